@@ -15,6 +15,7 @@ from .ComprEx import (Comprex, FastComprex, ThresholdNone, ThresholdConst, Thres
 from .allreduce import (AllToOneAllreduce, RingAllreduce, BigRingAllreduce, AutoAllreduce,  # noqa: F401
                         Comprex_AllToOneAllreduce, Comprex_RingAllreduce, Comprex_BigRingAllreduce,
                         select_schedule)
+from .adamw import AdamW  # noqa: F401
 from .utils import ComprexConfig  # noqa: F401
 
 __version__ = "0.1.0"

@@ -94,6 +94,18 @@ class Op(C.Structure):
                 ("tg", Targets), ("src", Sources), ("apply", ApplyArgs)]
 
 
+class AdamWClass(C.Structure):
+    _fields_ = [(n, C.c_float) for n in ("decay", "b1", "ob1", "b2", "ob2", "rate", "norm", "eps")]
+
+
+class AdamW(C.Structure):
+    """Arguments of cx_adamw_step (CxAdamW in csrc/cx_ops.h)."""
+    _fields_ = ([(n, C.c_void_p) for n in ("blk_seg", "seg_blk", "seg_len", "seg_param", "seg_grad", "seg_class", "master", "m",
+                                           "v", "m_scale", "v_scale")]
+                + [("blocks", C.c_int64), ("segs", C.c_int32), ("dtype", C.c_int32), ("bits", C.c_int32),
+                   ("noise", C.c_uint32), ("cls", AdamWClass * 64)])
+
+
 assert C.sizeof(Header) == 64 and C.sizeof(Stats) == 32
 
 _lock = threading.Lock()
@@ -167,6 +179,9 @@ def _declare(lib) -> None:
         "cx_host_alloc": (vp, [i64]),
         "cx_host_free": (i32, [vp]),
         "cx_host_wait_seq": (i32, [vp, u64, u64]),
+        "cx_adamw_noise": (u32, [u32]),
+        "cx_adamw_step": (i32, [i32, P(AdamW), vp]),
+        "cx_ops_sizeof": (i64, [i32]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)
@@ -196,6 +211,9 @@ def load():
             if mirror is not None and lib.cx_sizeof(what) != C.sizeof(mirror):
                 raise ComprexError(f"{path} does not match this binding ({mirror.__name__} is "
                                    f"{lib.cx_sizeof(what)} bytes there, {C.sizeof(mirror)} here): rebuild it")
+        for what, mirror in enumerate((AdamW,)):
+            if lib.cx_ops_sizeof(what) != C.sizeof(mirror):
+                raise ComprexError(f"{path} does not match this binding ({mirror.__name__}): rebuild it")
         _lib = lib
     return _lib
 

@@ -1,0 +1,253 @@
+"""AdamW over all tensors of a model in one kernel launch, with states in 32 bits or in 8.
+
+The optimizer for gradients that are ready to be applied: those of one GPU, or those that DistributedDataParallel has
+averaged through :func:`comprex_b200.ddp_hook.comprex_hook`.  (:class:`~comprex_b200.optim.ComprexOptimizer` exchanges
+the gradients itself and keeps one setting for the whole model.)
+
+    opt = cx.AdamW(model.parameters(), lr=3e-4, weight_decay=0.1, state_bits=8)
+
+Decoupled weight decay and bias corrections as in ``torch.optim.AdamW``:
+
+    m = b1 m + (1 - b1) g      v = b2 v + (1 - b2) g^2
+    p = (1 - lr wd) p - lr / (1 - b1^t) * m / (sqrt(v / (1 - b2^t)) + eps)
+
+Tensors of 16 bits have 32-bit weights behind them, which take the step; the tensor is their rounded copy.  Every
+parameter group has its own settings and every tensor its own step count: a tensor without a gradient is left alone.
+
+States live in flat buffers in which tensor ``i`` starts at a multiple of 256 elements, in the order of the
+parameters (:meth:`AdamW.flat_state`).  With ``state_bits=8`` each block of 256 elements keeps ``exp_avg`` and
+``exp_avg_rms``, the square root of the second moment, as ``float8_e4m3fn`` times a power of two: 2.03 bytes an
+element instead of 8.  They are rounded at random (up as often as what is cut off is part of a step), because a moving
+average with a beta near one would never leave its value under rounding to nearest; the random bits are a hash of the
+element's place, the step and ``seed``, so a run can be repeated bit for bit and does not depend on the launch.  A
+gradient that is no number spoils its own element, and the 8-bit states of its block.
+"""
+from __future__ import annotations
+
+import ctypes as C
+import math
+
+import numpy as np
+import torch
+
+from . import _lib
+from ._lib import ComprexError
+from .optim import _dense_layout
+
+_BLOCK = 256
+
+
+class AdamW(torch.optim.Optimizer):
+    """``params``: tensors of one type (float32, bfloat16, float16) on one device, each without gaps in memory."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, seed=0):
+        if state_bits not in (8, 32):
+            raise ValueError("state_bits must be 8 or 32")
+        self._check_settings(dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
+        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
+        self.state_bits, self.seed = int(state_bits), int(seed)
+        self._params = [p for g in self.param_groups for p in g["params"] if p.requires_grad]
+        if not self._params:
+            raise ValueError("optimizer got an empty parameter list")
+        self._group = np.array([i for i, g in enumerate(self.param_groups) for p in g["params"] if p.requires_grad])
+        first = self._params[0]
+        self._dtype, self._device = first.dtype, first.device
+        self._code, self._dev = _lib.dtype_code(first.dtype), _lib.dev_code(first)
+        if first.device.type not in ("cuda", "cpu"):
+            raise ComprexError(f"parameters on {first.device} are not supported")
+        for p in self._params:
+            if p.dtype != self._dtype or p.device != self._device:
+                raise ComprexError("all parameters must share one dtype and live on one device")
+            if p.layout != torch.strided or not _dense_layout(p):
+                raise ComprexError("a parameter has gaps in memory")
+        self._lay_out()
+
+    @staticmethod
+    def _check_settings(group):
+        b1, b2 = group["betas"]
+        if not (group["lr"] >= 0 and group["eps"] >= 0 and group["weight_decay"] >= 0 and 0 <= b1 < 1 and 0 <= b2 < 1):
+            raise ValueError("lr, eps and weight_decay must not be negative, betas lie in [0, 1)")
+
+    def add_param_group(self, param_group):
+        if hasattr(self, "_lay"):
+            raise ComprexError("the flat states are laid out at construction: give all parameter groups there")
+        super().add_param_group(param_group)
+
+    def _lay_out(self) -> None:
+        dev = self._device
+        numel = np.array([p.numel() for p in self._params], dtype=np.int64)
+        blocks = -(-numel // _BLOCK)
+        first = np.concatenate(([0], np.cumsum(blocks)))
+        self._first, self._numel = first, numel
+        k, nblk = len(numel), int(first[-1])
+        n = nblk * _BLOCK
+        put = lambda a, dt: torch.from_numpy(a.astype(dt)).to(dev)  # noqa: E731
+        self._lay = {
+            "blk_seg": put(np.repeat(np.arange(k), blocks), np.int32), "seg_blk": put(first[:-1], np.int64),
+            "seg_len": put(numel, np.int64), "seg_class": torch.zeros(k, dtype=torch.int32, device=dev),
+            "seg_param": torch.zeros(k, dtype=torch.int64, device=dev), "seg_grad": torch.zeros(k, dtype=torch.int64, device=dev),
+        }
+        state = {}
+        if self._dtype != torch.float32:
+            state["master"] = torch.zeros(n, dtype=torch.float32, device=dev)
+        if self.state_bits == 32:
+            state |= {s: torch.zeros(n, dtype=torch.float32, device=dev) for s in ("exp_avg", "exp_avg_sq")}
+        else:
+            for s in ("exp_avg", "exp_avg_rms"):
+                state[s] = torch.zeros(n, dtype=torch.uint8, device=dev).view(torch.float8_e4m3fn)
+                state[s + "_scale"] = torch.zeros(nblk, dtype=torch.float32, device=dev)
+        self._flat = state
+        self._steps = np.zeros(k, dtype=np.int64)
+        a = self._args = _lib.AdamW()
+        for name, t in self._lay.items():
+            setattr(a, name, t.data_ptr())
+        a.blocks, a.segs, a.dtype, a.bits = nblk, k, self._code, self.state_bits
+        names = ("exp_avg", "exp_avg_sq") if self.state_bits == 32 else ("exp_avg", "exp_avg_rms")
+        a.m, a.v = (state[s].data_ptr() for s in names)
+        if self.state_bits == 8:
+            a.m_scale, a.v_scale = (state[s + "_scale"].data_ptr() for s in names)
+        if "master" in state:
+            a.master = state["master"].data_ptr()
+            self.refresh_master()
+        # host copies of what the device holds, and pinned buffers to bring it there
+        self._now = {"seg_param": torch.zeros(k, dtype=torch.int64), "seg_grad": torch.zeros(k, dtype=torch.int64),
+                     "seg_class": torch.zeros(k, dtype=torch.int32)}
+        self._collect, self._scalar_type = _lib.host().collect, _lib.host().scalar_type(self._params[0])
+        self._ring = {}
+        self._classes, self._same = None, False
+        self._place()
+
+    def _place(self) -> None:
+        """The table of the tensors' addresses."""
+        if _lib.host().addresses(self._params, self._now["seg_param"].data_ptr()):
+            self._upload("seg_param")
+
+    def _upload(self, name) -> None:
+        """Table ``name`` to the device, in stream order and without waiting for it."""
+        src = self._now[name]
+        if self._device.type != "cuda":
+            self._lay[name].copy_(src)
+            return
+        ring = self._ring.setdefault(name, [0] + [(torch.empty_like(src).pin_memory(), torch.cuda.Event()) for _ in range(4)])
+        host, ev = ring[1 + ring[0]]
+        ring[0] = (ring[0] + 1) % 4
+        ev.synchronize()                      # the copy that last used this buffer has finished
+        host.copy_(src)
+        self._lay[name].copy_(host, non_blocking=True)
+        ev.record(torch.cuda.current_stream(self._device))
+
+    def _grads(self) -> bool:
+        """Bring the table of gradient addresses up to date (0: none); whether it has changed."""
+        now = self._now["seg_grad"]
+        changed = self._collect(self._params, self._scalar_type, 0, now.data_ptr())
+        if changed == 2:                      # rare: another type or memory order than the tensor's
+            now.fill_(-1)
+            for p in self._params:
+                g = p.grad
+                if g is None:
+                    continue
+                if g.layout != torch.strided or g.size() != p.size():
+                    raise ComprexError("a gradient is sparse or does not have its parameter's shape")
+                if g.dtype is not self._dtype or g.stride() != p.stride():
+                    p.grad = torch.empty_strided(p.size(), p.stride(), dtype=self._dtype, device=p.device).copy_(g)
+            changed = self._collect(self._params, self._scalar_type, 0, now.data_ptr())
+            if changed == 2:
+                now.fill_(-1)
+                raise ComprexError("a gradient does not have its parameter's shape")
+        if changed:
+            self._upload("seg_grad")
+        return bool(changed)
+
+    def _set_classes(self) -> None:
+        """Tensors with the same settings and step count share a row of settings."""
+        pair, of = np.unique(np.stack((self._group, self._steps)), axis=1, return_inverse=True)
+        if pair.shape[1] > len(self._args.cls):
+            raise ComprexError(f"more than {len(self._args.cls)} different settings and step counts")
+        self._classes = pair
+        of = torch.from_numpy(of.reshape(-1).astype(np.int32))
+        if not torch.equal(of, self._now["seg_class"]):
+            self._now["seg_class"].copy_(of)
+            self._upload("seg_class")
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for g in self.param_groups:
+            self._check_settings(g)
+        if self._device.type == "cuda" and torch.cuda.current_device() != self._device.index:
+            with torch.cuda.device(self._device):
+                self._step()
+        else:
+            self._step()
+        return loss
+
+    def _step(self) -> None:
+        self._place()
+        if self._grads() or self._classes is None:
+            has = (self._now["seg_grad"] != 0).numpy()
+            self._same = bool(has.all())
+            self._has = has
+            self._classes = None
+        a = self._args
+        if self._same and self._classes is not None:
+            # all tensors step: the classes stay what they are, one step further
+            self._steps += 1
+            self._classes[1] += 1
+        else:
+            self._steps += self._has
+            self._set_classes()
+        for i, (group, t) in enumerate(self._classes.T.tolist()):
+            g, c = self.param_groups[group], a.cls[i]
+            b1, b2 = g["betas"]
+            t = max(t, 1)                     # a class that has never stepped has no tensor with a gradient
+            c.decay = 1.0 - float(g["lr"]) * float(g["weight_decay"])
+            c.b1, c.ob1, c.b2, c.ob2 = b1, 1.0 - b1, b2, 1.0 - b2
+            c.rate, c.norm, c.eps = float(g["lr"]) / (1.0 - b1 ** t), 1.0 / math.sqrt(1.0 - b2 ** t), g["eps"]
+        lib = _lib.load()
+        a.noise = lib.cx_adamw_noise((self.seed + int(self._steps.max())) & 0xFFFFFFFF)
+        _lib.check(lib.cx_adamw_step(self._dev, C.byref(a), _lib.stream_ptr(self._device)), "cx_adamw_step")
+
+    def flat_state(self) -> dict:
+        """The buffers that hold the states of all tensors (not copies): ``master`` for 16-bit tensors, ``exp_avg`` and
+        ``exp_avg_sq``, or with 8 bits ``exp_avg`` and ``exp_avg_rms`` with a scale for each 256 elements."""
+        return dict(self._flat)
+
+    def spans(self) -> list:
+        """(start, elements) of every tensor in the flat buffers, in the order of the parameters."""
+        return [(int(a) * _BLOCK, int(n)) for a, n in zip(self._first, self._numel)]
+
+    @torch.no_grad()
+    def refresh_master(self) -> None:
+        """Take the tensors as they are as the 32-bit weights: after they were overwritten from outside."""
+        master = self._flat.get("master")
+        if master is not None:
+            for p, (a, n) in zip(self._params, self.spans()):
+                master[a:a + n].as_strided(p.size(), p.stride()).copy_(p)
+
+    # ---- checkpoint ------------------------------------------------------------------------------------------------
+    def state_dict(self):
+        sd = super().state_dict()
+        sd["comprex_adamw"] = {"version": 1, "bits": self.state_bits, "seed": self.seed, "numel": self._numel.tolist(),
+                               "steps": self._steps.tolist(), "flat": {k: t.detach().cpu().clone() for k, t in self._flat.items()}}
+        return sd
+
+    @torch.no_grad()
+    def load_state_dict(self, state_dict):
+        state_dict = dict(state_dict)
+        mine = state_dict.pop("comprex_adamw", None)
+        if mine is None:
+            raise ComprexError("not a checkpoint of this optimizer")
+        if mine["bits"] != self.state_bits or mine["numel"] != self._numel.tolist() or set(mine["flat"]) != set(self._flat):
+            raise ComprexError("checkpoint was written for other parameters or another width of states")
+        super().load_state_dict(state_dict)
+        for k, t in self._flat.items():
+            t.copy_(mine["flat"][k])
+        self.seed = int(mine["seed"])
+        self._steps = np.array(mine["steps"], dtype=np.int64)
+        self._classes = None
+        if "master" in self._flat:
+            for p, (a, n) in zip(self._params, self.spans()):
+                p.copy_(self._flat["master"][a:a + n].as_strided(p.size(), p.stride()))

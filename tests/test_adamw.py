@@ -1,0 +1,266 @@
+"""AdamW over many tensors (csrc/adamw.cu): against the formula in 64 bits, its 8-bit states, its refusals."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import comprex_b200 as cx
+from comprex_b200 import ComprexError
+
+SIZES = [1, 3, 255, 256, 257, 1000, 4096, 10007]
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+HYPER = dict(lr=1e-2, betas=(0.9, 0.99), eps=1e-8, weight_decay=0.1)
+EPS32 = 2.0 ** -24
+ROUND = {torch.float32: 0.0, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}     # of the stored copy
+
+
+def _params(dtype, device, sizes=SIZES, seed=0, shift=0):
+    """Leaves of the given sizes; ``shift``: start them that many elements off a 16-byte boundary."""
+    gen = torch.Generator().manual_seed(seed)
+    out = []
+    for n in sizes:
+        store = torch.zeros(n + shift, dtype=dtype, device=device)
+        store[shift:] = torch.randn(n, generator=gen).to(dtype)
+        out.append(torch.nn.Parameter(store[shift:]))
+    return out
+
+
+def _set_grads(params, seed, scale=1e-2):
+    gen = torch.Generator().manual_seed(seed)
+    for p in params:
+        p.grad = (torch.randn(p.numel(), generator=gen) * scale).to(p.dtype).to(p.device).view(p.size())
+
+
+def _formula(p, m, v, g, t, lr, betas, eps, weight_decay):
+    b1, b2 = betas
+    m = b1 * m + (1 - b1) * g
+    v = b2 * v + (1 - b2) * g * g
+    p = (1 - lr * weight_decay) * p - lr * (m / (1 - b1 ** t)) / (torch.sqrt(v / (1 - b2 ** t)) + eps)
+    return p, m, v
+
+
+def _weights(opt, params):
+    flat = opt.flat_state().get("master")
+    if flat is None:
+        return [p.detach().double().cpu().flatten() for p in params]
+    return [flat[a:a + n].double().cpu() for a, n in opt.spans()]
+
+
+def _decoded(opt, name):
+    flat = opt.flat_state()
+    x = flat[name].cpu().float().double().view(-1, 256) * flat[name + "_scale"].cpu().double()[:, None]
+    return [x.flatten()[a:a + n] for a, n in opt.spans()]
+
+
+@pytest.mark.parametrize("shift", [0, 1])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_32_bit_states_against_the_formula(device, dtype, shift):
+    params = _params(dtype, device, shift=shift)
+    opt = cx.AdamW(params, state_bits=32, **HYPER)
+    want = [(p.detach().double().cpu(), 0.0, 0.0) for p in params]
+    steps = 5
+    for t in range(1, steps + 1):
+        _set_grads(params, seed=t)
+        want = [_formula(*w, p.grad.double().cpu(), t, **HYPER) for w, p in zip(want, params)]
+        opt.step()
+    flat = opt.flat_state()
+    for got, p, (wp, wm, wv), (a, n) in zip(_weights(opt, params), params, want, opt.spans()):
+        # per step: two roundings of p, and a change of at most ~10 lr (a cancelled m over a small v) with eight roundings
+        assert (got - wp).abs().max() <= steps * EPS32 * (2 * wp.abs().max() + 10 * HYPER["lr"] * 8) + 1e-7
+        # per step three roundings of sums of magnitudes that the largest gradient bounds
+        assert (flat["exp_avg"][a:a + n].double().cpu() - wm).abs().max() <= 4 * steps * EPS32 * 0.06
+        assert ((flat["exp_avg_sq"][a:a + n].double().cpu() - wv).abs() <= 6 * steps * EPS32 * wv + 1e-30).all()
+        # the tensor is the rounded weight
+        assert torch.equal(p.detach().cpu(), got.float().to(dtype))
+    # the gaps between the tensors stay empty
+    gap = torch.ones(flat["exp_avg"].numel(), dtype=torch.bool)
+    for a, n in opt.spans():
+        gap[a:a + n] = False
+    assert not flat["exp_avg"].cpu()[gap].any() and not flat["exp_avg_sq"].cpu()[gap].any()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_8_bit_states_hold_the_moments(device, dtype):
+    params = _params(dtype, device)
+    opt = cx.AdamW(params, state_bits=8, seed=3, **HYPER)
+    want = [p.detach().double().cpu() for p in params]
+    held_m, held_r = ([torch.zeros_like(w) for w in want] for _ in range(2))
+    for t in range(1, 6):
+        _set_grads(params, seed=t)
+        new = [_formula(w, m, r * r, p.grad.double().cpu(), t, **HYPER) for w, m, r, p in zip(want, held_m, held_r, params)]
+        opt.step()
+        want = _weights(opt, params)
+        for (wp, _, _), got in zip(new, want):
+            assert (got - wp).abs().max() <= EPS32 * (2 * wp.abs().max() + 10 * HYPER["lr"] * 8) + 1e-7
+        held_m, held_r = _decoded(opt, "exp_avg"), _decoded(opt, "exp_avg_rms")
+        flat = opt.flat_state()
+        for i, (_, m, v) in enumerate(new):
+            block = np.arange(m.numel()) // 256 + opt.spans()[i][0] // 256
+            for got, exact, scale in ((held_m[i], m, flat["exp_avg_scale"]), (held_r[i], v.sqrt(), flat["exp_avg_rms_scale"])):
+                s = scale.cpu().double()[block]
+                # one step of three bits of mantissa, or in the subnormals two of theirs (cut at random, then rounded)
+                assert ((got - exact).abs() <= exact.abs() * (2.0 ** -3 + 1e-6) + s * 2.0 ** -9 * 1.5).all()
+                assert ((exact.abs() / s) < 256.01).all()
+            assert ((held_r[i] > 0) == (v > 0)).all()
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.gpu
+def test_cuda_agrees_with_host_bit_for_bit(dtype, bits):
+    made = {}
+    for device in ("cpu", "cuda"):
+        params = _params(dtype, device)
+        opt = cx.AdamW(params, state_bits=bits, seed=7, **HYPER)
+        for t in range(4):
+            _set_grads(params, seed=t)
+            opt.step()
+        made[device] = {k: t.cpu() for k, t in opt.flat_state().items()}
+        made[device]["param"] = torch.cat([p.detach().cpu() for p in params])
+    for k, t in made["cpu"].items():
+        a, b = (x.view(torch.uint8) for x in (t, made["cuda"][k]))
+        assert torch.equal(a, b), k
+
+
+def test_rounding_is_unbiased(device):
+    """The same gradient everywhere: the mean of n states rounded at random is the moment itself."""
+    n, g = 1 << 16, 0.01
+    p = torch.nn.Parameter(torch.zeros(n, device=device))
+    opt = cx.AdamW([p], state_bits=8, lr=0.0, betas=(0.9, 0.99), weight_decay=0.0)
+    grad = torch.full((n,), g, device=device)
+    grad[::256] = 0.0137         # the largest of each block, so that the others lie inside a step
+    p.grad = grad
+    opt.step()
+    keep = torch.arange(n) % 256 != 0
+    for name, exact in (("exp_avg", 0.1 * g), ("exp_avg_rms", math.sqrt(0.01) * g)):
+        got = _decoded(opt, name)[0][keep]
+        step = (got.max() - got.min()).item()
+        assert got.min() <= exact <= got.max() and got.unique().numel() == 2
+        # five standard deviations of the mean of independent roundings, and the 16 bits' own resolution
+        assert abs(got.mean().item() - exact) <= step * (5 * 0.5 / math.sqrt(keep.sum().item()) + 2.0 ** -16)
+
+
+def test_a_second_moment_does_not_stick(device):
+    """b2 near one: the states of a block follow a gradient that has become small, though one change is below a step."""
+    n = 4096
+    p = torch.nn.Parameter(torch.zeros(n, device=device))
+    opt = cx.AdamW([p], state_bits=8, lr=0.0, betas=(0.9, 0.98), weight_decay=0.0)
+    first = torch.ones(n, device=device)
+    later = torch.full((n,), 0.25, device=device)
+    later[::256] = 1.0
+    p.grad = first
+    opt.step()
+    p.grad = later
+    steps = 60
+    for _ in range(steps):
+        opt.step()
+    got = (_decoded(opt, "exp_avg_rms")[0][torch.arange(n) % 256 != 0] ** 2).mean().item()
+    exact = 0.02 * 0.98 ** steps + 0.0625 * (1 - 0.98 ** steps)
+    # each step adds the variance of a rounded root (at most (2^-3)^2 / 4 of v) to the mean of v, which b2 forgets again
+    assert exact * 0.98 <= got <= exact * (1 + steps * 2.0 ** -8 * 1.05)
+
+
+def test_groups_and_missing_gradients(device):
+    a, b, c = _params(torch.float32, device, [300, 5, 700])
+    opt = cx.AdamW([{"params": [a, b], "lr": 0.1, "weight_decay": 0.0}, {"params": [c], "betas": (0.5, 0.9)}], lr=0.01, weight_decay=0.5)
+    hyper = [dict(lr=0.1, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0)] * 2 + [dict(lr=0.01, betas=(0.5, 0.9), eps=1e-8, weight_decay=0.5)]
+    want = [(p.detach().double().cpu(), torch.zeros(p.numel(), dtype=torch.float64), torch.zeros(p.numel(), dtype=torch.float64), 0) for p in (a, b, c)]
+    for turn, missing in enumerate([(), (1,), (0, 2), (), (1,), ()]):
+        _set_grads([a, b, c], seed=turn)
+        for i, p in enumerate((a, b, c)):
+            if i in missing:
+                p.grad = None
+                continue
+            w, m, v, t = want[i]
+            want[i] = (*_formula(w, m, v, p.grad.double().cpu(), t + 1, **hyper[i]), t + 1)
+        opt.step()
+    for p, (w, _, _, _) in zip((a, b, c), want):
+        assert (p.detach().double().cpu() - w).abs().max() <= 6 * EPS32 * (2 * w.abs().max() + 10 * 0.1 * 8) + 1e-7
+    opt.param_groups[0]["lr"] = 0.0
+    before = a.detach().clone()
+    opt.step()
+    assert torch.equal(a.detach(), before)
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_checkpoint_goes_on_where_it_was(device, bits):
+    def run(opt, params, steps):
+        for t in steps:
+            _set_grads(params, seed=t)
+            opt.step()
+    a = _params(torch.bfloat16, device)
+    whole = cx.AdamW(a, state_bits=bits, seed=5, **HYPER)
+    run(whole, a, range(4))
+    b = _params(torch.bfloat16, device)
+    part = cx.AdamW(b, state_bits=bits, seed=5, **HYPER)
+    run(part, b, range(2))
+    saved = part.state_dict()
+    c = _params(torch.bfloat16, device, seed=9)
+    other = cx.AdamW(c, state_bits=bits, **HYPER)
+    other.load_state_dict(saved)
+    run(other, c, range(2, 4))
+    for x, y in zip(a, c):
+        assert torch.equal(x, y)
+    for k, t in whole.flat_state().items():
+        assert torch.equal(t.view(torch.uint8), other.flat_state()[k].view(torch.uint8)), k
+
+
+def test_memory_orders_and_other_gradients(device):
+    """Channels-last weights keep their order; a gradient of another order or type is brought into the tensor's."""
+    w = torch.randn(6, 4, 5, 5).to(device).to(memory_format=torch.channels_last)
+    p, q = torch.nn.Parameter(w.clone(memory_format=torch.preserve_format)), torch.nn.Parameter(w.contiguous().clone())
+    g = torch.randn(6, 4, 5, 5).to(device)
+    p.grad, q.grad = g.contiguous(), g.contiguous()
+    cx.AdamW([p], lr=0.1).step()
+    cx.AdamW([q], lr=0.1).step()
+    assert p.stride() != q.stride() and torch.equal(p.detach(), q.detach())
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_a_bad_gradient_spoils_its_element(device, bits):
+    p = torch.nn.Parameter(torch.ones(600, device=device))
+    opt = cx.AdamW([p], state_bits=bits, lr=0.1)
+    g = torch.full((600,), 0.01, device=device)
+    g[17], g[300] = float("nan"), float("inf")
+    p.grad = g
+    opt.step()
+    p.grad = torch.full((600,), 0.01, device=device)
+    opt.step()
+    bad = ~torch.isfinite(p.detach().cpu())
+    assert bad.nonzero().flatten().tolist() == [17, 300]
+
+
+def test_zero_gradients_leave_zero_states(device):
+    p = torch.nn.Parameter(torch.ones(300, device=device))
+    opt = cx.AdamW([p], state_bits=8, lr=0.1, weight_decay=0.0)
+    p.grad = torch.zeros(300, device=device)
+    opt.step()
+    assert torch.equal(p.detach().cpu(), torch.ones(300))
+    for name in ("exp_avg", "exp_avg_rms"):
+        assert not _decoded(opt, name)[0].any()
+
+
+def test_refusals(device):
+    p = torch.nn.Parameter(torch.zeros(4, 4, device=device))
+    with pytest.raises(ValueError):
+        cx.AdamW([p], state_bits=16)
+    with pytest.raises(ValueError):
+        cx.AdamW([p], lr=-1.0)
+    with pytest.raises(ValueError):
+        cx.AdamW([p], betas=(0.9, 1.0))
+    with pytest.raises(ComprexError):
+        cx.AdamW([p, torch.nn.Parameter(torch.zeros(4, dtype=torch.bfloat16, device=device))])
+    with pytest.raises(ComprexError):
+        cx.AdamW([torch.nn.Parameter(torch.zeros(4, dtype=torch.float64, device=device))])
+    with pytest.raises(ComprexError):
+        cx.AdamW([torch.nn.Parameter(torch.zeros(4, 8, device=device)[:, :4])])
+    opt = cx.AdamW([p])
+    with pytest.raises(ComprexError):
+        opt.add_param_group({"params": [torch.nn.Parameter(torch.zeros(2, device=device))]})
+    with pytest.raises(ComprexError):
+        opt.load_state_dict(torch.optim.AdamW([p]).state_dict())
+    with pytest.raises(ComprexError):
+        opt.load_state_dict(cx.AdamW([p], state_bits=8).state_dict())
+    opt.step()                   # no gradient anywhere: nothing moves
+    assert not p.detach().any()
