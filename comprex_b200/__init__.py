@@ -16,6 +16,8 @@ from .allreduce import (AllToOneAllreduce, RingAllreduce, BigRingAllreduce, Auto
                         Comprex_AllToOneAllreduce, Comprex_RingAllreduce, Comprex_BigRingAllreduce,
                         select_schedule)
 from .adamw import AdamW  # noqa: F401
+from .ops.linear import linear  # noqa: F401
+from .ops.vocab_loss import linear_cross_entropy  # noqa: F401
 from .utils import ComprexConfig  # noqa: F401
 
 __version__ = "0.1.0"

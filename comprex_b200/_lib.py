@@ -106,6 +106,26 @@ class AdamW(C.Structure):
                    ("noise", C.c_uint32), ("cls", AdamWClass * 64)])
 
 
+ACTIVATIONS = {None: 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
+REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
+
+
+class Linear(C.Structure):
+    """Arguments of cx_linear_forward and cx_linear_backward (CxLinear in csrc/cx_ops.h)."""
+    _fields_ = ([(n, C.c_int64) for n in ("rows", "inner", "outer", "ldx", "ldw", "ldr", "ldg")]
+                + [(n, C.c_void_p) for n in ("x", "w", "bias", "residual", "y", "pre", "grad", "dx", "dw", "dbias", "workspace")]
+                + [("ws_bytes", C.c_int64), ("dtype", C.c_int32), ("act", C.c_int32)])
+
+
+class VocabLoss(C.Structure):
+    """Arguments of cx_vocab_loss_forward and cx_vocab_loss_backward (CxVocabLoss in csrc/cx_ops.h)."""
+    _fields_ = ([(n, C.c_int64) for n in ("rows", "vocab", "dim", "ldh", "ldw")]
+                + [(n, C.c_void_p) for n in ("h", "w", "targets")] + [("ignore_index", C.c_int64)]
+                + [(n, C.c_void_p) for n in ("loss", "lse", "count", "grad")] + [("grad_stride", C.c_int64)]
+                + [(n, C.c_void_p) for n in ("dh", "dw", "workspace")]
+                + [("ws_bytes", C.c_int64), ("dtype", C.c_int32), ("reduction", C.c_int32)])
+
+
 assert C.sizeof(Header) == 64 and C.sizeof(Stats) == 32
 
 _lock = threading.Lock()
@@ -181,6 +201,12 @@ def _declare(lib) -> None:
         "cx_host_wait_seq": (i32, [vp, u64, u64]),
         "cx_adamw_noise": (u32, [u32]),
         "cx_adamw_step": (i32, [i32, P(AdamW), vp]),
+        "cx_linear_workspace_bytes": (i64, [i32, P(Linear), i32]),
+        "cx_linear_forward": (i32, [i32, P(Linear), vp]),
+        "cx_linear_backward": (i32, [i32, P(Linear), vp]),
+        "cx_vocab_loss_workspace_bytes": (i64, [i32, P(VocabLoss), i32]),
+        "cx_vocab_loss_forward": (i32, [i32, P(VocabLoss), vp]),
+        "cx_vocab_loss_backward": (i32, [i32, P(VocabLoss), vp]),
         "cx_ops_sizeof": (i64, [i32]),
     }
     for name, (res, args) in sig.items():
@@ -211,7 +237,7 @@ def load():
             if mirror is not None and lib.cx_sizeof(what) != C.sizeof(mirror):
                 raise ComprexError(f"{path} does not match this binding ({mirror.__name__} is "
                                    f"{lib.cx_sizeof(what)} bytes there, {C.sizeof(mirror)} here): rebuild it")
-        for what, mirror in enumerate((AdamW,)):
+        for what, mirror in enumerate((AdamW, Linear, VocabLoss)):
             if lib.cx_ops_sizeof(what) != C.sizeof(mirror):
                 raise ComprexError(f"{path} does not match this binding ({mirror.__name__}): rebuild it")
         _lib = lib

@@ -44,7 +44,67 @@ typedef struct CxAdamW {
 uint32_t cx_adamw_noise(uint32_t number);
 int cx_adamw_step(int dev, const CxAdamW* a, void* stream);
 
-int64_t cx_ops_sizeof(int what); /* 0 CxAdamW */
+/* ---- y = act(x w^T + bias) + residual --------------------------------------------------------------------------- */
+#define CX_ACT_NONE 0
+#define CX_ACT_RELU 1
+#define CX_ACT_GELU 2        /* u Phi(u) */
+#define CX_ACT_GELU_TANH 3   /* its tanh form */
+#define CX_ACT_SILU 4
+
+/* Matrices are row-major with rows `ld*` elements apart; y, dx, dw are written without gaps.  All of one type. */
+typedef struct CxLinear {
+  int64_t rows, inner, outer;
+  int64_t ldx, ldw, ldr, ldg;
+  const void* x;         /* [rows][inner] */
+  const void* w;         /* [outer][inner] */
+  const void* bias;      /* [outer] or NULL */
+  const void* residual;  /* [rows][outer] or NULL */
+  void* y;               /* forward: [rows][outer] */
+  void* pre;             /* x w^T + bias: written by the forward call when not NULL, read by the backward call where the
+                            activation needs it; [rows][outer] */
+  const void* grad;      /* backward: of y */
+  void* dx;              /* each may be NULL */
+  void* dw;
+  void* dbias;
+  void* workspace;       /* cx_linear_workspace_bytes */
+  int64_t ws_bytes;
+  int32_t dtype, act;
+} CxLinear;
+
+int64_t cx_linear_workspace_bytes(int dev, const CxLinear* l, int backward);
+int cx_linear_forward(int dev, const CxLinear* l, void* stream);
+int cx_linear_backward(int dev, const CxLinear* l, void* stream);
+
+/* ---- softmax cross entropy of h w^T over a vocabulary, without the logits ---------------------------------------- */
+#define CX_REDUCE_NONE 0
+#define CX_REDUCE_SUM 1
+#define CX_REDUCE_MEAN 2     /* over the rows that are not ignored */
+
+typedef struct CxVocabLoss {
+  int64_t rows, vocab, dim;
+  int64_t ldh, ldw;
+  const void* h;           /* [rows][dim] */
+  const void* w;           /* [vocab][dim] */
+  const int64_t* targets;  /* [rows]; ignore_index: the row counts for nothing; any other value outside [0, vocab) makes
+                              the row's loss and gradients NaN */
+  int64_t ignore_index;
+  float* loss;             /* [rows] for CX_REDUCE_NONE, else [1] */
+  float* lse;              /* [rows] log sum exp of the logits: written by the forward call, read by the backward call */
+  float* count;            /* [1] rows that are not ignored: likewise */
+  const float* grad;       /* backward: of the loss */
+  int64_t grad_stride;     /* CX_REDUCE_NONE: from row to row (0 for a broadcast one) */
+  void* dh;                /* [rows][dim], may be NULL */
+  void* dw;                /* [vocab][dim], may be NULL */
+  void* workspace;         /* cx_vocab_loss_workspace_bytes */
+  int64_t ws_bytes;
+  int32_t dtype, reduction;
+} CxVocabLoss;
+
+int64_t cx_vocab_loss_workspace_bytes(int dev, const CxVocabLoss* l, int backward);
+int cx_vocab_loss_forward(int dev, const CxVocabLoss* l, void* stream);
+int cx_vocab_loss_backward(int dev, const CxVocabLoss* l, void* stream);
+
+int64_t cx_ops_sizeof(int what); /* 0 CxAdamW, 1 CxLinear, 2 CxVocabLoss */
 
 #ifdef __cplusplus
 }

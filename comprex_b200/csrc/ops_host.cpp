@@ -97,3 +97,150 @@ int cx_adamw_step_host(const CxAdamW* a) {
   }
   return 0;
 }
+
+// ---- linear -----------------------------------------------------------------------------------------------------
+namespace {
+
+float act_host(float u, int act, float* slope) {
+  const float k = 0.79788456080286536f;
+  switch (act) {
+    case CX_ACT_RELU:
+      *slope = u > 0.f ? 1.f : 0.f;
+      return u > 0.f || u != u ? u : 0.f;
+    case CX_ACT_GELU: {
+      const float cdf = 0.5f * (1.f + erff(u * 0.70710678118654752f));
+      *slope = cdf + u * 0.39894228040143268f * expf(-0.5f * u * u);
+      return u * cdf;
+    }
+    case CX_ACT_GELU_TANH: {
+      const float t = tanhf(k * (u + 0.044715f * u * u * u));
+      *slope = 0.5f * (1.f + t) + 0.5f * u * (1.f - t * t) * k * (1.f + 0.134145f * u * u);
+      return 0.5f * u * (1.f + t);
+    }
+    case CX_ACT_SILU: {
+      const float q = 1.f / (1.f + expf(-u));
+      *slope = q * (1.f + u * (1.f - q));
+      return u * q;
+    }
+    default:
+      *slope = 1.f;
+      return u;
+  }
+}
+
+std::vector<float> widen(int dtype, const void* p, int64_t rows, int64_t cols, int64_t ld) {
+  std::vector<float> out((size_t)(rows * cols));
+  for (int64_t r = 0; r < rows; ++r)
+    for (int64_t c = 0; c < cols; ++c) out[(size_t)(r * cols + c)] = load_elem(dtype, p, r * ld + c);
+  return out;
+}
+// out[c] += sum over i of a[i] b[i][c]
+void add_product(const float* a, const float* b, float* out, int64_t inner, int64_t cols) {
+  for (int64_t i = 0; i < inner; ++i) {
+    if (a[i] == 0.f) continue;
+    for (int64_t c = 0; c < cols; ++c) out[c] += a[i] * b[i * cols + c];
+  }
+}
+float dot(const float* a, const float* b, int64_t n) {
+  float sum = 0.f;
+  for (int64_t i = 0; i < n; ++i) sum += a[i] * b[i];
+  return sum;
+}
+
+}  // namespace
+
+int cx_linear_forward_host(const CxLinear* l) {
+  const std::vector<float> x = widen(l->dtype, l->x, l->rows, l->inner, l->ldx), w = widen(l->dtype, l->w, l->outer, l->inner, l->ldw);
+  for (int64_t r = 0; r < l->rows; ++r)
+    for (int64_t c = 0; c < l->outer; ++c) {
+      float u = dot(&x[(size_t)(r * l->inner)], &w[(size_t)(c * l->inner)], l->inner), slope;
+      if (l->bias) u += load_elem(l->dtype, l->bias, c);
+      if (l->pre) store_elem(l->dtype, l->pre, r * l->outer + c, u);
+      u = act_host(u, l->act, &slope);
+      if (l->residual) u += load_elem(l->dtype, l->residual, r * l->ldr + c);
+      store_elem(l->dtype, l->y, r * l->outer + c, u);
+    }
+  return 0;
+}
+
+int cx_linear_backward_host(const CxLinear* l) {
+  std::vector<float> du = widen(l->dtype, l->grad, l->rows, l->outer, l->ldg), sum((size_t)l->outer);
+  for (int64_t r = 0; r < l->rows; ++r)
+    for (int64_t c = 0; c < l->outer; ++c) {
+      float& d = du[(size_t)(r * l->outer + c)];
+      float slope = 1.f;
+      if (l->act != CX_ACT_NONE) act_host(load_elem(l->dtype, l->pre, r * l->outer + c), l->act, &slope);
+      d *= slope;
+      sum[(size_t)c] += d;
+    }
+  if (l->dbias)
+    for (int64_t c = 0; c < l->outer; ++c) store_elem(l->dtype, l->dbias, c, sum[(size_t)c]);
+  std::vector<float> row((size_t)l->inner);
+  if (l->dx) {
+    const std::vector<float> w = widen(l->dtype, l->w, l->outer, l->inner, l->ldw);
+    for (int64_t r = 0; r < l->rows; ++r) {
+      std::fill(row.begin(), row.end(), 0.f);
+      add_product(&du[(size_t)(r * l->outer)], w.data(), row.data(), l->outer, l->inner);
+      for (int64_t i = 0; i < l->inner; ++i) store_elem(l->dtype, l->dx, r * l->inner + i, row[(size_t)i]);
+    }
+  }
+  if (l->dw) {
+    const std::vector<float> x = widen(l->dtype, l->x, l->rows, l->inner, l->ldx);
+    for (int64_t c = 0; c < l->outer; ++c) {
+      std::fill(row.begin(), row.end(), 0.f);
+      for (int64_t r = 0; r < l->rows; ++r) add_product(&du[(size_t)(r * l->outer + c)], &x[(size_t)(r * l->inner)], row.data(), 1, l->inner);
+      for (int64_t i = 0; i < l->inner; ++i) store_elem(l->dtype, l->dw, c * l->inner + i, row[(size_t)i]);
+    }
+  }
+  return 0;
+}
+
+// ---- loss over a vocabulary ---------------------------------------------------------------------------------------
+int cx_vocab_loss_forward_host(const CxVocabLoss* l) {
+  const std::vector<float> h = widen(l->dtype, l->h, l->rows, l->dim, l->ldh), w = widen(l->dtype, l->w, l->vocab, l->dim, l->ldw);
+  std::vector<float> s((size_t)l->vocab);
+  float sum = 0.f, count = 0.f;
+  for (int64_t r = 0; r < l->rows; ++r) {
+    const int64_t t = l->targets[r];
+    float top = -INFINITY, z = 0.f;
+    for (int64_t v = 0; v < l->vocab; ++v) {
+      s[(size_t)v] = dot(&h[(size_t)(r * l->dim)], &w[(size_t)(v * l->dim)], l->dim);
+      if (s[(size_t)v] > top || s[(size_t)v] != s[(size_t)v]) top = s[(size_t)v];
+    }
+    for (int64_t v = 0; v < l->vocab; ++v) z += expf(s[(size_t)v] - top);
+    const bool ignored = t == l->ignore_index, inside = t >= 0 && t < l->vocab;
+    l->lse[r] = !ignored && !inside ? NAN : top + logf(z);
+    const float loss = ignored ? 0.f : inside ? l->lse[r] - s[(size_t)t] : NAN;
+    if (l->reduction == CX_REDUCE_NONE) l->loss[r] = loss;
+    sum += loss;
+    count += ignored ? 0.f : 1.f;
+  }
+  *l->count = count;
+  if (l->reduction != CX_REDUCE_NONE) *l->loss = l->reduction == CX_REDUCE_MEAN ? sum / count : sum;
+  return 0;
+}
+
+int cx_vocab_loss_backward_host(const CxVocabLoss* l) {
+  const std::vector<float> h = widen(l->dtype, l->h, l->rows, l->dim, l->ldh), w = widen(l->dtype, l->w, l->vocab, l->dim, l->ldw);
+  std::vector<float> p((size_t)l->vocab), dh((size_t)l->dim), dw((size_t)(l->vocab * l->dim));
+  for (int64_t r = 0; r < l->rows; ++r) {
+    const int64_t t = l->targets[r];
+    float g = l->grad[l->reduction == CX_REDUCE_NONE ? r * l->grad_stride : 0];
+    if (l->reduction == CX_REDUCE_MEAN) g /= *l->count;
+    if (t == l->ignore_index) g = 0.f;
+    const float* hr = &h[(size_t)(r * l->dim)];
+    std::fill(dh.begin(), dh.end(), 0.f);
+    if (g != 0.f) {
+      for (int64_t v = 0; v < l->vocab; ++v)
+        p[(size_t)v] = (expf(dot(hr, &w[(size_t)(v * l->dim)], l->dim) - l->lse[r]) - (v == t ? 1.f : 0.f)) * g;
+      add_product(p.data(), w.data(), dh.data(), l->vocab, l->dim);
+      if (l->dw)
+        for (int64_t v = 0; v < l->vocab; ++v) add_product(&p[(size_t)v], hr, &dw[(size_t)(v * l->dim)], 1, l->dim);
+    }
+    if (l->dh)
+      for (int64_t i = 0; i < l->dim; ++i) store_elem(l->dtype, l->dh, r * l->dim + i, dh[(size_t)i]);
+  }
+  if (l->dw)
+    for (int64_t i = 0; i < l->vocab * l->dim; ++i) store_elem(l->dtype, l->dw, i, dw[(size_t)i]);
+  return 0;
+}

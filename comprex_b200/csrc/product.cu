@@ -1,0 +1,121 @@
+// The product of cx_product.cuh on the CUDA cores: any type, layout and stride.
+#include "cx_product.cuh"
+
+namespace {
+
+constexpr int kTile = 64, kDepth = 16, kThreads = 256;
+
+template <typename T>
+__device__ __forceinline__ void finish(const CxProduct& p, int64_t row, int64_t col, float v) {
+  using E = cx::Elem<T>;
+  if (p.mode == kSums) {
+    float* at = p.addend + row * p.n + col;
+    *at = p.has_addend ? *at + v : v;
+    return;
+  }
+  if (p.mode == kProb) {
+    const float q = exp2f(v * cxprod::kLog2e - p.lse[row]) - (p.targets[row] == p.col0 + col ? 1.f : 0.f);
+    const float f = p.row_factor[row];
+    reinterpret_cast<T*>(p.out)[row * p.ldo + col] = E::from_f(f == 0.f ? 0.f : q * f);
+    return;
+  }
+  if (p.has_addend) v += p.addend[row * p.n + col];
+  if (p.scale) v *= *p.scale;
+  if (p.bias) v += E::to_f(reinterpret_cast<const T*>(p.bias)[col]);
+  if (p.pre) reinterpret_cast<T*>(p.pre)[row * p.ldo + col] = E::from_f(v);
+  v = cxprod::activate(v, p.act);
+  if (p.residual) v += E::to_f(reinterpret_cast<const T*>(p.residual)[row * p.ldr + col]);
+  reinterpret_cast<T*>(p.out)[row * p.ldo + col] = E::from_f(v);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) product_kernel(const __grid_constant__ CxProduct p) {
+  __shared__ float sa[kDepth][kTile + 1], sb[kDepth][kTile + 1];
+  __shared__ float2 stat[kTile][16];
+  using E = cx::Elem<T>;
+  const int64_t row0 = (int64_t)blockIdx.x * kTile, col0 = (int64_t)blockIdx.y * kTile;
+  const int tr = threadIdx.x / 16, tc = threadIdx.x % 16;
+  const T* a = reinterpret_cast<const T*>(p.a);
+  const T* b = reinterpret_cast<const T*>(p.b);
+  float acc[4][4] = {};
+  for (int64_t k0 = 0; k0 < p.k; k0 += kDepth) {
+#pragma unroll
+    for (int j = 0; j < kTile * kDepth / kThreads; ++j) {
+      const int i = threadIdx.x + j * kThreads;
+      // neighbouring threads along the operand's consecutive elements
+      const int ka = p.layout == kTN ? i / kTile : i % kDepth, ma = p.layout == kTN ? i % kTile : i / kDepth;
+      const int kb = p.layout == kNT ? i % kDepth : i / kTile, nb = p.layout == kNT ? i / kDepth : i % kTile;
+      const int64_t r = row0 + ma, c = col0 + nb;
+      const bool in_a = r < p.m && k0 + ka < p.k, in_b = c < p.n && k0 + kb < p.k;
+      sa[ka][ma] = !in_a ? 0.f : E::to_f(p.layout == kTN ? a[(k0 + ka) * p.lda + r] : a[r * p.lda + k0 + ka]);
+      sb[kb][nb] = !in_b ? 0.f : E::to_f(p.layout == kNT ? b[c * p.ldb + k0 + kb] : b[(k0 + kb) * p.ldb + c]);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kDepth; ++k) {
+      float x[4], y[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = sa[k][tr * 4 + i];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) y[i] = sb[k][tc * 4 + i];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = __fmaf_rn(x[i], y[j], acc[i][j]);
+    }
+    __syncthreads();
+  }
+  if (p.mode != kStats) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int64_t r = row0 + tr * 4 + i, c = col0 + tc * 4 + j;
+        if (r < p.m && c < p.n) finish<T>(p, r, c, acc[i][j]);
+      }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int64_t r = row0 + tr * 4 + i;
+    float top = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int64_t c = col0 + tc * 4 + j;
+      if (c >= p.n || r >= p.m) continue;
+      if (p.targets[r] == p.col0 + c) p.target_logit[r] = acc[i][j];
+      top = acc[i][j] > top || acc[i][j] != acc[i][j] ? acc[i][j] : top;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (col0 + tc * 4 + j < p.n && top != -INFINITY) sum += exp2f((acc[i][j] - top) * cxprod::kLog2e);
+    stat[tr * 4 + i][tc] = make_float2(top, sum);
+  }
+  __syncthreads();
+  if (threadIdx.x < kTile && row0 + threadIdx.x < p.m) {
+    float top = -INFINITY, sum = 0.f;
+    for (int j = 0; j < 16; ++j) {
+      const float t = stat[threadIdx.x][j].x;
+      top = t > top || t != t ? t : top;
+    }
+    for (int j = 0; j < 16; ++j) {
+      const float2 s = stat[threadIdx.x][j];
+      if (s.x != -INFINITY) sum += s.y * exp2f((s.x - top) * cxprod::kLog2e);
+    }
+    p.part[(int64_t)blockIdx.y * p.m + row0 + threadIdx.x] = make_float2(top, sum);
+  }
+}
+
+}  // namespace
+
+int cx_product_stat_columns(const CxProduct&) { return kTile; }
+int64_t cx_product_workspace_bytes(const CxProduct&) { return 0; }
+
+int cx_product(const CxProduct& p, cudaStream_t s) {
+  const dim3 grid((unsigned)((p.m + kTile - 1) / kTile), (unsigned)((p.n + kTile - 1) / kTile));
+  if (p.dtype == CX_F32) product_kernel<float><<<grid, kThreads, 0, s>>>(p);
+  else if (p.dtype == CX_BF16) product_kernel<__nv_bfloat16><<<grid, kThreads, 0, s>>>(p);
+  else product_kernel<__half><<<grid, kThreads, 0, s>>>(p);
+  cx_note_launch();
+  return cx_check_launch("cx_product");
+}

@@ -1,0 +1,200 @@
+// Softmax cross entropy of s = h w^T over a vocabulary, and its gradients, without the logits in memory.
+//
+//   loss_r = log sum_v exp(s_rv) - s_r,t(r)      P_rv = (exp(s_rv - lse_r) - [v = t(r)]) g_r      dh = P w      dw = P^T h
+//
+// Forward: the product's epilogue leaves per row and tile of columns the largest logit and the sum of exponentials under
+// it, and the target's logit; a second kernel joins a row's tiles and a third one sums the losses.  Backward goes over
+// the vocabulary in pieces: the piece's logits are computed once more, P of the piece goes to a workspace in 16 bits,
+// and two products take it from there while it is in L2.  dh grows over the pieces in 32 bits.
+//
+// P in 16 bits: a probability of a large vocabulary times the 1 / rows of a mean is below what fp16 can hold, so P is
+// stored times a power of two that brings the largest |g_r| to [2^13, 2^14), and both products take it out at the end.
+#include "cx_product.cuh"
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int64_t kPieceBytes = 64ll << 20;
+
+struct Join {
+  const float2* part;
+  const float* target_logit;
+  const int64_t* targets;
+  int64_t rows, tiles, vocab, ignore;
+  float* lse;
+  float* row_loss;
+};
+
+__global__ void __launch_bounds__(kThreads) join_kernel(const Join j) {
+  const int64_t r = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+  if (r >= j.rows) return;
+  const int64_t t = j.targets[r];
+  float top = -INFINITY, sum = 0.f;
+  for (int64_t i = 0; i < j.tiles; ++i) {
+    const float2 s = j.part[i * j.rows + r];
+    if (s.x > top || s.x != s.x) {
+      sum = top == -INFINITY ? s.y : sum * exp2f((top - s.x) * cxprod::kLog2e) + s.y;
+      top = s.x;
+    } else if (s.x != -INFINITY) {
+      sum += s.y * exp2f((s.x - top) * cxprod::kLog2e);
+    }
+  }
+  const bool ignored = t == j.ignore, inside = t >= 0 && t < j.vocab;
+  float lse = top + logf(sum);
+  if (!ignored && !inside) lse = NAN;
+  j.lse[r] = lse;
+  j.row_loss[r] = ignored ? 0.f : inside ? lse - j.target_logit[r] : NAN;
+}
+
+// one block: the sum of the rows' losses and the number of rows that count, in a fixed order
+__global__ void __launch_bounds__(1024) total_kernel(const float* row_loss, const int64_t* targets, int64_t rows, int64_t ignore,
+                                                     int reduction, float* loss, float* count) {
+  __shared__ float s_sum[32], s_cnt[32];
+  float sum = 0.f, cnt = 0.f;
+  for (int64_t r = threadIdx.x; r < rows; r += 1024) {
+    sum += row_loss[r];
+    cnt += targets[r] == ignore ? 0.f : 1.f;
+  }
+  for (int d = 16; d; d >>= 1) {
+    sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
+    cnt += __shfl_xor_sync(0xFFFFFFFFu, cnt, d);
+  }
+  if ((threadIdx.x & 31) == 0) {
+    s_sum[threadIdx.x >> 5] = sum;
+    s_cnt[threadIdx.x >> 5] = cnt;
+  }
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    sum = s_sum[threadIdx.x];
+    cnt = s_cnt[threadIdx.x];
+    for (int d = 16; d; d >>= 1) {
+      sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
+      cnt += __shfl_xor_sync(0xFFFFFFFFu, cnt, d);
+    }
+    if (threadIdx.x == 0) {
+      *count = cnt;
+      if (reduction != CX_REDUCE_NONE) *loss = reduction == CX_REDUCE_MEAN ? sum / cnt : sum;
+    }
+  }
+}
+
+struct Factors {
+  const float* grad;
+  const int64_t* targets;
+  const float* lse;
+  const float* count;
+  int64_t rows, grad_stride, ignore;
+  int reduction;
+  float* lse2;          // [rows] lse in units of log 2
+  float* factor;        // [rows] g_r times the power of two
+  float* scale;         // its inverse
+};
+
+__device__ __forceinline__ float row_grad(const Factors& f, int64_t r) {
+  if (f.targets[r] == f.ignore) return 0.f;
+  const float g = f.grad[f.reduction == CX_REDUCE_NONE ? r * f.grad_stride : 0];
+  return f.reduction == CX_REDUCE_MEAN ? g / *f.count : g;
+}
+
+__global__ void __launch_bounds__(1024) factor_kernel(const Factors f) {
+  __shared__ uint32_t s_top;
+  if (threadIdx.x == 0) s_top = 0;
+  __syncthreads();
+  uint32_t top = 0;
+  for (int64_t r = threadIdx.x; r < f.rows; r += 1024) top = max(top, __float_as_uint(row_grad(f, r)) & 0x7FFFFFFFu);
+  top = __reduce_max_sync(0xFFFFFFFFu, top);
+  if ((threadIdx.x & 31) == 0) atomicMax(&s_top, top);
+  __syncthreads();
+  // exponent e of the largest: 2^(13 - e) and back, both normal numbers for every e that is clamped to [-100, 120]
+  const int e = min(max((int)(s_top >> 23) - 127, -100), 120);
+  const float up = __uint_as_float((uint32_t)(13 - e + 127) << 23);
+  if (threadIdx.x == 0) *f.scale = __uint_as_float((uint32_t)(e - 13 + 127) << 23);
+  for (int64_t r = threadIdx.x; r < f.rows; r += 1024) {
+    f.factor[r] = row_grad(f, r) * up;
+    f.lse2[r] = f.lse[r] * cxprod::kLog2e;
+  }
+}
+
+int forward(const CxVocabLoss& l, cxprod::Arena& ws, cudaStream_t s, bool count_only) {
+  CxProduct p = {};
+  p.m = l.rows; p.n = l.vocab; p.k = l.dim;
+  p.a = l.h; p.lda = l.ldh; p.b = l.w; p.ldb = l.ldw;
+  p.layout = kNT; p.mode = kStats; p.dtype = l.dtype; p.targets = l.targets;
+  const int64_t bn = cx_product_stat_columns(p), tiles = (l.vocab + bn - 1) / bn;
+  p.part = reinterpret_cast<float2*>(ws.take(tiles * l.rows * 8));
+  p.target_logit = reinterpret_cast<float*>(ws.take(l.rows * 4));
+  float* row_loss = l.reduction == CX_REDUCE_NONE ? l.loss : reinterpret_cast<float*>(ws.take(l.rows * 4));
+  if (count_only) return 0;
+  if (!ws.ok()) return cx_set_error("cx_vocab_loss_forward: workspace too small", 0);
+  int rc = cx_product(p, s);
+  if (rc) return rc;
+  const Join j = {p.part, p.target_logit, l.targets, l.rows, tiles, l.vocab, l.ignore_index, l.lse, row_loss};
+  join_kernel<<<(unsigned)((l.rows + kThreads - 1) / kThreads), kThreads, 0, s>>>(j);
+  cx_note_launch();
+  total_kernel<<<1, 1024, 0, s>>>(row_loss, l.targets, l.rows, l.ignore_index, l.reduction, l.loss, l.count);
+  cx_note_launch();
+  return cx_check_launch("cx_vocab_loss_forward");
+}
+
+int backward(const CxVocabLoss& l, cxprod::Arena& ws, cudaStream_t s, bool count_only) {
+  const int64_t size = l.dtype == CX_F32 ? 4 : 2;
+  int64_t piece = kPieceBytes / (l.rows * size) / 256 * 256;
+  if (piece < 256) piece = 256;
+  if (piece > (l.vocab + 7) / 8 * 8) piece = (l.vocab + 7) / 8 * 8;
+  void* prob = ws.take(l.rows * piece * size);
+  float* sums = l.dh && piece < l.vocab ? reinterpret_cast<float*>(ws.take(l.rows * l.dim * 4)) : nullptr;
+  Factors f = {l.grad, l.targets, l.lse, l.count, l.rows, l.grad_stride, l.ignore_index, l.reduction, nullptr, nullptr, nullptr};
+  f.lse2 = reinterpret_cast<float*>(ws.take(l.rows * 4));
+  f.factor = reinterpret_cast<float*>(ws.take(l.rows * 4));
+  f.scale = reinterpret_cast<float*>(ws.take(4));
+  if (count_only) return 0;
+  if (!ws.ok()) return cx_set_error("cx_vocab_loss_backward: workspace too small", 0);
+  factor_kernel<<<1, 1024, 0, s>>>(f);
+  cx_note_launch();
+  int rc = cx_check_launch("cx_vocab_loss_backward");
+  for (int64_t v0 = 0; v0 < l.vocab && !rc; v0 += piece) {
+    const int64_t n = piece < l.vocab - v0 ? piece : l.vocab - v0;
+    const char* w = reinterpret_cast<const char*>(l.w) + v0 * l.ldw * size;
+    CxProduct p = {};
+    p.m = l.rows; p.n = n; p.k = l.dim;
+    p.a = l.h; p.lda = l.ldh; p.b = w; p.ldb = l.ldw;
+    p.layout = kNT; p.mode = kProb; p.dtype = l.dtype;
+    p.out = prob; p.ldo = piece; p.targets = l.targets; p.col0 = v0; p.lse = f.lse2; p.row_factor = f.factor;
+    if ((rc = cx_product(p, s))) break;
+    if (l.dh) {
+      CxProduct q = {};
+      q.m = l.rows; q.n = l.dim; q.k = n;
+      q.a = prob; q.lda = piece; q.b = w; q.ldb = l.ldw;
+      q.layout = kNN; q.dtype = l.dtype; q.addend = sums; q.has_addend = v0 > 0; q.scale = f.scale;
+      q.mode = v0 + n < l.vocab ? kSums : kOut;
+      q.out = l.dh; q.ldo = l.dim;
+      if ((rc = cx_product(q, s))) break;
+    }
+    if (l.dw) {
+      CxProduct q = {};
+      q.m = n; q.n = l.dim; q.k = l.rows;
+      q.a = prob; q.lda = piece; q.b = l.h; q.ldb = l.ldh;
+      q.layout = kTN; q.dtype = l.dtype; q.scale = f.scale;
+      q.out = reinterpret_cast<char*>(l.dw) + v0 * l.dim * size; q.ldo = l.dim;
+      rc = cx_product(q, s);
+    }
+  }
+  return rc;
+}
+
+}  // namespace
+
+int64_t cx_vocab_loss_workspace_bytes_cuda(const CxVocabLoss* l, int back) {
+  cxprod::Arena ws = {nullptr, 0, 0};
+  if (back) backward(*l, ws, nullptr, true);
+  else forward(*l, ws, nullptr, true);
+  return ws.used;
+}
+int cx_vocab_loss_forward_cuda(const CxVocabLoss* l, void* stream) {
+  cxprod::Arena ws = {reinterpret_cast<char*>(l->workspace), 0, l->ws_bytes};
+  return forward(*l, ws, static_cast<cudaStream_t>(stream), false);
+}
+int cx_vocab_loss_backward_cuda(const CxVocabLoss* l, void* stream) {
+  cxprod::Arena ws = {reinterpret_cast<char*>(l->workspace), 0, l->ws_bytes};
+  return backward(*l, ws, static_cast<cudaStream_t>(stream), false);
+}

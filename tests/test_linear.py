@@ -1,0 +1,181 @@
+"""The product with bias, activation and residual (csrc/linear.cu) and its gradients, against 64 bits."""
+import pytest
+import torch
+
+import comprex_b200 as cx
+from comprex_b200 import ComprexError
+
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+UNIT = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}     # unit roundoff: 24, 8 and 11 bits
+SMALL = {torch.float32: 0.0, torch.bfloat16: 0.0, torch.float16: 2.0 ** -25}                 # half a subnormal step
+ACTS = [None, "relu", "gelu", "gelu_tanh", "silu"]
+# rows, inner, outer: one token, one of everything, tile borders, odd sizes, a long sum
+SIZES = [(1, 64, 128), (1, 1, 1), (2, 1024, 40), (5, 7, 3), (16, 256, 512), (17, 96, 264), (128, 64, 128), (129, 72, 136), (257, 520, 255), (100, 1001, 33), (700, 8, 16)]
+
+
+def _act(u, act):
+    f = torch.nn.functional
+    return {None: lambda v: v * 1.0, "relu": torch.relu, "gelu": f.gelu, "gelu_tanh": lambda v: f.gelu(v, approximate="tanh"), "silu": f.silu}[act](u)
+
+
+def _inputs(rows, inner, outer, dtype, device, bias=True, residual=True, seed=0):
+    gen = torch.Generator().manual_seed(seed)
+    make = lambda *s: torch.randn(*s, generator=gen).to(dtype).to(device)  # noqa: E731
+    w = (torch.randn(outer, inner, generator=gen) / inner ** 0.5).to(dtype).to(device)
+    return make(rows, inner), w, make(outer) if bias else None, make(rows, outer) if residual else None, make(rows, outer)
+
+
+def _check(x, w, b, r, g, act, got, grads):
+    """Elementwise bounds: sums of n products in 32 bits are off by at most n 2^-23 times the sum of magnitudes (the
+    order is free), every rounding to the type by UNIT, exponentials by 2^-20; the slopes change by at most 1.2 per unit."""
+    dtype = x.dtype
+    unit, small = UNIT[dtype], SMALL[dtype]
+    X, W, G = x.double().cpu(), w.double().cpu(), g.double().cpu()
+    B = torch.zeros(w.size(0), dtype=torch.float64) if b is None else b.double().cpu()
+    R = 0.0 if r is None else r.double().cpu()
+    n, k, m = w.size(0), w.size(1), x.size(0)
+    u = (X @ W.T + B).requires_grad_()
+    a = _act(u, act)
+    du, = torch.autograd.grad(a, u, G)
+    u, a = u.detach(), a.detach()
+    e_u = (k + 4) * 2.0 ** -23 * (X.abs() @ W.abs().T + B.abs())
+    y = a + R
+    bound = unit * y.abs() + small + 1.2 * e_u + 2.0 ** -20 * (u.abs() + a.abs()) + 2.0 ** -23 * y.abs()
+    assert ((got.detach().double().cpu() - y).abs() <= bound).all()
+    if grads is None:
+        return
+    dx, dw, db = (None if t is None else t.double().cpu() for t in grads)
+    # du before its rounding: from u in the operands' type
+    e_du = G.abs() * (1.2 * (unit * u.abs() + small + e_u) + 2.0 ** -20 * (1 + u.abs())) * (act is not None)
+    if act == "relu":                   # a jump where u is within its own error of zero
+        e_du = torch.where(u.abs() <= e_u, G.abs(), e_du)
+    e_all = e_du + (unit * (du.abs() + e_du) + small) * (act is not None)
+    if dx is not None:
+        bound = e_all @ W.abs() + (n + 4) * 2.0 ** -23 * (du.abs() @ W.abs()) + unit * (du @ W).abs() + small
+        assert ((dx - du @ W).abs() <= 1.01 * bound).all()
+    if dw is not None:
+        bound = e_all.T @ X.abs() + (m + 4) * 2.0 ** -23 * (du.abs().T @ X.abs()) + unit * (du.T @ X).abs() + small
+        assert ((dw - du.T @ X).abs() <= 1.01 * bound).all()
+    if db is not None:
+        bound = e_du.sum(0) + (m + 4) * 2.0 ** -23 * du.abs().sum(0) + unit * du.sum(0).abs() + small
+        assert ((db - du.sum(0)).abs() <= 1.01 * bound).all()
+
+
+@pytest.mark.parametrize("size", SIZES)
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("dtype", TYPES)
+def test_against_64_bits(device, dtype, act, size):
+    x, w, b, r, g = _inputs(*size, dtype, device)
+    leaves = [t.requires_grad_() for t in (x, w, b, r)]
+    y = cx.linear(x, w, b, activation=act, residual=r)
+    dx, dw, db, dr = torch.autograd.grad(y, leaves, g)
+    assert torch.equal(dr, g)
+    _check(*(t.detach() for t in leaves), g, act, y, (dx, dw, db))
+    with torch.no_grad():
+        assert torch.equal(cx.linear(x, w, b, activation=act, residual=r), y)
+
+
+@pytest.mark.parametrize("bias,residual", [(False, False), (True, False), (False, True)])
+def test_without_bias_or_residual(device, bias, residual):
+    for act in (None, "gelu_tanh"):
+        x, w, b, r, g = _inputs(33, 48, 56, torch.bfloat16, device, bias, residual)
+        leaves = [t.requires_grad_() for t in (x, w, b) if t is not None]
+        y = cx.linear(x, w, b, activation=act, residual=r)
+        got = iter(torch.autograd.grad(y, leaves, g))
+        grads = [next(got) if t is not None else None for t in (x, w, b)]
+        _check(x.detach(), w.detach(), None if b is None else b.detach(), r, g, act, y, grads)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size", [(8192, 64, 64), (64, 4096, 64), (40, 64, 5000), (2049, 1024, 1032), (1, 4096, 1024), (8, 1000, 4096), (3, 4096, 4096),
+                                  (513, 4095, 130), (256, 256, 512), (300, 2048, 256)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_larger_sizes(size, dtype):
+    for act in (None, "silu"):
+        x, w, b, r, g = _inputs(*size, dtype, "cuda")
+        leaves = [t.requires_grad_() for t in (x, w, b)]
+        y = cx.linear(x, w, b, activation=act, residual=r)
+        grads = torch.autograd.grad(y, leaves, g)
+        _check(*(t.detach() for t in leaves), r, g, act, y, grads)
+        again = cx.linear(x, w, b, activation=act, residual=r)
+        assert torch.equal(again, y) and all(torch.equal(a, c) for a, c in zip(torch.autograd.grad(again, leaves, g), grads))
+
+
+def test_memory_orders(device):
+    """Rows that lie apart, transposed and expanded operands, a gradient of zero stride, more dimensions."""
+    gen = torch.Generator().manual_seed(1)
+    make = lambda *s: torch.randn(*s, generator=gen).to(torch.bfloat16).to(device)  # noqa: E731
+    wide_x, wide_w, wide_r = make(20, 3, 100), make(50, 90), make(60, 77)
+    x, w, r, b = wide_x[:, :, 8:72], wide_w[::2, 16:80], wide_r[:, 3:28], make(50)[::2]
+    y = cx.linear(x, w, b, residual=r.view(20, 3, 25))
+    assert y.shape == (20, 3, 25)
+    assert torch.equal(y.view(60, 25), cx.linear(x.reshape(60, 64).contiguous(), w.contiguous(), b.contiguous(), residual=r.contiguous()))
+    assert torch.equal(cx.linear(x.reshape(60, 64), w.T.contiguous().T, b), cx.linear(x.reshape(60, 64), w, b))
+    one = make(1, 64).expand(60, 64)
+    assert torch.equal(cx.linear(one, w), cx.linear(one.contiguous(), w))
+    # off a 16-byte boundary
+    odd = make(60 * 64 + 1)[1:].view(60, 64)
+    assert torch.equal(cx.linear(odd, w), cx.linear(odd.clone(), w))
+    xr, wr = x.detach().requires_grad_(), w.detach().requires_grad_()
+    ones = torch.autograd.grad(cx.linear(xr, wr, activation="silu").sum(), (xr, wr))
+    full = torch.autograd.grad(cx.linear(xr, wr, activation="silu"), (xr, wr), torch.ones(20, 3, 25, dtype=x.dtype, device=device))
+    assert all(torch.equal(a, c) for a, c in zip(ones, full))
+
+
+def test_gradient_against_differences(device):
+    """Central differences in 32 bits; the step's error is h^2 times a third derivative below 3, the sums' 2^-20 / h."""
+    x, w, b, r, g = _inputs(6, 10, 8, torch.float32, device)
+    for act in ("gelu", "gelu_tanh", "silu"):
+        leaves = [t.clone().requires_grad_() for t in (x, w, b)]
+        grads = torch.autograd.grad(cx.linear(*leaves, activation=act, residual=r), leaves, g)
+        for leaf, grad in zip(leaves, grads):
+            way = torch.randn_like(leaf)
+            h = 1e-2
+            with torch.no_grad():
+                high, low = ((cx.linear(*(t + s * h * way if t is leaf else t for t in leaves), activation=act, residual=r).double() * g.double()).sum() for s in (1, -1))
+            want = ((high - low) / (2 * h)).item()
+            size = g.abs().sum().item()
+            assert abs((grad.double() * way.double()).sum().item() - want) <= size * (3 * h * h * way.abs().max().item() ** 3 * 10 + 2.0 ** -20 / h * 4)
+
+
+def test_empty_and_special_values(device):
+    x, w, b, _, _ = _inputs(4, 16, 24, torch.float16, device)
+    assert cx.linear(x[:0], w, b).shape == (0, 24)
+    leaves = [t.requires_grad_() for t in (x[:0].clone(), w, b)]
+    dx, dw, db = torch.autograd.grad(cx.linear(*leaves, activation="relu").sum(), leaves)
+    assert dx.shape == (0, 16) and not dw.any() and not db.any()
+    bad = x.detach().clone()
+    bad[2, 5] = float("nan")
+    for act in ACTS:
+        y = cx.linear(bad, w.detach(), activation=act)
+        assert torch.isnan(y[2]).all() and torch.isfinite(y[[0, 1, 3]]).all()
+
+
+@pytest.mark.gpu
+def test_on_another_stream_and_without_a_gradient_for_all():
+    x, w, b, r, g = _inputs(300, 256, 128, torch.bfloat16, "cuda")
+    want = cx.linear(x, w, b, activation="gelu_tanh", residual=r)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = cx.linear(x, w, b, activation="gelu_tanh", residual=r)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(got, want)
+    for only in range(3):
+        leaves = [t.clone().requires_grad_(i == only) for i, t in enumerate((x, w, b))]
+        part, = torch.autograd.grad(cx.linear(*leaves, activation="silu"), [leaves[only]], g)
+        every = [t.clone().requires_grad_() for t in (x, w, b)]
+        assert torch.equal(part, torch.autograd.grad(cx.linear(*every, activation="silu"), every, g)[only])
+
+
+def test_refusals(device):
+    x, w, b, r, _ = _inputs(4, 16, 24, torch.bfloat16, device)
+    with pytest.raises(ValueError):
+        cx.linear(x, w, activation="tanh")
+    for bad in (dict(x=x.float()), dict(x=x[:, :8]), dict(weight=w[0]), dict(bias=b[:3]), dict(residual=r[:2]), dict(bias=b.float()), dict(residual=r.half())):
+        with pytest.raises(ComprexError):
+            cx.linear(**(dict(x=x, weight=w, bias=b, residual=r) | bad))
+    with pytest.raises(ComprexError):
+        cx.linear(x.double(), w.double())
+    with pytest.raises(ComprexError):
+        cx.linear(x, w[:, :0].expand(24, 0))
