@@ -41,11 +41,6 @@ struct CxProduct {
   int64_t ws_bytes;
 };
 
-// columns of a kStats tile
-int cx_product_stat_columns(const CxProduct& p);
-int64_t cx_product_workspace_bytes(const CxProduct& p);
-int cx_product(const CxProduct& p, cudaStream_t s);
-
 namespace cxprod {
 
 struct Arena {                 // workspace handed out front to back; without a base it only counts
@@ -58,6 +53,23 @@ struct Arena {                 // workspace handed out front to back; without a 
   }
   bool ok() const { return used <= size; }
 };
+
+}  // namespace cxprod
+
+// Takes the product's own workspace from `ws`; without a base nothing is launched and the arena counts.
+int cx_product(CxProduct& p, cxprod::Arena& ws, cudaStream_t s);
+// An operand as the tensor cores can read it: itself, or a copy in `ws` whose rows are 16-byte aligned (16-bit types).
+int cx_product_operand(const void** base, int64_t* ld, int dtype, int64_t rows, int64_t cols, cxprod::Arena& ws, cudaStream_t s);
+// columns of a kStats tile
+int cx_product_stat_columns(const CxProduct& p);
+
+// tensor_product.cu: 16-bit types, operands that a tile copy can read (16-byte aligned rows)
+bool cx_tensor_product_takes(const CxProduct& p);
+int cx_tensor_product_stat_columns(const CxProduct& p);
+int64_t cx_tensor_product_workspace_bytes(const CxProduct& p);
+int cx_tensor_product(const CxProduct& p, cudaStream_t s);
+
+namespace cxprod {
 
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -86,6 +98,51 @@ __device__ __forceinline__ float slope(float u, int act) {
       return q * (1.f + u * (1.f - q));
     }
     default: return 1.f;
+  }
+}
+
+// 8 neighbouring elements of a row, as 16 bytes where `wide`, else the first `left` one by one
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, bool wide, int left, float (&v)[8]) {
+  if (wide) {
+    float lo[4], hi[4];
+    if (sizeof(T) == 2) {
+      const uint4 t = *reinterpret_cast<const uint4*>(p);
+      cx::Raw4<T>::to_f(reinterpret_cast<const typename cx::Raw4<T>::type*>(&t)[0], lo);
+      cx::Raw4<T>::to_f(reinterpret_cast<const typename cx::Raw4<T>::type*>(&t)[1], hi);
+    } else {
+      cx::load4(p, lo);
+      cx::load4(p + 4, hi);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[i] = lo[i];
+      v[4 + i] = hi[i];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i < left ? cx::Elem<T>::to_f(p[i]) : 0.f;
+  }
+}
+__device__ __forceinline__ void pack4(const float* v, uint2* out, __nv_bfloat16) {
+  const float t[4] = {v[0], v[1], v[2], v[3]};
+  cx::store4(reinterpret_cast<__nv_bfloat16*>(out), t);
+}
+__device__ __forceinline__ void pack4(const float* v, uint2* out, __half) {
+  const float t[4] = {v[0], v[1], v[2], v[3]};
+  cx::store4(reinterpret_cast<__half*>(out), t);
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, bool wide, int left, const float (&v)[8]) {
+  if (wide) {
+    uint2 t[2];
+    pack4(v, t, T());
+    pack4(v + 4, t + 1, T());
+    *reinterpret_cast<uint4*>(p) = make_uint4(t[0].x, t[0].y, t[1].x, t[1].y);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < left) p[i] = cx::Elem<T>::from_f(v[i]);
   }
 }
 

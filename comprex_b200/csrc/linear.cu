@@ -58,66 +58,67 @@ int du_pass(const Du& d, void* dbias, cudaStream_t s) {
   return cx_check_launch("cx_linear_backward");
 }
 
-int backward(const CxLinear& l, cxprod::Arena& ws, cudaStream_t s, bool count_only) {
+// Both calls also run without a workspace: they launch nothing then and count the bytes that they need.
+int forward(const CxLinear& l, cxprod::Arena& ws, cudaStream_t s) {
+  CxProduct p = {};
+  p.m = l.rows; p.n = l.outer; p.k = l.inner;
+  p.a = l.x; p.lda = l.ldx; p.b = l.w; p.ldb = l.ldw;
+  p.layout = kNT; p.dtype = l.dtype; p.act = l.act;
+  p.out = l.y; p.ldo = l.outer; p.bias = l.bias; p.residual = l.residual; p.ldr = l.ldr; p.pre = l.pre;
+  int rc = cx_product_operand(&p.a, &p.lda, l.dtype, l.rows, l.inner, ws, s);
+  if (!rc) rc = cx_product_operand(&p.b, &p.ldb, l.dtype, l.outer, l.inner, ws, s);
+  return rc ? rc : cx_product(p, ws, s);
+}
+
+int backward(const CxLinear& l, cxprod::Arena& ws, cudaStream_t s) {
   const int64_t size = l.dtype == CX_F32 ? 4 : 2;
-  const bool act = l.act != CX_ACT_NONE;
   Du d = {};
-  d.grad = l.grad;
-  d.pre = l.pre;
-  d.rows = l.rows;
-  d.outer = l.outer;
-  d.ldg = l.ldg;
-  d.act = l.act;
+  d.grad = l.grad; d.pre = l.pre;
+  d.rows = l.rows; d.outer = l.outer; d.ldg = l.ldg; d.act = l.act;
   const void* du = l.grad;
   int64_t ldd = l.ldg;
-  if (act && (l.dx || l.dw)) {
-    d.ldd = ldd = l.outer;
-    du = d.du = ws.take(l.rows * d.ldd * size);
+  if (l.act != CX_ACT_NONE && (l.dx || l.dw)) {
+    d.ldd = ldd = (l.outer + 7) / 8 * 8;
+    du = d.du = ws.take(l.rows * ldd * size);
   }
   if (l.dbias) d.part = reinterpret_cast<float*>(ws.take((l.rows + kRowsPer - 1) / kRowsPer * l.outer * 4));
-  if (count_only) return 0;
   int rc = 0;
-  if (!ws.ok()) return cx_set_error("cx_linear_backward: workspace too small", 0);
-  if (d.du || d.part) {
+  if (ws.base && !ws.ok()) return cx_set_error("cx_linear_backward: workspace too small", 0);
+  if (ws.base && (d.du || d.part))
     rc = l.dtype == CX_F32 ? du_pass<float>(d, l.dbias, s)
          : l.dtype == CX_BF16 ? du_pass<__nv_bfloat16>(d, l.dbias, s) : du_pass<__half>(d, l.dbias, s);
-    if (rc) return rc;
-  }
-  if (l.dx) {
+  if (!rc && (l.dx || l.dw)) rc = cx_product_operand(&du, &ldd, l.dtype, l.rows, l.outer, ws, s);
+  if (l.dx && !rc) {
     CxProduct p = {};
     p.m = l.rows; p.n = l.inner; p.k = l.outer;
     p.a = du; p.lda = ldd; p.b = l.w; p.ldb = l.ldw;
     p.layout = kNN; p.dtype = l.dtype; p.out = l.dx; p.ldo = l.inner;
-    if ((rc = cx_product(p, s))) return rc;
+    rc = cx_product_operand(&p.b, &p.ldb, l.dtype, l.outer, l.inner, ws, s);
+    if (!rc) rc = cx_product(p, ws, s);
   }
-  if (l.dw) {
+  if (l.dw && !rc) {
     CxProduct p = {};
     p.m = l.outer; p.n = l.inner; p.k = l.rows;
     p.a = du; p.lda = ldd; p.b = l.x; p.ldb = l.ldx;
     p.layout = kTN; p.dtype = l.dtype; p.out = l.dw; p.ldo = l.inner;
-    if ((rc = cx_product(p, s))) return rc;
+    rc = cx_product_operand(&p.b, &p.ldb, l.dtype, l.rows, l.inner, ws, s);
+    if (!rc) rc = cx_product(p, ws, s);
   }
-  return 0;
+  return rc;
 }
 
 }  // namespace
 
 int64_t cx_linear_workspace_bytes_cuda(const CxLinear* l, int back) {
   cxprod::Arena ws = {nullptr, 0, 0};
-  if (back) backward(*l, ws, nullptr, true);
-  return ws.used;
+  (back ? backward : forward)(*l, ws, nullptr);
+  return ws.used + 256;          // never none: without a base nothing runs
 }
-
 int cx_linear_forward_cuda(const CxLinear* l, void* stream) {
-  CxProduct p = {};
-  p.m = l->rows; p.n = l->outer; p.k = l->inner;
-  p.a = l->x; p.lda = l->ldx; p.b = l->w; p.ldb = l->ldw;
-  p.layout = kNT; p.dtype = l->dtype; p.act = l->act;
-  p.out = l->y; p.ldo = l->outer; p.bias = l->bias; p.residual = l->residual; p.ldr = l->ldr; p.pre = l->pre;
-  return cx_product(p, static_cast<cudaStream_t>(stream));
+  cxprod::Arena ws = {reinterpret_cast<char*>(l->workspace), 0, l->ws_bytes};
+  return ws.base ? forward(*l, ws, static_cast<cudaStream_t>(stream)) : cx_set_error("cx_linear_forward: no workspace", 0);
 }
-
 int cx_linear_backward_cuda(const CxLinear* l, void* stream) {
   cxprod::Arena ws = {reinterpret_cast<char*>(l->workspace), 0, l->ws_bytes};
-  return backward(*l, ws, static_cast<cudaStream_t>(stream), false);
+  return ws.base ? backward(*l, ws, static_cast<cudaStream_t>(stream)) : cx_set_error("cx_linear_backward: no workspace", 0);
 }

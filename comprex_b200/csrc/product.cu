@@ -106,12 +106,48 @@ __global__ void __launch_bounds__(kThreads) product_kernel(const __grid_constant
   }
 }
 
+// rows of `cols` elements, `ld` apart, to rows of `to_ld` (a multiple of 8); what is beyond a row's end is zero
+__global__ void __launch_bounds__(kThreads) align_kernel(const uint16_t* from, int64_t ld, int64_t rows, int64_t cols, uint16_t* to, int64_t to_ld) {
+  const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x, per = to_ld / 8;
+  if (i >= rows * per) return;
+  const int64_t row = i / per, col = i % per * 8;
+  uint16_t v[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) v[k] = col + k < cols ? from[row * ld + col + k] : 0;
+  uint4 t;
+  memcpy(&t, v, 16);
+  *reinterpret_cast<uint4*>(to + row * to_ld + col) = t;
+}
+
 }  // namespace
 
-int cx_product_stat_columns(const CxProduct&) { return kTile; }
-int64_t cx_product_workspace_bytes(const CxProduct&) { return 0; }
+int cx_product_operand(const void** base, int64_t* ld, int dtype, int64_t rows, int64_t cols, cxprod::Arena& ws, cudaStream_t s) {
+  if (dtype == CX_F32 || ((reinterpret_cast<uintptr_t>(*base) & 15) == 0 && *ld % 8 == 0)) return 0;
+  const int64_t to_ld = (cols + 7) / 8 * 8;
+  void* to = ws.take(rows * to_ld * 2);
+  const void* from = *base;
+  const int64_t from_ld = *ld;
+  *base = to;
+  *ld = to_ld;
+  if (!ws.base) return 0;
+  if (!ws.ok()) return cx_set_error("cx_product: workspace too small", 0);
+  align_kernel<<<(unsigned)((rows * (to_ld / 8) + kThreads - 1) / kThreads), kThreads, 0, s>>>(
+      reinterpret_cast<const uint16_t*>(from), from_ld, rows, cols, reinterpret_cast<uint16_t*>(to), to_ld);
+  cx_note_launch();
+  return cx_check_launch("cx_product");
+}
 
-int cx_product(const CxProduct& p, cudaStream_t s) {
+int cx_product_stat_columns(const CxProduct& p) { return cx_tensor_product_takes(p) ? cx_tensor_product_stat_columns(p) : kTile; }
+
+int cx_product(CxProduct& p, cxprod::Arena& ws, cudaStream_t s) {
+  const bool tensor = cx_tensor_product_takes(p);
+  if (tensor) {
+    p.ws_bytes = cx_tensor_product_workspace_bytes(p);
+    if (p.ws_bytes) p.workspace = ws.take(p.ws_bytes);
+  }
+  if (!ws.base) return 0;
+  if (!ws.ok()) return cx_set_error("cx_product: workspace too small", 0);
+  if (tensor) return cx_tensor_product(p, s);
   const dim3 grid((unsigned)((p.m + kTile - 1) / kTile), (unsigned)((p.n + kTile - 1) / kTile));
   if (p.dtype == CX_F32) product_kernel<float><<<grid, kThreads, 0, s>>>(p);
   else if (p.dtype == CX_BF16) product_kernel<__nv_bfloat16><<<grid, kThreads, 0, s>>>(p);

@@ -31,13 +31,11 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const Join j) {
   const int64_t t = j.targets[r];
   float top = -INFINITY, sum = 0.f;
   for (int64_t i = 0; i < j.tiles; ++i) {
+    // a tile without a finite logit has top -inf, and its sum is 0, or NaN where a logit was no number
     const float2 s = j.part[i * j.rows + r];
-    if (s.x > top || s.x != s.x) {
-      sum = top == -INFINITY ? s.y : sum * exp2f((top - s.x) * cxprod::kLog2e) + s.y;
-      top = s.x;
-    } else if (s.x != -INFINITY) {
-      sum += s.y * exp2f((s.x - top) * cxprod::kLog2e);
-    }
+    const float m = fmaxf(top, s.x), base = m == -INFINITY ? 0.f : m;
+    sum = sum * exp2f((top - base) * cxprod::kLog2e) + s.y * exp2f((s.x - base) * cxprod::kLog2e);
+    top = m;
   }
   const bool ignored = t == j.ignore, inside = t >= 0 && t < j.vocab;
   float lse = top + logf(sum);
@@ -115,19 +113,21 @@ __global__ void __launch_bounds__(1024) factor_kernel(const Factors f) {
   }
 }
 
-int forward(const CxVocabLoss& l, cxprod::Arena& ws, cudaStream_t s, bool count_only) {
+// Both calls also run without a workspace: they launch nothing then and count the bytes that they need.
+int forward(const CxVocabLoss& l, cxprod::Arena& ws, cudaStream_t s) {
   CxProduct p = {};
   p.m = l.rows; p.n = l.vocab; p.k = l.dim;
   p.a = l.h; p.lda = l.ldh; p.b = l.w; p.ldb = l.ldw;
   p.layout = kNT; p.mode = kStats; p.dtype = l.dtype; p.targets = l.targets;
+  int rc = cx_product_operand(&p.a, &p.lda, l.dtype, l.rows, l.dim, ws, s);
+  if (!rc) rc = cx_product_operand(&p.b, &p.ldb, l.dtype, l.vocab, l.dim, ws, s);
+  if (rc) return rc;
   const int64_t bn = cx_product_stat_columns(p), tiles = (l.vocab + bn - 1) / bn;
   p.part = reinterpret_cast<float2*>(ws.take(tiles * l.rows * 8));
   p.target_logit = reinterpret_cast<float*>(ws.take(l.rows * 4));
   float* row_loss = l.reduction == CX_REDUCE_NONE ? l.loss : reinterpret_cast<float*>(ws.take(l.rows * 4));
-  if (count_only) return 0;
-  if (!ws.ok()) return cx_set_error("cx_vocab_loss_forward: workspace too small", 0);
-  int rc = cx_product(p, s);
-  if (rc) return rc;
+  rc = cx_product(p, ws, s);
+  if (rc || !ws.base) return rc;
   const Join j = {p.part, p.target_logit, l.targets, l.rows, tiles, l.vocab, l.ignore_index, l.lse, row_loss};
   join_kernel<<<(unsigned)((l.rows + kThreads - 1) / kThreads), kThreads, 0, s>>>(j);
   cx_note_launch();
@@ -136,8 +136,13 @@ int forward(const CxVocabLoss& l, cxprod::Arena& ws, cudaStream_t s, bool count_
   return cx_check_launch("cx_vocab_loss_forward");
 }
 
-int backward(const CxVocabLoss& l, cxprod::Arena& ws, cudaStream_t s, bool count_only) {
+int backward(const CxVocabLoss& l, cxprod::Arena& ws, cudaStream_t s) {
   const int64_t size = l.dtype == CX_F32 ? 4 : 2;
+  const void *h = l.h, *w = l.w;
+  int64_t ldh = l.ldh, ldw = l.ldw;
+  int rc = cx_product_operand(&h, &ldh, l.dtype, l.rows, l.dim, ws, s);
+  if (!rc) rc = cx_product_operand(&w, &ldw, l.dtype, l.vocab, l.dim, ws, s);
+  if (rc) return rc;
   int64_t piece = kPieceBytes / (l.rows * size) / 256 * 256;
   if (piece < 256) piece = 256;
   if (piece > (l.vocab + 7) / 8 * 8) piece = (l.vocab + 7) / 8 * 8;
@@ -147,38 +152,44 @@ int backward(const CxVocabLoss& l, cxprod::Arena& ws, cudaStream_t s, bool count
   f.lse2 = reinterpret_cast<float*>(ws.take(l.rows * 4));
   f.factor = reinterpret_cast<float*>(ws.take(l.rows * 4));
   f.scale = reinterpret_cast<float*>(ws.take(4));
-  if (count_only) return 0;
-  if (!ws.ok()) return cx_set_error("cx_vocab_loss_backward: workspace too small", 0);
-  factor_kernel<<<1, 1024, 0, s>>>(f);
-  cx_note_launch();
-  int rc = cx_check_launch("cx_vocab_loss_backward");
+  if (ws.base) {
+    if (!ws.ok()) return cx_set_error("cx_vocab_loss_backward: workspace too small", 0);
+    factor_kernel<<<1, 1024, 0, s>>>(f);
+    cx_note_launch();
+    rc = cx_check_launch("cx_vocab_loss_backward");
+  }
+  const int64_t begin = ws.used;               // what the products need is used again by the next piece
+  int64_t most = begin;
   for (int64_t v0 = 0; v0 < l.vocab && !rc; v0 += piece) {
     const int64_t n = piece < l.vocab - v0 ? piece : l.vocab - v0;
-    const char* w = reinterpret_cast<const char*>(l.w) + v0 * l.ldw * size;
+    const char* at = reinterpret_cast<const char*>(w) + v0 * ldw * size;
+    ws.used = begin;
     CxProduct p = {};
     p.m = l.rows; p.n = n; p.k = l.dim;
-    p.a = l.h; p.lda = l.ldh; p.b = w; p.ldb = l.ldw;
+    p.a = h; p.lda = ldh; p.b = at; p.ldb = ldw;
     p.layout = kNT; p.mode = kProb; p.dtype = l.dtype;
     p.out = prob; p.ldo = piece; p.targets = l.targets; p.col0 = v0; p.lse = f.lse2; p.row_factor = f.factor;
-    if ((rc = cx_product(p, s))) break;
-    if (l.dh) {
+    rc = cx_product(p, ws, s);
+    if (l.dh && !rc) {
       CxProduct q = {};
       q.m = l.rows; q.n = l.dim; q.k = n;
-      q.a = prob; q.lda = piece; q.b = w; q.ldb = l.ldw;
+      q.a = prob; q.lda = piece; q.b = at; q.ldb = ldw;
       q.layout = kNN; q.dtype = l.dtype; q.addend = sums; q.has_addend = v0 > 0; q.scale = f.scale;
       q.mode = v0 + n < l.vocab ? kSums : kOut;
       q.out = l.dh; q.ldo = l.dim;
-      if ((rc = cx_product(q, s))) break;
+      rc = cx_product(q, ws, s);
     }
-    if (l.dw) {
+    if (l.dw && !rc) {
       CxProduct q = {};
       q.m = n; q.n = l.dim; q.k = l.rows;
-      q.a = prob; q.lda = piece; q.b = l.h; q.ldb = l.ldh;
+      q.a = prob; q.lda = piece; q.b = h; q.ldb = ldh;
       q.layout = kTN; q.dtype = l.dtype; q.scale = f.scale;
       q.out = reinterpret_cast<char*>(l.dw) + v0 * l.dim * size; q.ldo = l.dim;
-      rc = cx_product(q, s);
+      rc = cx_product(q, ws, s);
     }
+    if (ws.used > most) most = ws.used;
   }
+  ws.used = most;
   return rc;
 }
 
@@ -186,15 +197,14 @@ int backward(const CxVocabLoss& l, cxprod::Arena& ws, cudaStream_t s, bool count
 
 int64_t cx_vocab_loss_workspace_bytes_cuda(const CxVocabLoss* l, int back) {
   cxprod::Arena ws = {nullptr, 0, 0};
-  if (back) backward(*l, ws, nullptr, true);
-  else forward(*l, ws, nullptr, true);
-  return ws.used;
+  (back ? backward : forward)(*l, ws, nullptr);
+  return ws.used + 256;          // never none: without a base nothing runs
 }
 int cx_vocab_loss_forward_cuda(const CxVocabLoss* l, void* stream) {
   cxprod::Arena ws = {reinterpret_cast<char*>(l->workspace), 0, l->ws_bytes};
-  return forward(*l, ws, static_cast<cudaStream_t>(stream), false);
+  return ws.base ? forward(*l, ws, static_cast<cudaStream_t>(stream)) : cx_set_error("cx_vocab_loss_forward: no workspace", 0);
 }
 int cx_vocab_loss_backward_cuda(const CxVocabLoss* l, void* stream) {
   cxprod::Arena ws = {reinterpret_cast<char*>(l->workspace), 0, l->ws_bytes};
-  return backward(*l, ws, static_cast<cudaStream_t>(stream), false);
+  return ws.base ? backward(*l, ws, static_cast<cudaStream_t>(stream)) : cx_set_error("cx_vocab_loss_backward: no workspace", 0);
 }
