@@ -90,7 +90,7 @@ typedef struct CxVocabLoss {
   int64_t ignore_index;
   float* loss;             /* [rows] for CX_REDUCE_NONE, else [1] */
   float* lse;              /* [rows] log sum exp of the logits: written by the forward call, read by the backward call */
-  float* count;            /* [1] rows that are not ignored: likewise */
+  float* count;            /* [1] rows that are not ignored: likewise (CX_REDUCE_MEAN) */
   const float* grad;       /* backward: of the loss */
   int64_t grad_stride;     /* CX_REDUCE_NONE: from row to row (0 for a broadcast one) */
   void* dh;                /* [rows][dim], may be NULL */

@@ -69,33 +69,70 @@ int cx_tensor_product_stat_columns(const CxProduct& p);
 int64_t cx_tensor_product_workspace_bytes(const CxProduct& p);
 int cx_tensor_product(const CxProduct& p, cudaStream_t s);
 
+// A launch that may become resident while the kernel in front is ending; every kernel launched so calls cx::pdl_wait
+// before it touches memory.
+template <typename K, typename P>
+void cx_launch_pdl2(K kernel, dim3 grid, int threads, cudaStream_t s, const P& params) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cx_pdl_enabled() ? 1 : 0;
+  cudaLaunchKernelEx(&cfg, kernel, params);           // (an error is the next cx_check_launch's)
+}
+
 namespace cxprod {
 
 constexpr float kLog2e = 1.4426950408889634f;
 
+__device__ __forceinline__ float pow2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float inverse(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 // Activations in terms of u = x w^T + b.  gelu_tanh(u) = u / (1 + exp(-2 z)), z = sqrt(2 / pi) (u + 0.044715 u^3): the
-// same function as u / 2 (1 + tanh z), with one exponential.
-__device__ __forceinline__ float sigmoid(float z) { return __fdividef(1.f, 1.f + __expf(-z)); }
-__device__ __forceinline__ float activate(float u, int act) {
-  switch (act) {
-    case CX_ACT_RELU: return u > 0.f || u != u ? u : 0.f;
-    case CX_ACT_GELU: return 0.5f * u * (1.f + erff(u * 0.70710678118654752f));
-    case CX_ACT_GELU_TANH: return u * sigmoid(1.5957691216057308f * (u + 0.044715f * u * u * u));
-    case CX_ACT_SILU: return u * sigmoid(u);
-    default: return u;
+// same function as u / 2 (1 + tanh z), with one exponential.  Power of two and reciprocal are the hardware's (about 2
+// units of 2^-23): three bits below what the result is rounded to in 16 bits, and inside the sums' own error in 32.
+constexpr float kGelu = 1.5957691216057308f;       // 2 sqrt(2 / pi)
+__device__ __forceinline__ float sigmoid(float z) { return inverse(1.f + pow2(-kLog2e * z)); }
+__device__ __forceinline__ float gelu_gate(float u) { return inverse(1.f + pow2(u * __fmaf_rn(u * u, -0.044715f * kGelu * kLog2e, -kGelu * kLog2e))); }
+template <int N>
+__device__ __forceinline__ void activate(float (&v)[N], int act) {
+  if (act == CX_ACT_RELU) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = v[i] > 0.f || v[i] != v[i] ? v[i] : 0.f;
+  } else if (act == CX_ACT_GELU) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = 0.5f * v[i] * (1.f + erff(v[i] * 0.70710678118654752f));
+  } else if (act == CX_ACT_GELU_TANH) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] *= gelu_gate(v[i]);
+  } else if (act == CX_ACT_SILU) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] *= sigmoid(v[i]);
   }
 }
 __device__ __forceinline__ float slope(float u, int act) {
   switch (act) {
     case CX_ACT_RELU: return u > 0.f ? 1.f : 0.f;
-    case CX_ACT_GELU: return 0.5f * (1.f + erff(u * 0.70710678118654752f)) + u * 0.39894228040143268f * __expf(-0.5f * u * u);
+    case CX_ACT_GELU: return 0.5f * (1.f + erff(u * 0.70710678118654752f)) + u * 0.39894228040143268f * pow2(-0.5f * kLog2e * u * u);
     case CX_ACT_GELU_TANH: {
-      const float q = sigmoid(1.5957691216057308f * (u + 0.044715f * u * u * u));
-      return q + u * q * (1.f - q) * 1.5957691216057308f * (1.f + 0.134145f * u * u);
+      const float q = gelu_gate(u);
+      return q + u * q * (1.f - q) * kGelu * __fmaf_rn(u * u, 0.134145f, 1.f);
     }
     case CX_ACT_SILU: {
       const float q = sigmoid(u);
-      return q * (1.f + u * (1.f - q));
+      return q * __fmaf_rn(u, 1.f - q, 1.f);
     }
     default: return 1.f;
   }
@@ -132,9 +169,13 @@ __device__ __forceinline__ void pack4(const float* v, uint2* out, __half) {
   const float t[4] = {v[0], v[1], v[2], v[3]};
   cx::store4(reinterpret_cast<__half*>(out), t);
 }
+__device__ __forceinline__ void pack4(const float*, uint2*, float) {}
 template <typename T>
-__device__ __forceinline__ void store8(T* p, bool wide, int left, const float (&v)[8]) {
-  if (wide) {
+__device__ __forceinline__ void store8(T* p, bool wide, int left, const float* v) {
+  if (wide && sizeof(T) == 4) {
+    reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+    reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+  } else if (wide) {
     uint2 t[2];
     pack4(v, t, T());
     pack4(v + 4, t + 1, T());

@@ -9,7 +9,7 @@
 
 namespace {
 
-constexpr int kThreads = 256, kRowsPer = 64;
+constexpr int kThreads = 256, kRowsPer = 64;      // a block of du_kernel: 64 rows of 256 columns
 
 struct Du {
   const void* grad;
@@ -18,41 +18,103 @@ struct Du {
   float* part;          // [chunks][outer], NULL: no sums
   int64_t rows, outer, ldg, ldd;
   int32_t act;
+  int32_t wide_in, wide_out;       // 16-byte accesses are aligned
 };
 
-// du and the sums of its columns over kRowsPer rows; a thread has a column
+// du, and the sums of its columns over 64 rows.  Bound by memory: a thread has 8 neighbouring columns of 8 rows, all of
+// them under way at once; the 8 threads of a column join their sums in shared memory, in a fixed order.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) du_kernel(const Du d) {
-  using E = cx::Elem<T>;
-  const int64_t c = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  if (c >= d.outer) return;
-  const int64_t r0 = (int64_t)blockIdx.y * kRowsPer, r1 = min(d.rows, r0 + kRowsPer);
-  float sum = 0.f;
-  for (int64_t r = r0; r < r1; ++r) {
-    float g = E::to_f(reinterpret_cast<const T*>(d.grad)[r * d.ldg + c]);
-    if (d.act != CX_ACT_NONE) g *= cxprod::slope(E::to_f(reinterpret_cast<const T*>(d.pre)[r * d.outer + c]), d.act);
-    sum += g;
-    if (d.du) reinterpret_cast<T*>(d.du)[r * d.ldd + c] = E::from_f(g);
+__global__ void __launch_bounds__(kThreads) du_kernel(const __grid_constant__ Du d) {
+  __shared__ float sums[8][256 + 8];
+  cx::pdl_trigger();
+  cx::pdl_wait();
+  const int lane = threadIdx.x % 32, group = threadIdx.x / 32;
+  const int64_t c = (int64_t)blockIdx.x * 256 + lane * 8, r0 = (int64_t)blockIdx.y * kRowsPer + group;
+  const int left = (int)max((int64_t)0, min((int64_t)8, d.outer - c));
+  const bool act = d.act != CX_ACT_NONE;
+  float sum[8] = {};
+  const T* grad = reinterpret_cast<const T*>(d.grad) + c;
+  const T* pre = reinterpret_cast<const T*>(d.pre) + c;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    float g[4][8], u[4][8];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int64_t r = r0 + 8 * (4 * h + j);
+      const int have = r < d.rows ? left : 0;
+      cxprod::load8(grad + r * d.ldg, have == 8 && d.wide_in, have, g[j]);
+      if (act) cxprod::load8(pre + r * d.outer, have == 8 && d.wide_in, have, u[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int64_t r = r0 + 8 * (4 * h + j);
+      if (r >= d.rows || left == 0) continue;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (act) g[j][i] *= cxprod::slope(u[j][i], d.act);
+        sum[i] += i < left ? g[j][i] : 0.f;
+      }
+      if (d.du) cxprod::store8(reinterpret_cast<T*>(d.du) + r * d.ldd + c, left == 8 && d.wide_out, left, g[j]);
+    }
   }
-  if (d.part) d.part[blockIdx.y * d.outer + c] = sum;
+  if (!d.part) return;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) sums[group][lane * 8 + i] = sum[i];
+  __syncthreads();
+  const int64_t mine = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (mine >= d.outer) return;
+  float all = 0.f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) all += sums[j][threadIdx.x];
+  d.part[blockIdx.y * d.outer + mine] = all;
 }
 
+struct ColumnSums {
+  const float* part;
+  int64_t chunks, outer;
+  void* out;
+};
+
 template <typename T>
-__global__ void __launch_bounds__(kThreads) column_sum_kernel(const float* part, int64_t chunks, int64_t outer, T* out) {
-  const int64_t c = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  if (c >= outer) return;
+__global__ void __launch_bounds__(kThreads) column_sum_kernel(const __grid_constant__ ColumnSums d) {
+  __shared__ float sums[8][33];
+  cx::pdl_trigger();
+  cx::pdl_wait();
+  const int lane = threadIdx.x % 32, group = threadIdx.x / 32;
+  const int64_t c = (int64_t)blockIdx.x * 32 + lane;
   float sum = 0.f;
-  for (int64_t i = 0; i < chunks; ++i) sum += part[i * outer + c];
-  out[c] = cx::Elem<T>::from_f(sum);
+  if (c < d.outer) {
+#pragma unroll 4
+    for (int64_t i = group; i < d.chunks; i += 8) sum += d.part[i * d.outer + c];
+  }
+  sums[group][lane] = sum;
+  __syncthreads();
+  if (group || c >= d.outer) return;
+#pragma unroll
+  for (int j = 1; j < 8; ++j) sum += sums[j][lane];
+  reinterpret_cast<T*>(d.out)[c] = cx::Elem<T>::from_f(sum);
 }
 
 template <typename T>
-int du_pass(const Du& d, void* dbias, cudaStream_t s) {
-  const int64_t chunks = (d.rows + kRowsPer - 1) / kRowsPer, cols = (d.outer + kThreads - 1) / kThreads;
-  du_kernel<T><<<dim3((unsigned)cols, (unsigned)chunks), kThreads, 0, s>>>(d);
-  cx_note_launch();
+int du_pass(Du& d, void* dbias, cudaStream_t s) {
+  const int64_t chunks = (d.rows + kRowsPer - 1) / kRowsPer;
+  const uintptr_t in = reinterpret_cast<uintptr_t>(d.grad) | (d.act != CX_ACT_NONE ? reinterpret_cast<uintptr_t>(d.pre) : 0);
+  d.wide_in = (in & 15) == 0 && d.ldg % 8 == 0 && (d.act == CX_ACT_NONE || d.outer % 8 == 0);
+  d.wide_out = (reinterpret_cast<uintptr_t>(d.du) & 15) == 0 && d.ldd % 8 == 0;
+  for (int64_t first = 0; first < chunks; first += 65535) {        // a grid's second dimension ends there
+    Du part = d;
+    part.grad = reinterpret_cast<const T*>(d.grad) + first * kRowsPer * d.ldg;
+    if (d.pre) part.pre = reinterpret_cast<const T*>(d.pre) + first * kRowsPer * d.outer;
+    if (d.du) part.du = reinterpret_cast<T*>(d.du) + first * kRowsPer * d.ldd;
+    if (d.part) part.part = d.part + first * d.outer;
+    part.rows = d.rows - first * kRowsPer;
+    const dim3 grid((unsigned)((d.outer + 255) / 256), (unsigned)(chunks - first < 65535 ? chunks - first : 65535));
+    cx_launch_pdl2(du_kernel<T>, grid, kThreads, s, part);
+    cx_note_launch();
+  }
   if (dbias) {
-    column_sum_kernel<T><<<(unsigned)cols, kThreads, 0, s>>>(d.part, chunks, d.outer, reinterpret_cast<T*>(dbias));
+    const ColumnSums c = {d.part, chunks, d.outer, dbias};
+    cx_launch_pdl2(column_sum_kernel<T>, dim3((unsigned)((d.outer + 31) / 32)), kThreads, s, c);
     cx_note_launch();
   }
   return cx_check_launch("cx_linear_backward");

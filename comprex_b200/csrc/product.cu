@@ -23,7 +23,9 @@ __device__ __forceinline__ void finish(const CxProduct& p, int64_t row, int64_t 
   if (p.scale) v *= *p.scale;
   if (p.bias) v += E::to_f(reinterpret_cast<const T*>(p.bias)[col]);
   if (p.pre) reinterpret_cast<T*>(p.pre)[row * p.ldo + col] = E::from_f(v);
-  v = cxprod::activate(v, p.act);
+  float one[1] = {v};
+  cxprod::activate(one, p.act);
+  v = one[0];
   if (p.residual) v += E::to_f(reinterpret_cast<const T*>(p.residual)[row * p.ldr + col]);
   reinterpret_cast<T*>(p.out)[row * p.ldo + col] = E::from_f(v);
 }
@@ -106,17 +108,25 @@ __global__ void __launch_bounds__(kThreads) product_kernel(const __grid_constant
   }
 }
 
+struct Align {
+  const uint16_t* from;
+  uint16_t* to;
+  int64_t ld, rows, cols, to_ld;
+};
+
 // rows of `cols` elements, `ld` apart, to rows of `to_ld` (a multiple of 8); what is beyond a row's end is zero
-__global__ void __launch_bounds__(kThreads) align_kernel(const uint16_t* from, int64_t ld, int64_t rows, int64_t cols, uint16_t* to, int64_t to_ld) {
-  const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x, per = to_ld / 8;
-  if (i >= rows * per) return;
+__global__ void __launch_bounds__(kThreads) align_kernel(const __grid_constant__ Align d) {
+  cx::pdl_trigger();
+  cx::pdl_wait();
+  const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x, per = d.to_ld / 8;
+  if (i >= d.rows * per) return;
   const int64_t row = i / per, col = i % per * 8;
   uint16_t v[8];
 #pragma unroll
-  for (int k = 0; k < 8; ++k) v[k] = col + k < cols ? from[row * ld + col + k] : 0;
+  for (int k = 0; k < 8; ++k) v[k] = col + k < d.cols ? d.from[row * d.ld + col + k] : 0;
   uint4 t;
   memcpy(&t, v, 16);
-  *reinterpret_cast<uint4*>(to + row * to_ld + col) = t;
+  *reinterpret_cast<uint4*>(d.to + row * d.to_ld + col) = t;
 }
 
 }  // namespace
@@ -131,8 +141,8 @@ int cx_product_operand(const void** base, int64_t* ld, int dtype, int64_t rows, 
   *ld = to_ld;
   if (!ws.base) return 0;
   if (!ws.ok()) return cx_set_error("cx_product: workspace too small", 0);
-  align_kernel<<<(unsigned)((rows * (to_ld / 8) + kThreads - 1) / kThreads), kThreads, 0, s>>>(
-      reinterpret_cast<const uint16_t*>(from), from_ld, rows, cols, reinterpret_cast<uint16_t*>(to), to_ld);
+  const Align d = {reinterpret_cast<const uint16_t*>(from), reinterpret_cast<uint16_t*>(to), from_ld, rows, cols, to_ld};
+  cx_launch_pdl2(align_kernel, dim3((unsigned)((rows * (to_ld / 8) + kThreads - 1) / kThreads)), kThreads, s, d);
   cx_note_launch();
   return cx_check_launch("cx_product");
 }

@@ -2,7 +2,7 @@
 //
 // A persistent grid of CTAs, or of pairs of CTAs that share a tile, walks over the output's tiles.  One thread per CTA
 // brings 64-deep slices of both operands into a ring of stages with tile copies, one thread per tile issues the matrix
-// instructions, whose sums stay in tensor memory, and four warps take finished sums from there: the tensor memory holds
+// instructions, whose sums stay in tensor memory, and eight warps take finished sums from there: the tensor memory holds
 // two tiles, so the matrix instructions of a tile run under the epilogue of the tile before.  Each layout of the operands
 // is read as it lies: consecutive along k or along m and n is a bit of the instruction and another shape of the copy.
 #include "cx_product.cuh"
@@ -11,9 +11,11 @@
 namespace {
 
 constexpr int kDepth = 64;               // elements of k in a stage: one 128-byte line
-constexpr int kThreads = 256;            // warp 0 copies, warp 1 multiplies, warp 2 has the tensor memory, 4 to 7 finish
+constexpr int kThreads = 384;            // warp 0 copies, warp 1 multiplies, warp 2 has the tensor memory, 4 to 11 finish
+constexpr int kJoinThreads = 256;
 constexpr int kPitch = 36;               // floats of a row of the epilogue's scratch: 16-byte accesses without conflicts
-constexpr int kScratch = 4 * 32 * kPitch * 4;
+constexpr int kFinish = 8;               // finishing warps: four have the left half of a tile's columns, four the right one
+constexpr int kScratch = kFinish * 32 * kPitch * 4;
 constexpr int kShared = 232448;          // of a CTA
 constexpr int kGroup = 8;                // tiles along m that are walked together: their operands stay in L2
 
@@ -52,100 +54,150 @@ __device__ __forceinline__ Unit unit_of(const Plan& t, int u) {
   return r;
 }
 
-// what is done to 8 neighbouring sums of a row (kOut, kSums)
-template <typename T>
-__device__ __forceinline__ void finish8(const Plan& t, int64_t row, int64_t col, float (&v)[8]) {
+// What is done to sums (kOut, kSums) of R rows, `apart` rows apart, each 8 neighbouring columns.
+template <typename T, int R>
+__device__ __forceinline__ void finish(const Plan& t, int64_t row, int apart, int64_t col, float (&v)[8 * R]) {
   const CxProduct& p = t.p;
-  if (row >= p.m || col >= p.n) return;
   const int left = (int)min((int64_t)8, p.n - col);
+  if (left <= 0) return;
   float x[8];
   if (p.has_addend) {
-    cxprod::load8(p.addend + row * p.n + col, left == 8 && t.wide_add, left, x);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] += x[i];
+    for (int j = 0; j < R; ++j)
+      if (row + j * apart < p.m) {
+        cxprod::load8(p.addend + (row + j * apart) * p.n + col, left == 8 && t.wide_add, left, x);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[8 * j + i] += x[i];
+      }
   }
   if (p.mode == kSums) {
-    float* at = p.addend + row * p.n + col;
-    if (left == 8 && t.wide_add) {
-      *reinterpret_cast<float4*>(at) = make_float4(v[0], v[1], v[2], v[3]);
-      *reinterpret_cast<float4*>(at + 4) = make_float4(v[4], v[5], v[6], v[7]);
-    } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (i < left) at[i] = v[i];
-    }
+    for (int j = 0; j < R; ++j)
+      if (row + j * apart < p.m) {
+        float* at = p.addend + (row + j * apart) * p.n + col;
+        if (left == 8 && t.wide_add) {
+          *reinterpret_cast<float4*>(at) = make_float4(v[8 * j], v[8 * j + 1], v[8 * j + 2], v[8 * j + 3]);
+          *reinterpret_cast<float4*>(at + 4) = make_float4(v[8 * j + 4], v[8 * j + 5], v[8 * j + 6], v[8 * j + 7]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (i < left) at[i] = v[8 * j + i];
+        }
+      }
     return;
   }
   const bool wide = left == 8 && t.wide_out;
-  T* out = reinterpret_cast<T*>(p.out) + row * p.ldo + col;
   if (p.scale) {
     const float f = *p.scale;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] *= f;
+    for (int i = 0; i < 8 * R; ++i) v[i] *= f;
   }
   if (p.bias) {
     cxprod::load8(reinterpret_cast<const T*>(p.bias) + col, left == 8 && t.wide_bias, left, x);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] += x[i];
+    for (int i = 0; i < 8 * R; ++i) v[i] += x[i % 8];
   }
-  if (p.pre) cxprod::store8(reinterpret_cast<T*>(p.pre) + row * p.ldo + col, wide, left, v);
-  if (p.act != CX_ACT_NONE) {
+  if (p.pre) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = cxprod::activate(v[i], p.act);
+    for (int j = 0; j < R; ++j)
+      if (row + j * apart < p.m)
+        cxprod::store8(reinterpret_cast<T*>(p.pre) + (row + j * apart) * p.ldo + col, wide, left, v + 8 * j);
   }
-  if (p.residual) {
-    cxprod::load8(reinterpret_cast<const T*>(p.residual) + row * p.ldr + col, left == 8 && t.wide_res, left, x);
+  cxprod::activate(v, p.act);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] += x[i];
-  }
-  cxprod::store8(out, wide, left, v);
+  for (int j = 0; j < R; ++j)
+    if (row + j * apart < p.m) {
+      if (p.residual) {
+        cxprod::load8(reinterpret_cast<const T*>(p.residual) + (row + j * apart) * p.ldr + col, left == 8 && t.wide_res, left, x);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[8 * j + i] += x[i];
+      }
+      cxprod::store8(reinterpret_cast<T*>(p.out) + (row + j * apart) * p.ldo + col, wide, left, v + 8 * j);
+    }
 }
 
 // Rows of the warp's 32 x 32 sums, one per lane, through shared memory to four lanes per row: every access of the
 // output is then 16 bytes, 64 neighbouring bytes a row.
 template <typename T>
-__device__ __forceinline__ void finish32(const Plan& t, const Unit& u, int64_t row0, int64_t col, float* scratch, const uint32_t (&r)[32]) {
-  const int lane = threadIdx.x & 31;
+__device__ __forceinline__ void finish32(const Plan& t, int split, int64_t row0, int64_t col, float* scratch, const uint32_t (&r)[32]) {
+  const int lane = threadIdx.x & 31, c = lane % 4 * 8;
 #pragma unroll
   for (int j = 0; j < 8; ++j)
     *reinterpret_cast<uint4*>(scratch + lane * kPitch + 4 * j) = make_uint4(r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
   __syncwarp();
+  float v[32];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const int row = 8 * j + lane / 4, c = lane % 4 * 8;
-    float v[8];
-    *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(scratch + row * kPitch + c);
-    *reinterpret_cast<float4*>(v + 4) = *reinterpret_cast<const float4*>(scratch + row * kPitch + c + 4);
-    if (t.partial) {
-      if (row0 + row < t.p.m && col + c < t.p.n) {       // part_ld is a multiple of 8
-        float* at = t.partial + ((int64_t)u.split * t.p.m + row0 + row) * t.part_ld + col + c;
-        *reinterpret_cast<float4*>(at) = make_float4(v[0], v[1], v[2], v[3]);
-        *reinterpret_cast<float4*>(at + 4) = make_float4(v[4], v[5], v[6], v[7]);
-      }
-    } else if (t.p.mode == kProb) {
-      if (row0 + row < t.p.m && col + c < t.p.n) {
-        const int left = (int)min((int64_t)8, t.p.n - col - c);
-        cxprod::store8(reinterpret_cast<T*>(t.p.out) + (row0 + row) * t.p.ldo + col + c, left == 8 && t.wide_out, left, v);
-      }
-    } else {
-      finish8<T>(t, row0 + row, col + c, v);
-    }
+    const float* at = scratch + (8 * j + lane / 4) * kPitch + c;
+    *reinterpret_cast<float4*>(v + 8 * j) = *reinterpret_cast<const float4*>(at);
+    *reinterpret_cast<float4*>(v + 8 * j + 4) = *reinterpret_cast<const float4*>(at + 4);
   }
   __syncwarp();
+  row0 += lane / 4;
+  col += c;
+  if (!t.partial) return finish<T, 4>(t, row0, 8, col, v);
+  if (col >= t.p.n) return;
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (row0 + 8 * j < t.p.m) {                              // part_ld is a multiple of 8
+      float* at = t.partial + ((int64_t)split * t.p.m + row0 + 8 * j) * t.part_ld + col;
+      *reinterpret_cast<float4*>(at) = make_float4(v[8 * j], v[8 * j + 1], v[8 * j + 2], v[8 * j + 3]);
+      *reinterpret_cast<float4*>(at + 4) = make_float4(v[8 * j + 4], v[8 * j + 5], v[8 * j + 6], v[8 * j + 7]);
+    }
 }
 
-template <typename T, int BN>
-__device__ __forceinline__ void finish_tile(const Plan& t, const Unit& u, int64_t row0, uint32_t tmem, float* scratch) {
+// The same for values that only have to be rounded and stored: they go through shared memory in 16 bits.
+template <typename T>
+__device__ __forceinline__ void store32(const Plan& t, int64_t row0, int64_t col, float* scratch, const uint32_t (&r)[32]) {
+  const int lane = threadIdx.x & 31, c = lane % 4 * 8;
+  const CxProduct& p = t.p;
+  uint4* mine = reinterpret_cast<uint4*>(scratch) + lane * 5;          // 64 bytes of a row, 16 of padding
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    uint2 lo, hi;
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(r[8 * j + i]);
+    cxprod::pack4(x, &lo, T());
+    cxprod::pack4(x + 4, &hi, T());
+    mine[j] = make_uint4(lo.x, lo.y, hi.x, hi.y);
+  }
+  __syncwarp();
+  uint4 q[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) q[j] = reinterpret_cast<const uint4*>(scratch)[(8 * j + lane / 4) * 5 + lane % 4];
+  __syncwarp();
+  const int left = (int)min((int64_t)8, p.n - col - c);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int64_t row = row0 + 8 * j + lane / 4;
+    if (row >= p.m || left <= 0) continue;
+    T* at = reinterpret_cast<T*>(p.out) + row * p.ldo + col + c;
+    if (left == 8 && t.wide_out) {
+      *reinterpret_cast<uint4*>(at) = q[j];
+    } else {
+      const T* e = reinterpret_cast<const T*>(&q[j]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i < left) at[i] = e[i];
+    }
+  }
+}
+
+// A finishing warp's part of a tile: 32 rows, WIDTH columns from col0 on.
+template <typename T, int WIDTH>
+__device__ __forceinline__ void finish_part(const Plan& t, int split, int64_t part, int64_t row0, int64_t col0, uint32_t tmem, float* scratch) {
   const CxProduct& p = t.p;
   const int lane = threadIdx.x & 31;
-  const int64_t row = row0 + lane, col0 = (int64_t)u.tn * BN;
+  const int64_t row = row0 + lane;
   const bool in = row < p.m;
   uint32_t r[32];
   if (p.mode == kStats) {
-    const int64_t hot = (in ? p.targets[row] : -1) - p.col0 - col0;      // where the row's target is in this tile
+    if (col0 >= p.n) return;
+    const int64_t hot = (in ? p.targets[row] : -1) - p.col0 - col0;      // where the row's target is in this part
     float top = -INFINITY, sum = 0.f;
 #pragma unroll 1
-    for (int c = 0; c < BN; c += 32) {
+    for (int c = 0; c < WIDTH; c += 32) {
       if (col0 + c >= p.n) break;
       cxt::tmem_load32(tmem + c, r);
       cxt::tmem_load_wait();
@@ -162,43 +214,56 @@ __device__ __forceinline__ void finish_tile(const Plan& t, const Unit& u, int64_
           if (hot == c + j) x = __uint_as_float(r[j]);
         p.target_logit[row] = x;
       }
-      float m = top;
+      float m[4] = {top, top, top, top}, add[4] = {};
 #pragma unroll
-      for (int j = 0; j < 32; ++j) m = fmaxf(m, __uint_as_float(r[j]));
-      const float base = (m == -INFINITY ? 0.f : m) * cxprod::kLog2e;
-      sum *= exp2f(top * cxprod::kLog2e - base);                         // (top = -inf: 0)
+      for (int j = 0; j < 32; ++j) m[j % 4] = fmaxf(m[j % 4], __uint_as_float(r[j]));
+      m[0] = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+      const float base = (m[0] == -INFINITY ? 0.f : m[0]) * cxprod::kLog2e;
 #pragma unroll
-      for (int j = 0; j < 32; ++j) sum += exp2f(__fmaf_rn(__uint_as_float(r[j]), cxprod::kLog2e, -base));
-      top = m;
+      for (int j = 0; j < 32; ++j) add[j % 4] += cxprod::pow2(__fmaf_rn(__uint_as_float(r[j]), cxprod::kLog2e, -base));
+      sum = sum * cxprod::pow2(__fmaf_rn(top, cxprod::kLog2e, -base)) + ((add[0] + add[1]) + (add[2] + add[3]));   // (top = -inf: 0)
+      top = m[0];
     }
-    if (in) p.part[(int64_t)u.tn * p.m + row] = make_float2(top, sum);
+    if (in) p.part[part * p.m + row] = make_float2(top, sum);
     return;
   }
-  float lse = 0.f, factor = 0.f;
-  int64_t hot = -1;
-  if (p.mode == kProb && in) {
-    lse = p.lse[row];
-    factor = p.row_factor[row];
-    hot = p.targets[row] - p.col0 - col0;
-  }
+  if (p.mode == kProb) {
+    const float lse = in ? p.lse[row] : 0.f, factor = in ? p.row_factor[row] : 0.f;
+    const int64_t hot = in ? p.targets[row] - p.col0 - col0 : -1;
 #pragma unroll 1
-  for (int c = 0; c < BN; c += 32) {
-    if (col0 + c >= p.n) break;
-    cxt::tmem_load32(tmem + c, r);
-    cxt::tmem_load_wait();
-    if (p.mode == kProb) {
+    for (int c = 0; c < WIDTH; c += 32) {
+      if (col0 + c >= p.n) break;
+      cxt::tmem_load32(tmem + c, r);
+      cxt::tmem_load_wait();
 #pragma unroll
-      for (int j = 0; j < 32; ++j) {
-        const float q = exp2f(__fmaf_rn(__uint_as_float(r[j]), cxprod::kLog2e, -lse));
-        r[j] = __float_as_uint(factor == 0.f ? 0.f : q * factor);
-      }
+      for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(cxprod::pow2(__fmaf_rn(__uint_as_float(r[j]), cxprod::kLog2e, -lse)) * factor);
       if (hot >= c && hot < c + 32) {
 #pragma unroll
         for (int j = 0; j < 32; ++j)
           if (hot == c + j) r[j] = __float_as_uint(__uint_as_float(r[j]) - factor);
       }
+      if (factor == 0.f) {                 // a row that does not count, whatever its logits are
+#pragma unroll
+        for (int j = 0; j < 32; ++j) r[j] = 0;
+      }
+      store32<T>(t, row0, col0 + c, scratch, r);
     }
-    finish32<T>(t, u, row0, col0 + c, scratch, r);
+    return;
+  }
+  const bool plain = p.mode == kOut && !t.partial && !p.has_addend && !p.bias && !p.pre && !p.residual && p.act == CX_ACT_NONE;
+  const float scale = plain && p.scale ? *p.scale : 1.f;
+#pragma unroll 1
+  for (int c = 0; c < WIDTH; c += 32) {
+    if (col0 + c >= p.n) break;
+    cxt::tmem_load32(tmem + c, r);
+    cxt::tmem_load_wait();
+    if (plain) {
+#pragma unroll
+      for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * scale);
+      store32<T>(t, row0, col0 + c, scratch, r);
+    } else {
+      finish32<T>(t, split, row0, col0 + c, scratch, r);
+    }
   }
 }
 
@@ -224,7 +289,7 @@ tensor_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
     }
     for (int i = 0; i < 2; ++i) {
       cx::mbar_init(bars + 2 * S::kStages + i, 1);
-      cx::mbar_init(bars + 2 * S::kStages + 2 + i, 4 * CG);
+      cx::mbar_init(bars + 2 * S::kStages + 2 + i, kFinish * CG);
     }
     cxt::fence_barrier_init();
     cxt::prefetch_map(&map_a);
@@ -325,10 +390,11 @@ tensor_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
         break;
       }
       cxt::fence_after_sync();
-      const int64_t row0 = (int64_t)(w.tm * CG + (int)rank) * 128 + (warp - 4) * 32;
-      const uint32_t at = tmem + (turn & 1) * BN + ((uint32_t)(warp - 4) * 32u << 16);
-      if (t.p.dtype == CX_BF16) finish_tile<__nv_bfloat16, BN>(t, w, row0, at, mine);
-      else finish_tile<__half, BN>(t, w, row0, at, mine);
+      const int quarter = warp % 4, half = (warp - 4) / 4;
+      const int64_t row0 = (int64_t)(w.tm * CG + (int)rank) * 128 + quarter * 32, col0 = (int64_t)w.tn * BN + half * (BN / 2);
+      const uint32_t at = tmem + (turn & 1) * BN + half * (BN / 2) + ((uint32_t)quarter * 32u << 16);
+      if (t.p.dtype == CX_BF16) finish_part<__nv_bfloat16, BN / 2>(t, w.split, 2 * w.tn + half, row0, col0, at, mine);
+      else finish_part<__half, BN / 2>(t, w.split, 2 * w.tn + half, row0, col0, at, mine);
       cxt::fence_before_sync();
       __syncwarp();
       if (lane == 0) cxt::arrive_cluster(taken + 8 * (turn & 1));
@@ -345,10 +411,10 @@ tensor_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
 
 // the splits' sums, added in their order, and the rest of the epilogue
 template <typename T>
-__global__ void __launch_bounds__(kThreads) join_splits_kernel(const __grid_constant__ Plan t) {
+__global__ void __launch_bounds__(kJoinThreads) join_splits_kernel(const __grid_constant__ Plan t) {
   cx::pdl_trigger();
   cx::pdl_wait();
-  const int64_t per = t.part_ld / 8, i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+  const int64_t per = t.part_ld / 8, i = (int64_t)blockIdx.x * kJoinThreads + threadIdx.x;
   if (i >= t.p.m * per) return;
   const int64_t row = i / per, col = i % per * 8;
   float v[8] = {};
@@ -358,7 +424,7 @@ __global__ void __launch_bounds__(kThreads) join_splits_kernel(const __grid_cons
     v[0] += lo.x; v[1] += lo.y; v[2] += lo.z; v[3] += lo.w;
     v[4] += hi.x; v[5] += hi.y; v[6] += hi.z; v[7] += hi.w;
   }
-  finish8<T>(t, row, col, v);
+  finish<T, 1>(t, row, 1, col, v);
 }
 
 // ---- host ----------------------------------------------------------------------------------------------------------
@@ -474,7 +540,7 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 bool cx_tensor_product_takes(const CxProduct& p) {
   return p.dtype != CX_F32 && aligned16(p.a) && aligned16(p.b) && p.lda % 8 == 0 && p.ldb % 8 == 0;
 }
-int cx_tensor_product_stat_columns(const CxProduct& p) { return choose(p).bn; }
+int cx_tensor_product_stat_columns(const CxProduct& p) { return choose(p).bn / 2; }
 int64_t cx_tensor_product_workspace_bytes(const CxProduct& p) {
   const Choice c = choose(p);
   return c.splits > 1 ? c.splits * p.m * ((p.n + 7) / 8 * 8) * 4 : 0;
@@ -509,9 +575,9 @@ int cx_tensor_product(const CxProduct& p, cudaStream_t s) {
   }
   int rc = c.cg == 2 ? launch_layout<2, 256>(t, s) : c.bn == 128 ? launch_layout<1, 128>(t, s) : launch_layout<1, 64>(t, s);
   if (rc || t.splits == 1) return rc;
-  const int grid = (int)ceil_div(p.m * (t.part_ld / 8), kThreads);
-  if (p.dtype == CX_BF16) cx_launch_pdl(join_splits_kernel<__nv_bfloat16>, grid, kThreads, 0, s, t, false);
-  else cx_launch_pdl(join_splits_kernel<__half>, grid, kThreads, 0, s, t, false);
+  const int grid = (int)ceil_div(p.m * (t.part_ld / 8), kJoinThreads);
+  if (p.dtype == CX_BF16) cx_launch_pdl2(join_splits_kernel<__nv_bfloat16>, dim3(grid), kJoinThreads, s, t);
+  else cx_launch_pdl2(join_splits_kernel<__half>, dim3(grid), kJoinThreads, s, t);
   cx_note_launch();
   return cx_check_launch("cx_product");
 }
