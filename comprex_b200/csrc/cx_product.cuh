@@ -28,7 +28,8 @@ struct CxProduct {
   const void* residual;    // kOut
   int64_t ldr;
   void* pre;               // kOut: (C + addend) * scale + bias, rounded, rows ldo apart
-  float* addend;           // [m][n] without gaps
+  float* addend;           // [m][ldadd], 32-byte aligned rows
+  int64_t ldadd;
   int32_t has_addend;      // it holds sums already
   const float* scale;      // device cell, NULL: 1
   float2* part;            // kStats: [tile][m]
@@ -56,8 +57,9 @@ struct Arena {                 // workspace handed out front to back; without a 
 
 }  // namespace cxprod
 
-// Takes the product's own workspace from `ws`; without a base nothing is launched and the arena counts.
-int cx_product(CxProduct& p, cxprod::Arena& ws, cudaStream_t s);
+// One product, or two that do not depend on one another and share the GPU.  Takes their own workspace from `ws`;
+// without a base nothing is launched and the arena counts.
+int cx_product(CxProduct* p, int count, cxprod::Arena& ws, cudaStream_t s);
 // An operand as the tensor cores can read it: itself, or a copy in `ws` whose rows are 16-byte aligned (16-bit types).
 int cx_product_operand(const void** base, int64_t* ld, int dtype, int64_t rows, int64_t cols, cxprod::Arena& ws, cudaStream_t s);
 // columns of a kStats tile
@@ -66,8 +68,7 @@ int cx_product_stat_columns(const CxProduct& p);
 // tensor_product.cu: 16-bit types, operands that a tile copy can read (16-byte aligned rows)
 bool cx_tensor_product_takes(const CxProduct& p);
 int cx_tensor_product_stat_columns(const CxProduct& p);
-int64_t cx_tensor_product_workspace_bytes(const CxProduct& p);
-int cx_tensor_product(const CxProduct& p, cudaStream_t s);
+int cx_tensor_product(CxProduct* p, int count, cxprod::Arena& ws, cudaStream_t s);
 
 // A launch that may become resident while the kernel in front is ending; every kernel launched so calls cx::pdl_wait
 // before it touches memory.
@@ -122,20 +123,19 @@ __device__ __forceinline__ void activate(float (&v)[N], int act) {
     for (int i = 0; i < N; ++i) v[i] *= sigmoid(v[i]);
   }
 }
-__device__ __forceinline__ float slope(float u, int act) {
-  switch (act) {
-    case CX_ACT_RELU: return u > 0.f ? 1.f : 0.f;
-    case CX_ACT_GELU: return 0.5f * (1.f + erff(u * 0.70710678118654752f)) + u * 0.39894228040143268f * pow2(-0.5f * kLog2e * u * u);
-    case CX_ACT_GELU_TANH: {
-      const float q = gelu_gate(u);
-      return q + u * q * (1.f - q) * kGelu * __fmaf_rn(u * u, 0.134145f, 1.f);
-    }
-    case CX_ACT_SILU: {
-      const float q = sigmoid(u);
-      return q * __fmaf_rn(u, 1.f - q, 1.f);
-    }
-    default: return 1.f;
+template <int ACT>
+__device__ __forceinline__ float slope(float u) {
+  if (ACT == CX_ACT_RELU) return u > 0.f ? 1.f : 0.f;
+  if (ACT == CX_ACT_GELU) return 0.5f * (1.f + erff(u * 0.70710678118654752f)) + u * 0.39894228040143268f * pow2(-0.5f * kLog2e * u * u);
+  if (ACT == CX_ACT_GELU_TANH) {
+    const float q = gelu_gate(u);
+    return q + u * q * (1.f - q) * kGelu * __fmaf_rn(u * u, 0.134145f, 1.f);
   }
+  if (ACT == CX_ACT_SILU) {
+    const float q = sigmoid(u);
+    return q * __fmaf_rn(u, 1.f - q, 1.f);
+  }
+  return 1.f;
 }
 
 // 8 neighbouring elements of a row, as 16 bytes where `wide`, else the first `left` one by one

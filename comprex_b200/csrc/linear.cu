@@ -23,7 +23,7 @@ struct Du {
 
 // du, and the sums of its columns over 64 rows.  Bound by memory: a thread has 8 neighbouring columns of 8 rows, all of
 // them under way at once; the 8 threads of a column join their sums in shared memory, in a fixed order.
-template <typename T>
+template <typename T, int ACT>
 __global__ void __launch_bounds__(kThreads) du_kernel(const __grid_constant__ Du d) {
   __shared__ float sums[8][256 + 8];
   cx::pdl_trigger();
@@ -31,7 +31,7 @@ __global__ void __launch_bounds__(kThreads) du_kernel(const __grid_constant__ Du
   const int lane = threadIdx.x % 32, group = threadIdx.x / 32;
   const int64_t c = (int64_t)blockIdx.x * 256 + lane * 8, r0 = (int64_t)blockIdx.y * kRowsPer + group;
   const int left = (int)max((int64_t)0, min((int64_t)8, d.outer - c));
-  const bool act = d.act != CX_ACT_NONE;
+  constexpr bool act = ACT != CX_ACT_NONE;
   float sum[8] = {};
   const T* grad = reinterpret_cast<const T*>(d.grad) + c;
   const T* pre = reinterpret_cast<const T*>(d.pre) + c;
@@ -51,7 +51,7 @@ __global__ void __launch_bounds__(kThreads) du_kernel(const __grid_constant__ Du
       if (r >= d.rows || left == 0) continue;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        if (act) g[j][i] *= cxprod::slope(u[j][i], d.act);
+        if (act) g[j][i] *= cxprod::slope<ACT>(u[j][i]);
         sum[i] += i < left ? g[j][i] : 0.f;
       }
       if (d.du) cxprod::store8(reinterpret_cast<T*>(d.du) + r * d.ldd + c, left == 8 && d.wide_out, left, g[j]);
@@ -109,7 +109,13 @@ int du_pass(Du& d, void* dbias, cudaStream_t s) {
     if (d.part) part.part = d.part + first * d.outer;
     part.rows = d.rows - first * kRowsPer;
     const dim3 grid((unsigned)((d.outer + 255) / 256), (unsigned)(chunks - first < 65535 ? chunks - first : 65535));
-    cx_launch_pdl2(du_kernel<T>, grid, kThreads, s, part);
+    switch (d.act) {
+      case CX_ACT_RELU: cx_launch_pdl2(du_kernel<T, CX_ACT_RELU>, grid, kThreads, s, part); break;
+      case CX_ACT_GELU: cx_launch_pdl2(du_kernel<T, CX_ACT_GELU>, grid, kThreads, s, part); break;
+      case CX_ACT_GELU_TANH: cx_launch_pdl2(du_kernel<T, CX_ACT_GELU_TANH>, grid, kThreads, s, part); break;
+      case CX_ACT_SILU: cx_launch_pdl2(du_kernel<T, CX_ACT_SILU>, grid, kThreads, s, part); break;
+      default: cx_launch_pdl2(du_kernel<T, CX_ACT_NONE>, grid, kThreads, s, part);
+    }
     cx_note_launch();
   }
   if (dbias) {
@@ -129,7 +135,7 @@ int forward(const CxLinear& l, cxprod::Arena& ws, cudaStream_t s) {
   p.out = l.y; p.ldo = l.outer; p.bias = l.bias; p.residual = l.residual; p.ldr = l.ldr; p.pre = l.pre;
   int rc = cx_product_operand(&p.a, &p.lda, l.dtype, l.rows, l.inner, ws, s);
   if (!rc) rc = cx_product_operand(&p.b, &p.ldb, l.dtype, l.outer, l.inner, ws, s);
-  return rc ? rc : cx_product(p, ws, s);
+  return rc ? rc : cx_product(&p, 1, ws, s);
 }
 
 int backward(const CxLinear& l, cxprod::Arena& ws, cudaStream_t s) {
@@ -150,23 +156,23 @@ int backward(const CxLinear& l, cxprod::Arena& ws, cudaStream_t s) {
     rc = l.dtype == CX_F32 ? du_pass<float>(d, l.dbias, s)
          : l.dtype == CX_BF16 ? du_pass<__nv_bfloat16>(d, l.dbias, s) : du_pass<__half>(d, l.dbias, s);
   if (!rc && (l.dx || l.dw)) rc = cx_product_operand(&du, &ldd, l.dtype, l.rows, l.outer, ws, s);
+  CxProduct both[2] = {};
+  int count = 0;
   if (l.dx && !rc) {
-    CxProduct p = {};
+    CxProduct& p = both[count++];
     p.m = l.rows; p.n = l.inner; p.k = l.outer;
     p.a = du; p.lda = ldd; p.b = l.w; p.ldb = l.ldw;
     p.layout = kNN; p.dtype = l.dtype; p.out = l.dx; p.ldo = l.inner;
     rc = cx_product_operand(&p.b, &p.ldb, l.dtype, l.outer, l.inner, ws, s);
-    if (!rc) rc = cx_product(p, ws, s);
   }
   if (l.dw && !rc) {
-    CxProduct p = {};
+    CxProduct& p = both[count++];
     p.m = l.outer; p.n = l.inner; p.k = l.rows;
     p.a = du; p.lda = ldd; p.b = l.x; p.ldb = l.ldx;
     p.layout = kTN; p.dtype = l.dtype; p.out = l.dw; p.ldo = l.inner;
     rc = cx_product_operand(&p.b, &p.ldb, l.dtype, l.rows, l.inner, ws, s);
-    if (!rc) rc = cx_product(p, ws, s);
   }
-  return rc;
+  return rc || !count ? rc : cx_product(both, count, ws, s);
 }
 
 }  // namespace

@@ -9,7 +9,7 @@ template <typename T>
 __device__ __forceinline__ void finish(const CxProduct& p, int64_t row, int64_t col, float v) {
   using E = cx::Elem<T>;
   if (p.mode == kSums) {
-    float* at = p.addend + row * p.n + col;
+    float* at = p.addend + row * p.ldadd + col;
     *at = p.has_addend ? *at + v : v;
     return;
   }
@@ -19,7 +19,7 @@ __device__ __forceinline__ void finish(const CxProduct& p, int64_t row, int64_t 
     reinterpret_cast<T*>(p.out)[row * p.ldo + col] = E::from_f(f == 0.f ? 0.f : q * f);
     return;
   }
-  if (p.has_addend) v += p.addend[row * p.n + col];
+  if (p.has_addend) v += p.addend[row * p.ldadd + col];
   if (p.scale) v *= *p.scale;
   if (p.bias) v += E::to_f(reinterpret_cast<const T*>(p.bias)[col]);
   if (p.pre) reinterpret_cast<T*>(p.pre)[row * p.ldo + col] = E::from_f(v);
@@ -149,19 +149,22 @@ int cx_product_operand(const void** base, int64_t* ld, int dtype, int64_t rows, 
 
 int cx_product_stat_columns(const CxProduct& p) { return cx_tensor_product_takes(p) ? cx_tensor_product_stat_columns(p) : kTile; }
 
-int cx_product(CxProduct& p, cxprod::Arena& ws, cudaStream_t s) {
-  const bool tensor = cx_tensor_product_takes(p);
-  if (tensor) {
-    p.ws_bytes = cx_tensor_product_workspace_bytes(p);
-    if (p.ws_bytes) p.workspace = ws.take(p.ws_bytes);
-  }
-  if (!ws.base) return 0;
-  if (!ws.ok()) return cx_set_error("cx_product: workspace too small", 0);
-  if (tensor) return cx_tensor_product(p, s);
+static int plain_product(const CxProduct& p, cudaStream_t s) {
   const dim3 grid((unsigned)((p.m + kTile - 1) / kTile), (unsigned)((p.n + kTile - 1) / kTile));
   if (p.dtype == CX_F32) product_kernel<float><<<grid, kThreads, 0, s>>>(p);
   else if (p.dtype == CX_BF16) product_kernel<__nv_bfloat16><<<grid, kThreads, 0, s>>>(p);
   else product_kernel<__half><<<grid, kThreads, 0, s>>>(p);
   cx_note_launch();
   return cx_check_launch("cx_product");
+}
+
+int cx_product(CxProduct* p, int count, cxprod::Arena& ws, cudaStream_t s) {
+  bool tensor = true;
+  for (int i = 0; i < count; ++i) tensor = tensor && cx_tensor_product_takes(p[i]);
+  if (tensor) return cx_tensor_product(p, count, ws, s);
+  if (!ws.base) return 0;
+  if (!ws.ok()) return cx_set_error("cx_product: workspace too small", 0);
+  int rc = 0;
+  for (int i = 0; i < count && !rc; ++i) rc = plain_product(p[i], s);
+  return rc;
 }

@@ -12,36 +12,61 @@ namespace {
 
 constexpr int kDepth = 64;               // elements of k in a stage: one 128-byte line
 constexpr int kThreads = 384;            // warp 0 copies, warp 1 multiplies, warp 2 has the tensor memory, 4 to 11 finish
-constexpr int kJoinThreads = 256;
-constexpr int kPitch = 36;               // floats of a row of the epilogue's scratch: 16-byte accesses without conflicts
 constexpr int kFinish = 8;               // finishing warps: four have the left half of a tile's columns, four the right one
-constexpr int kScratch = kFinish * 32 * kPitch * 4;
+constexpr int kJoinThreads = 256;
 constexpr int kShared = 232448;          // of a CTA
 constexpr int kGroup = 8;                // tiles along m that are walked together: their operands stay in L2
 
 template <int CG, int BN>
 struct Shape {
   static constexpr int kA = 128 * kDepth * 2, kB = BN / CG * kDepth * 2, kStage = kA + kB;
-  static constexpr int kFit = (kShared - 1024 - 512 - kScratch) / kStage;
+  static constexpr int kBias = kFinish * BN / 2 * 4;
+  static constexpr int kFit = (kShared - 1024 - 512 - kBias) / kStage;
   static constexpr int kStages = kFit < 8 ? kFit : 8;
-  static constexpr int kBytes = 1024 + 512 + kScratch + kStages * kStage;
+  static constexpr int kBytes = 1024 + 512 + kBias + kStages * kStage;
   static constexpr int kColumns = 2 * BN;
 };
 
-struct Plan {
+struct Job {
   CxProduct p;
-  int tiles_m, tiles_n, splits;
+  int tiles_m, tiles_n, units;
   int slices, slices_per;      // of kDepth along k: all, and per split
   float* partial;              // sums of the splits: [split][m][part_ld]
   int64_t part_ld;
+  int splits;
+  int wide_out, wide_res, wide_bias;   // alignment of their rows: 2 for 32 bytes, 1 for 16, 0 for less
+};
+
+// The units of the first job go round the workers, those of the second one fill up: `extra` workers have one more of the
+// first and take `few` of the second, the others `many`.
+struct Plan {
+  Job job[2];
+  int extra, few, many;
   uint32_t* status;            // set when a wait has run out
-  int wide_out, wide_add, wide_res, wide_bias;   // 16-byte accesses are aligned
+};
+
+struct Walk {
+  const Plan& t;
+  int worker, workers, job, u, end;
+  __device__ __forceinline__ Walk(const Plan& plan, int w, int n) : t(plan), worker(w), workers(n), job(0), u(w), end(plan.job[0].units) {
+    if (u >= end) second();
+  }
+  __device__ __forceinline__ void second() {
+    job = 1;
+    u = worker < t.extra ? worker * t.few : t.extra * t.few + (worker - t.extra) * t.many;
+    end = min(u + (worker < t.extra ? t.few : t.many), t.job[1].units);
+  }
+  __device__ __forceinline__ bool more() const { return u < end; }
+  __device__ __forceinline__ void next() {
+    u += job ? 1 : workers;
+    if (!job && u >= end) second();
+  }
 };
 
 struct Unit {
   int tm, tn, split, s0, s1;
 };
-__device__ __forceinline__ Unit unit_of(const Plan& t, int u) {
+__device__ __forceinline__ Unit unit_of(const Job& t, int u) {
   Unit r;
   const int tiles = t.tiles_m * t.tiles_n;
   r.split = u / tiles;
@@ -54,233 +79,210 @@ __device__ __forceinline__ Unit unit_of(const Plan& t, int u) {
   return r;
 }
 
-// What is done to sums (kOut, kSums) of R rows, `apart` rows apart, each 8 neighbouring columns.
-template <typename T, int R>
-__device__ __forceinline__ void finish(const Plan& t, int64_t row, int apart, int64_t col, float (&v)[8 * R]) {
+// ---- neighbouring columns of one row: a lane has a row, so it moves whole 32-byte sectors ---------------------------
+__device__ __forceinline__ void load_words8(const void* p, uint32_t (&w)[8]) {
+  asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7]) : "l"(p) : "memory");
+}
+__device__ __forceinline__ void store_words8(void* p, const uint32_t* w) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+               ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+  const __half2 v = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+template <typename T, int W>
+__device__ __forceinline__ void store_row(T* at, int wide, int left, const float (&v)[W]) {
+  if (left >= W && wide) {
+    uint32_t w[W / 2];
+#pragma unroll
+    for (int i = 0; i < W / 2; ++i) w[i] = pack2<T>(v[2 * i], v[2 * i + 1]);
+    if (W >= 16 && wide == 2) {
+#pragma unroll
+      for (int i = 0; i < W / 16; ++i) store_words8(at + 16 * i, w + 8 * i);
+    } else {
+#pragma unroll
+      for (int i = 0; i < W / 8; ++i) reinterpret_cast<uint4*>(at)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < W; ++i)
+      if (i < left) at[i] = cx::Elem<T>::from_f(v[i]);
+  }
+}
+template <typename T, int W>
+__device__ __forceinline__ void add_row(const T* at, int wide, int left, float (&v)[W]) {
+  if (left >= W && wide) {
+    uint32_t w[W / 2];
+    if (W >= 16 && wide == 2) {
+#pragma unroll
+      for (int i = 0; i < W / 16; ++i) load_words8(at + 16 * i, reinterpret_cast<uint32_t(&)[8]>(w[8 * i]));
+    } else {
+#pragma unroll
+      for (int i = 0; i < W / 8; ++i) {
+        const uint4 q = reinterpret_cast<const uint4*>(at)[i];
+        w[4 * i] = q.x, w[4 * i + 1] = q.y, w[4 * i + 2] = q.z, w[4 * i + 3] = q.w;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < W; ++i) v[i] += cx::Elem<T>::to_f(reinterpret_cast<const T*>(w)[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < W; ++i)
+      if (i < left) v[i] += cx::Elem<T>::to_f(at[i]);
+  }
+}
+// 32-bit sums in aligned rows, whole groups of 8
+template <int W>
+__device__ __forceinline__ void store_sums(float* at, int left, const float (&v)[W]) {
+#pragma unroll
+  for (int i = 0; i < W / 8; ++i)
+    if (8 * i < left) store_words8(at + 8 * i, reinterpret_cast<const uint32_t*>(v) + 8 * i);
+}
+template <int W>
+__device__ __forceinline__ void add_sums(const float* at, int left, float (&v)[W]) {
+#pragma unroll
+  for (int i = 0; i < W / 8; ++i)
+    if (8 * i < left) {
+      uint32_t w[8];
+      load_words8(at + 8 * i, w);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[8 * i + k] += __uint_as_float(w[k]);
+    }
+}
+
+// What is done to the sums (kOut, kSums) of W columns of a row.  `scale`: what p.scale holds; `bias`: in shared memory, or NULL where it is read from
+// the operand.
+template <typename T, int W>
+__device__ __forceinline__ void finish(const Job& t, int64_t row, int64_t col, float (&v)[W], float scale, const float* bias) {
   const CxProduct& p = t.p;
-  const int left = (int)min((int64_t)8, p.n - col);
-  if (left <= 0) return;
-  float x[8];
-  if (p.has_addend) {
-#pragma unroll
-    for (int j = 0; j < R; ++j)
-      if (row + j * apart < p.m) {
-        cxprod::load8(p.addend + (row + j * apart) * p.n + col, left == 8 && t.wide_add, left, x);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[8 * j + i] += x[i];
-      }
-  }
-  if (p.mode == kSums) {
-#pragma unroll
-    for (int j = 0; j < R; ++j)
-      if (row + j * apart < p.m) {
-        float* at = p.addend + (row + j * apart) * p.n + col;
-        if (left == 8 && t.wide_add) {
-          *reinterpret_cast<float4*>(at) = make_float4(v[8 * j], v[8 * j + 1], v[8 * j + 2], v[8 * j + 3]);
-          *reinterpret_cast<float4*>(at + 4) = make_float4(v[8 * j + 4], v[8 * j + 5], v[8 * j + 6], v[8 * j + 7]);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (i < left) at[i] = v[8 * j + i];
-        }
-      }
-    return;
-  }
-  const bool wide = left == 8 && t.wide_out;
+  const int left = (int)min((int64_t)W, p.n - col);
+  if (p.has_addend) add_sums(p.addend + row * p.ldadd + col, left, v);
+  if (p.mode == kSums) return store_sums(p.addend + row * p.ldadd + col, left, v);
   if (p.scale) {
-    const float f = *p.scale;
 #pragma unroll
-    for (int i = 0; i < 8 * R; ++i) v[i] *= f;
+    for (int i = 0; i < W; ++i) v[i] *= scale;
   }
   if (p.bias) {
-    cxprod::load8(reinterpret_cast<const T*>(p.bias) + col, left == 8 && t.wide_bias, left, x);
+    if (bias) {
 #pragma unroll
-    for (int i = 0; i < 8 * R; ++i) v[i] += x[i % 8];
-  }
-  if (p.pre) {
-#pragma unroll
-    for (int j = 0; j < R; ++j)
-      if (row + j * apart < p.m)
-        cxprod::store8(reinterpret_cast<T*>(p.pre) + (row + j * apart) * p.ldo + col, wide, left, v + 8 * j);
-  }
-  cxprod::activate(v, p.act);
-#pragma unroll
-  for (int j = 0; j < R; ++j)
-    if (row + j * apart < p.m) {
-      if (p.residual) {
-        cxprod::load8(reinterpret_cast<const T*>(p.residual) + (row + j * apart) * p.ldr + col, left == 8 && t.wide_res, left, x);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[8 * j + i] += x[i];
+      for (int i = 0; i < W / 4; ++i) {
+        const float4 b = reinterpret_cast<const float4*>(bias)[i];
+        v[4 * i] += b.x, v[4 * i + 1] += b.y, v[4 * i + 2] += b.z, v[4 * i + 3] += b.w;
       }
-      cxprod::store8(reinterpret_cast<T*>(p.out) + (row + j * apart) * p.ldo + col, wide, left, v + 8 * j);
-    }
-}
-
-// Rows of the warp's 32 x 32 sums, one per lane, through shared memory to four lanes per row: every access of the
-// output is then 16 bytes, 64 neighbouring bytes a row.
-template <typename T>
-__device__ __forceinline__ void finish32(const Plan& t, int split, int64_t row0, int64_t col, float* scratch, const uint32_t (&r)[32]) {
-  const int lane = threadIdx.x & 31, c = lane % 4 * 8;
-#pragma unroll
-  for (int j = 0; j < 8; ++j)
-    *reinterpret_cast<uint4*>(scratch + lane * kPitch + 4 * j) = make_uint4(r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
-  __syncwarp();
-  float v[32];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const float* at = scratch + (8 * j + lane / 4) * kPitch + c;
-    *reinterpret_cast<float4*>(v + 8 * j) = *reinterpret_cast<const float4*>(at);
-    *reinterpret_cast<float4*>(v + 8 * j + 4) = *reinterpret_cast<const float4*>(at + 4);
-  }
-  __syncwarp();
-  row0 += lane / 4;
-  col += c;
-  if (!t.partial) return finish<T, 4>(t, row0, 8, col, v);
-  if (col >= t.p.n) return;
-#pragma unroll
-  for (int j = 0; j < 4; ++j)
-    if (row0 + 8 * j < t.p.m) {                              // part_ld is a multiple of 8
-      float* at = t.partial + ((int64_t)split * t.p.m + row0 + 8 * j) * t.part_ld + col;
-      *reinterpret_cast<float4*>(at) = make_float4(v[8 * j], v[8 * j + 1], v[8 * j + 2], v[8 * j + 3]);
-      *reinterpret_cast<float4*>(at + 4) = make_float4(v[8 * j + 4], v[8 * j + 5], v[8 * j + 6], v[8 * j + 7]);
-    }
-}
-
-// The same for values that only have to be rounded and stored: they go through shared memory in 16 bits.
-template <typename T>
-__device__ __forceinline__ void store32(const Plan& t, int64_t row0, int64_t col, float* scratch, const uint32_t (&r)[32]) {
-  const int lane = threadIdx.x & 31, c = lane % 4 * 8;
-  const CxProduct& p = t.p;
-  uint4* mine = reinterpret_cast<uint4*>(scratch) + lane * 5;          // 64 bytes of a row, 16 of padding
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    uint2 lo, hi;
-    float x[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(r[8 * j + i]);
-    cxprod::pack4(x, &lo, T());
-    cxprod::pack4(x + 4, &hi, T());
-    mine[j] = make_uint4(lo.x, lo.y, hi.x, hi.y);
-  }
-  __syncwarp();
-  uint4 q[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) q[j] = reinterpret_cast<const uint4*>(scratch)[(8 * j + lane / 4) * 5 + lane % 4];
-  __syncwarp();
-  const int left = (int)min((int64_t)8, p.n - col - c);
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int64_t row = row0 + 8 * j + lane / 4;
-    if (row >= p.m || left <= 0) continue;
-    T* at = reinterpret_cast<T*>(p.out) + row * p.ldo + col + c;
-    if (left == 8 && t.wide_out) {
-      *reinterpret_cast<uint4*>(at) = q[j];
     } else {
-      const T* e = reinterpret_cast<const T*>(&q[j]);
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (i < left) at[i] = e[i];
+      add_row(reinterpret_cast<const T*>(p.bias) + col, t.wide_bias, left, v);
     }
+  }
+  if (p.pre) store_row(reinterpret_cast<T*>(p.pre) + row * p.ldo + col, t.wide_out, left, v);
+  cxprod::activate(v, p.act);
+  if (p.residual) add_row(reinterpret_cast<const T*>(p.residual) + row * p.ldr + col, t.wide_res, left, v);
+  store_row(reinterpret_cast<T*>(p.out) + row * p.ldo + col, t.wide_out, left, v);
+}
+
+// A finishing warp's part of a tile: 32 rows, one per lane, WIDTH columns from col0 on.  The next 32 columns come from
+// the tensor memory while these are worked on.
+template <typename T, int WIDTH, typename F>
+__device__ __forceinline__ void each32(uint32_t tmem, int64_t left, const F& work) {
+  uint32_t r[2][32];
+  cxt::tmem_load32(tmem, r[0]);
+#pragma unroll
+  for (int c = 0; c < WIDTH; c += 32) {
+    cxt::tmem_load_wait(r[(c / 32) % 2]);
+    if (c + 32 < WIDTH) cxt::tmem_load32(tmem + c + 32, r[(c / 32 + 1) % 2]);
+    if (c < left) work(c, reinterpret_cast<float(&)[32]>(r[(c / 32) % 2]));
   }
 }
 
-// A finishing warp's part of a tile: 32 rows, WIDTH columns from col0 on.
 template <typename T, int WIDTH>
-__device__ __forceinline__ void finish_part(const Plan& t, int split, int64_t part, int64_t row0, int64_t col0, uint32_t tmem, float* scratch) {
+__device__ __forceinline__ void finish_part(const Job& t, const Unit& u, int half, int64_t row0, int64_t col0, uint32_t tmem, const float* bias) {
   const CxProduct& p = t.p;
   const int lane = threadIdx.x & 31;
-  const int64_t row = row0 + lane;
+  const int64_t row = row0 + lane, left = p.n - col0;
   const bool in = row < p.m;
-  uint32_t r[32];
+  if (left <= 0) return;
   if (p.mode == kStats) {
-    if (col0 >= p.n) return;
     const int64_t hot = (in ? p.targets[row] : -1) - p.col0 - col0;      // where the row's target is in this part
     float top = -INFINITY, sum = 0.f;
-#pragma unroll 1
-    for (int c = 0; c < WIDTH; c += 32) {
-      if (col0 + c >= p.n) break;
-      cxt::tmem_load32(tmem + c, r);
-      cxt::tmem_load_wait();
-      if (col0 + c + 32 > p.n) {
-        const int left = (int)(p.n - col0 - c);
+    each32<T, WIDTH>(tmem, left, [&](int c, float(&v)[32]) {
+      if (c + 32 > left) {
 #pragma unroll
         for (int j = 0; j < 32; ++j)
-          if (j >= left) r[j] = 0xFF800000u;
+          if (c + j >= left) v[j] = -INFINITY;
       }
       if (hot >= c && hot < c + 32) {
         float x = 0.f;
 #pragma unroll
         for (int j = 0; j < 32; ++j)
-          if (hot == c + j) x = __uint_as_float(r[j]);
+          if (hot == c + j) x = v[j];
         p.target_logit[row] = x;
       }
       float m[4] = {top, top, top, top}, add[4] = {};
 #pragma unroll
-      for (int j = 0; j < 32; ++j) m[j % 4] = fmaxf(m[j % 4], __uint_as_float(r[j]));
+      for (int j = 0; j < 32; ++j) m[j % 4] = fmaxf(m[j % 4], v[j]);
       m[0] = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
       const float base = (m[0] == -INFINITY ? 0.f : m[0]) * cxprod::kLog2e;
 #pragma unroll
-      for (int j = 0; j < 32; ++j) add[j % 4] += cxprod::pow2(__fmaf_rn(__uint_as_float(r[j]), cxprod::kLog2e, -base));
+      for (int j = 0; j < 32; ++j) add[j % 4] += cxprod::pow2(__fmaf_rn(v[j], cxprod::kLog2e, -base));
       sum = sum * cxprod::pow2(__fmaf_rn(top, cxprod::kLog2e, -base)) + ((add[0] + add[1]) + (add[2] + add[3]));   // (top = -inf: 0)
       top = m[0];
-    }
-    if (in) p.part[part * p.m + row] = make_float2(top, sum);
-    return;
-  }
-  if (p.mode == kProb) {
+    });
+    if (in) p.part[(2ll * u.tn + half) * p.m + row] = make_float2(top, sum);
+  } else if (p.mode == kProb) {
     const float lse = in ? p.lse[row] : 0.f, factor = in ? p.row_factor[row] : 0.f;
     const int64_t hot = in ? p.targets[row] - p.col0 - col0 : -1;
-#pragma unroll 1
-    for (int c = 0; c < WIDTH; c += 32) {
-      if (col0 + c >= p.n) break;
-      cxt::tmem_load32(tmem + c, r);
-      cxt::tmem_load_wait();
+    T* out = reinterpret_cast<T*>(p.out) + row * p.ldo + col0;
+    each32<T, WIDTH>(tmem, left, [&](int c, float(&v)[32]) {
 #pragma unroll
-      for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(cxprod::pow2(__fmaf_rn(__uint_as_float(r[j]), cxprod::kLog2e, -lse)) * factor);
+      for (int j = 0; j < 32; ++j) v[j] = cxprod::pow2(__fmaf_rn(v[j], cxprod::kLog2e, -lse)) * factor;
       if (hot >= c && hot < c + 32) {
 #pragma unroll
         for (int j = 0; j < 32; ++j)
-          if (hot == c + j) r[j] = __float_as_uint(__uint_as_float(r[j]) - factor);
+          if (hot == c + j) v[j] -= factor;
       }
       if (factor == 0.f) {                 // a row that does not count, whatever its logits are
 #pragma unroll
-        for (int j = 0; j < 32; ++j) r[j] = 0;
+        for (int j = 0; j < 32; ++j) v[j] = 0.f;
       }
-      store32<T>(t, row0, col0 + c, scratch, r);
-    }
-    return;
-  }
-  const bool plain = p.mode == kOut && !t.partial && !p.has_addend && !p.bias && !p.pre && !p.residual && p.act == CX_ACT_NONE;
-  const float scale = plain && p.scale ? *p.scale : 1.f;
-#pragma unroll 1
-  for (int c = 0; c < WIDTH; c += 32) {
-    if (col0 + c >= p.n) break;
-    cxt::tmem_load32(tmem + c, r);
-    cxt::tmem_load_wait();
-    if (plain) {
-#pragma unroll
-      for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * scale);
-      store32<T>(t, row0, col0 + c, scratch, r);
-    } else {
-      finish32<T>(t, split, row0, col0 + c, scratch, r);
-    }
+      if (in) store_row(out + c, t.wide_out, (int)min((int64_t)32, left - c), v);
+    });
+  } else if (t.partial) {
+    float* at = t.partial + ((int64_t)u.split * p.m + row) * t.part_ld + col0;
+    each32<T, WIDTH>(tmem, left, [&](int c, float(&v)[32]) {
+      if (in) store_sums(at + c, (int)min((int64_t)32, left - c), v);
+    });
+  } else {
+    const float scale = p.scale ? *p.scale : 1.f;
+    each32<T, WIDTH>(tmem, left, [&](int c, float(&v)[32]) {
+      if (in) finish<T>(t, row, col0 + c, v, scale, bias + c);
+    });
   }
 }
 
-template <int CG, int BN, int LAYOUT>
+template <int CG, int BN>
 __global__ void __launch_bounds__(kThreads, 1)
-tensor_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ Plan t) {
+tensor_product_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_constant__ CUtensorMap map_b0,
+                      const __grid_constant__ CUtensorMap map_a1, const __grid_constant__ CUtensorMap map_b1, const __grid_constant__ Plan t) {
   using S = Shape<CG, BN>;
   extern __shared__ char shared_raw[];
   char* shared = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(shared_raw) + 1023) & ~(uintptr_t)1023);
   char* stages = shared;
-  float* scratch = reinterpret_cast<float*>(shared + S::kStages * S::kStage);
-  uint64_t* bars = reinterpret_cast<uint64_t*>(shared + S::kStages * S::kStage + kScratch);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(shared + S::kStages * S::kStage + S::kBias);
   const uint32_t bar_full = cx::smem_u32(bars), bar_empty = bar_full + 8 * S::kStages, bar_sums = bar_empty + 8 * S::kStages,
                  bar_taken = bar_sums + 16, tmem_cell = bar_taken + 16;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = CG == 2 ? cxt::cluster_rank() : 0;
-  const int units = t.tiles_m * t.tiles_n * t.splits, first = blockIdx.x / CG, step = gridDim.x / CG;
+  const int worker = blockIdx.x / CG, workers = gridDim.x / CG;
   cx::pdl_trigger();
   if (threadIdx.x == 0) {
     for (int i = 0; i < S::kStages; ++i) {
@@ -292,8 +294,8 @@ tensor_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
       cx::mbar_init(bars + 2 * S::kStages + 2 + i, kFinish * CG);
     }
     cxt::fence_barrier_init();
-    cxt::prefetch_map(&map_a);
-    cxt::prefetch_map(&map_b);
+    cxt::prefetch_map(&map_a0);
+    cxt::prefetch_map(&map_b0);
   }
   if (warp == 2) cxt::tmem_alloc<CG>(tmem_cell, S::kColumns);
   cxt::fence_before_sync();
@@ -307,10 +309,12 @@ tensor_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
   if (warp == 0 && lane == 0) {
     int stage = 0;
     uint32_t phase = 0, filled = 0;
-    for (int u = first; u < units && !gave_up; u += step) {
-      const Unit w = unit_of(t, u);
-      const int m0 = (w.tm * CG + (int)rank) * 128, n0 = w.tn * BN + (int)rank * (BN / CG);
-      for (int s = w.s0; s < w.s1; ++s) {
+    for (Walk w(t, worker, workers); w.more() && !gave_up; w.next()) {
+      const Job& job = t.job[w.job];
+      const Unit u = unit_of(job, w.u);
+      const CUtensorMap *map_a = w.job ? &map_a1 : &map_a0, *map_b = w.job ? &map_b1 : &map_b0;
+      const int layout = job.p.layout, m0 = (u.tm * CG + (int)rank) * 128, n0 = u.tn * BN + (int)rank * (BN / CG);
+      for (int s = u.s0; s < u.s1; ++s) {
         if (!cxt::wait(bar_empty + 8 * stage, phase ^ 1u)) {
           gave_up = true;
           break;
@@ -318,17 +322,17 @@ tensor_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
         const uint32_t full = CG == 2 ? cxt::in_cta(bar_full + 8 * stage, 0) : bar_full + 8 * stage;
         if (rank == 0) cxt::expect_bytes(bar_full + 8 * stage, CG * S::kStage);
         const uint32_t a = cx::smem_u32(stages + stage * S::kStage), b = a + S::kA;
-        if (LAYOUT == kTN) {
+        if (layout == kTN) {
 #pragma unroll
-          for (int i = 0; i < 2; ++i) cxt::load_tile<CG>(a + i * 8192, &map_a, m0 + 64 * i, s * kDepth, full);
+          for (int i = 0; i < 2; ++i) cxt::load_tile<CG>(a + i * 8192, map_a, m0 + 64 * i, s * kDepth, full);
         } else {
-          cxt::load_tile<CG>(a, &map_a, s * kDepth, m0, full);
+          cxt::load_tile<CG>(a, map_a, s * kDepth, m0, full);
         }
-        if (LAYOUT == kNT) {
-          cxt::load_tile<CG>(b, &map_b, s * kDepth, n0, full);
+        if (layout == kNT) {
+          cxt::load_tile<CG>(b, map_b, s * kDepth, n0, full);
         } else {
 #pragma unroll
-          for (int i = 0; i < BN / CG / 64; ++i) cxt::load_tile<CG>(b + i * 8192, &map_b, n0 + 64 * i, s * kDepth, full);
+          for (int i = 0; i < BN / CG / 64; ++i) cxt::load_tile<CG>(b + i * 8192, map_b, n0 + 64 * i, s * kDepth, full);
         }
         ++filled;
         if (++stage == S::kStages) {
@@ -349,18 +353,22 @@ tensor_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
       }
     }
   } else if (warp == 1 && lane == 0 && rank == 0) {
-    const uint32_t instr = cxt::instruction(t.p.dtype == CX_BF16, LAYOUT == kTN, LAYOUT != kNT, 128 * CG, BN);
     int stage = 0, turn = 0;
     uint32_t phase = 0;
-    for (int u = first; u < units && !gave_up; u += step, ++turn) {
-      const Unit w = unit_of(t, u);
+    for (Walk w(t, worker, workers); w.more() && !gave_up; w.next(), ++turn) {
+      const Job& job = t.job[w.job];
+      const Unit u = unit_of(job, w.u);
+      const bool along_m = job.p.layout == kTN, along_n = job.p.layout != kNT;
+      const uint32_t instr = cxt::instruction(job.p.dtype == CX_BF16, along_m, along_n, 128 * CG, BN);
+      // 16 of k: 32 bytes along a line, or 16 lines
+      const uint32_t step_a = along_m ? 2048 : 32, step_b = along_n ? 2048 : 32, chunk_a = along_m ? 8192 : 16, chunk_b = along_n ? 8192 : 16;
       if (!cxt::wait(bar_taken + 8 * (turn & 1), ((turn >> 1) & 1) ^ 1u)) {
         gave_up = true;
         break;
       }
       cxt::fence_after_sync();
       const uint32_t sums = tmem + (turn & 1) * BN;
-      for (int s = w.s0; s < w.s1; ++s) {
+      for (int s = u.s0; s < u.s1; ++s) {
         if (!cxt::wait(bar_full + 8 * stage, phase)) {
           gave_up = true;
           break;
@@ -368,9 +376,8 @@ tensor_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
         cxt::fence_after_sync();
         const uint32_t a = cx::smem_u32(stages + stage * S::kStage), b = a + S::kA;
 #pragma unroll
-        for (int k = 0; k < kDepth / 16; ++k)         // 16 of k: 32 bytes along a line, or 16 lines
-          cxt::mma<CG>(sums, cxt::smem_operand(a + k * (LAYOUT == kTN ? 2048 : 32), LAYOUT == kTN ? 8192 : 16),
-                       cxt::smem_operand(b + k * (LAYOUT != kNT ? 2048 : 32), LAYOUT != kNT ? 8192 : 16), instr, s > w.s0 || k > 0);
+        for (int k = 0; k < kDepth / 16; ++k)
+          cxt::mma<CG>(sums, cxt::smem_operand(a + k * step_a, chunk_a), cxt::smem_operand(b + k * step_b, chunk_b), instr, s > u.s0 || k > 0);
         cxt::commit<CG>(bar_empty + 8 * stage);
         if (++stage == S::kStages) {
           stage = 0;
@@ -381,20 +388,30 @@ tensor_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
     }
   } else if (warp >= 4) {
     const uint32_t taken = CG == 2 ? cxt::in_cta(bar_taken, 0) : bar_taken;
-    float* mine = scratch + (warp - 4) * 32 * kPitch;
+    const int quarter = warp % 4, half = (warp - 4) / 4;
+    float* bias = reinterpret_cast<float*>(shared + S::kStages * S::kStage) + (warp - 4) * (BN / 2);
     int turn = 0;
-    for (int u = first; u < units; u += step, ++turn) {
-      const Unit w = unit_of(t, u);
+    for (Walk w(t, worker, workers); w.more(); w.next(), ++turn) {
+      const Job& job = t.job[w.job];
+      const Unit u = unit_of(job, w.u);
+      const int64_t row0 = (int64_t)(u.tm * CG + (int)rank) * 128 + quarter * 32, col0 = (int64_t)u.tn * BN + half * (BN / 2);
+      if (job.p.bias) {                    // before the sums are there: nothing waits for it
+        for (int i = lane; i < BN / 2; i += 32) {
+          const bool have = col0 + i < job.p.n;
+          bias[i] = !have ? 0.f : job.p.dtype == CX_BF16 ? __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(job.p.bias)[col0 + i])
+                                                         : __half2float(reinterpret_cast<const __half*>(job.p.bias)[col0 + i]);
+        }
+        __syncwarp();
+      }
       if (!cxt::wait(bar_sums + 8 * (turn & 1), (turn >> 1) & 1)) {
         gave_up = true;
         break;
       }
+      __syncwarp();
       cxt::fence_after_sync();
-      const int quarter = warp % 4, half = (warp - 4) / 4;
-      const int64_t row0 = (int64_t)(w.tm * CG + (int)rank) * 128 + quarter * 32, col0 = (int64_t)w.tn * BN + half * (BN / 2);
       const uint32_t at = tmem + (turn & 1) * BN + half * (BN / 2) + ((uint32_t)quarter * 32u << 16);
-      if (t.p.dtype == CX_BF16) finish_part<__nv_bfloat16, BN / 2>(t, w.split, 2 * w.tn + half, row0, col0, at, mine);
-      else finish_part<__half, BN / 2>(t, w.split, 2 * w.tn + half, row0, col0, at, mine);
+      if (job.p.dtype == CX_BF16) finish_part<__nv_bfloat16, BN / 2>(job, u, half, row0, col0, at, bias);
+      else finish_part<__half, BN / 2>(job, u, half, row0, col0, at, bias);
       cxt::fence_before_sync();
       __syncwarp();
       if (lane == 0) cxt::arrive_cluster(taken + 8 * (turn & 1));
@@ -409,22 +426,19 @@ tensor_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
   if (warp == 2) cxt::tmem_free<CG>(tmem, S::kColumns);
 }
 
-// the splits' sums, added in their order, and the rest of the epilogue
+// the splits' sums, added in their order, and the rest of the epilogue; a block has a part of one of the jobs
 template <typename T>
 __global__ void __launch_bounds__(kJoinThreads) join_splits_kernel(const __grid_constant__ Plan t) {
   cx::pdl_trigger();
   cx::pdl_wait();
-  const int64_t per = t.part_ld / 8, i = (int64_t)blockIdx.x * kJoinThreads + threadIdx.x;
-  if (i >= t.p.m * per) return;
+  const Job& job = t.job[blockIdx.y];
+  if (!job.partial) return;
+  const int64_t per = job.part_ld / 8, i = (int64_t)blockIdx.x * kJoinThreads + threadIdx.x;
+  if (i >= job.p.m * per) return;
   const int64_t row = i / per, col = i % per * 8;
   float v[8] = {};
-  for (int s = 0; s < t.splits; ++s) {
-    const float* at = t.partial + ((int64_t)s * t.p.m + row) * t.part_ld + col;
-    const float4 lo = *reinterpret_cast<const float4*>(at), hi = *reinterpret_cast<const float4*>(at + 4);
-    v[0] += lo.x; v[1] += lo.y; v[2] += lo.z; v[3] += lo.w;
-    v[4] += hi.x; v[5] += hi.y; v[6] += hi.z; v[7] += hi.w;
-  }
-  finish<T, 1>(t, row, 1, col, v);
+  for (int s = 0; s < job.splits; ++s) add_sums(job.partial + ((int64_t)s * job.p.m + row) * job.part_ld + col, 8, v);
+  finish<T>(job, row, col, v, job.p.scale ? *job.p.scale : 1.f, nullptr);
 }
 
 // ---- host ----------------------------------------------------------------------------------------------------------
@@ -471,43 +485,70 @@ uint32_t* status_word(bool host) {
   return cudaHostGetDevicePointer(&d, word, 0) == cudaSuccess ? static_cast<uint32_t*>(d) : nullptr;
 }
 
-struct Choice {
-  int cg, bn, splits;
-};
-
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-Choice choose(const CxProduct& p) {
-  const int64_t slices = ceil_div(p.k, kDepth);
-  Choice best = {1, 128, 1};
-  if (p.mode == kStats || p.mode == kProb) {
-    if (ceil_div(p.m, 256) * ceil_div(p.n, 256) >= 74) best = {2, 256, 1};
-    return best;
+struct Choice {
+  int cg, bn, splits[2];
+};
+
+Choice choose(const CxProduct* p, int count) {
+  int64_t big = 0, tiles = 0;
+  bool sums = true;
+  for (int i = 0; i < count; ++i) {
+    big += ceil_div(p[i].m, 256) * ceil_div(p[i].n, 256);
+    tiles += ceil_div(p[i].m, 128) * ceil_div(p[i].n, 128);
+    sums = sums && (p[i].mode == kOut || p[i].mode == kSums);
   }
-  if (ceil_div(p.m, 256) * ceil_div(p.n, 256) >= 60) return {2, 256, 1};
-  const int64_t tiles = ceil_div(p.m, 128) * ceil_div(p.n, 128);
-  if (tiles < 74) best.bn = 64;
-  const int64_t now = ceil_div(p.m, 128) * ceil_div(p.n, best.bn);
-  int64_t splits = 148 / now;
-  if (splits > slices / 8) splits = slices / 8;
-  best.splits = (int)(splits < 1 ? 1 : splits);
-  return best;
+  if (big >= 60) return {2, 256, {1, 1}};
+  Choice c = {1, tiles < 74 && sums ? 64 : 128, {1, 1}};
+  if (!sums) return c;
+  tiles = 0;
+  for (int i = 0; i < count; ++i) tiles += ceil_div(p[i].m, 128) * ceil_div(p[i].n, c.bn);
+  for (int i = 0; i < count; ++i) {
+    const int64_t most = ceil_div(p[i].k, kDepth) / 8, splits = 148 / tiles;
+    c.splits[i] = (int)(splits < most ? splits : most);
+    if (c.splits[i] < 1) c.splits[i] = 1;
+  }
+  return c;
 }
 
-template <int CG, int BN, int LAYOUT>
-int launch(Plan& t, cudaStream_t s) {
+int align_of(const void* p, int64_t ld) {
+  const uintptr_t a = reinterpret_cast<uintptr_t>(p) | (uintptr_t)(ld * 2);
+  return a % 32 == 0 ? 2 : a % 16 == 0 ? 1 : 0;
+}
+
+template <int CG, int BN>
+int launch(const Plan& t, int count, cudaStream_t s) {
   using S = Shape<CG, BN>;
-  CUtensorMap a, b;
-  const CxProduct& p = t.p;
-  int rc = LAYOUT == kTN ? make_map(&a, p.a, p.dtype, p.k, p.m, p.lda, kDepth) : make_map(&a, p.a, p.dtype, p.m, p.k, p.lda, 128);
+  CUtensorMap map[4] = {};
+  int rc = 0;
+  for (int i = 0; i < count && !rc; ++i) {
+    const CxProduct& p = t.job[i].p;
+    rc = p.layout == kTN ? make_map(&map[2 * i], p.a, p.dtype, p.k, p.m, p.lda, kDepth) : make_map(&map[2 * i], p.a, p.dtype, p.m, p.k, p.lda, 128);
+    if (!rc)
+      rc = p.layout == kNT ? make_map(&map[2 * i + 1], p.b, p.dtype, p.n, p.k, p.ldb, BN / CG)
+                           : make_map(&map[2 * i + 1], p.b, p.dtype, p.k, p.n, p.ldb, kDepth);
+  }
   if (rc) return rc;
-  rc = LAYOUT == kNT ? make_map(&b, p.b, p.dtype, p.n, p.k, p.ldb, BN / CG) : make_map(&b, p.b, p.dtype, p.k, p.n, p.ldb, kDepth);
-  if (rc) return rc;
-  static const int ready = (int)cudaFuncSetAttribute(tensor_product_kernel<CG, BN, LAYOUT>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes);
+  static const int ready = (int)cudaFuncSetAttribute(tensor_product_kernel<CG, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes);
   if (ready) return cx_set_error("cx_product", ready);
-  const int64_t units = (int64_t)t.tiles_m * t.tiles_n * t.splits, most = cx_sm_count() / CG;
+  // Who takes what: a unit lasts as long as its slices.  The first job's go round; the second one's are given out so
+  // that the last worker is done as early as can be.
+  Plan plan = t;
+  const int64_t units = (int64_t)t.job[0].units + t.job[1].units, most = cx_sm_count() / CG, workers = units < most ? units : most;
+  const int64_t a = t.job[0].units, b = t.job[1].units, la = t.job[0].slices_per, lb = t.job[1].slices_per;
+  const int64_t rounds = a / workers, extra = a % workers;
+  int64_t few = 0, many = 0;
+  while (extra * few + (workers - extra) * many < b) {
+    const int64_t end_few = (rounds + 1) * la + (few + 1) * lb, end_many = rounds * la + (many + 1) * lb;
+    if (end_many <= end_few || !extra) ++many;
+    else ++few;
+  }
+  plan.extra = (int)extra;
+  plan.few = (int)few;
+  plan.many = (int)many;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(CG * (units < most ? units : most)));
+  cfg.gridDim = dim3((unsigned)(CG * workers));
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = S::kBytes;
   cfg.stream = s;
@@ -519,65 +560,62 @@ int launch(Plan& t, cudaStream_t s) {
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = cx_pdl_enabled() ? 2 : 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, tensor_product_kernel<CG, BN, LAYOUT>, a, b, t);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, tensor_product_kernel<CG, BN>, map[0], map[1], map[2], map[3], plan);
   cx_note_launch();
   return e == cudaSuccess ? 0 : cx_set_error("cx_product", (int)e);
 }
 
-template <int CG, int BN>
-int launch_layout(Plan& t, cudaStream_t s) {
-  switch (t.p.layout) {
-    case kNT: return launch<CG, BN, kNT>(t, s);
-    case kNN: return launch<CG, BN, kNN>(t, s);
-    default: return launch<CG, BN, kTN>(t, s);
-  }
-}
-
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-
 }  // namespace
 
 bool cx_tensor_product_takes(const CxProduct& p) {
-  return p.dtype != CX_F32 && aligned16(p.a) && aligned16(p.b) && p.lda % 8 == 0 && p.ldb % 8 == 0;
+  return p.dtype != CX_F32 && ((reinterpret_cast<uintptr_t>(p.a) | reinterpret_cast<uintptr_t>(p.b)) & 15) == 0 && p.lda % 8 == 0 && p.ldb % 8 == 0;
 }
-int cx_tensor_product_stat_columns(const CxProduct& p) { return choose(p).bn / 2; }
-int64_t cx_tensor_product_workspace_bytes(const CxProduct& p) {
-  const Choice c = choose(p);
-  return c.splits > 1 ? c.splits * p.m * ((p.n + 7) / 8 * 8) * 4 : 0;
-}
+int cx_tensor_product_stat_columns(const CxProduct& p) { return choose(&p, 1).bn / 2; }
 
-int cx_tensor_product(const CxProduct& p, cudaStream_t s) {
-  const Choice c = choose(p);
+int cx_tensor_product(CxProduct* p, int count, cxprod::Arena& ws, cudaStream_t s) {
+  const Choice c = choose(p, count);
+  Plan t = {};
+  int64_t most = 0, units = 0;
+  // the longer units first
+  const bool swap = count == 2 && ceil_div(ceil_div(p[0].k, kDepth), c.splits[0]) < ceil_div(ceil_div(p[1].k, kDepth), c.splits[1]);
+  for (int i = 0; i < count; ++i) {
+    const int from = swap ? 1 - i : i;
+    Job& job = t.job[i];
+    const CxProduct& q = job.p = p[from];
+    const int64_t tm = ceil_div(q.m, 128 * c.cg), tn = ceil_div(q.n, c.bn);
+    job.slices = (int)ceil_div(q.k, kDepth);
+    job.slices_per = (int)ceil_div(job.slices, c.splits[from]);
+    job.splits = (int)ceil_div(job.slices, job.slices_per);
+    units += tm * tn * job.splits;
+    job.tiles_m = (int)tm;
+    job.tiles_n = (int)tn;
+    job.units = (int)(tm * tn * job.splits);
+    job.wide_out = align_of(q.out, q.ldo);
+    if (q.pre && align_of(q.pre, q.ldo) < job.wide_out) job.wide_out = align_of(q.pre, q.ldo);
+    job.wide_res = align_of(q.residual, q.ldr);
+    job.wide_bias = align_of(q.bias, 0);
+    if (job.splits > 1) {
+      job.part_ld = (q.n + 7) / 8 * 8;
+      job.partial = reinterpret_cast<float*>(ws.take((int64_t)job.splits * q.m * job.part_ld * 4));
+      const int64_t blocks = ceil_div(q.m * (job.part_ld / 8), kJoinThreads);
+      if (blocks > most) most = blocks;
+    }
+  }
+  if (!ws.base) return 0;
+  if (!ws.ok()) return cx_set_error("cx_product: workspace too small", 0);
+  if (units > 0x3FFFFFFF) return cx_set_error("cx_product: too many tiles", 0);
   uint32_t* said = status_word(true);
   if (!said) return cx_set_error("cx_product: no pinned memory for the status word", 0);
   if (*reinterpret_cast<volatile uint32_t*>(said)) {
     *reinterpret_cast<volatile uint32_t*>(said) = 0;
     return cx_set_error("cx_product: an earlier product gave up waiting, its results are not valid", 0);
   }
-  if (ceil_div(p.m, 128 * c.cg) * ceil_div(p.n, c.bn) > 0x7FFFFFFF / (c.splits + 1))
-    return cx_set_error("cx_product: too many tiles", 0);
-  Plan t = {};
-  t.p = p;
-  t.tiles_m = (int)ceil_div(p.m, 128 * c.cg);
-  t.tiles_n = (int)ceil_div(p.n, c.bn);
-  t.slices = (int)ceil_div(p.k, kDepth);
-  t.slices_per = (int)ceil_div(t.slices, c.splits);
-  t.splits = (int)ceil_div(t.slices, t.slices_per);
   t.status = status_word(false);
-  t.wide_out = aligned16(p.out) && aligned16(p.pre) && p.ldo % 8 == 0;
-  t.wide_add = aligned16(p.addend) && p.n % 4 == 0;
-  t.wide_res = aligned16(p.residual) && p.ldr % 8 == 0;
-  t.wide_bias = aligned16(p.bias);
-  if (t.splits > 1) {
-    if (p.ws_bytes < cx_tensor_product_workspace_bytes(p)) return cx_set_error("cx_product: workspace too small", 0);
-    t.partial = reinterpret_cast<float*>(p.workspace);
-    t.part_ld = (p.n + 7) / 8 * 8;
-  }
-  int rc = c.cg == 2 ? launch_layout<2, 256>(t, s) : c.bn == 128 ? launch_layout<1, 128>(t, s) : launch_layout<1, 64>(t, s);
-  if (rc || t.splits == 1) return rc;
-  const int grid = (int)ceil_div(p.m * (t.part_ld / 8), kJoinThreads);
-  if (p.dtype == CX_BF16) cx_launch_pdl2(join_splits_kernel<__nv_bfloat16>, dim3(grid), kJoinThreads, s, t);
-  else cx_launch_pdl2(join_splits_kernel<__half>, dim3(grid), kJoinThreads, s, t);
+  const int rc = c.cg == 2 ? launch<2, 256>(t, count, s) : c.bn == 128 ? launch<1, 128>(t, count, s) : launch<1, 64>(t, count, s);
+  if (rc || !most) return rc;
+  const dim3 grid((unsigned)most, (unsigned)count);
+  if (p[0].dtype == CX_BF16) cx_launch_pdl2(join_splits_kernel<__nv_bfloat16>, grid, kJoinThreads, s, t);
+  else cx_launch_pdl2(join_splits_kernel<__half>, grid, kJoinThreads, s, t);
   cx_note_launch();
   return cx_check_launch("cx_product");
 }

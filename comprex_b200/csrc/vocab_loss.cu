@@ -167,7 +167,7 @@ int forward(const CxVocabLoss& l, cxprod::Arena& ws, cudaStream_t s) {
   p.part = reinterpret_cast<float2*>(ws.take(tiles * l.rows * 8));
   p.target_logit = reinterpret_cast<float*>(ws.take(l.rows * 4));
   float* row_loss = l.reduction == CX_REDUCE_NONE ? l.loss : reinterpret_cast<float*>(ws.take(l.rows * 4));
-  rc = cx_product(p, ws, s);
+  rc = cx_product(&p, 1, ws, s);
   if (rc || !ws.base) return rc;
   const Join j = {p.part, p.target_logit, l.targets, l.rows, tiles, l.vocab, l.ignore_index, l.lse, row_loss};
   cx_launch_pdl2(join_kernel, dim3((unsigned)((l.rows + 31) / 32)), kThreads, s, j);
@@ -191,7 +191,8 @@ int backward(const CxVocabLoss& l, cxprod::Arena& ws, cudaStream_t s) {
   if (piece < 256) piece = 256;
   if (piece > (l.vocab + 7) / 8 * 8) piece = (l.vocab + 7) / 8 * 8;
   void* prob = ws.take(l.rows * piece * size);
-  float* sums = l.dh && piece < l.vocab ? reinterpret_cast<float*>(ws.take(l.rows * l.dim * 4)) : nullptr;
+  const int64_t sums_ld = (l.dim + 7) / 8 * 8;
+  float* sums = l.dh && piece < l.vocab ? reinterpret_cast<float*>(ws.take(l.rows * sums_ld * 4)) : nullptr;
   Factors f = {l.grad, l.targets, l.lse, l.count, l.rows, l.grad_stride, l.ignore_index, l.reduction, nullptr, nullptr, nullptr};
   f.lse2 = reinterpret_cast<float*>(ws.take(l.rows * 4));
   f.factor = reinterpret_cast<float*>(ws.take(l.rows * 4));
@@ -214,24 +215,25 @@ int backward(const CxVocabLoss& l, cxprod::Arena& ws, cudaStream_t s) {
     p.a = h; p.lda = ldh; p.b = at; p.ldb = ldw;
     p.layout = kNT; p.mode = kProb; p.dtype = l.dtype;
     p.out = prob; p.ldo = piece; p.targets = l.targets; p.col0 = v0; p.lse = f.lse2; p.row_factor = f.factor;
-    rc = cx_product(p, ws, s);
-    if (l.dh && !rc) {
-      CxProduct q = {};
+    rc = cx_product(&p, 1, ws, s);
+    CxProduct both[2] = {};
+    int count = 0;
+    if (l.dh) {
+      CxProduct& q = both[count++];
       q.m = l.rows; q.n = l.dim; q.k = n;
       q.a = prob; q.lda = piece; q.b = at; q.ldb = ldw;
-      q.layout = kNN; q.dtype = l.dtype; q.addend = sums; q.has_addend = v0 > 0; q.scale = f.scale;
+      q.layout = kNN; q.dtype = l.dtype; q.addend = sums; q.ldadd = sums_ld; q.has_addend = v0 > 0; q.scale = f.scale;
       q.mode = v0 + n < l.vocab ? kSums : kOut;
       q.out = l.dh; q.ldo = l.dim;
-      rc = cx_product(q, ws, s);
     }
-    if (l.dw && !rc) {
-      CxProduct q = {};
+    if (l.dw) {
+      CxProduct& q = both[count++];
       q.m = n; q.n = l.dim; q.k = l.rows;
       q.a = prob; q.lda = piece; q.b = h; q.ldb = ldh;
       q.layout = kTN; q.dtype = l.dtype; q.scale = f.scale;
       q.out = reinterpret_cast<char*>(l.dw) + v0 * l.dim * size; q.ldo = l.dim;
-      rc = cx_product(q, ws, s);
     }
+    if (!rc) rc = cx_product(both, count, ws, s);
     if (ws.used > most) most = ws.used;
   }
   ws.used = most;
