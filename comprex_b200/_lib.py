@@ -264,6 +264,10 @@ def host():
         loader = importlib.machinery.ExtensionFileLoader("_cxhost", path)
         mod = importlib.util.module_from_spec(importlib.util.spec_from_loader("_cxhost", loader))
         loader.exec_module(mod)
+        lib = load()
+        mod.bind_operators(ComprexError, *(C.cast(getattr(lib, f), C.c_void_p).value for f in (
+            "cx_linear_workspace_bytes", "cx_linear_forward", "cx_linear_backward", "cx_vocab_loss_workspace_bytes",
+            "cx_vocab_loss_forward", "cx_vocab_loss_backward", "cx_last_error")))
         _host_mod = mod
     return _host_mod
 

@@ -77,18 +77,27 @@ def _build_host(verbose: bool) -> None:
     import sysconfig
     import torch
     from torch.utils.cpp_extension import include_paths, library_paths
-    src = CSRC / "python" / "host.cpp"
-    if not _stale(HOST, [src, CSRC / "cx_common.h", Path(__file__)]):
+    srcs = sorted((CSRC / "python").glob("*.cpp"))
+    headers = list((CSRC / "python").glob("*.h")) + list(CSRC.glob("*.h")) + [Path(__file__)]
+    if not _stale(HOST, srcs + headers):
         return
-    cmd = ([os.environ.get("CXX", "g++"), "-shared"] + CXX_FLAGS
-           + [f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
-           + [f"-I{d}" for d in include_paths() + [sysconfig.get_paths()["include"]]] + [str(src), "-o", str(HOST)]
-           + [f"-L{d}" for d in library_paths()] + ["-ltorch_python", "-ltorch_cpu", "-lc10"])
-    if verbose:
-        print(" ".join(cmd), flush=True)
-    res = subprocess.run(cmd, capture_output=True, text=True)
-    if res.returncode != 0:
-        raise RuntimeError(f"compiling {src.name} failed:\n{res.stdout}\n{res.stderr}")
+    flags = (CXX_FLAGS + [f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+             + [f"-I{d}" for d in include_paths() + [sysconfig.get_paths()["include"]]])
+
+    def run(cmd, what):
+        if verbose:
+            print(" ".join(cmd), flush=True)
+        res = subprocess.run(cmd, capture_output=True, text=True)
+        if res.returncode != 0:
+            raise RuntimeError(f"compiling {what} failed:\n{res.stdout}\n{res.stderr}")
+
+    cxx = os.environ.get("CXX", "g++")
+    objs = [OBJDIR / ("python_" + src.name + ".o") for src in srcs]
+    for src, obj in zip(srcs, objs):
+        if _stale(obj, [src] + headers):
+            run([cxx] + flags + ["-c", str(src), "-o", str(obj)], src.name)
+    run([cxx, "-shared"] + [str(o) for o in objs] + ["-o", str(HOST)] + [f"-L{d}" for d in library_paths()]
+        + ["-ltorch_python", "-ltorch_cpu", "-lc10"], HOST.name)
 
 
 def build(verbose: bool = False, force: bool = False, ptxas_v: bool = False) -> Path:

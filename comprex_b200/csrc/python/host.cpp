@@ -5,7 +5,8 @@
 //  * addresses: those of the tensors themselves,
 //  * run_vector: the launches of one message of a prepared connection.  Checks of the vector,
 //    descriptors and native calls took 20 us per exchange in Python, the kernels of a 64 k-element
-//    exchange take 15 us.
+//    exchange take 15 us,
+//  * linear, vocab_loss: the operators of operators.cpp.
 // Tensors of unusual kinds (nested, sparse, wrapped by a transform) throw at the questions asked here.  No
 // exception may leave these functions: such a tensor is not the plain case, and the caller's general path
 // says what is wrong with it.
@@ -14,6 +15,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include "../cx_common.h"
+#include "operators.h"
 
 namespace {
 
@@ -213,6 +215,9 @@ PyMethodDef methods[] = {{"collect", collect, METH_VARARGS, nullptr},
                           METH_FASTCALL, nullptr},
                          {"install", install, METH_O, nullptr},
                          {"scalar_type", scalar_type, METH_O, nullptr},
+                         {"linear", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(cx_py_linear)), METH_FASTCALL, nullptr},
+                         {"vocab_loss", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(cx_py_vocab_loss)), METH_FASTCALL, nullptr},
+                         {"bind_operators", cx_py_bind_operators, METH_VARARGS, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_cxhost", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

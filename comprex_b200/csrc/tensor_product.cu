@@ -15,7 +15,6 @@ constexpr int kThreads = 384;            // warp 0 copies, warp 1 multiplies, wa
 constexpr int kFinish = 8;               // finishing warps: four have the left half of a tile's columns, four the right one
 constexpr int kJoinThreads = 256;
 constexpr int kShared = 232448;          // of a CTA
-constexpr int kGroup = 8;                // tiles along m that are walked together: their operands stay in L2
 
 template <int CG, int BN>
 struct Shape {
@@ -30,6 +29,7 @@ struct Shape {
 struct Job {
   CxProduct p;
   int tiles_m, tiles_n, units;
+  int group;                   // tiles along m that are walked together, column of tiles after column
   int slices, slices_per;      // of kDepth along k: all, and per split
   float* partial;              // sums of the splits: [split][m][part_ld]
   int64_t part_ld;
@@ -70,8 +70,8 @@ __device__ __forceinline__ Unit unit_of(const Job& t, int u) {
   Unit r;
   const int tiles = t.tiles_m * t.tiles_n;
   r.split = u / tiles;
-  const int tile = u - r.split * tiles, per = kGroup * t.tiles_n, first = tile / per * kGroup;
-  const int rows = min(kGroup, t.tiles_m - first), in = tile % per;
+  const int tile = u - r.split * tiles, per = t.group * t.tiles_n, first = tile / per * t.group;
+  const int rows = min(t.group, t.tiles_m - first), in = tile % per;
   r.tm = first + in % rows;
   r.tn = in / rows;
   r.s0 = r.split * t.slices_per;
@@ -517,6 +517,30 @@ int align_of(const void* p, int64_t ld) {
   return a % 32 == 0 ? 2 : a % 16 == 0 ? 1 : 0;
 }
 
+// Who takes what: a unit lasts as long as its slices.  The first job's `a` units go round the workers, the second one's
+// are given out so that the last worker is done as early as can be; returns that time.
+int64_t share_out(int64_t a, int64_t la, int64_t b, int64_t lb, int64_t workers, int* extra, int* few, int* many) {
+  const int64_t rounds = a / workers, more = a % workers, base = b * lb / workers / (lb ? lb : 1);
+  int64_t f = 0, m = 0;
+  // with one first unit more a worker takes la / lb fewer of the others: start below that and add the cheapest one
+  if (base > 4) {
+    const int64_t gap = lb ? la / lb + 2 : 0;
+    m = base - 4;
+    f = m > gap ? m - gap : 0;
+    while (m > 0 && more * f + (workers - more) * m > b) --m;
+  }
+  while (more * f + (workers - more) * m < b) {
+    const int64_t end_few = (rounds + 1) * la + (f + 1) * lb, end_many = rounds * la + (m + 1) * lb;
+    if (!more || end_many <= end_few) ++m;
+    else ++f;
+  }
+  *extra = (int)more;
+  *few = (int)f;
+  *many = (int)m;
+  const int64_t t_few = more ? (rounds + 1) * la + f * lb : 0, t_many = rounds * la + m * lb;
+  return t_few > t_many ? t_few : t_many;
+}
+
 template <int CG, int BN>
 int launch(const Plan& t, int count, cudaStream_t s) {
   using S = Shape<CG, BN>;
@@ -532,21 +556,9 @@ int launch(const Plan& t, int count, cudaStream_t s) {
   if (rc) return rc;
   static const int ready = (int)cudaFuncSetAttribute(tensor_product_kernel<CG, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes);
   if (ready) return cx_set_error("cx_product", ready);
-  // Who takes what: a unit lasts as long as its slices.  The first job's go round; the second one's are given out so
-  // that the last worker is done as early as can be.
   Plan plan = t;
   const int64_t units = (int64_t)t.job[0].units + t.job[1].units, most = cx_sm_count() / CG, workers = units < most ? units : most;
-  const int64_t a = t.job[0].units, b = t.job[1].units, la = t.job[0].slices_per, lb = t.job[1].slices_per;
-  const int64_t rounds = a / workers, extra = a % workers;
-  int64_t few = 0, many = 0;
-  while (extra * few + (workers - extra) * many < b) {
-    const int64_t end_few = (rounds + 1) * la + (few + 1) * lb, end_many = rounds * la + (many + 1) * lb;
-    if (end_many <= end_few || !extra) ++many;
-    else ++few;
-  }
-  plan.extra = (int)extra;
-  plan.few = (int)few;
-  plan.many = (int)many;
+  share_out(t.job[0].units, t.job[0].slices_per, t.job[1].units, t.job[1].slices_per, workers, &plan.extra, &plan.few, &plan.many);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(CG * workers));
   cfg.blockDim = dim3(kThreads);
@@ -570,6 +582,20 @@ int launch(const Plan& t, int count, cudaStream_t s) {
 bool cx_tensor_product_takes(const CxProduct& p) {
   return p.dtype != CX_F32 && ((reinterpret_cast<uintptr_t>(p.a) | reinterpret_cast<uintptr_t>(p.b)) & 15) == 0 && p.lda % 8 == 0 && p.ldb % 8 == 0;
 }
+double cx_tensor_product_time(const CxProduct* p, int count) {
+  const Choice c = choose(p, count);
+  int64_t units[2] = {}, slices[2] = {}, all = 0;
+  const bool swap = count == 2 && ceil_div(ceil_div(p[0].k, kDepth), c.splits[0]) < ceil_div(ceil_div(p[1].k, kDepth), c.splits[1]);
+  for (int i = 0; i < count; ++i) {
+    const CxProduct& q = p[swap ? 1 - i : i];
+    slices[i] = ceil_div(ceil_div(q.k, kDepth), c.splits[swap ? 1 - i : i]);
+    units[i] = ceil_div(q.m, 128 * c.cg) * ceil_div(q.n, c.bn) * c.splits[swap ? 1 - i : i];
+    all += units[i];
+  }
+  int extra, few, many;
+  const int64_t most = cx_sm_count() / c.cg;
+  return (double)share_out(units[0], slices[0], units[1], slices[1], all < most ? all : most, &extra, &few, &many) + 12.0;
+}
 int cx_tensor_product_stat_columns(const CxProduct& p) { return choose(&p, 1).bn / 2; }
 
 int cx_tensor_product(CxProduct* p, int count, cxprod::Arena& ws, cudaStream_t s) {
@@ -590,6 +616,11 @@ int cx_tensor_product(CxProduct* p, int count, cxprod::Arena& ws, cudaStream_t s
     job.tiles_m = (int)tm;
     job.tiles_n = (int)tn;
     job.units = (int)(tm * tn * job.splits);
+    // The rows of A that a group walks with stay in L2 while B goes by once: as many as take 32 MB, or where k is long
+    // about as many rows as columns at a time.  (8192 x 50257 x 1024, 8 / 16 rows of tiles: 700 / 684 us; 8192^3,
+    // 4 / 8 / 16: 877 / 855 / 881 us.)
+    const int64_t fit = (32ll << 20) / (q.k * 2 * 128 * c.cg);
+    job.group = (int)(fit < 8 ? 8 : fit < tm ? fit : tm);
     job.wide_out = align_of(q.out, q.ldo);
     if (q.pre && align_of(q.pre, q.ldo) < job.wide_out) job.wide_out = align_of(q.pre, q.ldo);
     job.wide_res = align_of(q.residual, q.ldr);

@@ -14,7 +14,7 @@
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int64_t kPieceBytes = 64ll << 20;
+constexpr int64_t kPieceBytes = 288ll << 20;
 
 struct Join {
   const float2* part;
@@ -180,6 +180,68 @@ int forward(const CxVocabLoss& l, cxprod::Arena& ws, cudaStream_t s) {
   return cx_check_launch("cx_vocab_loss_forward");
 }
 
+// The products of a piece of the vocabulary, [v0, v0 + n): its probabilities, and what they give to the gradients.
+struct Piece {
+  CxProduct prob, both[2];
+  int count;
+  Piece(const CxVocabLoss& l, const void* h, int64_t ldh, const void* w, int64_t ldw, int64_t v0, int64_t n, void* p, int64_t ldp) : prob(), both(), count(0) {
+    const int64_t size = l.dtype == CX_F32 ? 4 : 2;
+    const void* at = reinterpret_cast<const char*>(w) + v0 * ldw * size;
+    prob.m = l.rows; prob.n = n; prob.k = l.dim;
+    prob.a = h; prob.lda = ldh; prob.b = at; prob.ldb = ldw;
+    prob.layout = kNT; prob.mode = kProb; prob.dtype = l.dtype;
+    prob.out = p; prob.ldo = ldp; prob.targets = l.targets; prob.col0 = v0;
+    if (l.dh) {
+      CxProduct& q = both[count++];
+      q.m = l.rows; q.n = l.dim; q.k = n;
+      q.a = p; q.lda = ldp; q.b = at; q.ldb = ldw;
+      q.layout = kNN; q.dtype = l.dtype; q.has_addend = v0 > 0;
+      q.mode = v0 + n < l.vocab ? kSums : kOut;
+      q.out = l.dh; q.ldo = l.dim;
+    }
+    if (l.dw) {
+      CxProduct& q = both[count++];
+      q.m = n; q.n = l.dim; q.k = l.rows;
+      q.a = p; q.lda = ldp; q.b = h; q.ldb = ldh;
+      q.layout = kTN; q.dtype = l.dtype;
+      q.out = reinterpret_cast<char*>(l.dw) + v0 * l.dim * size; q.ldo = l.dim;
+    }
+  }
+};
+
+// Columns of a piece.  A piece that fits in L2 with its operands saves its trip to memory, but what bounds the products
+// is how their tiles fill the GPU: of the sizes up to kPieceBytes the one whose tiles leave the least of it idle
+// (8192 rows of width 1024, vocabulary 50257: ...).
+int64_t piece_columns(const CxVocabLoss& l) {
+  const int64_t size = l.dtype == CX_F32 ? 4 : 2, whole = (l.vocab + 7) / 8 * 8;
+  int64_t most = kPieceBytes / (l.rows * size) / 256 * 256;
+  if (most < 256) most = 256;
+  if (whole <= most && l.rows * whole * size <= kPieceBytes / 4) return whole;
+  if (l.dtype == CX_F32) return whole < most ? whole : most;
+  int64_t best = whole < most ? whole : most;
+  double least = 1e30;
+  const int64_t fewest = (l.vocab + most - 1) / most;
+  for (int64_t pieces = fewest; pieces < fewest + 4; ++pieces)
+    for (int64_t more = 0; more < 6; ++more) {
+      int64_t n = ((l.vocab + pieces - 1) / pieces + 255) / 256 * 256 + (more - 2) * 256;
+      if (n > whole) n = whole;
+      if (n < 256 || n > most) continue;
+      double time = 0;
+      const int64_t full = l.vocab / n, rest = l.vocab % n;
+      const Piece a(l, nullptr, 8, nullptr, 8, 0, n, nullptr, 8);
+      time += full * (cx_tensor_product_time(&a.prob, 1) + cx_tensor_product_time(a.both, a.count));
+      if (rest) {
+        const Piece b(l, nullptr, 8, nullptr, 8, 0, rest, nullptr, 8);
+        time += cx_tensor_product_time(&b.prob, 1) + cx_tensor_product_time(b.both, b.count);
+      }
+      if (time < least) {
+        least = time;
+        best = n;
+      }
+    }
+  return best;
+}
+
 int backward(const CxVocabLoss& l, cxprod::Arena& ws, cudaStream_t s) {
   const int64_t size = l.dtype == CX_F32 ? 4 : 2;
   const void *h = l.h, *w = l.w;
@@ -187,10 +249,9 @@ int backward(const CxVocabLoss& l, cxprod::Arena& ws, cudaStream_t s) {
   int rc = cx_product_operand(&h, &ldh, l.dtype, l.rows, l.dim, ws, s);
   if (!rc) rc = cx_product_operand(&w, &ldw, l.dtype, l.vocab, l.dim, ws, s);
   if (rc) return rc;
-  int64_t piece = kPieceBytes / (l.rows * size) / 256 * 256;
-  if (piece < 256) piece = 256;
-  if (piece > (l.vocab + 7) / 8 * 8) piece = (l.vocab + 7) / 8 * 8;
-  void* prob = ws.take(l.rows * piece * size);
+  const int64_t piece = piece_columns(l);
+  const int64_t ldp = (piece + 63) / 64 * 64;          // whole lines
+  void* prob = ws.take(l.rows * ldp * size);
   const int64_t sums_ld = (l.dim + 7) / 8 * 8;
   float* sums = l.dh && piece < l.vocab ? reinterpret_cast<float*>(ws.take(l.rows * sums_ld * 4)) : nullptr;
   Factors f = {l.grad, l.targets, l.lse, l.count, l.rows, l.grad_stride, l.ignore_index, l.reduction, nullptr, nullptr, nullptr};
@@ -207,33 +268,19 @@ int backward(const CxVocabLoss& l, cxprod::Arena& ws, cudaStream_t s) {
   const int64_t begin = ws.used;               // what the products need is used again by the next piece
   int64_t most = begin;
   for (int64_t v0 = 0; v0 < l.vocab && !rc; v0 += piece) {
-    const int64_t n = piece < l.vocab - v0 ? piece : l.vocab - v0;
-    const char* at = reinterpret_cast<const char*>(w) + v0 * ldw * size;
     ws.used = begin;
-    CxProduct p = {};
-    p.m = l.rows; p.n = n; p.k = l.dim;
-    p.a = h; p.lda = ldh; p.b = at; p.ldb = ldw;
-    p.layout = kNT; p.mode = kProb; p.dtype = l.dtype;
-    p.out = prob; p.ldo = piece; p.targets = l.targets; p.col0 = v0; p.lse = f.lse2; p.row_factor = f.factor;
-    rc = cx_product(&p, 1, ws, s);
-    CxProduct both[2] = {};
-    int count = 0;
-    if (l.dh) {
-      CxProduct& q = both[count++];
-      q.m = l.rows; q.n = l.dim; q.k = n;
-      q.a = prob; q.lda = piece; q.b = at; q.ldb = ldw;
-      q.layout = kNN; q.dtype = l.dtype; q.addend = sums; q.ldadd = sums_ld; q.has_addend = v0 > 0; q.scale = f.scale;
-      q.mode = v0 + n < l.vocab ? kSums : kOut;
-      q.out = l.dh; q.ldo = l.dim;
+    Piece p(l, h, ldh, w, ldw, v0, piece < l.vocab - v0 ? piece : l.vocab - v0, prob, ldp);
+    p.prob.lse = f.lse2;
+    p.prob.row_factor = f.factor;
+    for (int i = 0; i < p.count; ++i) {
+      p.both[i].scale = f.scale;
+      if (p.both[i].layout == kNN) {
+        p.both[i].addend = sums;
+        p.both[i].ldadd = sums_ld;
+      }
     }
-    if (l.dw) {
-      CxProduct& q = both[count++];
-      q.m = n; q.n = l.dim; q.k = l.rows;
-      q.a = prob; q.lda = piece; q.b = h; q.ldb = ldh;
-      q.layout = kTN; q.dtype = l.dtype; q.scale = f.scale;
-      q.out = reinterpret_cast<char*>(l.dw) + v0 * l.dim * size; q.ldo = l.dim;
-    }
-    if (!rc) rc = cx_product(both, count, ws, s);
+    rc = cx_product(&p.prob, 1, ws, s);
+    if (!rc) rc = cx_product(p.both, p.count, ws, s);
     if (ws.used > most) most = ws.used;
   }
   ws.used = most;
