@@ -26,10 +26,25 @@ struct Shape {
   static constexpr int kColumns = 2 * BN;
 };
 
+// Division of numbers below 2^31 by a number that is known at launch: n / d = n m >> (31 + l), l = ceil(log2 d), m =
+// ceil(2^(31 + l) / d).
+struct Divisor {
+  uint32_t d, m, shift;
+  void set(uint32_t by) {
+    d = by;
+    shift = 0;
+    while ((1ull << shift) < by) ++shift;
+    m = (uint32_t)(((1ull << (31 + shift)) + by - 1) / by);
+    shift += 31;
+  }
+  __device__ __forceinline__ int of(int n) const { return (int)(((uint64_t)(uint32_t)n * m) >> shift); }
+};
+
 struct Job {
   CxProduct p;
   int tiles_m, tiles_n, units;
-  int group;                   // tiles along m that are walked together, column of tiles after column
+  Divisor tiles, per, group, last;   // tiles; tiles of a group: `group` rows of tiles (the last one: `last`) are walked
+                                     // together, column after column
   int slices, slices_per;      // of kDepth along k: all, and per split
   float* partial;              // sums of the splits: [split][m][part_ld]
   int64_t part_ld;
@@ -68,12 +83,11 @@ struct Unit {
 };
 __device__ __forceinline__ Unit unit_of(const Job& t, int u) {
   Unit r;
-  const int tiles = t.tiles_m * t.tiles_n;
-  r.split = u / tiles;
-  const int tile = u - r.split * tiles, per = t.group * t.tiles_n, first = tile / per * t.group;
-  const int rows = min(t.group, t.tiles_m - first), in = tile % per;
-  r.tm = first + in % rows;
-  r.tn = in / rows;
+  r.split = t.tiles.of(u);
+  const int tile = u - r.split * (int)t.tiles.d, g = t.per.of(tile), in = tile - g * (int)t.per.d, first = g * (int)t.group.d;
+  const Divisor& rows = first + (int)t.group.d <= t.tiles_m ? t.group : t.last;
+  r.tn = rows.of(in);
+  r.tm = first + in - r.tn * (int)rows.d;
   r.s0 = r.split * t.slices_per;
   r.s1 = min(t.slices, r.s0 + t.slices_per);
   return r;
@@ -161,46 +175,72 @@ __device__ __forceinline__ void add_sums(const float* at, int left, float (&v)[W
     }
 }
 
-// What is done to the sums (kOut, kSums) of W columns of a row.  `scale`: what p.scale holds; `bias`: in shared memory, or NULL where it is read from
-// the operand.
-template <typename T, int W>
-__device__ __forceinline__ void finish(const Job& t, int64_t row, int64_t col, float (&v)[W], float scale, const float* bias) {
-  const CxProduct& p = t.p;
-  const int left = (int)min((int64_t)W, p.n - col);
-  if (p.has_addend) add_sums(p.addend + row * p.ldadd + col, left, v);
-  if (p.mode == kSums) return store_sums(p.addend + row * p.ldadd + col, left, v);
-  if (p.scale) {
-#pragma unroll
-    for (int i = 0; i < W; ++i) v[i] *= scale;
+// What is done to the sums of a row (kOut, kSums), from column `col` on: everything that the descriptor says, in registers.
+// (Read from the descriptor for each 16 columns it took 880 cycles for them.)
+template <typename T>
+struct Row {
+  T *out, *pre;
+  const T *residual, *bias;
+  float* addend;
+  float scale;
+  int left, act, wide_out, wide_res, wide_bias;
+  bool add, sums, scaled;
+  __device__ __forceinline__ Row(const Job& t, int64_t row, int64_t col) {
+    const CxProduct& p = t.p;
+    out = reinterpret_cast<T*>(p.out) + row * p.ldo + col;
+    pre = p.pre ? reinterpret_cast<T*>(p.pre) + row * p.ldo + col : nullptr;
+    residual = p.residual ? reinterpret_cast<const T*>(p.residual) + row * p.ldr + col : nullptr;
+    bias = p.bias ? reinterpret_cast<const T*>(p.bias) + col : nullptr;
+    addend = p.addend + row * p.ldadd + col;
+    scaled = p.scale != nullptr;
+    scale = scaled ? *p.scale : 1.f;
+    left = (int)min((int64_t)0x40000000, p.n - col);
+    act = p.act;
+    wide_out = t.wide_out;
+    wide_res = t.wide_res;
+    wide_bias = t.wide_bias;
+    add = p.has_addend;
+    sums = p.mode == kSums;
   }
-  if (p.bias) {
-    if (bias) {
+  // W columns, `c` further on; `shared`: their biases in shared memory, or NULL where they are read from the operand
+  template <int W>
+  __device__ __forceinline__ void finish(int c, float (&v)[W], const float* shared) const {
+    const int have = left - c;
+    if (add) add_sums(addend + c, have, v);
+    if (sums) return store_sums(addend + c, have, v);
+    if (scaled) {
 #pragma unroll
-      for (int i = 0; i < W / 4; ++i) {
-        const float4 b = reinterpret_cast<const float4*>(bias)[i];
-        v[4 * i] += b.x, v[4 * i + 1] += b.y, v[4 * i + 2] += b.z, v[4 * i + 3] += b.w;
-      }
-    } else {
-      add_row(reinterpret_cast<const T*>(p.bias) + col, t.wide_bias, left, v);
+      for (int i = 0; i < W; ++i) v[i] *= scale;
     }
-  }
-  if (p.pre) store_row(reinterpret_cast<T*>(p.pre) + row * p.ldo + col, t.wide_out, left, v);
-  cxprod::activate(v, p.act);
-  if (p.residual) add_row(reinterpret_cast<const T*>(p.residual) + row * p.ldr + col, t.wide_res, left, v);
-  store_row(reinterpret_cast<T*>(p.out) + row * p.ldo + col, t.wide_out, left, v);
-}
-
-// A finishing warp's part of a tile: 32 rows, one per lane, WIDTH columns from col0 on.  The next 32 columns come from
-// the tensor memory while these are worked on.
-template <typename T, int WIDTH, typename F>
-__device__ __forceinline__ void each32(uint32_t tmem, int64_t left, const F& work) {
-  uint32_t r[2][32];
-  cxt::tmem_load32(tmem, r[0]);
+    if (bias) {
+      if (shared) {
 #pragma unroll
-  for (int c = 0; c < WIDTH; c += 32) {
-    cxt::tmem_load_wait(r[(c / 32) % 2]);
-    if (c + 32 < WIDTH) cxt::tmem_load32(tmem + c + 32, r[(c / 32 + 1) % 2]);
-    if (c < left) work(c, reinterpret_cast<float(&)[32]>(r[(c / 32) % 2]));
+        for (int i = 0; i < W / 4; ++i) {
+          const float4 b = reinterpret_cast<const float4*>(shared)[i];
+          v[4 * i] += b.x, v[4 * i + 1] += b.y, v[4 * i + 2] += b.z, v[4 * i + 3] += b.w;
+        }
+      } else {
+        add_row(bias + c, wide_bias, have, v);
+      }
+    }
+    if (pre) store_row(pre + c, wide_out, have, v);
+    cxprod::activate(v, act);
+    if (residual) add_row(residual + c, wide_res, have, v);
+    store_row(out + c, wide_out, have, v);
+  }
+};
+
+// A finishing warp's part of a tile: 32 rows, one per lane, WIDTH columns from col0 on, 16 at a time.  The loops are not
+// unrolled: instructions of a tile that are fetched once per tile cost more than they do (one unrolled 32 columns at a
+// time took 1600 cycles for each 32).
+template <int WIDTH, typename F>
+__device__ __forceinline__ void each16(uint32_t tmem, int64_t left, const F& work) {
+#pragma unroll 1
+  for (int c = 0; c < WIDTH && c < left; c += 16) {
+    uint32_t r[16];
+    cxt::tmem_load16(tmem + c, r);
+    cxt::tmem_load_wait(r);
+    work(c, reinterpret_cast<float(&)[16]>(r));
   }
 }
 
@@ -214,26 +254,26 @@ __device__ __forceinline__ void finish_part(const Job& t, const Unit& u, int hal
   if (p.mode == kStats) {
     const int64_t hot = (in ? p.targets[row] : -1) - p.col0 - col0;      // where the row's target is in this part
     float top = -INFINITY, sum = 0.f;
-    each32<T, WIDTH>(tmem, left, [&](int c, float(&v)[32]) {
-      if (c + 32 > left) {
+    each16<WIDTH>(tmem, left, [&](int c, float(&v)[16]) {
+      if (c + 16 > left) {
 #pragma unroll
-        for (int j = 0; j < 32; ++j)
+        for (int j = 0; j < 16; ++j)
           if (c + j >= left) v[j] = -INFINITY;
       }
-      if (hot >= c && hot < c + 32) {
+      if (hot >= c && hot < c + 16) {
         float x = 0.f;
 #pragma unroll
-        for (int j = 0; j < 32; ++j)
+        for (int j = 0; j < 16; ++j)
           if (hot == c + j) x = v[j];
         p.target_logit[row] = x;
       }
       float m[4] = {top, top, top, top}, add[4] = {};
 #pragma unroll
-      for (int j = 0; j < 32; ++j) m[j % 4] = fmaxf(m[j % 4], v[j]);
+      for (int j = 0; j < 16; ++j) m[j % 4] = fmaxf(m[j % 4], v[j]);
       m[0] = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
       const float base = (m[0] == -INFINITY ? 0.f : m[0]) * cxprod::kLog2e;
 #pragma unroll
-      for (int j = 0; j < 32; ++j) add[j % 4] += cxprod::pow2(__fmaf_rn(v[j], cxprod::kLog2e, -base));
+      for (int j = 0; j < 16; ++j) add[j % 4] += cxprod::pow2(__fmaf_rn(v[j], cxprod::kLog2e, -base));
       sum = sum * cxprod::pow2(__fmaf_rn(top, cxprod::kLog2e, -base)) + ((add[0] + add[1]) + (add[2] + add[3]));   // (top = -inf: 0)
       top = m[0];
     });
@@ -242,29 +282,30 @@ __device__ __forceinline__ void finish_part(const Job& t, const Unit& u, int hal
     const float lse = in ? p.lse[row] : 0.f, factor = in ? p.row_factor[row] : 0.f;
     const int64_t hot = in ? p.targets[row] - p.col0 - col0 : -1;
     T* out = reinterpret_cast<T*>(p.out) + row * p.ldo + col0;
-    each32<T, WIDTH>(tmem, left, [&](int c, float(&v)[32]) {
+    const int wide = t.wide_out;
+    each16<WIDTH>(tmem, left, [&](int c, float(&v)[16]) {
 #pragma unroll
-      for (int j = 0; j < 32; ++j) v[j] = cxprod::pow2(__fmaf_rn(v[j], cxprod::kLog2e, -lse)) * factor;
-      if (hot >= c && hot < c + 32) {
+      for (int j = 0; j < 16; ++j) v[j] = cxprod::pow2(__fmaf_rn(v[j], cxprod::kLog2e, -lse)) * factor;
+      if (hot >= c && hot < c + 16) {
 #pragma unroll
-        for (int j = 0; j < 32; ++j)
+        for (int j = 0; j < 16; ++j)
           if (hot == c + j) v[j] -= factor;
       }
       if (factor == 0.f) {                 // a row that does not count, whatever its logits are
 #pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] = 0.f;
+        for (int j = 0; j < 16; ++j) v[j] = 0.f;
       }
-      if (in) store_row(out + c, t.wide_out, (int)min((int64_t)32, left - c), v);
+      if (in) store_row(out + c, wide, (int)min((int64_t)16, left - c), v);
     });
   } else if (t.partial) {
     float* at = t.partial + ((int64_t)u.split * p.m + row) * t.part_ld + col0;
-    each32<T, WIDTH>(tmem, left, [&](int c, float(&v)[32]) {
-      if (in) store_sums(at + c, (int)min((int64_t)32, left - c), v);
+    each16<WIDTH>(tmem, left, [&](int c, float(&v)[16]) {
+      if (in) store_sums(at + c, (int)min((int64_t)16, left - c), v);
     });
   } else {
-    const float scale = p.scale ? *p.scale : 1.f;
-    each32<T, WIDTH>(tmem, left, [&](int c, float(&v)[32]) {
-      if (in) finish<T>(t, row, col0 + c, v, scale, bias + c);
+    const Row<T> to(t, row, col0);
+    each16<WIDTH>(tmem, left, [&](int c, float(&v)[16]) {
+      if (in) to.finish(c, v, bias + c);
     });
   }
 }
@@ -280,9 +321,10 @@ tensor_product_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_c
   uint64_t* bars = reinterpret_cast<uint64_t*>(shared + S::kStages * S::kStage + S::kBias);
   const uint32_t bar_full = cx::smem_u32(bars), bar_empty = bar_full + 8 * S::kStages, bar_sums = bar_empty + 8 * S::kStages,
                  bar_taken = bar_sums + 16, tmem_cell = bar_taken + 16;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xFFFFFFFFu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const uint32_t rank = CG == 2 ? cxt::cluster_rank() : 0;
-  const int worker = blockIdx.x / CG, workers = gridDim.x / CG;
+  Walk w(t, blockIdx.x / CG, gridDim.x / CG);
+  Unit u = unit_of(t.job[w.job], w.u);       // (under the allocation below)
   cx::pdl_trigger();
   if (threadIdx.x == 0) {
     for (int i = 0; i < S::kStages; ++i) {
@@ -306,12 +348,13 @@ tensor_product_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_c
   cx::pdl_wait();                        // everything above needs nothing from the kernel in front
   bool gave_up = false;
 
-  if (warp == 0 && lane == 0) {
+  if (warp == 0 && cxt::elect_one()) {
+    const uint32_t lead_full = CG == 2 ? cxt::in_cta(bar_full, 0) : bar_full;      // the pair's matrix instructions wait there
     int stage = 0;
     uint32_t phase = 0, filled = 0;
-    for (Walk w(t, worker, workers); w.more() && !gave_up; w.next()) {
+    for (; w.more() && !gave_up; w.next()) {
       const Job& job = t.job[w.job];
-      const Unit u = unit_of(job, w.u);
+      if (filled) u = unit_of(job, w.u);
       const CUtensorMap *map_a = w.job ? &map_a1 : &map_a0, *map_b = w.job ? &map_b1 : &map_b0;
       const int layout = job.p.layout, m0 = (u.tm * CG + (int)rank) * 128, n0 = u.tn * BN + (int)rank * (BN / CG);
       for (int s = u.s0; s < u.s1; ++s) {
@@ -319,7 +362,7 @@ tensor_product_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_c
           gave_up = true;
           break;
         }
-        const uint32_t full = CG == 2 ? cxt::in_cta(bar_full + 8 * stage, 0) : bar_full + 8 * stage;
+        const uint32_t full = lead_full + 8 * stage;
         if (rank == 0) cxt::expect_bytes(bar_full + 8 * stage, CG * S::kStage);
         const uint32_t a = cx::smem_u32(stages + stage * S::kStage), b = a + S::kA;
         if (layout == kTN) {
@@ -352,12 +395,12 @@ tensor_product_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_c
         break;
       }
     }
-  } else if (warp == 1 && lane == 0 && rank == 0) {
+  } else if (warp == 1 && rank == 0 && cxt::elect_one()) {
     int stage = 0, turn = 0;
     uint32_t phase = 0;
-    for (Walk w(t, worker, workers); w.more() && !gave_up; w.next(), ++turn) {
+    for (; w.more() && !gave_up; w.next(), ++turn) {
       const Job& job = t.job[w.job];
-      const Unit u = unit_of(job, w.u);
+      if (turn) u = unit_of(job, w.u);
       const bool along_m = job.p.layout == kTN, along_n = job.p.layout != kNT;
       const uint32_t instr = cxt::instruction(job.p.dtype == CX_BF16, along_m, along_n, 128 * CG, BN);
       // 16 of k: 32 bytes along a line, or 16 lines
@@ -391,9 +434,9 @@ tensor_product_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_c
     const int quarter = warp % 4, half = (warp - 4) / 4;
     float* bias = reinterpret_cast<float*>(shared + S::kStages * S::kStage) + (warp - 4) * (BN / 2);
     int turn = 0;
-    for (Walk w(t, worker, workers); w.more(); w.next(), ++turn) {
+    for (; w.more(); w.next(), ++turn) {
       const Job& job = t.job[w.job];
-      const Unit u = unit_of(job, w.u);
+      if (turn) u = unit_of(job, w.u);
       const int64_t row0 = (int64_t)(u.tm * CG + (int)rank) * 128 + quarter * 32, col0 = (int64_t)u.tn * BN + half * (BN / 2);
       if (job.p.bias) {                    // before the sums are there: nothing waits for it
         for (int i = lane; i < BN / 2; i += 32) {
@@ -438,7 +481,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_splits_kernel(const __grid_
   const int64_t row = i / per, col = i % per * 8;
   float v[8] = {};
   for (int s = 0; s < job.splits; ++s) add_sums(job.partial + ((int64_t)s * job.p.m + row) * job.part_ld + col, 8, v);
-  finish<T>(job, row, col, v, job.p.scale ? *job.p.scale : 1.f, nullptr);
+  Row<T>(job, row, col).finish(0, v, nullptr);
 }
 
 // ---- host ----------------------------------------------------------------------------------------------------------
@@ -620,7 +663,11 @@ int cx_tensor_product(CxProduct* p, int count, cxprod::Arena& ws, cudaStream_t s
     // about as many rows as columns at a time.  (8192 x 50257 x 1024, 8 / 16 rows of tiles: 700 / 684 us; 8192^3,
     // 4 / 8 / 16: 877 / 855 / 881 us.)
     const int64_t fit = (32ll << 20) / (q.k * 2 * 128 * c.cg);
-    job.group = (int)(fit < 8 ? 8 : fit < tm ? fit : tm);
+    const int64_t group = fit < 8 ? 8 : fit < tm ? fit : tm;
+    job.tiles.set((uint32_t)(tm * tn));
+    job.per.set((uint32_t)(group * tn));
+    job.group.set((uint32_t)group);
+    job.last.set((uint32_t)(tm % group ? tm % group : group));
     job.wide_out = align_of(q.out, q.ldo);
     if (q.pre && align_of(q.pre, q.ldo) < job.wide_out) job.wide_out = align_of(q.pre, q.ldo);
     job.wide_res = align_of(q.residual, q.ldr);
