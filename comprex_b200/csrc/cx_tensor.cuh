@@ -12,9 +12,9 @@ __device__ __forceinline__ uint32_t cluster_rank() {
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
   return r;
 }
-// True in one lane of the warp.  What one thread issues here takes its operands from the warp's uniform registers; behind
-// a test of the lane's number the compiler has to find out first which lanes are there: a tile copy took 250 cycles, 40
-// behind this.
+// True in one lane of the warp.  What one thread issues here takes its operands from the warp's uniform registers, which
+// the compiler fills where the whole warp comes by: the loops around are the warp's, only the instructions themselves are
+// behind this.  (Behind a test of the lane's number a tile copy took 250 cycles.)
 __device__ __forceinline__ bool elect_one() {
   uint32_t yes;
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(yes));
@@ -49,15 +49,17 @@ __device__ __forceinline__ bool try_wait(uint32_t bar, uint32_t parity) {
       : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
   return ok != 0;
 }
-// at most about two seconds (and 2^26 tries), then false
+// The whole warp waits: at most about two seconds (and 2^26 tries), then false, in all lanes alike.
 __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity) {
-  if (try_wait(bar, parity)) return true;
-  const uint64_t t0 = cx::globaltimer_ns();
-  for (uint32_t it = 0; it < (1u << 26); ++it) {
-    if (try_wait(bar, parity)) return true;
-    if ((it & 255u) == 255u && cx::globaltimer_ns() - t0 > 2000000000ull) return false;
+  bool there = try_wait(bar, parity);
+  if (!there) {
+    const uint64_t t0 = cx::globaltimer_ns();
+    for (uint32_t it = 0; it < (1u << 26) && !there; ++it) {
+      there = try_wait(bar, parity);
+      if ((it & 255u) == 255u && cx::globaltimer_ns() - t0 > 2000000000ull) break;
+    }
   }
-  return false;
+  return __all_sync(0xFFFFFFFFu, there);
 }
 
 // ---- tile copies (global -> shared, 128-byte swizzle; the inner coordinate is a multiple of 64 elements) ----------
@@ -94,19 +96,24 @@ __device__ __forceinline__ void tmem_free(uint32_t tmem, uint32_t columns) {
 __device__ __forceinline__ void fence_before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
-// 16 columns of the warp's 32 lanes: lane i gets row i
-__device__ __forceinline__ void tmem_load16(uint32_t tmem, uint32_t (&r)[16]) {
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-               "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+// 32 columns of the warp's 32 lanes: lane i gets row i
+__device__ __forceinline__ void tmem_load32(uint32_t tmem, uint32_t (&r)[32]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+               "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+               "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-                 "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+                 "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+                 "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
                : "r"(tmem));
 }
 // Until all of the warp's loads are there.  `r`, which one of them fills, is an operand: no use of it may move up.
-__device__ __forceinline__ void tmem_load_wait(uint32_t (&r)[16]) {
+__device__ __forceinline__ void tmem_load_wait(uint32_t (&r)[32]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;"
                : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
-                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                 "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+                 "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
                :: "memory");
 }
 
@@ -115,25 +122,24 @@ __device__ __forceinline__ void tmem_load_wait(uint32_t (&r)[16]) {
 //   consecutive along k:       rows are the operand's rows, an atom is 8 rows of 64 elements of k, atoms 1024 bytes apart
 //   consecutive along m or n:  rows are k, an atom is 8 of k by 64 elements, the next 8 of k 1024 bytes on, the next 64
 //                              elements `chunk` bytes on
-__device__ __forceinline__ uint64_t smem_operand(uint32_t addr, uint32_t chunk) {
-  return (uint64_t)((addr >> 4) & 0x3FFFu) | (uint64_t)((chunk >> 4) & 0x3FFFu) << 16 | (uint64_t)(1024u >> 4) << 32 |
-         1ull << 46 | 2ull << 61;
-}
+// The lower word holds the address and `chunk`, in 16 bytes: adding to it moves the tile (shared memory ends below 2^18).
+__device__ __forceinline__ uint32_t operand_at(uint32_t addr, uint32_t chunk) { return addr >> 4 | (chunk >> 4) << 16; }
+constexpr uint32_t kOperandHigh = 1024u >> 4 | 1u << 14 | 2u << 29;
 // kind::f16, sums in 32 bits; both operands bf16, or both f16
 __host__ __device__ constexpr uint32_t instruction(bool bf16, bool a_along_m, bool b_along_n, int m, int n) {
   return 1u << 4 | (bf16 ? 1u : 0u) << 7 | (bf16 ? 1u : 0u) << 10 | (a_along_m ? 1u : 0u) << 15 | (b_along_n ? 1u : 0u) << 16 |
          (uint32_t)(n / 8) << 17 | (uint32_t)(m / 16) << 24;
 }
 template <int CG>
-__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t instr, bool add) {
+__device__ __forceinline__ void mma(uint32_t d, uint32_t a, uint32_t b, uint32_t instr, bool add) {
   if (CG == 1)
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-                 ::"r"(d), "l"(a), "l"(b), "r"(instr), "r"((uint32_t)add) : "memory");
+    asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 x, y;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 x, {%1, %5};\n\tmov.b64 y, {%2, %5};\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n\t}"
+                 ::"r"(d), "r"(a), "r"(b), "r"(instr), "r"((uint32_t)add), "r"(kOperandHigh) : "memory");
   else
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-                 ::"r"(d), "l"(a), "l"(b), "r"(instr), "r"((uint32_t)add) : "memory");
+    asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 x, y;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 x, {%1, %5};\n\tmov.b64 y, {%2, %5};\n\t"
+                 "tcgen05.mma.cta_group::2.kind::f16 [%0], x, y, %3, p;\n\t}"
+                 ::"r"(d), "r"(a), "r"(b), "r"(instr), "r"((uint32_t)add), "r"(kOperandHigh) : "memory");
 }
 // the barrier (CG == 2: of both CTAs of the pair) gets an arrival when all matrix instructions so far are complete
 template <int CG>

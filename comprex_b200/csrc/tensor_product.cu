@@ -50,6 +50,7 @@ struct Job {
   int64_t part_ld;
   int splits;
   int wide_out, wide_res, wide_bias;   // alignment of their rows: 2 for 32 bytes, 1 for 16, 0 for less
+  int plain;                   // kOut with nothing to it but a factor
 };
 
 // The units of the first job go round the workers, those of the second one fill up: `extra` workers have one more of the
@@ -175,8 +176,8 @@ __device__ __forceinline__ void add_sums(const float* at, int left, float (&v)[W
     }
 }
 
-// What is done to the sums of a row (kOut, kSums), from column `col` on: everything that the descriptor says, in registers.
-// (Read from the descriptor for each 16 columns it took 880 cycles for them.)
+// What the descriptor says of a row's results from column `col` on, in registers: read from the descriptor for each few
+// columns it took 880 cycles for 16 of them.
 template <typename T>
 struct Row {
   T *out, *pre;
@@ -184,7 +185,6 @@ struct Row {
   float* addend;
   float scale;
   int left, act, wide_out, wide_res, wide_bias;
-  bool add, sums, scaled;
   __device__ __forceinline__ Row(const Job& t, int64_t row, int64_t col) {
     const CxProduct& p = t.p;
     out = reinterpret_cast<T*>(p.out) + row * p.ldo + col;
@@ -192,122 +192,160 @@ struct Row {
     residual = p.residual ? reinterpret_cast<const T*>(p.residual) + row * p.ldr + col : nullptr;
     bias = p.bias ? reinterpret_cast<const T*>(p.bias) + col : nullptr;
     addend = p.addend + row * p.ldadd + col;
-    scaled = p.scale != nullptr;
-    scale = scaled ? *p.scale : 1.f;
+    scale = p.scale ? *p.scale : 1.f;
     left = (int)min((int64_t)0x40000000, p.n - col);
     act = p.act;
     wide_out = t.wide_out;
     wide_res = t.wide_res;
     wide_bias = t.wide_bias;
-    add = p.has_addend;
-    sums = p.mode == kSums;
-  }
-  // W columns, `c` further on; `shared`: their biases in shared memory, or NULL where they are read from the operand
-  template <int W>
-  __device__ __forceinline__ void finish(int c, float (&v)[W], const float* shared) const {
-    const int have = left - c;
-    if (add) add_sums(addend + c, have, v);
-    if (sums) return store_sums(addend + c, have, v);
-    if (scaled) {
-#pragma unroll
-      for (int i = 0; i < W; ++i) v[i] *= scale;
-    }
-    if (bias) {
-      if (shared) {
-#pragma unroll
-        for (int i = 0; i < W / 4; ++i) {
-          const float4 b = reinterpret_cast<const float4*>(shared)[i];
-          v[4 * i] += b.x, v[4 * i + 1] += b.y, v[4 * i + 2] += b.z, v[4 * i + 3] += b.w;
-        }
-      } else {
-        add_row(bias + c, wide_bias, have, v);
-      }
-    }
-    if (pre) store_row(pre + c, wide_out, have, v);
-    cxprod::activate(v, act);
-    if (residual) add_row(residual + c, wide_res, have, v);
-    store_row(out + c, wide_out, have, v);
   }
 };
 
-// A finishing warp's part of a tile: 32 rows, one per lane, WIDTH columns from col0 on, 16 at a time.  The loops are not
-// unrolled: instructions of a tile that are fetched once per tile cost more than they do (one unrolled 32 columns at a
-// time took 1600 cycles for each 32).
+// A finishing warp's part of a tile, 32 rows, one per lane, 32 columns at a time.  The loop is not unrolled: fetching
+// instructions that a tile needs once costs more than they do.
 template <int WIDTH, typename F>
-__device__ __forceinline__ void each16(uint32_t tmem, int64_t left, const F& work) {
+__device__ __forceinline__ void each32(uint32_t tmem, int left, const F& work) {
 #pragma unroll 1
-  for (int c = 0; c < WIDTH && c < left; c += 16) {
-    uint32_t r[16];
-    cxt::tmem_load16(tmem + c, r);
+  for (int c = 0; c < WIDTH && c < left; c += 32) {
+    uint32_t r[32];
+    cxt::tmem_load32(tmem + c, r);
     cxt::tmem_load_wait(r);
-    work(c, reinterpret_cast<float(&)[16]>(r));
+    work(c, reinterpret_cast<float(&)[32]>(r));
   }
 }
 
 template <typename T, int WIDTH>
+__device__ __forceinline__ void finish_stats(const Job& t, const Unit& u, int half, int64_t row, int64_t col0, uint32_t tmem) {
+  const CxProduct& p = t.p;
+  const bool in = row < p.m;
+  const int left = (int)min((int64_t)WIDTH, p.n - col0);
+  const int64_t hot = (in ? p.targets[row] : -1) - p.col0 - col0;      // where the row's target is in this part
+  float top = -INFINITY, sum = 0.f;
+  each32<WIDTH>(tmem, left, [&](int c, float(&v)[32]) {
+    if (c + 32 > left) {
+#pragma unroll
+      for (int j = 0; j < 32; ++j)
+        if (c + j >= left) v[j] = -INFINITY;
+    }
+    if (hot >= c && hot < c + 32) {
+      float x = 0.f;
+#pragma unroll
+      for (int j = 0; j < 32; ++j)
+        if (hot == c + j) x = v[j];
+      p.target_logit[row] = x;
+    }
+    float m[4] = {top, top, top, top}, add[4] = {};
+#pragma unroll
+    for (int j = 0; j < 32; ++j) m[j % 4] = fmaxf(m[j % 4], v[j]);
+    m[0] = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+    const float base = (m[0] == -INFINITY ? 0.f : m[0]) * cxprod::kLog2e;
+#pragma unroll
+    for (int j = 0; j < 32; ++j) add[j % 4] += cxprod::pow2(__fmaf_rn(v[j], cxprod::kLog2e, -base));
+    sum = sum * cxprod::pow2(__fmaf_rn(top, cxprod::kLog2e, -base)) + ((add[0] + add[1]) + (add[2] + add[3]));   // (top = -inf: 0)
+    top = m[0];
+  });
+  if (in) p.part[(2ll * u.tn + half) * p.m + row] = make_float2(top, sum);
+}
+
+template <typename T, int WIDTH>
+__device__ __forceinline__ void finish_prob(const Job& t, int64_t row, int64_t col0, uint32_t tmem) {
+  const CxProduct& p = t.p;
+  const bool in = row < p.m;
+  const int left = (int)min((int64_t)WIDTH, p.n - col0), wide = t.wide_out;
+  const float lse = in ? p.lse[row] : 0.f, factor = in ? p.row_factor[row] : 0.f;
+  const int64_t hot = in ? p.targets[row] - p.col0 - col0 : -1;
+  T* out = reinterpret_cast<T*>(p.out) + row * p.ldo + col0;
+  each32<WIDTH>(tmem, left, [&](int c, float(&v)[32]) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] = cxprod::pow2(__fmaf_rn(v[j], cxprod::kLog2e, -lse)) * factor;
+    if (hot >= c && hot < c + 32) {
+#pragma unroll
+      for (int j = 0; j < 32; ++j)
+        if (hot == c + j) v[j] -= factor;
+    }
+    if (factor == 0.f) {                 // a row that does not count, whatever its logits are
+#pragma unroll
+      for (int j = 0; j < 32; ++j) v[j] = 0.f;
+    }
+    if (in) store_row(out + c, wide, left - c, v);
+  });
+}
+
+// kOut without anything to it but a factor
+template <typename T, int WIDTH>
+__device__ __forceinline__ void finish_plain(const Job& t, int64_t row, int64_t col0, uint32_t tmem) {
+  const CxProduct& p = t.p;
+  const bool in = row < p.m;
+  const int left = (int)min((int64_t)WIDTH, p.n - col0), wide = t.wide_out;
+  const float scale = p.scale ? *p.scale : 1.f;
+  T* out = reinterpret_cast<T*>(p.out) + row * p.ldo + col0;
+  each32<WIDTH>(tmem, left, [&](int c, float(&v)[32]) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] *= scale;
+    if (in) store_row(out + c, wide, left - c, v);
+  });
+}
+
+// 32-bit sums: of a split, or those that a later product goes on with
+template <int WIDTH>
+__device__ __forceinline__ void finish_sums(float* at, bool add, bool in, int left, uint32_t tmem) {
+  each32<WIDTH>(tmem, left, [&](int c, float(&v)[32]) {
+    if (!in) return;
+    if (add) add_sums(at + c, left - c, v);
+    store_sums(at + c, left - c, v);
+  });
+}
+
+// kOut with all that can be in it.  The residual's next 32 columns are on their way while these are worked on.
+template <typename T, int WIDTH>
+__device__ __forceinline__ void finish_linear(const Job& t, int64_t row, int64_t col0, uint32_t tmem, const float* bias) {
+  const Row<T> to(t, row, col0);
+  const bool in = row < t.p.m, add = t.p.has_addend, ahead = to.residual && to.wide_res == 2 && in && to.left >= WIDTH;
+  uint32_t next[16];
+  if (ahead) {
+    load_words8(to.residual, reinterpret_cast<uint32_t(&)[8]>(next[0]));
+    load_words8(to.residual + 16, reinterpret_cast<uint32_t(&)[8]>(next[8]));
+  }
+  each32<WIDTH>(tmem, min(to.left, WIDTH), [&](int c, float(&v)[32]) {
+    const int have = to.left - c;
+    if (add && in) add_sums(to.addend + c, have, v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float4 b = reinterpret_cast<const float4*>(bias + c)[i];      // zeros where there is none
+      v[4 * i] = __fmaf_rn(v[4 * i], to.scale, b.x);
+      v[4 * i + 1] = __fmaf_rn(v[4 * i + 1], to.scale, b.y);
+      v[4 * i + 2] = __fmaf_rn(v[4 * i + 2], to.scale, b.z);
+      v[4 * i + 3] = __fmaf_rn(v[4 * i + 3], to.scale, b.w);
+    }
+    if (to.pre && in) store_row(to.pre + c, to.wide_out, have, v);
+    cxprod::activate(v, to.act);
+    if (ahead) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[i] += cx::Elem<T>::to_f(reinterpret_cast<const T*>(next)[i]);
+      if (c + 32 < WIDTH) {
+        load_words8(to.residual + c + 32, reinterpret_cast<uint32_t(&)[8]>(next[0]));
+        load_words8(to.residual + c + 48, reinterpret_cast<uint32_t(&)[8]>(next[8]));
+      }
+    } else if (to.residual && in) {
+      add_row(to.residual + c, to.wide_res, have, v);
+    }
+    if (in) store_row(to.out + c, to.wide_out, have, v);
+  });
+}
+
+// A finishing warp's part of a tile: rows row0 to row0 + 31, WIDTH columns from col0 on.
+template <typename T, int WIDTH>
 __device__ __forceinline__ void finish_part(const Job& t, const Unit& u, int half, int64_t row0, int64_t col0, uint32_t tmem, const float* bias) {
   const CxProduct& p = t.p;
-  const int lane = threadIdx.x & 31;
-  const int64_t row = row0 + lane, left = p.n - col0;
-  const bool in = row < p.m;
-  if (left <= 0) return;
-  if (p.mode == kStats) {
-    const int64_t hot = (in ? p.targets[row] : -1) - p.col0 - col0;      // where the row's target is in this part
-    float top = -INFINITY, sum = 0.f;
-    each16<WIDTH>(tmem, left, [&](int c, float(&v)[16]) {
-      if (c + 16 > left) {
-#pragma unroll
-        for (int j = 0; j < 16; ++j)
-          if (c + j >= left) v[j] = -INFINITY;
-      }
-      if (hot >= c && hot < c + 16) {
-        float x = 0.f;
-#pragma unroll
-        for (int j = 0; j < 16; ++j)
-          if (hot == c + j) x = v[j];
-        p.target_logit[row] = x;
-      }
-      float m[4] = {top, top, top, top}, add[4] = {};
-#pragma unroll
-      for (int j = 0; j < 16; ++j) m[j % 4] = fmaxf(m[j % 4], v[j]);
-      m[0] = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
-      const float base = (m[0] == -INFINITY ? 0.f : m[0]) * cxprod::kLog2e;
-#pragma unroll
-      for (int j = 0; j < 16; ++j) add[j % 4] += cxprod::pow2(__fmaf_rn(v[j], cxprod::kLog2e, -base));
-      sum = sum * cxprod::pow2(__fmaf_rn(top, cxprod::kLog2e, -base)) + ((add[0] + add[1]) + (add[2] + add[3]));   // (top = -inf: 0)
-      top = m[0];
-    });
-    if (in) p.part[(2ll * u.tn + half) * p.m + row] = make_float2(top, sum);
-  } else if (p.mode == kProb) {
-    const float lse = in ? p.lse[row] : 0.f, factor = in ? p.row_factor[row] : 0.f;
-    const int64_t hot = in ? p.targets[row] - p.col0 - col0 : -1;
-    T* out = reinterpret_cast<T*>(p.out) + row * p.ldo + col0;
-    const int wide = t.wide_out;
-    each16<WIDTH>(tmem, left, [&](int c, float(&v)[16]) {
-#pragma unroll
-      for (int j = 0; j < 16; ++j) v[j] = cxprod::pow2(__fmaf_rn(v[j], cxprod::kLog2e, -lse)) * factor;
-      if (hot >= c && hot < c + 16) {
-#pragma unroll
-        for (int j = 0; j < 16; ++j)
-          if (hot == c + j) v[j] -= factor;
-      }
-      if (factor == 0.f) {                 // a row that does not count, whatever its logits are
-#pragma unroll
-        for (int j = 0; j < 16; ++j) v[j] = 0.f;
-      }
-      if (in) store_row(out + c, wide, (int)min((int64_t)16, left - c), v);
-    });
-  } else if (t.partial) {
-    float* at = t.partial + ((int64_t)u.split * p.m + row) * t.part_ld + col0;
-    each16<WIDTH>(tmem, left, [&](int c, float(&v)[16]) {
-      if (in) store_sums(at + c, (int)min((int64_t)16, left - c), v);
-    });
-  } else {
-    const Row<T> to(t, row, col0);
-    each16<WIDTH>(tmem, left, [&](int c, float(&v)[16]) {
-      if (in) to.finish(c, v, bias + c);
-    });
-  }
+  const int64_t row = row0 + (threadIdx.x & 31);
+  if (col0 >= p.n) return;
+  const int left = (int)min((int64_t)WIDTH, p.n - col0);
+  if (p.mode == kStats) return finish_stats<T, WIDTH>(t, u, half, row, col0, tmem);
+  if (p.mode == kProb) return finish_prob<T, WIDTH>(t, row, col0, tmem);
+  if (t.partial) return finish_sums<WIDTH>(t.partial + ((int64_t)u.split * p.m + row) * t.part_ld + col0, false, row < p.m, left, tmem);
+  if (p.mode == kSums) return finish_sums<WIDTH>(p.addend + row * p.ldadd + col0, p.has_addend, row < p.m, left, tmem);
+  if (t.plain) return finish_plain<T, WIDTH>(t, row, col0, tmem);
+  finish_linear<T, WIDTH>(t, row, col0, tmem, bias);
 }
 
 template <int CG, int BN>
@@ -348,7 +386,7 @@ tensor_product_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_c
   cx::pdl_wait();                        // everything above needs nothing from the kernel in front
   bool gave_up = false;
 
-  if (warp == 0 && cxt::elect_one()) {
+  if (warp == 0) {
     const uint32_t lead_full = CG == 2 ? cxt::in_cta(bar_full, 0) : bar_full;      // the pair's matrix instructions wait there
     int stage = 0;
     uint32_t phase = 0, filled = 0;
@@ -362,21 +400,23 @@ tensor_product_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_c
           gave_up = true;
           break;
         }
-        const uint32_t full = lead_full + 8 * stage;
-        if (rank == 0) cxt::expect_bytes(bar_full + 8 * stage, CG * S::kStage);
-        const uint32_t a = cx::smem_u32(stages + stage * S::kStage), b = a + S::kA;
-        if (layout == kTN) {
+        const uint32_t full = lead_full + 8 * stage, a = cx::smem_u32(stages) + stage * S::kStage, b = a + S::kA;
+        if (cxt::elect_one()) {
+          if (rank == 0) cxt::expect_bytes(bar_full + 8 * stage, CG * S::kStage);
+          if (layout == kTN) {
 #pragma unroll
-          for (int i = 0; i < 2; ++i) cxt::load_tile<CG>(a + i * 8192, map_a, m0 + 64 * i, s * kDepth, full);
-        } else {
-          cxt::load_tile<CG>(a, map_a, s * kDepth, m0, full);
-        }
-        if (layout == kNT) {
-          cxt::load_tile<CG>(b, map_b, s * kDepth, n0, full);
-        } else {
+            for (int i = 0; i < 2; ++i) cxt::load_tile<CG>(a + i * 8192, map_a, m0 + 64 * i, s * kDepth, full);
+          } else {
+            cxt::load_tile<CG>(a, map_a, s * kDepth, m0, full);
+          }
+          if (layout == kNT) {
+            cxt::load_tile<CG>(b, map_b, s * kDepth, n0, full);
+          } else {
 #pragma unroll
-          for (int i = 0; i < BN / CG / 64; ++i) cxt::load_tile<CG>(b + i * 8192, map_b, n0 + 64 * i, s * kDepth, full);
+            for (int i = 0; i < BN / CG / 64; ++i) cxt::load_tile<CG>(b + i * 8192, map_b, n0 + 64 * i, s * kDepth, full);
+          }
         }
+        __syncwarp();
         ++filled;
         if (++stage == S::kStages) {
           stage = 0;
@@ -395,7 +435,7 @@ tensor_product_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_c
         break;
       }
     }
-  } else if (warp == 1 && rank == 0 && cxt::elect_one()) {
+  } else if (warp == 1 && rank == 0) {
     int stage = 0, turn = 0;
     uint32_t phase = 0;
     for (; w.more() && !gave_up; w.next(), ++turn) {
@@ -404,7 +444,9 @@ tensor_product_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_c
       const bool along_m = job.p.layout == kTN, along_n = job.p.layout != kNT;
       const uint32_t instr = cxt::instruction(job.p.dtype == CX_BF16, along_m, along_n, 128 * CG, BN);
       // 16 of k: 32 bytes along a line, or 16 lines
-      const uint32_t step_a = along_m ? 2048 : 32, step_b = along_n ? 2048 : 32, chunk_a = along_m ? 8192 : 16, chunk_b = along_n ? 8192 : 16;
+      const uint32_t step_a = along_m ? 128 : 2, step_b = along_n ? 128 : 2;
+      const uint32_t first_a = cxt::operand_at(cx::smem_u32(stages), along_m ? 8192 : 16);
+      const uint32_t first_b = cxt::operand_at(cx::smem_u32(stages) + S::kA, along_n ? 8192 : 16);
       if (!cxt::wait(bar_taken + 8 * (turn & 1), ((turn >> 1) & 1) ^ 1u)) {
         gave_up = true;
         break;
@@ -417,17 +459,20 @@ tensor_product_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_c
           break;
         }
         cxt::fence_after_sync();
-        const uint32_t a = cx::smem_u32(stages + stage * S::kStage), b = a + S::kA;
+        const uint32_t a = first_a + stage * (S::kStage >> 4), b = first_b + stage * (S::kStage >> 4);
+        if (cxt::elect_one()) {
 #pragma unroll
-        for (int k = 0; k < kDepth / 16; ++k)
-          cxt::mma<CG>(sums, cxt::smem_operand(a + k * step_a, chunk_a), cxt::smem_operand(b + k * step_b, chunk_b), instr, s > u.s0 || k > 0);
-        cxt::commit<CG>(bar_empty + 8 * stage);
+          for (int k = 0; k < kDepth / 16; ++k) cxt::mma<CG>(sums, a + k * step_a, b + k * step_b, instr, s > u.s0 || k > 0);
+          cxt::commit<CG>(bar_empty + 8 * stage);
+        }
+        __syncwarp();
         if (++stage == S::kStages) {
           stage = 0;
           phase ^= 1u;
         }
       }
-      cxt::commit<CG>(bar_sums + 8 * (turn & 1));
+      if (cxt::elect_one()) cxt::commit<CG>(bar_sums + 8 * (turn & 1));
+      __syncwarp();
     }
   } else if (warp >= 4) {
     const uint32_t taken = CG == 2 ? cxt::in_cta(bar_taken, 0) : bar_taken;
@@ -438,9 +483,9 @@ tensor_product_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_c
       const Job& job = t.job[w.job];
       if (turn) u = unit_of(job, w.u);
       const int64_t row0 = (int64_t)(u.tm * CG + (int)rank) * 128 + quarter * 32, col0 = (int64_t)u.tn * BN + half * (BN / 2);
-      if (job.p.bias) {                    // before the sums are there: nothing waits for it
+      if (!job.plain && job.p.mode == kOut && !job.partial) {      // before the sums are there: nothing waits for it
         for (int i = lane; i < BN / 2; i += 32) {
-          const bool have = col0 + i < job.p.n;
+          const bool have = job.p.bias && col0 + i < job.p.n;
           bias[i] = !have ? 0.f : job.p.dtype == CX_BF16 ? __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(job.p.bias)[col0 + i])
                                                          : __half2float(reinterpret_cast<const __half*>(job.p.bias)[col0 + i]);
         }
@@ -481,7 +526,16 @@ __global__ void __launch_bounds__(kJoinThreads) join_splits_kernel(const __grid_
   const int64_t row = i / per, col = i % per * 8;
   float v[8] = {};
   for (int s = 0; s < job.splits; ++s) add_sums(job.partial + ((int64_t)s * job.p.m + row) * job.part_ld + col, 8, v);
-  Row<T>(job, row, col).finish(0, v, nullptr);
+  const Row<T> to(job, row, col);
+  if (job.p.has_addend) add_sums(to.addend, to.left, v);
+  if (job.p.mode == kSums) return store_sums(to.addend, to.left, v);
+#pragma unroll
+  for (int k = 0; k < 8; ++k) v[k] *= to.scale;
+  if (to.bias) add_row(to.bias, to.wide_bias, to.left, v);
+  if (to.pre) store_row(to.pre, to.wide_out, to.left, v);
+  cxprod::activate(v, to.act);
+  if (to.residual) add_row(to.residual, to.wide_res, to.left, v);
+  store_row(to.out, to.wide_out, to.left, v);
 }
 
 // ---- host ----------------------------------------------------------------------------------------------------------
@@ -672,6 +726,7 @@ int cx_tensor_product(CxProduct* p, int count, cxprod::Arena& ws, cudaStream_t s
     if (q.pre && align_of(q.pre, q.ldo) < job.wide_out) job.wide_out = align_of(q.pre, q.ldo);
     job.wide_res = align_of(q.residual, q.ldr);
     job.wide_bias = align_of(q.bias, 0);
+    job.plain = q.mode == kOut && !q.has_addend && !q.bias && !q.pre && !q.residual && q.act == CX_ACT_NONE;
     if (job.splits > 1) {
       job.part_ld = (q.n + 7) / 8 * 8;
       job.partial = reinterpret_cast<float*>(ws.take((int64_t)job.splits * q.m * job.part_ld * 4));
