@@ -1,7 +1,7 @@
 // The product of cx_product.cuh on the fifth-generation tensor cores, for 16-bit operands.
 //
-// A persistent grid of CTAs, or of pairs of CTAs that share a tile, walks over the output's tiles.  One thread per CTA
-// brings 64-deep slices of both operands into a ring of stages with tile copies, one thread per tile issues the matrix
+// A persistent grid of CTAs, or of pairs of CTAs that share a tile, walks over the output's tiles.  Two warps per
+// CTA bring 64-deep slices of the operands into a ring of stages with tile copies, one per tile issues the matrix
 // instructions, whose sums stay in tensor memory, and eight warps take finished sums from there: the tensor memory holds
 // two tiles, so the matrix instructions of a tile run under the epilogue of the tile before.  Each layout of the operands
 // is read as it lies: consecutive along k or along m and n is a bit of the instruction and another shape of the copy.
@@ -11,7 +11,7 @@
 namespace {
 
 constexpr int kDepth = 64;               // elements of k in a stage: one 128-byte line
-constexpr int kThreads = 384;            // warp 0 copies, warp 1 multiplies, warp 2 has the tensor memory, 4 to 11 finish
+constexpr int kThreads = 384;            // warps 0 and 3 copy, 1 multiplies, 2 has the tensor memory, 4 to 11 finish
 constexpr int kFinish = 8;               // finishing warps: four have the left half of a tile's columns, four the right one
 constexpr int kJoinThreads = 256;
 constexpr int kShared = 232448;          // of a CTA
@@ -366,7 +366,7 @@ tensor_product_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_c
   cx::pdl_trigger();
   if (threadIdx.x == 0) {
     for (int i = 0; i < S::kStages; ++i) {
-      cx::mbar_init(bars + i, 1);
+      cx::mbar_init(bars + i, 2);
       cx::mbar_init(bars + S::kStages + i, 1);
     }
     for (int i = 0; i < 2; ++i) {
@@ -386,38 +386,38 @@ tensor_product_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_c
   cx::pdl_wait();                        // everything above needs nothing from the kernel in front
   bool gave_up = false;
 
-  if (warp == 0) {
+  if (warp == 0 || warp == 3) {
+    // Each has an operand: a turn of such a loop takes 200 cycles whatever it copies, a slice's matrix instructions 128
+    // to 512 (one warp for both operands: 360 a slice).
+    const bool is_b = warp == 3;
     const uint32_t lead_full = CG == 2 ? cxt::in_cta(bar_full, 0) : bar_full;      // the pair's matrix instructions wait there
-    int stage = 0;
-    uint32_t phase = 0, filled = 0;
+    const uint32_t base = cx::smem_u32(stages) + (is_b ? S::kA : 0), bytes = CG * (is_b ? S::kB : S::kA);
+    int stage = 0, filled = 0;
+    uint32_t phase = 0;
     for (; w.more() && !gave_up; w.next()) {
       const Job& job = t.job[w.job];
       if (filled) u = unit_of(job, w.u);
-      const CUtensorMap *map_a = w.job ? &map_a1 : &map_a0, *map_b = w.job ? &map_b1 : &map_b0;
-      const int layout = job.p.layout, m0 = (u.tm * CG + (int)rank) * 128, n0 = u.tn * BN + (int)rank * (BN / CG);
+      const CUtensorMap* map = is_b ? (w.job ? &map_b1 : &map_b0) : (w.job ? &map_a1 : &map_a0);
+      const bool across = is_b ? job.p.layout != kNT : job.p.layout == kTN;          // consecutive along m or n, not along k
+      const int first = is_b ? u.tn * BN + (int)rank * (BN / CG) : (u.tm * CG + (int)rank) * 128;
+      const int boxes = !across ? 1 : is_b ? BN / CG / 64 : 2;
       for (int s = u.s0; s < u.s1; ++s) {
-        if (!cxt::wait(bar_empty + 8 * stage, phase ^ 1u)) {
+        if (filled >= S::kStages && !cxt::wait(bar_empty + 8 * stage, phase ^ 1u)) {
           gave_up = true;
           break;
         }
-        const uint32_t full = lead_full + 8 * stage, a = cx::smem_u32(stages) + stage * S::kStage, b = a + S::kA;
+        const uint32_t full = lead_full + 8 * stage, at = base + stage * S::kStage;
         if (cxt::elect_one()) {
-          if (rank == 0) cxt::expect_bytes(bar_full + 8 * stage, CG * S::kStage);
-          if (layout == kTN) {
-#pragma unroll
-            for (int i = 0; i < 2; ++i) cxt::load_tile<CG>(a + i * 8192, map_a, m0 + 64 * i, s * kDepth, full);
+          if (rank == 0) cxt::expect_bytes(bar_full + 8 * stage, bytes);
+          if (!across) {
+            cxt::load_tile<CG>(at, map, s * kDepth, first, full);
           } else {
-            cxt::load_tile<CG>(a, map_a, s * kDepth, m0, full);
-          }
-          if (layout == kNT) {
-            cxt::load_tile<CG>(b, map_b, s * kDepth, n0, full);
-          } else {
-#pragma unroll
-            for (int i = 0; i < BN / CG / 64; ++i) cxt::load_tile<CG>(b + i * 8192, map_b, n0 + 64 * i, s * kDepth, full);
+#pragma unroll 1
+            for (int i = 0; i < boxes; ++i) cxt::load_tile<CG>(at + i * 8192, map, first + 64 * i, s * kDepth, full);
           }
         }
         __syncwarp();
-        ++filled;
+        if (filled < S::kStages) ++filled;
         if (++stage == S::kStages) {
           stage = 0;
           phase ^= 1u;
@@ -425,7 +425,7 @@ tensor_product_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_c
       }
     }
     // until the stages are free again: no copy is in flight, and no arrival of the pair's on its way, when the CTA ends
-    for (int i = 0; i < S::kStages && i < (int)filled; ++i) {
+    for (int i = 0; i < filled; ++i) {
       if (--stage < 0) {
         stage = S::kStages - 1;
         phase ^= 1u;
