@@ -68,7 +68,7 @@ int cx_product_stat_columns(const CxProduct& p);
 // tensor_product.cu: 16-bit types, operands that a tile copy can read (16-byte aligned rows)
 bool cx_tensor_product_takes(const CxProduct& p);
 int cx_tensor_product_stat_columns(const CxProduct& p);
-// about how long that takes, in slices of 64 along k (0.3 to 0.4 us), the launch counted as 12
+// about how long that takes, in us
 double cx_tensor_product_time(const CxProduct* p, int count);
 int cx_tensor_product(CxProduct* p, int count, cxprod::Arena& ws, cudaStream_t s);
 

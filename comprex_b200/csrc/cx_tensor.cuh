@@ -38,29 +38,34 @@ __device__ __forceinline__ void arrive_cluster(uint32_t bar) {
 __device__ __forceinline__ void expect_bytes(uint32_t bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
-// (Acquire at the scope of the CTA: what the barriers here guard comes by tile copies, matrix instructions and loads of
-// tensor memory, which their own completion and fences order.  At the scope of the cluster each wait took 500 cycles.)
-__device__ __forceinline__ bool try_wait(uint32_t bar, uint32_t parity) {
+// Waits for a phase of a barrier: at most 2^21 tries of about a microsecond each, then false.  Acquire at the scope of the
+// CTA: what the barriers here guard comes by tile copies, matrix instructions and loads of tensor memory, which their own
+// completion and fences order.  (At the scope of the cluster a wait took 500 cycles; as a loop in C++ with a vote 220; so,
+// where the phase is there already, 40.)
+__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .u32 n;\n\tmov.u32 n, 2097152;\n"
+      "again:\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 1000;\n\t"
+      "@p bra there;\n\t"
+      "sub.u32 n, n, 1;\n\tsetp.ne.u32 q, n, 0;\n\t@q bra again;\n"
+      "there:\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+  return ok != 0;
+}
+// One look at it.  The answer takes 200 cycles: ask for the next phase before the work on this one.
+__device__ __forceinline__ bool look(uint32_t bar, uint32_t parity) {
   uint32_t ok;
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
       "selp.u32 %0, 1, 0, p;\n\t}"
       : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
   return ok != 0;
 }
-// The whole warp waits: at most about two seconds (and 2^26 tries), then false, in all lanes alike.
-__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity) {
-  bool there = try_wait(bar, parity);
-  if (!there) {
-    const uint64_t t0 = cx::globaltimer_ns();
-    for (uint32_t it = 0; it < (1u << 26) && !there; ++it) {
-      there = try_wait(bar, parity);
-      if ((it & 255u) == 255u && cx::globaltimer_ns() - t0 > 2000000000ull) break;
-    }
-  }
-  return __all_sync(0xFFFFFFFFu, there);
-}
+// the same answer in all lanes of the warp
+__device__ __forceinline__ bool wait_together(uint32_t bar, uint32_t parity) { return __all_sync(0xFFFFFFFFu, wait(bar, parity)); }
 
 // ---- tile copies (global -> shared, 128-byte swizzle; the inner coordinate is a multiple of 64 elements) ----------
 // CG == 2: the barrier may be the one of the other CTA of the pair.

@@ -394,7 +394,8 @@ tensor_product_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_c
     const uint32_t base = cx::smem_u32(stages) + (is_b ? S::kA : 0), bytes = CG * (is_b ? S::kB : S::kA);
     int stage = 0, filled = 0;
     uint32_t phase = 0;
-    for (; w.more() && !gave_up; w.next()) {
+    bool ready = true;
+    for (; w.more(); w.next()) {
       const Job& job = t.job[w.job];
       if (filled) u = unit_of(job, w.u);
       const CUtensorMap* map = is_b ? (w.job ? &map_b1 : &map_b0) : (w.job ? &map_a1 : &map_a0);
@@ -402,13 +403,17 @@ tensor_product_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_c
       const int first = is_b ? u.tn * BN + (int)rank * (BN / CG) : (u.tm * CG + (int)rank) * 128;
       const int boxes = !across ? 1 : is_b ? BN / CG / 64 : 2;
       for (int s = u.s0; s < u.s1; ++s) {
-        if (filled >= S::kStages && !cxt::wait(bar_empty + 8 * stage, phase ^ 1u)) {
-          gave_up = true;
-          break;
+        // a lane whose wait has run out copies nothing more and waits no more; the warp stays together
+        if (!ready && !gave_up) gave_up = !cxt::wait(bar_empty + 8 * stage, phase ^ 1u);
+        const uint32_t full = lead_full + 8 * stage, at = base + stage * S::kStage, own = bar_full + 8 * stage;
+        if (filled < S::kStages) ++filled;
+        if (++stage == S::kStages) {
+          stage = 0;
+          phase ^= 1u;
         }
-        const uint32_t full = lead_full + 8 * stage, at = base + stage * S::kStage;
-        if (cxt::elect_one()) {
-          if (rank == 0) cxt::expect_bytes(bar_full + 8 * stage, bytes);
+        ready = filled < S::kStages || cxt::look(bar_empty + 8 * stage, phase ^ 1u);
+        if (cxt::elect_one() && !gave_up) {
+          if (rank == 0) cxt::expect_bytes(own, bytes);
           if (!across) {
             cxt::load_tile<CG>(at, map, s * kDepth, first, full);
           } else {
@@ -417,11 +422,6 @@ tensor_product_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_c
           }
         }
         __syncwarp();
-        if (filled < S::kStages) ++filled;
-        if (++stage == S::kStages) {
-          stage = 0;
-          phase ^= 1u;
-        }
       }
     }
     // until the stages are free again: no copy is in flight, and no arrival of the pair's on its way, when the CTA ends
@@ -430,15 +430,13 @@ tensor_product_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_c
         stage = S::kStages - 1;
         phase ^= 1u;
       }
-      if (!cxt::wait(bar_empty + 8 * stage, phase)) {
-        gave_up = true;
-        break;
-      }
+      if (!gave_up) gave_up = !cxt::wait(bar_empty + 8 * stage, phase);
     }
   } else if (warp == 1 && rank == 0) {
     int stage = 0, turn = 0;
     uint32_t phase = 0;
-    for (; w.more() && !gave_up; w.next(), ++turn) {
+    bool ready = false;
+    for (; w.more(); w.next(), ++turn) {
       const Job& job = t.job[w.job];
       if (turn) u = unit_of(job, w.u);
       const bool along_m = job.p.layout == kTN, along_n = job.p.layout != kNT;
@@ -447,31 +445,26 @@ tensor_product_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_c
       const uint32_t step_a = along_m ? 128 : 2, step_b = along_n ? 128 : 2;
       const uint32_t first_a = cxt::operand_at(cx::smem_u32(stages), along_m ? 8192 : 16);
       const uint32_t first_b = cxt::operand_at(cx::smem_u32(stages) + S::kA, along_n ? 8192 : 16);
-      if (!cxt::wait(bar_taken + 8 * (turn & 1), ((turn >> 1) & 1) ^ 1u)) {
-        gave_up = true;
-        break;
-      }
+      if (!gave_up) gave_up = !cxt::wait(bar_taken + 8 * (turn & 1), ((turn >> 1) & 1) ^ 1u);
       cxt::fence_after_sync();
       const uint32_t sums = tmem + (turn & 1) * BN;
       for (int s = u.s0; s < u.s1; ++s) {
-        if (!cxt::wait(bar_full + 8 * stage, phase)) {
-          gave_up = true;
-          break;
-        }
+        if (!ready && !gave_up) gave_up = !cxt::wait(bar_full + 8 * stage, phase);
         cxt::fence_after_sync();
-        const uint32_t a = first_a + stage * (S::kStage >> 4), b = first_b + stage * (S::kStage >> 4);
-        if (cxt::elect_one()) {
-#pragma unroll
-          for (int k = 0; k < kDepth / 16; ++k) cxt::mma<CG>(sums, a + k * step_a, b + k * step_b, instr, s > u.s0 || k > 0);
-          cxt::commit<CG>(bar_empty + 8 * stage);
-        }
-        __syncwarp();
+        const uint32_t a = first_a + stage * (S::kStage >> 4), b = first_b + stage * (S::kStage >> 4), free = bar_empty + 8 * stage;
         if (++stage == S::kStages) {
           stage = 0;
           phase ^= 1u;
         }
+        ready = cxt::look(bar_full + 8 * stage, phase);
+        if (cxt::elect_one() && !gave_up) {
+#pragma unroll
+          for (int k = 0; k < kDepth / 16; ++k) cxt::mma<CG>(sums, a + k * step_a, b + k * step_b, instr, s > u.s0 || k > 0);
+          cxt::commit<CG>(free);
+        }
+        __syncwarp();
       }
-      if (cxt::elect_one()) cxt::commit<CG>(bar_sums + 8 * (turn & 1));
+      if (cxt::elect_one() && !gave_up) cxt::commit<CG>(bar_sums + 8 * (turn & 1));
       __syncwarp();
     }
   } else if (warp >= 4) {
@@ -491,7 +484,7 @@ tensor_product_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_c
         }
         __syncwarp();
       }
-      if (!cxt::wait(bar_sums + 8 * (turn & 1), (turn >> 1) & 1)) {
+      if (!cxt::wait_together(bar_sums + 8 * (turn & 1), (turn >> 1) & 1)) {
         gave_up = true;
         break;
       }
@@ -586,33 +579,8 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 struct Choice {
   int cg, bn, splits[2];
+  double time;
 };
-
-Choice choose(const CxProduct* p, int count) {
-  int64_t big = 0, tiles = 0;
-  bool sums = true;
-  for (int i = 0; i < count; ++i) {
-    big += ceil_div(p[i].m, 256) * ceil_div(p[i].n, 256);
-    tiles += ceil_div(p[i].m, 128) * ceil_div(p[i].n, 128);
-    sums = sums && (p[i].mode == kOut || p[i].mode == kSums);
-  }
-  if (big >= 60) return {2, 256, {1, 1}};
-  Choice c = {1, tiles < 74 && sums ? 64 : 128, {1, 1}};
-  if (!sums) return c;
-  tiles = 0;
-  for (int i = 0; i < count; ++i) tiles += ceil_div(p[i].m, 128) * ceil_div(p[i].n, c.bn);
-  for (int i = 0; i < count; ++i) {
-    const int64_t most = ceil_div(p[i].k, kDepth) / 8, splits = 148 / tiles;
-    c.splits[i] = (int)(splits < most ? splits : most);
-    if (c.splits[i] < 1) c.splits[i] = 1;
-  }
-  return c;
-}
-
-int align_of(const void* p, int64_t ld) {
-  const uintptr_t a = reinterpret_cast<uintptr_t>(p) | (uintptr_t)(ld * 2);
-  return a % 32 == 0 ? 2 : a % 16 == 0 ? 1 : 0;
-}
 
 // Who takes what: a unit lasts as long as its slices.  The first job's `a` units go round the workers, the second one's
 // are given out so that the last worker is done as early as can be; returns that time.
@@ -636,6 +604,60 @@ int64_t share_out(int64_t a, int64_t la, int64_t b, int64_t lb, int64_t workers,
   *many = (int)m;
   const int64_t t_few = more ? (rounds + 1) * la + f * lb : 0, t_many = rounds * la + m * lb;
   return t_few > t_many ? t_few : t_many;
+}
+
+// What a launch takes, in us: `fixed`, and for the last worker `slice` for each of its slices of k and `tile` for each of
+// its units.  Measured alone on the GPU at 1.9 GHz: 128 x 64 tiles 5.4 / 6.5 / 13.5 us for one unit of 8 / 16 / 64 slices and
+// 47 for 14 units of 16, 128 x 128 tiles 6.1 / 7.4 / 14.7 and 35 for 7 of 16, pairs' 256 x 256 tiles 7.9 / 11.6 / 24 and 29.5
+// for 4 of 16; joining the splits of 1 M results 3.1 us for two, 3.9 for four.
+struct Cost {
+  int cg, bn;
+  double fixed, slice, tile;
+};
+constexpr Cost kCosts[3] = {{2, 256, 5.7, 0.27, 1.3}, {1, 128, 4.2, 0.17, 1.0}, {1, 64, 3.7, 0.146, 0.65}};
+constexpr double kJoin = 2.2, kJoinBytes = 6e6;      // us, and bytes of partial sums a us
+
+// The tile and the splits along k that are done first.  A product is split where its own units are longer than an even
+// share of all there is: few rows (or few results of a long sum) fill the GPU so, others are not worth the joining.
+Choice choose(const CxProduct* p, int count) {
+  const bool sums = p[0].mode == kOut || p[0].mode == kSums;
+  Choice best = {};
+  for (const Cost& c : kCosts) {
+    const int64_t most = cx_sm_count() / c.cg;
+    int64_t tiles[2] = {}, slices[2] = {}, total = 0;
+    for (int i = 0; i < count; ++i) {
+      tiles[i] = ceil_div(p[i].m, 128 * c.cg) * ceil_div(p[i].n, c.bn);
+      slices[i] = ceil_div(p[i].k, kDepth);
+      total += tiles[i] * slices[i];
+    }
+    int64_t limit[2] = {1, 1};
+    for (int i = 0; i < count; ++i)
+      if (sums && slices[i] * most > total + total / 4) limit[i] = slices[i] / 4 < 16 ? slices[i] / 4 : 16;
+    for (int64_t s0 = 1; s0 == 1 || s0 <= limit[0]; s0 += s0 < 4 ? 1 : s0 / 2)
+      for (int64_t s1 = 1; s1 == 1 || s1 <= limit[1]; s1 += s1 < 4 ? 1 : s1 / 2) {
+        const int64_t split[2] = {s0, s1};
+        int64_t units[2] = {}, len[2] = {}, all = 0;
+        double join = 0;
+        for (int i = 0; i < count; ++i) {
+          len[i] = ceil_div(slices[i], split[i]);
+          units[i] = tiles[i] * ceil_div(slices[i], len[i]);
+          all += units[i];
+          if (split[i] > 1) join += (double)split[i] * p[i].m * p[i].n * 4 / kJoinBytes;
+        }
+        int extra, few, many;
+        const int64_t workers = all < most ? all : most;
+        const bool swap = len[0] < len[1];
+        const int64_t last = share_out(units[swap], len[swap], units[!swap], len[!swap], workers, &extra, &few, &many);
+        const double time = c.fixed + c.slice * last + c.tile * ceil_div(all, workers) + (join > 0 ? join + kJoin : 0);
+        if (!best.cg || time < best.time) best = {c.cg, c.bn, {(int)s0, (int)s1}, time};
+      }
+  }
+  return best;
+}
+
+int align_of(const void* p, int64_t ld) {
+  const uintptr_t a = reinterpret_cast<uintptr_t>(p) | (uintptr_t)(ld * 2);
+  return a % 32 == 0 ? 2 : a % 16 == 0 ? 1 : 0;
 }
 
 template <int CG, int BN>
@@ -679,20 +701,7 @@ int launch(const Plan& t, int count, cudaStream_t s) {
 bool cx_tensor_product_takes(const CxProduct& p) {
   return p.dtype != CX_F32 && ((reinterpret_cast<uintptr_t>(p.a) | reinterpret_cast<uintptr_t>(p.b)) & 15) == 0 && p.lda % 8 == 0 && p.ldb % 8 == 0;
 }
-double cx_tensor_product_time(const CxProduct* p, int count) {
-  const Choice c = choose(p, count);
-  int64_t units[2] = {}, slices[2] = {}, all = 0;
-  const bool swap = count == 2 && ceil_div(ceil_div(p[0].k, kDepth), c.splits[0]) < ceil_div(ceil_div(p[1].k, kDepth), c.splits[1]);
-  for (int i = 0; i < count; ++i) {
-    const CxProduct& q = p[swap ? 1 - i : i];
-    slices[i] = ceil_div(ceil_div(q.k, kDepth), c.splits[swap ? 1 - i : i]);
-    units[i] = ceil_div(q.m, 128 * c.cg) * ceil_div(q.n, c.bn) * c.splits[swap ? 1 - i : i];
-    all += units[i];
-  }
-  int extra, few, many;
-  const int64_t most = cx_sm_count() / c.cg;
-  return (double)share_out(units[0], slices[0], units[1], slices[1], all < most ? all : most, &extra, &few, &many) + 12.0;
-}
+double cx_tensor_product_time(const CxProduct* p, int count) { return choose(p, count).time; }
 int cx_tensor_product_stat_columns(const CxProduct& p) { return choose(&p, 1).bn / 2; }
 
 int cx_tensor_product(CxProduct* p, int count, cxprod::Arena& ws, cudaStream_t s) {
