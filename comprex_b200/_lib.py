@@ -112,7 +112,7 @@ REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
 
 class Linear(C.Structure):
     """Arguments of cx_linear_forward and cx_linear_backward (CxLinear in csrc/cx_ops.h)."""
-    _fields_ = ([(n, C.c_int64) for n in ("rows", "inner", "outer", "ldx", "ldw", "ldr", "ldg")]
+    _fields_ = ([(n, C.c_int64) for n in ("rows", "inner", "outer", "ldx", "ldw", "ldr", "ldg", "ldpre")]
                 + [(n, C.c_void_p) for n in ("x", "w", "bias", "residual", "y", "pre", "grad", "dx", "dw", "dbias", "workspace")]
                 + [("ws_bytes", C.c_int64), ("dtype", C.c_int32), ("act", C.c_int32)])
 

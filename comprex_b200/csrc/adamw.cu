@@ -25,12 +25,8 @@ __device__ __forceinline__ void step1(const CxAdamWClass& c, float g, float& p, 
   p = p * c.decay - (m * c.rate) / (root * c.norm + c.eps);
 }
 
-// |x| < 256 with 16 random bits under the mantissa's end; NaN where x is no number
-__device__ __forceinline__ float cut(float x, uint32_t bits16) {
-  const uint32_t raw = __float_as_uint(x) & 0x7FFFFFFFu;
-  const float q = __uint_as_float(((raw + (bits16 << 4)) & ~0xFFFFFu) | (__float_as_uint(x) & 0x80000000u));
-  return raw < 0x7F800000u ? q : __uint_as_float(0x7FC00000u);
-}
+// |x| < 256 with 16 random bits under the mantissa's end: they are added below the sign, and what is below is cut off
+__device__ __forceinline__ float cut(float x, uint32_t bits16) { return __uint_as_float((__float_as_uint(x) + (bits16 << 4)) & 0xFFF00000u); }
 __device__ __forceinline__ uint32_t pack4(const float (&x)[4]) {
   const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(x[0], x[1]), __NV_SATFINITE, __NV_E4M3);
   const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(x[2], x[3]), __NV_SATFINITE, __NV_E4M3);
@@ -106,9 +102,12 @@ __global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__
         }
       }
     float inv_m = 0.f, inv_v = 0.f;
+    bool fine = true;                     // no element of the block is infinite or no number
     if (EIGHT) {
-      const uint32_t e_m = __reduce_max_sync(0xFFFFFFFFu, top_m) >> 23;
-      const uint32_t e_v = cxadam::root_exponent(__reduce_max_sync(0xFFFFFFFFu, top_v) >> 23);
+      top_m = __reduce_max_sync(0xFFFFFFFFu, top_m);
+      top_v = __reduce_max_sync(0xFFFFFFFFu, top_v);
+      const uint32_t e_m = top_m >> 23, e_v = cxadam::root_exponent(top_v >> 23);
+      fine = max(top_m, top_v) < 0x7F800000u;
       inv_m = __uint_as_float(cxadam::inverse_bits(e_m));
       inv_v = __uint_as_float(cxadam::inverse_bits(e_v));
       if (lane == 0) {
@@ -134,8 +133,15 @@ __global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__
         for (int k = 0; k < 4; ++k) {
           const uint32_t bits = cxadam::random_bits((uint32_t)(flat + e + k), a.noise);
           qm[k] = cut(s[h].m[k] * inv_m, bits & 0xFFFFu);
-          const float q = cut(root[h][k] * inv_v, bits >> 16);
-          qv[k] = s[h].v[k] == 0.f ? 0.f : q < 0x1p-9f ? 0x1p-9f : q;
+          const float q = fmaxf(cut(root[h][k] * inv_v, bits >> 16), 0x1p-9f);
+          qv[k] = s[h].v[k] == 0.f ? 0.f : q;
+        }
+        if (!fine) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            if (!(fabsf(s[h].m[k]) < INFINITY)) qm[k] = NAN;
+            if (!(s[h].v[k] < INFINITY)) qv[k] = NAN;
+          }
         }
         reinterpret_cast<uint32_t*>(a.m)[(flat + e) / 4] = pack4(qm);
         reinterpret_cast<uint32_t*>(a.v)[(flat + e) / 4] = pack4(qv);

@@ -51,17 +51,18 @@ int cx_adamw_step(int dev, const CxAdamW* a, void* stream);
 #define CX_ACT_GELU_TANH 3   /* its tanh form */
 #define CX_ACT_SILU 4
 
-/* Matrices are row-major with rows `ld*` elements apart; y, dx, dw are written without gaps.  All of one type. */
+/* Matrices are row-major with rows `ld*` elements apart (ldpre: 16-byte aligned rows are the fast case); y, dx, dw are
+ * written without gaps.  All of one type. */
 typedef struct CxLinear {
   int64_t rows, inner, outer;
-  int64_t ldx, ldw, ldr, ldg;
+  int64_t ldx, ldw, ldr, ldg, ldpre;
   const void* x;         /* [rows][inner] */
   const void* w;         /* [outer][inner] */
   const void* bias;      /* [outer] or NULL */
   const void* residual;  /* [rows][outer] or NULL */
   void* y;               /* forward: [rows][outer] */
   void* pre;             /* x w^T + bias: written by the forward call when not NULL, read by the backward call where the
-                            activation needs it; [rows][outer] */
+                            activation needs it; [rows][outer], rows ldpre apart */
   const void* grad;      /* backward: of y */
   void* dx;              /* each may be NULL */
   void* dw;

@@ -27,7 +27,8 @@ struct CxProduct {
   const void* bias;        // kOut: [n]
   const void* residual;    // kOut
   int64_t ldr;
-  void* pre;               // kOut: (C + addend) * scale + bias, rounded, rows ldo apart
+  void* pre;               // kOut: (C + addend) * scale + bias, rounded
+  int64_t ldpre;
   float* addend;           // [m][ldadd], 32-byte aligned rows
   int64_t ldadd;
   int32_t has_addend;      // it holds sums already
@@ -65,8 +66,7 @@ int cx_product_operand(const void** base, int64_t* ld, int dtype, int64_t rows, 
 // columns of a kStats tile
 int cx_product_stat_columns(const CxProduct& p);
 
-// tensor_product.cu: 16-bit types, operands that a tile copy can read (16-byte aligned rows)
-bool cx_tensor_product_takes(const CxProduct& p);
+// tensor_product.cu: 16-bit types, operands as cx_product_operand leaves them
 int cx_tensor_product_stat_columns(const CxProduct& p);
 // about how long that takes, in us
 double cx_tensor_product_time(const CxProduct* p, int count);

@@ -16,9 +16,9 @@ struct Du {
   const void* pre;
   void* du;             // NULL: not stored
   float* part;          // [chunks][outer], NULL: no sums
-  int64_t rows, outer, ldg, ldd;
+  int64_t rows, outer, ldg, ldpre, ldd;
   int32_t act;
-  int32_t wide_in, wide_out;       // 16-byte accesses are aligned
+  int32_t wide_grad, wide_pre, wide_out;       // 16-byte accesses are aligned
 };
 
 // du, and the sums of its columns over 64 rows.  Bound by memory: a thread has 8 neighbouring columns of 8 rows, all of
@@ -42,8 +42,8 @@ __global__ void __launch_bounds__(kThreads) du_kernel(const __grid_constant__ Du
     for (int j = 0; j < 4; ++j) {
       const int64_t r = r0 + 8 * (4 * h + j);
       const int have = r < d.rows ? left : 0;
-      cxprod::load8(grad + r * d.ldg, have == 8 && d.wide_in, have, g[j]);
-      if (act) cxprod::load8(pre + r * d.outer, have == 8 && d.wide_in, have, u[j]);
+      cxprod::load8(grad + r * d.ldg, have == 8 && d.wide_grad, have, g[j]);
+      if (act) cxprod::load8(pre + r * d.ldpre, have == 8 && d.wide_pre, have, u[j]);
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -98,13 +98,13 @@ __global__ void __launch_bounds__(kThreads) column_sum_kernel(const __grid_const
 template <typename T>
 int du_pass(Du& d, void* dbias, cudaStream_t s) {
   const int64_t chunks = (d.rows + kRowsPer - 1) / kRowsPer;
-  const uintptr_t in = reinterpret_cast<uintptr_t>(d.grad) | (d.act != CX_ACT_NONE ? reinterpret_cast<uintptr_t>(d.pre) : 0);
-  d.wide_in = (in & 15) == 0 && d.ldg % 8 == 0 && (d.act == CX_ACT_NONE || d.outer % 8 == 0);
+  d.wide_grad = (reinterpret_cast<uintptr_t>(d.grad) & 15) == 0 && d.ldg % 8 == 0;
+  d.wide_pre = (reinterpret_cast<uintptr_t>(d.pre) & 15) == 0 && d.ldpre % 8 == 0;
   d.wide_out = (reinterpret_cast<uintptr_t>(d.du) & 15) == 0 && d.ldd % 8 == 0;
   for (int64_t first = 0; first < chunks; first += 65535) {        // a grid's second dimension ends there
     Du part = d;
     part.grad = reinterpret_cast<const T*>(d.grad) + first * kRowsPer * d.ldg;
-    if (d.pre) part.pre = reinterpret_cast<const T*>(d.pre) + first * kRowsPer * d.outer;
+    if (d.pre) part.pre = reinterpret_cast<const T*>(d.pre) + first * kRowsPer * d.ldpre;
     if (d.du) part.du = reinterpret_cast<T*>(d.du) + first * kRowsPer * d.ldd;
     if (d.part) part.part = d.part + first * d.outer;
     part.rows = d.rows - first * kRowsPer;
@@ -126,15 +126,132 @@ int du_pass(Du& d, void* dbias, cudaStream_t s) {
   return cx_check_launch("cx_linear_backward");
 }
 
+// ---- few rows: tokens that are being decoded ------------------------------------------------------------------------
+// Bound by reading w, and at these sizes by latency: every weight is used once per row, so the tensor cores have nothing to
+// do.  A warp has four rows of w and a share of k, 256 elements at a time, all loads of a turn under way at once; `share`
+// warps of a block join their sums in a fixed order, and one thread per result does the rest.
+constexpr int kFewRows = 16, kFewColumns = 4, kWarps = kThreads / 32;
+
+struct Few {
+  const void* x;
+  const void* w;
+  const void* bias;
+  const void* residual;
+  void* y;
+  void* pre;
+  int64_t inner, outer, ldx, ldw, ldr, ldpre;
+  int rows, act, share;
+};
+
+// Sums of V values (4 to 16) over the warp, each in the lanes whose highest bits are its number.  A step halves what a lane
+// holds, so that V values take about V shuffles instead of 5 V.
+template <int V>
+__device__ __forceinline__ void warp_sums(float (&v)[V], int lane) {
+  int have = V;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    if (have > 1) {
+      have /= 2;
+#pragma unroll
+      for (int i = 0; i < V / 2; ++i)
+        if (i < have) {
+          const float give = lane & o ? v[i] : v[i + have], keep = lane & o ? v[i + have] : v[i];
+          v[i] = keep + __shfl_xor_sync(0xFFFFFFFFu, give, o);
+        }
+    } else {
+      v[0] += __shfl_xor_sync(0xFFFFFFFFu, v[0], o);
+    }
+  }
+}
+
+template <typename T, int R, bool WIDE>
+__global__ void __launch_bounds__(kThreads) few_rows_kernel(const __grid_constant__ Few d) {
+  constexpr int V = R * kFewColumns;
+  __shared__ float sums[kWarps][V];
+  cx::pdl_trigger();
+  cx::pdl_wait();
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, groups = kWarps / d.share;
+  const int64_t c0 = ((int64_t)blockIdx.x * groups + warp / d.share) * kFewColumns;
+  const T* x = reinterpret_cast<const T*>(d.x);
+  const T* w = reinterpret_cast<const T*>(d.w) + c0 * d.ldw;
+  const int columns = (int)max((int64_t)0, min((int64_t)kFewColumns, d.outer - c0));
+  float acc[V] = {};
+  for (int64_t k = (warp % d.share) * 256 + lane * 8; k < d.inner; k += d.share * 256) {
+    const int left = (int)min((int64_t)8, d.inner - k);
+    float b[kFewColumns][8];
+#pragma unroll
+    for (int c = 0; c < kFewColumns; ++c) cxprod::load8(w + c * d.ldw + k, WIDE && left == 8 && c < columns, c < columns ? left : 0, b[c]);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      float a[8];
+      cxprod::load8(x + r * d.ldx + k, WIDE && left == 8 && r < d.rows, r < d.rows ? left : 0, a);
+#pragma unroll
+      for (int c = 0; c < kFewColumns; ++c)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) acc[r * kFewColumns + c] = __fmaf_rn(a[i], b[c][i], acc[r * kFewColumns + c]);
+    }
+  }
+  warp_sums<V>(acc, lane);
+  // a lane holds the value that its number says, highest bit first
+  constexpr int kBits = V == 16 ? 4 : V == 8 ? 3 : 2;
+  int at = 0, size = V;
+#pragma unroll
+  for (int i = 0; i < kBits; ++i) {
+    size /= 2;
+    at += lane & (16 >> i) ? size : 0;
+  }
+  sums[warp][at] = acc[0];
+  __syncthreads();
+  for (int i = threadIdx.x; i < groups * V; i += kThreads) {
+    const int g = i / V, r = i % V / kFewColumns;
+    const int64_t c = ((int64_t)blockIdx.x * groups + g) * kFewColumns + i % kFewColumns;
+    if (r >= d.rows || c >= d.outer) continue;
+    float v[1] = {0.f};
+    for (int j = 0; j < d.share; ++j) v[0] += sums[g * d.share + j][i % V];
+    using E = cx::Elem<T>;
+    if (d.bias) v[0] += E::to_f(reinterpret_cast<const T*>(d.bias)[c]);
+    if (d.pre) reinterpret_cast<T*>(d.pre)[r * d.ldpre + c] = E::from_f(v[0]);
+    cxprod::activate(v, d.act);
+    if (d.residual) v[0] += E::to_f(reinterpret_cast<const T*>(d.residual)[r * d.ldr + c]);
+    reinterpret_cast<T*>(d.y)[r * d.outer + c] = E::from_f(v[0]);
+  }
+}
+
+template <typename T, int R>
+void few_rows_of(const Few& d, bool wide, dim3 grid, cudaStream_t s) {
+  if (wide) cx_launch_pdl2(few_rows_kernel<T, R, true>, grid, kThreads, s, d);
+  else cx_launch_pdl2(few_rows_kernel<T, R, false>, grid, kThreads, s, d);
+}
+
+template <typename T>
+int few_rows(const CxLinear& l, cudaStream_t s) {
+  Few d = {l.x, l.w, l.bias, l.residual, l.y, l.pre, l.inner, l.outer, l.ldx, l.ldw, l.ldr, l.ldpre, (int)l.rows, l.act, 1};
+  while (d.share < kWarps && d.share * 512 < l.inner) d.share *= 2;
+  constexpr int64_t per = 16 / sizeof(T);
+  const bool wide = ((reinterpret_cast<uintptr_t>(l.x) | reinterpret_cast<uintptr_t>(l.w)) & 15) == 0 && l.ldx % per == 0 && l.ldw % per == 0;
+  const int64_t columns = kFewColumns * kWarps / d.share;
+  const dim3 grid((unsigned)((l.outer + columns - 1) / columns));
+  if (l.rows == 1) few_rows_of<T, 1>(d, wide, grid, s);
+  else if (l.rows <= 2) few_rows_of<T, 2>(d, wide, grid, s);
+  else few_rows_of<T, 4>(d, wide, grid, s);
+  cx_note_launch();
+  return cx_check_launch("cx_linear_forward");
+}
+
 // Both calls also run without a workspace: they launch nothing then and count the bytes that they need.
 int forward(const CxLinear& l, cxprod::Arena& ws, cudaStream_t s) {
+  if (l.rows <= 2 || (l.rows <= 4 && l.outer * l.inner <= (8 << 20))) {
+    if (!ws.base) return 0;
+    return l.dtype == CX_F32 ? few_rows<float>(l, s) : l.dtype == CX_BF16 ? few_rows<__nv_bfloat16>(l, s) : few_rows<__half>(l, s);
+  }
   CxProduct p = {};
   p.m = l.rows; p.n = l.outer; p.k = l.inner;
   p.a = l.x; p.lda = l.ldx; p.b = l.w; p.ldb = l.ldw;
   p.layout = kNT; p.dtype = l.dtype; p.act = l.act;
-  p.out = l.y; p.ldo = l.outer; p.bias = l.bias; p.residual = l.residual; p.ldr = l.ldr; p.pre = l.pre;
+  p.out = l.y; p.ldo = l.outer; p.bias = l.bias; p.residual = l.residual; p.ldr = l.ldr; p.pre = l.pre; p.ldpre = l.ldpre;
   int rc = cx_product_operand(&p.a, &p.lda, l.dtype, l.rows, l.inner, ws, s);
   if (!rc) rc = cx_product_operand(&p.b, &p.ldb, l.dtype, l.outer, l.inner, ws, s);
+  if (!rc && p.residual) rc = cx_product_operand(&p.residual, &p.ldr, l.dtype, l.rows, l.outer, ws, s);
   return rc ? rc : cx_product(&p, 1, ws, s);
 }
 
@@ -142,7 +259,7 @@ int backward(const CxLinear& l, cxprod::Arena& ws, cudaStream_t s) {
   const int64_t size = l.dtype == CX_F32 ? 4 : 2;
   Du d = {};
   d.grad = l.grad; d.pre = l.pre;
-  d.rows = l.rows; d.outer = l.outer; d.ldg = l.ldg; d.act = l.act;
+  d.rows = l.rows; d.outer = l.outer; d.ldg = l.ldg; d.ldpre = l.ldpre; d.act = l.act;
   const void* du = l.grad;
   int64_t ldd = l.ldg;
   if (l.act != CX_ACT_NONE && (l.dx || l.dw)) {

@@ -61,7 +61,7 @@ int64_t cx_linear_workspace_bytes(int dev, const CxLinear* l, int backward) {
 int cx_linear_forward(int dev, const CxLinear* l, void* stream) {
   if (const char* why = wrong(l)) return cx_set_error(why, 0);
   if (!l->x || !l->w || !l->y) return cx_set_error("cx_linear_forward: an operand is missing", 0);
-  if (l->ldx < l->inner || l->ldw < l->inner || (l->residual && l->ldr < l->outer))
+  if (l->ldx < l->inner || l->ldw < l->inner || (l->residual && l->ldr < l->outer) || (l->pre && l->ldpre < l->outer))
     return cx_set_error("cx_linear_forward: rows overlap", 0);
   return dev == CX_DEV_CUDA ? cx_linear_forward_cuda(l, stream) : cx_linear_forward_host(l);
 }
@@ -70,7 +70,7 @@ int cx_linear_backward(int dev, const CxLinear* l, void* stream) {
   if (const char* why = wrong(l)) return cx_set_error(why, 0);
   if (!l->grad || (l->dx && !l->w) || (l->dw && !l->x) || (l->act != CX_ACT_NONE && !l->pre))
     return cx_set_error("cx_linear_backward: an operand is missing", 0);
-  if (l->ldg < l->outer || (l->dw && l->ldx < l->inner) || (l->dx && l->ldw < l->inner))
+  if (l->ldg < l->outer || (l->act != CX_ACT_NONE && l->ldpre < l->outer) || (l->dw && l->ldx < l->inner) || (l->dx && l->ldw < l->inner))
     return cx_set_error("cx_linear_backward: rows overlap", 0);
   return dev == CX_DEV_CUDA ? cx_linear_backward_cuda(l, stream) : cx_linear_backward_host(l);
 }

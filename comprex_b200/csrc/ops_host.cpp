@@ -155,7 +155,7 @@ int cx_linear_forward_host(const CxLinear* l) {
     for (int64_t c = 0; c < l->outer; ++c) {
       float u = dot(&x[(size_t)(r * l->inner)], &w[(size_t)(c * l->inner)], l->inner), slope;
       if (l->bias) u += load_elem(l->dtype, l->bias, c);
-      if (l->pre) store_elem(l->dtype, l->pre, r * l->outer + c, u);
+      if (l->pre) store_elem(l->dtype, l->pre, r * l->ldpre + c, u);
       u = act_host(u, l->act, &slope);
       if (l->residual) u += load_elem(l->dtype, l->residual, r * l->ldr + c);
       store_elem(l->dtype, l->y, r * l->outer + c, u);
@@ -169,7 +169,7 @@ int cx_linear_backward_host(const CxLinear* l) {
     for (int64_t c = 0; c < l->outer; ++c) {
       float& d = du[(size_t)(r * l->outer + c)];
       float slope = 1.f;
-      if (l->act != CX_ACT_NONE) act_host(load_elem(l->dtype, l->pre, r * l->outer + c), l->act, &slope);
+      if (l->act != CX_ACT_NONE) act_host(load_elem(l->dtype, l->pre, r * l->ldpre + c), l->act, &slope);
       d *= slope;
       sum[(size_t)c] += d;
     }

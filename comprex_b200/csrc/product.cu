@@ -1,13 +1,12 @@
-// The product of cx_product.cuh on the CUDA cores: any type, layout and stride.
+// The product of cx_product.cuh for operands of 32 bits, on the CUDA cores (the tensor cores round them to 11 bits): any
+// layout and stride.  Not what this package trains large models in; 20 TFLOP/s.
 #include "cx_product.cuh"
 
 namespace {
 
 constexpr int kTile = 64, kDepth = 16, kThreads = 256;
 
-template <typename T>
 __device__ __forceinline__ void finish(const CxProduct& p, int64_t row, int64_t col, float v) {
-  using E = cx::Elem<T>;
   if (p.mode == kSums) {
     float* at = p.addend + row * p.ldadd + col;
     *at = p.has_addend ? *at + v : v;
@@ -16,29 +15,27 @@ __device__ __forceinline__ void finish(const CxProduct& p, int64_t row, int64_t 
   if (p.mode == kProb) {
     const float q = exp2f(v * cxprod::kLog2e - p.lse[row]) - (p.targets[row] == p.col0 + col ? 1.f : 0.f);
     const float f = p.row_factor[row];
-    reinterpret_cast<T*>(p.out)[row * p.ldo + col] = E::from_f(f == 0.f ? 0.f : q * f);
+    reinterpret_cast<float*>(p.out)[row * p.ldo + col] = f == 0.f ? 0.f : q * f;
     return;
   }
   if (p.has_addend) v += p.addend[row * p.ldadd + col];
   if (p.scale) v *= *p.scale;
-  if (p.bias) v += E::to_f(reinterpret_cast<const T*>(p.bias)[col]);
-  if (p.pre) reinterpret_cast<T*>(p.pre)[row * p.ldo + col] = E::from_f(v);
+  if (p.bias) v += reinterpret_cast<const float*>(p.bias)[col];
+  if (p.pre) reinterpret_cast<float*>(p.pre)[row * p.ldpre + col] = v;
   float one[1] = {v};
   cxprod::activate(one, p.act);
   v = one[0];
-  if (p.residual) v += E::to_f(reinterpret_cast<const T*>(p.residual)[row * p.ldr + col]);
-  reinterpret_cast<T*>(p.out)[row * p.ldo + col] = E::from_f(v);
+  if (p.residual) v += reinterpret_cast<const float*>(p.residual)[row * p.ldr + col];
+  reinterpret_cast<float*>(p.out)[row * p.ldo + col] = v;
 }
 
-template <typename T>
 __global__ void __launch_bounds__(kThreads) product_kernel(const __grid_constant__ CxProduct p) {
   __shared__ float sa[kDepth][kTile + 1], sb[kDepth][kTile + 1];
   __shared__ float2 stat[kTile][16];
-  using E = cx::Elem<T>;
   const int64_t row0 = (int64_t)blockIdx.x * kTile, col0 = (int64_t)blockIdx.y * kTile;
   const int tr = threadIdx.x / 16, tc = threadIdx.x % 16;
-  const T* a = reinterpret_cast<const T*>(p.a);
-  const T* b = reinterpret_cast<const T*>(p.b);
+  const float* a = reinterpret_cast<const float*>(p.a);
+  const float* b = reinterpret_cast<const float*>(p.b);
   float acc[4][4] = {};
   for (int64_t k0 = 0; k0 < p.k; k0 += kDepth) {
 #pragma unroll
@@ -49,8 +46,8 @@ __global__ void __launch_bounds__(kThreads) product_kernel(const __grid_constant
       const int kb = p.layout == kNT ? i % kDepth : i / kTile, nb = p.layout == kNT ? i / kDepth : i % kTile;
       const int64_t r = row0 + ma, c = col0 + nb;
       const bool in_a = r < p.m && k0 + ka < p.k, in_b = c < p.n && k0 + kb < p.k;
-      sa[ka][ma] = !in_a ? 0.f : E::to_f(p.layout == kTN ? a[(k0 + ka) * p.lda + r] : a[r * p.lda + k0 + ka]);
-      sb[kb][nb] = !in_b ? 0.f : E::to_f(p.layout == kNT ? b[c * p.ldb + k0 + kb] : b[(k0 + kb) * p.ldb + c]);
+      sa[ka][ma] = !in_a ? 0.f : p.layout == kTN ? a[(k0 + ka) * p.lda + r] : a[r * p.lda + k0 + ka];
+      sb[kb][nb] = !in_b ? 0.f : p.layout == kNT ? b[c * p.ldb + k0 + kb] : b[(k0 + kb) * p.ldb + c];
     }
     __syncthreads();
 #pragma unroll
@@ -73,7 +70,7 @@ __global__ void __launch_bounds__(kThreads) product_kernel(const __grid_constant
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int64_t r = row0 + tr * 4 + i, c = col0 + tc * 4 + j;
-        if (r < p.m && c < p.n) finish<T>(p, r, c, acc[i][j]);
+        if (r < p.m && c < p.n) finish(p, r, c, acc[i][j]);
       }
     return;
   }
@@ -147,24 +144,16 @@ int cx_product_operand(const void** base, int64_t* ld, int dtype, int64_t rows, 
   return cx_check_launch("cx_product");
 }
 
-int cx_product_stat_columns(const CxProduct& p) { return cx_tensor_product_takes(p) ? cx_tensor_product_stat_columns(p) : kTile; }
-
-static int plain_product(const CxProduct& p, cudaStream_t s) {
-  const dim3 grid((unsigned)((p.m + kTile - 1) / kTile), (unsigned)((p.n + kTile - 1) / kTile));
-  if (p.dtype == CX_F32) product_kernel<float><<<grid, kThreads, 0, s>>>(p);
-  else if (p.dtype == CX_BF16) product_kernel<__nv_bfloat16><<<grid, kThreads, 0, s>>>(p);
-  else product_kernel<__half><<<grid, kThreads, 0, s>>>(p);
-  cx_note_launch();
-  return cx_check_launch("cx_product");
-}
+int cx_product_stat_columns(const CxProduct& p) { return p.dtype != CX_F32 ? cx_tensor_product_stat_columns(p) : kTile; }
 
 int cx_product(CxProduct* p, int count, cxprod::Arena& ws, cudaStream_t s) {
-  bool tensor = true;
-  for (int i = 0; i < count; ++i) tensor = tensor && cx_tensor_product_takes(p[i]);
-  if (tensor) return cx_tensor_product(p, count, ws, s);
+  if (p[0].dtype != CX_F32) return cx_tensor_product(p, count, ws, s);
   if (!ws.base) return 0;
   if (!ws.ok()) return cx_set_error("cx_product: workspace too small", 0);
-  int rc = 0;
-  for (int i = 0; i < count && !rc; ++i) rc = plain_product(p[i], s);
-  return rc;
+  for (int i = 0; i < count; ++i) {
+    const dim3 grid((unsigned)((p[i].m + kTile - 1) / kTile), (unsigned)((p[i].n + kTile - 1) / kTile));
+    product_kernel<<<grid, kThreads, 0, s>>>(p[i]);
+    cx_note_launch();
+  }
+  return cx_check_launch("cx_product");
 }

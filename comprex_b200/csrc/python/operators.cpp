@@ -133,8 +133,10 @@ Tensor linear_forward(const Tensor& x, const Tensor& w, const Maybe& bias, int a
   std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
   shape.back() = outer;
   Tensor y = at::empty(shape, x.options());
-  if (pre) *pre = at::empty(shape, x.options());
-  if (!y.numel()) return y;
+  if (!y.numel()) {
+    if (pre) *pre = at::empty({0}, x.options());
+    return y;
+  }
   const c10::OptionalDeviceGuard guard(x.is_cuda() ? std::make_optional(x.device()) : std::nullopt);
   const Tensor xm = rows_of(x, inner), wm = rows_of(w, inner), b = bias ? bias->contiguous() : Tensor(), r = residual ? rows_of(*residual, outer) : Tensor();
   CxLinear d = describe(xm, wm, act);
@@ -144,7 +146,11 @@ Tensor linear_forward(const Tensor& x, const Tensor& w, const Maybe& bias, int a
     d.ldr = ld_of(r);
   }
   d.y = y.data_ptr();
-  if (pre) d.pre = pre->data_ptr();
+  if (pre) {                                  // kept for the backward call, in aligned rows
+    d.ldpre = (outer + 15) / 16 * 16;
+    *pre = at::empty({d.rows, d.ldpre}, x.options());
+    d.pre = pre->data_ptr();
+  }
   const Tensor ws = workspace(d, x, native.linear_bytes(dev_of(x), &d, 0));
   done(native.linear_forward(dev_of(x), &d, stream_of(x)), "cx_linear_forward");
   return y;
@@ -185,7 +191,10 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
       CxLinear d = describe(xm, wm, (int)act);
       d.grad = gm.data_ptr();
       d.ldg = ld_of(gm);
-      if (pre.defined()) d.pre = pre.data_ptr();
+      if (pre.defined()) {
+        d.pre = pre.data_ptr();
+        d.ldpre = pre.size(1);
+      }
       if (out[0].defined()) d.dx = out[0].data_ptr();
       if (out[1].defined()) d.dw = out[1].data_ptr();
       if (out[2].defined()) d.dbias = out[2].data_ptr();
