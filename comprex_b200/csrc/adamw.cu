@@ -14,15 +14,23 @@ namespace {
 
 constexpr int kThreads = 256;
 
-struct State4 {
-  float p[4], m[4], v[4];
-};
-
-__device__ __forceinline__ void step1(const CxAdamWClass& c, float g, float& p, float& m, float& v, float& root) {
-  m = m * c.b1 + g * c.ob1;
-  v = v * c.b2 + (g * c.ob2) * g;
-  root = sqrtf(v);
-  p = p * c.decay - (m * c.rate) / (root * c.norm + c.eps);
+// The hardware's square root and reciprocal, about 2^-23 off each, one instruction instead of ten: the moments themselves
+// are exact sums, the step is lr-sized, and what the root is kept as has 3 bits of mantissa.
+__device__ __forceinline__ float approx_root(float x) {
+  float y;
+  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float approx_inverse(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// The larger magnitude of three; NaN where one is
+__device__ __forceinline__ float top3(float a, float b, float c) {
+  float d;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
 }
 
 // |x| < 256 with 16 random bits under the mantissa's end: they are added below the sign, and what is below is cut off
@@ -32,123 +40,163 @@ __device__ __forceinline__ uint32_t pack4(const float (&x)[4]) {
   const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(x[2], x[3]), __NV_SATFINITE, __NV_E4M3);
   return lo | hi << 16;
 }
-__device__ __forceinline__ void unpack4(uint32_t w, float scale, float (&x)[4]) {
+__device__ __forceinline__ void unpack4(uint32_t w, float (&x)[4]) {
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> (16 * h)), __NV_E4M3);
     const float2 f = __half22float2(__half2(r));
-    x[2 * h] = f.x * scale;
-    x[2 * h + 1] = f.y * scale;
+    x[2 * h] = f.x;
+    x[2 * h + 1] = f.y;
   }
 }
 
+// four elements as they lie in memory, and what a lane holds of a block: elements 4 lane to 4 lane + 3 of both halves
 template <typename T, bool EIGHT>
-__global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__ CxAdamW a) {
+struct Loaded {
+  typename cx::Raw4<T>::type g[2];
+  float4 p[2];
+  float4 m[EIGHT ? 1 : 2], v[EIGHT ? 1 : 2];
+  uint32_t m8[2], v8[2];
+};
+
+template <typename T, bool EIGHT>
+__global__ void __launch_bounds__(kThreads, 4) adamw_kernel(const __grid_constant__ CxAdamW a) {
+  using Raw = cx::Raw4<T>;
   const int lane = threadIdx.x & 31;
   const int64_t warps = (int64_t)gridDim.x * (kThreads / 32);
-  for (int64_t b = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); b < a.blocks; b += warps) {
-    const int seg = a.blk_seg[b];
-    const T* grad = reinterpret_cast<const T*>(a.seg_grad[seg]);
-    if (grad == nullptr) continue;
-    const CxAdamWClass& c = a.cls[a.seg_class[seg]];
-    const int64_t at = (b - a.seg_blk[seg]) * CX_ADAMW_BLOCK;          // in the tensor
-    const int64_t flat = b * CX_ADAMW_BLOCK;
-    const int left = (int)min((int64_t)CX_ADAMW_BLOCK, a.seg_len[seg] - at);
-    T* param = reinterpret_cast<T*>(a.seg_param[seg]) + at;
-    grad += at;
+  int64_t b = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
+  if (b >= a.blocks) return;
+  // a tensor's row of the tables is read when a block of another tensor comes; which tensor that is, a block ahead
+  int seg = a.blk_seg[b], known = -1;
+  const T* grad0 = nullptr;
+  T* param0 = nullptr;
+  int64_t first = 0, len = 0;
+  int cls = 0;
+  for (; b < a.blocks; b += warps) {
+    if (seg != known) {
+      known = seg;
+      grad0 = reinterpret_cast<const T*>(a.seg_grad[seg]);
+      param0 = reinterpret_cast<T*>(a.seg_param[seg]);
+      first = a.seg_blk[seg];
+      len = a.seg_len[seg];
+      cls = a.seg_class[seg];
+    }
+    if (b + warps < a.blocks) seg = a.blk_seg[b + warps];
+    if (grad0 == nullptr) continue;
+    const int64_t at = (b - first) * CX_ADAMW_BLOCK, flat = b * CX_ADAMW_BLOCK;
+    const int left = (int)min((int64_t)CX_ADAMW_BLOCK, len - at);
+    const T* grad = grad0 + at;
+    T* param = param0 + at;
     constexpr uintptr_t kWide = 4 * sizeof(T) - 1;
     const bool wide = left == CX_ADAMW_BLOCK && (((uintptr_t)param | (uintptr_t)grad) & kWide) == 0;
-    float scale_m = 0.f, scale_v = 0.f;
+    Loaded<T, EIGHT> in;
+    const CxAdamWClass& c = a.cls[cls];
+    // of what is kept, this much stays: with 8 bits times the scale, or its square (powers of two: the products with beta
+    // are what they are without them)
+    float keep_m = c.b1, keep_v = c.b2;
     if (EIGHT) {
-      scale_m = a.m_scale[b];
-      scale_v = a.v_scale[b];
+      const float scale = a.v_scale[b];
+      keep_m *= a.m_scale[b];
+      keep_v *= scale * scale;
     }
-    State4 s[2];
-    float g[2][4];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int e = h * 128 + lane * 4;
       if (wide) {
-        cx::load4(grad + e, g[h]);
-        if (sizeof(T) == 4) cx::load4(reinterpret_cast<const float*>(param) + e, s[h].p);
+        in.g[h] = Raw::load(grad + e);
+        if (sizeof(T) == 4) in.p[h] = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(param) + e);
       } else {
+        T g[4];
+        float p[4] = {};
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          g[h][k] = e + k < left ? cx::Elem<T>::to_f(grad[e + k]) : 0.f;
-          if (sizeof(T) == 4) s[h].p[k] = e + k < left ? cx::Elem<T>::to_f(param[e + k]) : 0.f;
+          g[k] = e + k < left ? grad[e + k] : cx::Elem<T>::from_f(0.f);
+          if (sizeof(T) == 4 && e + k < left) p[k] = cx::Elem<T>::to_f(param[e + k]);
         }
+        memcpy(&in.g[h], g, sizeof(g));
+        in.p[h] = make_float4(p[0], p[1], p[2], p[3]);
       }
-      if (sizeof(T) != 4) cx::load4(a.master + flat + e, s[h].p);
+      if (sizeof(T) != 4) in.p[h] = *reinterpret_cast<const float4*>(a.master + flat + e);
       if (EIGHT) {
-        unpack4(reinterpret_cast<const uint32_t*>(a.m)[(flat + e) / 4], scale_m, s[h].m);
-        unpack4(reinterpret_cast<const uint32_t*>(a.v)[(flat + e) / 4], scale_v, s[h].v);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) s[h].v[k] *= s[h].v[k];
+        in.m8[h] = reinterpret_cast<const uint32_t*>(a.m)[(flat + e) / 4];
+        in.v8[h] = reinterpret_cast<const uint32_t*>(a.v)[(flat + e) / 4];
       } else {
-        cx::load4(reinterpret_cast<const float*>(a.m) + flat + e, s[h].m);
-        cx::load4(reinterpret_cast<const float*>(a.v) + flat + e, s[h].v);
+        in.m[h] = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(a.m) + flat + e);
+        in.v[h] = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(a.v) + flat + e);
       }
     }
-    float root[2][4];
-    uint32_t top_m = 0, top_v = 0;
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        step1(c, g[h][k], s[h].p[k], s[h].m[k], s[h].v[k], root[h][k]);
-        if (EIGHT) {
-          top_m = max(top_m, __float_as_uint(s[h].m[k]) & 0x7FFFFFFFu);
-          top_v = max(top_v, __float_as_uint(s[h].v[k]) & 0x7FFFFFFFu);
-        }
-      }
-    float inv_m = 0.f, inv_v = 0.f;
-    bool fine = true;                     // no element of the block is infinite or no number
-    if (EIGHT) {
-      top_m = __reduce_max_sync(0xFFFFFFFFu, top_m);
-      top_v = __reduce_max_sync(0xFFFFFFFFu, top_v);
-      const uint32_t e_m = top_m >> 23, e_v = cxadam::root_exponent(top_v >> 23);
-      fine = max(top_m, top_v) < 0x7F800000u;
-      inv_m = __uint_as_float(cxadam::inverse_bits(e_m));
-      inv_v = __uint_as_float(cxadam::inverse_bits(e_v));
-      if (lane == 0) {
-        a.m_scale[b] = __uint_as_float(cxadam::scale_bits(e_m));
-        a.v_scale[b] = __uint_as_float(cxadam::scale_bits(e_v));
-      }
-    }
+    // the step; what is done with an element is stored at once, but for the states of 8 bits, which wait for their scale
+    float m[2][4], root[2][4], most_m = 0.f, most_v = 0.f;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int e = h * 128 + lane * 4;
+      float g[4], p[4] = {in.p[h].x, in.p[h].y, in.p[h].z, in.p[h].w}, v[4];
+      Raw::to_f(in.g[h], g);
+      if (EIGHT) {
+        unpack4(in.m8[h], m[h]);
+        unpack4(in.v8[h], v);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] *= v[k];            // 4 bits squared: exact
+      } else {
+        const float4 x = in.m[h], y = in.v[h];
+        m[h][0] = x.x, m[h][1] = x.y, m[h][2] = x.z, m[h][3] = x.w;
+        v[0] = y.x, v[1] = y.y, v[2] = y.z, v[3] = y.w;
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        m[h][k] = m[h][k] * keep_m + g[k] * c.ob1;
+        v[k] = v[k] * keep_v + (g[k] * c.ob2) * g[k];
+        root[h][k] = approx_root(v[k]);
+        p[k] = __fmaf_rn(p[k], c.decay, -(m[h][k] * c.rate * approx_inverse(__fmaf_rn(root[h][k], c.norm, c.eps))));
+      }
+      if (EIGHT) {
+        most_m = top3(most_m, m[h][0], top3(m[h][1], m[h][2], m[h][3]));
+        most_v = top3(most_v, v[0], top3(v[1], v[2], v[3]));
+      }
       if (wide) {
-        if (sizeof(T) == 4) cx::store4(reinterpret_cast<float*>(param) + e, s[h].p);
-        else cx::store4(param + e, s[h].p);
+        if (sizeof(T) == 4) cx::store4(reinterpret_cast<float*>(param) + e, p);
+        else cx::store4(param + e, p);
       } else {
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-          if (e + k < left) param[e + k] = cx::Elem<T>::from_f(s[h].p[k]);
+          if (e + k < left) param[e + k] = cx::Elem<T>::from_f(p[k]);
       }
-      if (sizeof(T) != 4) cx::store4(a.master + flat + e, s[h].p);
-      if (EIGHT) {
-        float qm[4], qv[4];
+      if (sizeof(T) != 4) cx::store4(a.master + flat + e, p);
+      if (!EIGHT) {
+        cx::store4(reinterpret_cast<float*>(a.m) + flat + e, m[h]);
+        cx::store4(reinterpret_cast<float*>(a.v) + flat + e, v);
+      }
+    }
+    if (!EIGHT) continue;
+    const uint32_t top_m = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(most_m) & 0x7FFFFFFFu);
+    const uint32_t top_v = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(most_v) & 0x7FFFFFFFu);
+    const uint32_t e_m = top_m >> 23, e_v = cxadam::root_exponent(top_v >> 23);
+    const bool fine = max(top_m, top_v) < 0x7F800000u;       // no element of the block is infinite or no number
+    const float inv_m = __uint_as_float(cxadam::inverse_bits(e_m)), inv_v = __uint_as_float(cxadam::inverse_bits(e_v));
+    if (lane == 0) {
+      a.m_scale[b] = __uint_as_float(cxadam::scale_bits(e_m));
+      a.v_scale[b] = __uint_as_float(cxadam::scale_bits(e_v));
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int e = h * 128 + lane * 4;
+      float qm[4], qv[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t bits = cxadam::random_bits((uint32_t)(flat + e + k), a.noise);
+        qm[k] = cut(m[h][k] * inv_m, bits & 0xFFFFu);
+        const float q = fmaxf(cut(root[h][k] * inv_v, bits >> 16), 0x1p-9f);
+        qv[k] = root[h][k] == 0.f ? 0.f : q;                 // (v is zero, or below 2^-126)
+      }
+      if (!fine) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const uint32_t bits = cxadam::random_bits((uint32_t)(flat + e + k), a.noise);
-          qm[k] = cut(s[h].m[k] * inv_m, bits & 0xFFFFu);
-          const float q = fmaxf(cut(root[h][k] * inv_v, bits >> 16), 0x1p-9f);
-          qv[k] = s[h].v[k] == 0.f ? 0.f : q;
+          if (!(fabsf(m[h][k]) < INFINITY)) qm[k] = NAN;
+          if (!(root[h][k] < INFINITY)) qv[k] = NAN;
         }
-        if (!fine) {
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            if (!(fabsf(s[h].m[k]) < INFINITY)) qm[k] = NAN;
-            if (!(s[h].v[k] < INFINITY)) qv[k] = NAN;
-          }
-        }
-        reinterpret_cast<uint32_t*>(a.m)[(flat + e) / 4] = pack4(qm);
-        reinterpret_cast<uint32_t*>(a.v)[(flat + e) / 4] = pack4(qv);
-      } else {
-        cx::store4(reinterpret_cast<float*>(a.m) + flat + e, s[h].m);
-        cx::store4(reinterpret_cast<float*>(a.v) + flat + e, s[h].v);
       }
+      reinterpret_cast<uint32_t*>(a.m)[(flat + e) / 4] = pack4(qm);
+      reinterpret_cast<uint32_t*>(a.v)[(flat + e) / 4] = pack4(qv);
     }
   }
 }

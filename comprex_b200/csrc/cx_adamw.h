@@ -2,7 +2,8 @@
 //
 //   m = b1 m + (1 - b1) g     v = b2 v + (1 - b2) g^2     p = (1 - lr wd) p - lr / c1 * m / (sqrt(v / c2) + eps)
 //
-// (Decoupled weight decay; c1, c2 are the bias corrections.)  All of it in 32 bits, no multiply-add contraction.
+// (Decoupled weight decay; c1, c2 are the bias corrections.)  All of it in 32 bits; the moments without multiply-add
+// contraction, so that both back ends have the same ones, bit for bit.
 //
 // States of 8 bits: a block of 256 elements keeps m and r = sqrt(v) as e4m3 numbers times a power of two per block,
 // chosen so that the block's largest magnitude lies in [128, 256) (r: [128, 256)).  The root halves the range that the

@@ -58,18 +58,22 @@ int cx_adamw_step_host(const CxAdamW* a) {
     uint8_t *m8 = reinterpret_cast<uint8_t*>(a->m) + flat, *v8 = reinterpret_cast<uint8_t*>(a->v) + flat;
     float *m32 = reinterpret_cast<float*>(a->m) + flat, *v32 = reinterpret_cast<float*>(a->v) + flat;
     for (int e = 0; e < left; ++e) {
+      // with 8 bits what is kept is a power of two times what is stored: it goes with beta, as in the kernel
+      float keep_m = c.b1, keep_v = c.b2;
       if (a->bits == 8) {
-        m[e] = e4m3_to_f(m8[e]) * a->m_scale[b];
-        v[e] = e4m3_to_f(v8[e]) * a->v_scale[b];
+        m[e] = e4m3_to_f(m8[e]);
+        v[e] = e4m3_to_f(v8[e]);
         v[e] *= v[e];
+        keep_m *= a->m_scale[b];
+        keep_v *= a->v_scale[b] * a->v_scale[b];
       } else {
         m[e] = m32[e];
         v[e] = v32[e];
       }
       const float g = load_elem(a->dtype, grad, at + e);
       float p = a->master ? a->master[flat + e] : load_elem(a->dtype, a->seg_param[seg], at + e);
-      m[e] = m[e] * c.b1 + g * c.ob1;
-      v[e] = v[e] * c.b2 + (g * c.ob2) * g;
+      m[e] = m[e] * keep_m + g * c.ob1;
+      v[e] = v[e] * keep_v + (g * c.ob2) * g;
       root[e] = sqrtf(v[e]);
       p = p * c.decay - (m[e] * c.rate) / (root[e] * c.norm + c.eps);
       if (a->master) a->master[flat + e] = p;
