@@ -21,6 +21,28 @@ struct Du {
   int32_t wide_grad, wide_pre, wide_out;       // 16-byte accesses are aligned
 };
 
+// 8 neighbouring elements as they lie in memory
+template <typename T>
+struct Raw8 {
+  uint4 w[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T* p, bool wide, int have) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) w[i] = make_uint4(0, 0, 0, 0);
+    if (wide) {
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(T) / 2; ++i) w[i] = reinterpret_cast<const uint4*>(p)[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i < have) reinterpret_cast<T*>(w)[i] = p[i];
+    }
+  }
+  __device__ __forceinline__ void get(float (&v)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = cx::Elem<T>::to_f(reinterpret_cast<const T*>(w)[i]);
+  }
+};
+
 // du, and the sums of its columns over 64 rows.  Bound by memory: a thread has 8 neighbouring columns of 8 rows, all of
 // them under way at once; the 8 threads of a column join their sums in shared memory, in a fixed order.
 template <typename T, int ACT>
@@ -35,26 +57,31 @@ __global__ void __launch_bounds__(kThreads) du_kernel(const __grid_constant__ Du
   float sum[8] = {};
   const T* grad = reinterpret_cast<const T*>(d.grad) + c;
   const T* pre = reinterpret_cast<const T*>(d.pre) + c;
-#pragma unroll
+  const bool wide = left == 8 && d.wide_grad && (!act || d.wide_pre);
+#pragma unroll 1
   for (int h = 0; h < 2; ++h) {
-    float g[4][8], u[4][8];
+    // as they lie in memory until they are used: 16 loads of 16 bytes (of 16-bit types) under way in 64 registers
+    Raw8<T> g[4], u[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int64_t r = r0 + 8 * (4 * h + j);
       const int have = r < d.rows ? left : 0;
-      cxprod::load8(grad + r * d.ldg, have == 8 && d.wide_grad, have, g[j]);
-      if (act) cxprod::load8(pre + r * d.ldpre, have == 8 && d.wide_pre, have, u[j]);
+      g[j].load(grad + r * d.ldg, wide && have, have);
+      if (act) u[j].load(pre + r * d.ldpre, wide && have, have);
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int64_t r = r0 + 8 * (4 * h + j);
       if (r >= d.rows || left == 0) continue;
+      float x[8], y[8];
+      g[j].get(x);
+      if (act) u[j].get(y);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        if (act) g[j][i] *= cxprod::slope<ACT>(u[j][i]);
-        sum[i] += i < left ? g[j][i] : 0.f;
+        if (act) x[i] *= cxprod::slope<ACT>(y[i]);
+        sum[i] += x[i];                                   // (zero from `left` on)
       }
-      if (d.du) cxprod::store8(reinterpret_cast<T*>(d.du) + r * d.ldd + c, left == 8 && d.wide_out, left, g[j]);
+      if (d.du) cxprod::store8(reinterpret_cast<T*>(d.du) + r * d.ldd + c, left == 8 && d.wide_out, left, x);
     }
   }
   if (!d.part) return;
