@@ -128,13 +128,19 @@ class AdamW(torch.optim.Optimizer):
         if self._device.type != "cuda":
             self._lay[name].copy_(src)
             return
-        ring = self._ring.setdefault(name, [0] + [(torch.empty_like(src).pin_memory(), torch.cuda.Event()) for _ in range(4)])
-        host, ev = ring[1 + ring[0]]
-        ring[0] = (ring[0] + 1) % 4
-        ev.synchronize()                      # the copy that last used this buffer has finished
-        host.copy_(src)
-        self._lay[name].copy_(host, non_blocking=True)
-        ev.record(torch.cuda.current_stream(self._device))
+        ring = self._ring.setdefault(name, [])
+        stream = torch.cuda.current_stream(self._device)
+        slot = next((r for r in ring if r[1].query()), None)     # a buffer whose last copy has finished
+        if slot is None and len(ring) < 4:
+            slot = (torch.empty_like(src).pin_memory(), torch.cuda.Event())
+            ring.append(slot)
+        if slot is None:
+            slot = ring.pop(0)
+            slot[1].synchronize()
+            ring.append(slot)
+        slot[0].copy_(src)
+        self._lay[name].copy_(slot[0], non_blocking=True)
+        slot[1].record(stream)
 
     def _grads(self) -> bool:
         """Bring the table of gradient addresses up to date (0: none); whether it has changed."""

@@ -14,13 +14,9 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// The hardware's square root and reciprocal, about 2^-23 off each, one instruction instead of ten: the moments themselves
-// are exact sums, the step is lr-sized, and what the root is kept as has 3 bits of mantissa.
-__device__ __forceinline__ float approx_root(float x) {
-  float y;
-  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
+// The hardware's reciprocal, 2^-23 off, one instruction instead of ten: the step that it makes is lr-sized.  The root is the
+// exact one: what is kept of it is rounded at random, and must be the same whoever computes it (with an approximate root one
+// code in 500 000 differed, and the weights a step later).
 __device__ __forceinline__ float approx_inverse(float x) {
   float y;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -160,7 +156,7 @@ __global__ void __launch_bounds__(kThreads, EIGHT ? 4 : 3) adamw_kernel(const __
       for (int k = 0; k < 4; ++k) {
         m[h][k] = m[h][k] * keep_m + g[k] * c.ob1;
         v[k] = v[k] * keep_v + (g[k] * c.ob2) * g[k];
-        root[h][k] = approx_root(v[k]);
+        root[h][k] = sqrtf(v[k]);
         p[k] = __fmaf_rn(p[k], c.decay, -(m[h][k] * c.rate * approx_inverse(__fmaf_rn(root[h][k], c.norm, c.eps))));
       }
       if (EIGHT) {
@@ -200,7 +196,7 @@ __global__ void __launch_bounds__(kThreads, EIGHT ? 4 : 3) adamw_kernel(const __
         const uint32_t bits = cxadam::random_bits((uint32_t)(flat + e + k), a.noise);
         qm[k] = cut(m[h][k] * inv_m, bits & 0xFFFFu);
         const float q = fmaxf(cut(root[h][k] * inv_v, bits >> 16), 0x1p-9f);
-        qv[k] = root[h][k] == 0.f ? 0.f : q;                 // (v is zero, or below 2^-126)
+        qv[k] = root[h][k] == 0.f ? 0.f : q;                 // (only the root of zero is zero)
       }
       if (!fine) {
 #pragma unroll

@@ -109,25 +109,22 @@ def test_8_bit_states_hold_the_moments(device, dtype):
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.gpu
 def test_cuda_agrees_with_host(dtype, bits):
-    """One step from the same states: 32-bit moments and the scales of 8-bit ones bit for bit, the first moment's codes too.
-    The kernel takes the root and the quotient from the hardware's approximations, 2^-22 off: weights within that of the
-    step, and a root's code one step away where the random bits fall into the 2^-19 of a code's step that this moves it."""
+    """States bit for bit.  The kernel takes the quotient of the step from the hardware's approximate reciprocal: weights
+    within a few roundings of the step, which is at most 10 lr, and their own."""
     made = {}
     for device in ("cpu", "cuda"):
         params = _params(dtype, device)
         opt = cx.AdamW(params, state_bits=bits, seed=7, **HYPER)
-        _set_grads(params, seed=0)
-        opt.step()
+        for t in range(4):
+            _set_grads(params, seed=t)
+            opt.step()
         made[device] = {k: t.cpu() for k, t in opt.flat_state().items()}
         made[device]["weights"] = torch.cat(_weights(opt, params))
     host, cuda = made["cpu"], made["cuda"]
-    for k in ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_rms_scale"):
-        if k in host:
+    for k in host:
+        if k.startswith("exp_avg"):
             assert torch.equal(host[k].view(torch.uint8), cuda[k].view(torch.uint8)), k
-    assert ((host["weights"] - cuda["weights"]).abs() <= EPS32 * 2 * host["weights"].abs() + 2.0 ** -21 * 1.1 * HYPER["lr"]).all()
-    if bits == 8:
-        off = host["exp_avg_rms"].view(torch.uint8).int() - cuda["exp_avg_rms"].view(torch.uint8).int()
-        assert off.abs().max() <= 1 and off.ne(0).sum() <= 3         # 17 000 roots: 0.03 expected
+    assert ((host["weights"] - cuda["weights"]).abs() <= 4 * (EPS32 * 2 * host["weights"].abs() + 2.0 ** -21 * 10 * HYPER["lr"])).all()
 
 
 def test_rounding_is_unbiased(device):
