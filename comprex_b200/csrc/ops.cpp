@@ -1,4 +1,6 @@
 // Entry points of the operators of cx_ops.h: checks of the descriptors, then the back end that `dev` names.
+#include <exception>
+
 #include "cx_adamw.h"
 #include "cx_ops.h"
 
@@ -19,6 +21,16 @@ int cx_vocab_loss_backward_host(const CxVocabLoss*);
 namespace {
 
 bool type_ok(int dtype) { return dtype == CX_F32 || dtype == CX_BF16 || dtype == CX_F16; }
+// No exception leaves a C entry: the host back end allocates.
+template <typename F, typename D>
+int on_host(F f, const D* d) {
+  try {
+    return f(d);
+  } catch (const std::exception& e) {
+    return cx_set_error(e.what(), 0);
+  }
+}
+
 constexpr int64_t kMost = 0x7FFFFF00;      // rows, columns and entries of the vocabulary: 32-bit coordinates
 bool size_ok(int64_t n) { return n >= 1 && n <= kMost; }
 
@@ -51,7 +63,7 @@ int cx_adamw_step(int dev, const CxAdamW* a, void* stream) {
   if (!a->blk_seg || !a->seg_blk || !a->seg_len || !a->seg_param || !a->seg_grad || !a->seg_class || !a->m || !a->v ||
       (a->bits == 8 && (!a->m_scale || !a->v_scale)) || (a->dtype != CX_F32 && !a->master))
     return cx_set_error("cx_adamw_step: a table or state is missing", 0);
-  return dev == CX_DEV_CUDA ? cx_adamw_step_cuda(a, stream) : cx_adamw_step_host(a);
+  return dev == CX_DEV_CUDA ? cx_adamw_step_cuda(a, stream) : on_host(cx_adamw_step_host, a);
 }
 
 int64_t cx_linear_workspace_bytes(int dev, const CxLinear* l, int backward) {
@@ -63,7 +75,7 @@ int cx_linear_forward(int dev, const CxLinear* l, void* stream) {
   if (!l->x || !l->w || !l->y) return cx_set_error("cx_linear_forward: an operand is missing", 0);
   if (l->ldx < l->inner || l->ldw < l->inner || (l->residual && l->ldr < l->outer) || (l->pre && l->ldpre < l->outer))
     return cx_set_error("cx_linear_forward: rows overlap", 0);
-  return dev == CX_DEV_CUDA ? cx_linear_forward_cuda(l, stream) : cx_linear_forward_host(l);
+  return dev == CX_DEV_CUDA ? cx_linear_forward_cuda(l, stream) : on_host(cx_linear_forward_host, l);
 }
 
 int cx_linear_backward(int dev, const CxLinear* l, void* stream) {
@@ -72,7 +84,7 @@ int cx_linear_backward(int dev, const CxLinear* l, void* stream) {
     return cx_set_error("cx_linear_backward: an operand is missing", 0);
   if (l->ldg < l->outer || (l->act != CX_ACT_NONE && l->ldpre < l->outer) || (l->dw && l->ldx < l->inner) || (l->dx && l->ldw < l->inner))
     return cx_set_error("cx_linear_backward: rows overlap", 0);
-  return dev == CX_DEV_CUDA ? cx_linear_backward_cuda(l, stream) : cx_linear_backward_host(l);
+  return dev == CX_DEV_CUDA ? cx_linear_backward_cuda(l, stream) : on_host(cx_linear_backward_host, l);
 }
 
 int64_t cx_vocab_loss_workspace_bytes(int dev, const CxVocabLoss* l, int backward) {
@@ -82,14 +94,14 @@ int64_t cx_vocab_loss_workspace_bytes(int dev, const CxVocabLoss* l, int backwar
 int cx_vocab_loss_forward(int dev, const CxVocabLoss* l, void* stream) {
   if (const char* why = wrong(l)) return cx_set_error(why, 0);
   if (!l->loss) return cx_set_error("cx_vocab_loss_forward: an operand is missing", 0);
-  return dev == CX_DEV_CUDA ? cx_vocab_loss_forward_cuda(l, stream) : cx_vocab_loss_forward_host(l);
+  return dev == CX_DEV_CUDA ? cx_vocab_loss_forward_cuda(l, stream) : on_host(cx_vocab_loss_forward_host, l);
 }
 
 int cx_vocab_loss_backward(int dev, const CxVocabLoss* l, void* stream) {
   if (const char* why = wrong(l)) return cx_set_error(why, 0);
   if (!l->grad) return cx_set_error("cx_vocab_loss_backward: an operand is missing", 0);
   if (!l->dh && !l->dw) return 0;
-  return dev == CX_DEV_CUDA ? cx_vocab_loss_backward_cuda(l, stream) : cx_vocab_loss_backward_host(l);
+  return dev == CX_DEV_CUDA ? cx_vocab_loss_backward_cuda(l, stream) : on_host(cx_vocab_loss_backward_host, l);
 }
 
 int64_t cx_ops_sizeof(int what) {
