@@ -1,10 +1,12 @@
 // AdamW step over all tensors of a model in one launch, states in 32 bits or in 8 (the mathematics: cx_adamw.h).
 //
-// Bound by memory: an element moves its gradient, its 32-bit weight both ways, its 16-bit copy and two states both
-// ways, 16 bytes for a bf16 tensor with 8-bit states and 28 with 32-bit ones.  One warp takes one block of 256
-// elements at a time: the block is what shares a scale, so its largest values are two warp-wide integer maxima and
-// nothing crosses warps, and a lane's two groups of four consecutive elements make every access of the warp whole
-// lines.  Tensors are found through a table of blocks, so a model of many small tensors is one launch as well.
+// An element moves its gradient, its 32-bit weight both ways, its 16-bit copy and two states both ways: 16 bytes for a bf16
+// tensor with 8-bit states, 28 with 32-bit ones.  With 32 bits that bounds it (268 M elements bf16 / fp32 1270 / 1248 us, 5.9
+// / 6.0 TB/s); with 8 it is instructions as well, 78 an element, 18 of them the random bits (876 / 829 us, 4.9 / 5.2 TB/s;
+// without the random bits 727 / 706).  One warp takes one block of 256 elements at a time: the block is what shares a scale,
+// so its largest values are two warp-wide integer maxima and nothing crosses warps, and a lane's two groups of four
+// consecutive elements make every access of the warp whole lines.  Tensors are found through a table of blocks, so a model of
+// many small tensors is one launch as well.
 #include <cuda_fp8.h>
 
 #include "cx_adamw.h"
@@ -21,6 +23,32 @@ __device__ __forceinline__ float approx_inverse(float x) {
   float y;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+// Two products, sums or multiply-adds in one instruction, each rounded as one alone is
+struct Two {
+  unsigned long long w;
+  __device__ __forceinline__ Two() {}
+  __device__ __forceinline__ Two(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(w) : "f"(a), "f"(b)); }
+  __device__ __forceinline__ void get(float& a, float& b) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(w)); }
+};
+__device__ __forceinline__ Two operator*(Two a, Two b) {
+  Two d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d.w) : "l"(a.w), "l"(b.w));
+  return d;
+}
+__device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
+  Two d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.w) : "l"(a.w), "l"(b.w), "l"(c.w));
+  return d;
+}
+// a b + c d as three roundings.  (The sum is one of single numbers: as two in one instruction it would be joined with a
+// product into a multiply-add, and the moments would not be the host's.)
+__device__ __forceinline__ void sum_of_products(Two a, Two b, Two c, Two d, float& x, float& y) {
+  float p, q, r, s;
+  (a * b).get(p, q);
+  (c * d).get(r, s);
+  x = __fadd_rn(p, r);
+  y = __fadd_rn(q, s);
 }
 // The larger magnitude of three; NaN where one is
 __device__ __forceinline__ float top3(float a, float b, float c) {
@@ -56,27 +84,29 @@ struct Loaded {
 };
 
 template <typename T, bool EIGHT>
-__global__ void __launch_bounds__(kThreads, EIGHT ? 4 : 3) adamw_kernel(const __grid_constant__ CxAdamW a) {
+__global__ void __launch_bounds__(kThreads, EIGHT ? 4 : 2) adamw_kernel(const __grid_constant__ CxAdamW a) {
   using Raw = cx::Raw4<T>;
   const int lane = threadIdx.x & 31;
-  const int64_t warps = (int64_t)gridDim.x * (kThreads / 32);
-  int64_t b = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
-  if (b >= a.blocks) return;
+  // a CTA has a range of blocks, mostly of one tensor; its warps take them in turn
+  constexpr int64_t warps = kThreads / 32;
+  const int64_t share = (a.blocks + gridDim.x - 1) / gridDim.x, last = min(a.blocks, (blockIdx.x + 1) * share);
+  int64_t b = blockIdx.x * share + (threadIdx.x >> 5);
+  if (b >= last) return;
   // a tensor's row of the tables is read when a block of another tensor comes; which tensor that is, a block ahead
   int seg = a.blk_seg[b], known = -1;
   const T* grad0 = nullptr;
   T* param0 = nullptr;
   int64_t first = 0, len = 0;
   int cls = 0;
-  // With 8 bits the next block's lines are asked into L2 while this one is worked on, a lane has one of them: there are more
-  // instructions then than 32 warps an SM hide the loads behind (268 M elements, bf16 / fp32 with / without: 812 / 786 and
-  // 884 / 795 us).  With 32 bits 24 warps without it are faster (1259 / 1208 us, 1450 / 1417 with both).
+  // With 8 bits the next block's lines are asked into L2 while this one is worked on, a lane has one of them: there are
+  // more instructions then than 32 warps an SM hide the loads behind (268 M elements, bf16 / fp32: with it 8 / 1 % faster).
+  // With 32 bits 16 warps without it are fastest (1150 / 1125 us; 24 warps 1259 / 1208, 32 warps with it 1450 / 1417).
   constexpr int kT = (int)sizeof(T) * 2, kState = EIGHT ? 2 : 8;           // lines of a block: of a tensor, of a state
   constexpr int kLines = kT + 8 + 2 * kState;                              // gradient, weights, two states
   const int part = lane < kT ? 0 : lane < kT + 8 ? 1 : lane < kT + 8 + kState ? 2 : 3;
   const int64_t per = part == 0 ? kT * 128 : part == 1 ? 1024 : kState * 128;
   const char* line = nullptr;
-  for (; b < a.blocks; b += warps) {
+  for (; b < last; b += warps) {
     if (seg != known) {
       known = seg;
       grad0 = reinterpret_cast<const T*>(a.seg_grad[seg]);
@@ -89,9 +119,9 @@ __global__ void __launch_bounds__(kThreads, EIGHT ? 4 : 3) adamw_kernel(const __
                          : reinterpret_cast<const char*>(part == 2 ? a.m : a.v);
       line = base + 128 * (part == 0 ? lane : part == 1 ? lane - kT : part == 2 ? lane - kT - 8 : lane - kT - 8 - kState);
     }
-    if (b + warps < a.blocks) seg = a.blk_seg[b + warps];
+    if (b + warps < last) seg = a.blk_seg[b + warps];
     if (grad0 == nullptr) continue;
-    if (EIGHT && lane < kLines && seg == known && (b + warps - first + 1) * CX_ADAMW_BLOCK <= len)       // whole, and of this tensor
+    if (EIGHT && lane < kLines && b + warps < last && seg == known && (b + warps - first + 1) * CX_ADAMW_BLOCK <= len)       // whole, and of this tensor
       asm volatile("prefetch.global.L2 [%0];" ::"l"(line + (b + warps) * per));
     const int64_t at = (b - first) * CX_ADAMW_BLOCK, flat = b * CX_ADAMW_BLOCK;
     const int left = (int)min((int64_t)CX_ADAMW_BLOCK, len - at);
@@ -146,18 +176,26 @@ __global__ void __launch_bounds__(kThreads, EIGHT ? 4 : 3) adamw_kernel(const __
         unpack4(in.m8[h], m[h]);
         unpack4(in.v8[h], v);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] *= v[k];            // 4 bits squared: exact
+        for (int k = 0; k < 4; k += 2) {                     // 4 bits squared: exact
+          const Two r(v[k], v[k + 1]);
+          (r * r).get(v[k], v[k + 1]);
+        }
       } else {
         const float4 x = in.m[h], y = in.v[h];
         m[h][0] = x.x, m[h][1] = x.y, m[h][2] = x.z, m[h][3] = x.w;
         v[0] = y.x, v[1] = y.y, v[2] = y.z, v[3] = y.w;
       }
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        m[h][k] = m[h][k] * keep_m + g[k] * c.ob1;
-        v[k] = v[k] * keep_v + (g[k] * c.ob2) * g[k];
+      for (int k = 0; k < 4; k += 2) {
+        const Two g2(g[k], g[k + 1]);
+        sum_of_products(Two(m[h][k], m[h][k + 1]), Two(keep_m, keep_m), g2, Two(c.ob1, c.ob1), m[h][k], m[h][k + 1]);
+        sum_of_products(Two(v[k], v[k + 1]), Two(keep_v, keep_v), g2 * Two(c.ob2, c.ob2), g2, v[k], v[k + 1]);
+        const Two m2(m[h][k], m[h][k + 1]);
         root[h][k] = sqrtf(v[k]);
-        p[k] = __fmaf_rn(p[k], c.decay, -(m[h][k] * c.rate * approx_inverse(__fmaf_rn(root[h][k], c.norm, c.eps))));
+        root[h][k + 1] = sqrtf(v[k + 1]);
+        float low0, low1;
+        fma2(Two(root[h][k], root[h][k + 1]), Two(c.norm, c.norm), Two(c.eps, c.eps)).get(low0, low1);
+        fma2(Two(p[k], p[k + 1]), Two(c.decay, c.decay), m2 * Two(-c.rate, -c.rate) * Two(approx_inverse(low0), approx_inverse(low1))).get(p[k], p[k + 1]);
       }
       if (EIGHT) {
         most_m = top3(most_m, m[h][0], top3(m[h][1], m[h][2], m[h][3]));
@@ -192,10 +230,15 @@ __global__ void __launch_bounds__(kThreads, EIGHT ? 4 : 3) adamw_kernel(const __
       const int e = h * 128 + lane * 4;
       float qm[4], qv[4];
 #pragma unroll
+      for (int k = 0; k < 4; k += 2) {
+        (Two(m[h][k], m[h][k + 1]) * Two(inv_m, inv_m)).get(qm[k], qm[k + 1]);
+        (Two(root[h][k], root[h][k + 1]) * Two(inv_v, inv_v)).get(qv[k], qv[k + 1]);
+      }
+#pragma unroll
       for (int k = 0; k < 4; ++k) {
         const uint32_t bits = cxadam::random_bits((uint32_t)(flat + e + k), a.noise);
-        qm[k] = cut(m[h][k] * inv_m, bits & 0xFFFFu);
-        const float q = fmaxf(cut(root[h][k] * inv_v, bits >> 16), 0x1p-9f);
+        qm[k] = cut(qm[k], bits & 0xFFFFu);
+        const float q = fmaxf(cut(qv[k], bits >> 16), 0x1p-9f);
         qv[k] = root[h][k] == 0.f ? 0.f : q;                 // (only the root of zero is zero)
       }
       if (!fine) {
