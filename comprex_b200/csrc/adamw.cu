@@ -84,16 +84,16 @@ struct Loaded {
 };
 
 template <typename T, bool EIGHT>
-__global__ void __launch_bounds__(kThreads, EIGHT ? 4 : 2) adamw_kernel(const __grid_constant__ CxAdamW a) {
+__global__ void __launch_bounds__(kThreads, EIGHT ? 4 : 2) adamw_kernel(const __grid_constant__ CxAdamW a, const int64_t run) {
   using Raw = cx::Raw4<T>;
   const int lane = threadIdx.x & 31;
-  // a CTA has a range of blocks, mostly of one tensor; its warps take them in turn
+  // A CTA takes `run` neighbouring blocks, mostly of one tensor, its warps in turn, then those of its next turn: all CTAs
+  // together stay in a window of each array, and the tensors' tables are seldom read.  (355 M elements in 292 tensors, bf16,
+  // 8 bits, runs of 8 / 32 / 128 / 512 blocks and one range a CTA: 1387 / 1233 / 1147 / 1096 / 1223 us; 268 M in one tensor
+  // with 32 bits, 8 / 16 / 32 / 128: 1174 / 1137 / 1147 / 1185.)
   constexpr int64_t warps = kThreads / 32;
-  const int64_t share = (a.blocks + gridDim.x - 1) / gridDim.x, last = min(a.blocks, (blockIdx.x + 1) * share);
-  int64_t b = blockIdx.x * share + (threadIdx.x >> 5);
-  if (b >= last) return;
   // a tensor's row of the tables is read when a block of another tensor comes; which tensor that is, a block ahead
-  int seg = a.blk_seg[b], known = -1;
+  int seg = 0, known = -1;
   const T* grad0 = nullptr;
   T* param0 = nullptr;
   int64_t first = 0, len = 0;
@@ -106,150 +106,156 @@ __global__ void __launch_bounds__(kThreads, EIGHT ? 4 : 2) adamw_kernel(const __
   const int part = lane < kT ? 0 : lane < kT + 8 ? 1 : lane < kT + 8 + kState ? 2 : 3;
   const int64_t per = part == 0 ? kT * 128 : part == 1 ? 1024 : kState * 128;
   const char* line = nullptr;
-  for (; b < last; b += warps) {
-    if (seg != known) {
-      known = seg;
-      grad0 = reinterpret_cast<const T*>(a.seg_grad[seg]);
-      param0 = reinterpret_cast<T*>(a.seg_param[seg]);
-      first = a.seg_blk[seg];
-      len = a.seg_len[seg];
-      cls = a.seg_class[seg];
-      const char* base = part == 0 ? reinterpret_cast<const char*>(grad0) - first * per
-                         : part == 1 ? (sizeof(T) == 4 ? reinterpret_cast<const char*>(param0) - first * per : reinterpret_cast<const char*>(a.master))
-                         : reinterpret_cast<const char*>(part == 2 ? a.m : a.v);
-      line = base + 128 * (part == 0 ? lane : part == 1 ? lane - kT : part == 2 ? lane - kT - 8 : lane - kT - 8 - kState);
-    }
-    if (b + warps < last) seg = a.blk_seg[b + warps];
-    if (grad0 == nullptr) continue;
-    if (EIGHT && lane < kLines && b + warps < last && seg == known && (b + warps - first + 1) * CX_ADAMW_BLOCK <= len)       // whole, and of this tensor
-      asm volatile("prefetch.global.L2 [%0];" ::"l"(line + (b + warps) * per));
-    const int64_t at = (b - first) * CX_ADAMW_BLOCK, flat = b * CX_ADAMW_BLOCK;
-    const int left = (int)min((int64_t)CX_ADAMW_BLOCK, len - at);
-    const T* grad = grad0 + at;
-    T* param = param0 + at;
-    constexpr uintptr_t kWide = 4 * sizeof(T) - 1;
-    const bool wide = left == CX_ADAMW_BLOCK && (((uintptr_t)param | (uintptr_t)grad) & kWide) == 0;
-    Loaded<T, EIGHT> in;
-    const CxAdamWClass& c = a.cls[cls];
-    // of what is kept, this much stays: with 8 bits times the scale, or its square (powers of two: the products with beta
-    // are what they are without them)
-    float keep_m = c.b1, keep_v = c.b2;
-    if (EIGHT) {
-      const float scale = a.v_scale[b];
-      keep_m *= a.m_scale[b];
-      keep_v *= scale * scale;
-    }
+  for (int64_t turn = blockIdx.x; turn * run < a.blocks; turn += gridDim.x) {
+    const int64_t last = min(a.blocks, (turn + 1) * run);
+    int64_t b = turn * run + (threadIdx.x >> 5);
+    if (b >= last) continue;
+    seg = a.blk_seg[b];
+    for (; b < last; b += warps) {
+      if (seg != known) {
+        known = seg;
+        grad0 = reinterpret_cast<const T*>(a.seg_grad[seg]);
+        param0 = reinterpret_cast<T*>(a.seg_param[seg]);
+        first = a.seg_blk[seg];
+        len = a.seg_len[seg];
+        cls = a.seg_class[seg];
+        const char* base = part == 0 ? reinterpret_cast<const char*>(grad0) - first * per
+                           : part == 1 ? (sizeof(T) == 4 ? reinterpret_cast<const char*>(param0) - first * per : reinterpret_cast<const char*>(a.master))
+                           : reinterpret_cast<const char*>(part == 2 ? a.m : a.v);
+        line = base + 128 * (part == 0 ? lane : part == 1 ? lane - kT : part == 2 ? lane - kT - 8 : lane - kT - 8 - kState);
+      }
+      if (b + warps < last) seg = a.blk_seg[b + warps];
+      if (grad0 == nullptr) continue;
+      if (EIGHT && lane < kLines && b + warps < last && seg == known && (b + warps - first + 1) * CX_ADAMW_BLOCK <= len)       // whole, and of this tensor
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(line + (b + warps) * per));
+      const int64_t at = (b - first) * CX_ADAMW_BLOCK, flat = b * CX_ADAMW_BLOCK;
+      const int left = (int)min((int64_t)CX_ADAMW_BLOCK, len - at);
+      const T* grad = grad0 + at;
+      T* param = param0 + at;
+      constexpr uintptr_t kWide = 4 * sizeof(T) - 1;
+      const bool wide = left == CX_ADAMW_BLOCK && (((uintptr_t)param | (uintptr_t)grad) & kWide) == 0;
+      Loaded<T, EIGHT> in;
+      const CxAdamWClass& c = a.cls[cls];
+      // of what is kept, this much stays: with 8 bits times the scale, or its square (powers of two: the products with beta
+      // are what they are without them)
+      float keep_m = c.b1, keep_v = c.b2;
+      if (EIGHT) {
+        const float scale = a.v_scale[b];
+        keep_m *= a.m_scale[b];
+        keep_v *= scale * scale;
+      }
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int e = h * 128 + lane * 4;
-      if (wide) {
-        in.g[h] = Raw::load(grad + e);
-        if (sizeof(T) == 4) in.p[h] = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(param) + e);
-      } else {
-        T g[4];
-        float p[4] = {};
+      for (int h = 0; h < 2; ++h) {
+        const int e = h * 128 + lane * 4;
+        if (wide) {
+          in.g[h] = Raw::load(grad + e);
+          if (sizeof(T) == 4) in.p[h] = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(param) + e);
+        } else {
+          T g[4];
+          float p[4] = {};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            g[k] = e + k < left ? grad[e + k] : cx::Elem<T>::from_f(0.f);
+            if (sizeof(T) == 4 && e + k < left) p[k] = cx::Elem<T>::to_f(param[e + k]);
+          }
+          memcpy(&in.g[h], g, sizeof(g));
+          in.p[h] = make_float4(p[0], p[1], p[2], p[3]);
+        }
+        if (sizeof(T) != 4) in.p[h] = *reinterpret_cast<const float4*>(a.master + flat + e);
+        if (EIGHT) {
+          in.m8[h] = reinterpret_cast<const uint32_t*>(a.m)[(flat + e) / 4];
+          in.v8[h] = reinterpret_cast<const uint32_t*>(a.v)[(flat + e) / 4];
+        } else {
+          in.m[h] = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(a.m) + flat + e);
+          in.v[h] = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(a.v) + flat + e);
+        }
+      }
+      // the step; what is done with an element is stored at once, but for the states of 8 bits, which wait for their scale
+      float m[2][4], root[2][4], most_m = 0.f, most_v = 0.f;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int e = h * 128 + lane * 4;
+        float g[4], p[4] = {in.p[h].x, in.p[h].y, in.p[h].z, in.p[h].w}, v[4];
+        Raw::to_f(in.g[h], g);
+        if (EIGHT) {
+          unpack4(in.m8[h], m[h]);
+          unpack4(in.v8[h], v);
+#pragma unroll
+          for (int k = 0; k < 4; k += 2) {                     // 4 bits squared: exact
+            const Two r(v[k], v[k + 1]);
+            (r * r).get(v[k], v[k + 1]);
+          }
+        } else {
+          const float4 x = in.m[h], y = in.v[h];
+          m[h][0] = x.x, m[h][1] = x.y, m[h][2] = x.z, m[h][3] = x.w;
+          v[0] = y.x, v[1] = y.y, v[2] = y.z, v[3] = y.w;
+        }
+#pragma unroll
+        for (int k = 0; k < 4; k += 2) {
+          const Two g2(g[k], g[k + 1]);
+          sum_of_products(Two(m[h][k], m[h][k + 1]), Two(keep_m, keep_m), g2, Two(c.ob1, c.ob1), m[h][k], m[h][k + 1]);
+          sum_of_products(Two(v[k], v[k + 1]), Two(keep_v, keep_v), g2 * Two(c.ob2, c.ob2), g2, v[k], v[k + 1]);
+          const Two m2(m[h][k], m[h][k + 1]);
+          root[h][k] = sqrtf(v[k]);
+          root[h][k + 1] = sqrtf(v[k + 1]);
+          float low0, low1;
+          fma2(Two(root[h][k], root[h][k + 1]), Two(c.norm, c.norm), Two(c.eps, c.eps)).get(low0, low1);
+          fma2(Two(p[k], p[k + 1]), Two(c.decay, c.decay), m2 * Two(-c.rate, -c.rate) * Two(approx_inverse(low0), approx_inverse(low1))).get(p[k], p[k + 1]);
+        }
+        if (EIGHT) {
+          most_m = top3(most_m, m[h][0], top3(m[h][1], m[h][2], m[h][3]));
+          most_v = top3(most_v, v[0], top3(v[1], v[2], v[3]));
+        }
+        if (wide) {
+          if (sizeof(T) == 4) cx::store4(reinterpret_cast<float*>(param) + e, p);
+          else cx::store4(param + e, p);
+        } else {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (e + k < left) param[e + k] = cx::Elem<T>::from_f(p[k]);
+        }
+        if (sizeof(T) != 4) cx::store4(a.master + flat + e, p);
+        if (!EIGHT) {
+          cx::store4(reinterpret_cast<float*>(a.m) + flat + e, m[h]);
+          cx::store4(reinterpret_cast<float*>(a.v) + flat + e, v);
+        }
+      }
+      if (!EIGHT) continue;
+      const uint32_t top_m = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(most_m) & 0x7FFFFFFFu);
+      const uint32_t top_v = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(most_v) & 0x7FFFFFFFu);
+      const uint32_t e_m = top_m >> 23, e_v = cxadam::root_exponent(top_v >> 23);
+      const bool fine = max(top_m, top_v) < 0x7F800000u;       // no element of the block is infinite or no number
+      const float inv_m = __uint_as_float(cxadam::inverse_bits(e_m)), inv_v = __uint_as_float(cxadam::inverse_bits(e_v));
+      if (lane == 0) {
+        a.m_scale[b] = __uint_as_float(cxadam::scale_bits(e_m));
+        a.v_scale[b] = __uint_as_float(cxadam::scale_bits(e_v));
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int e = h * 128 + lane * 4;
+        float qm[4], qv[4];
+#pragma unroll
+        for (int k = 0; k < 4; k += 2) {
+          (Two(m[h][k], m[h][k + 1]) * Two(inv_m, inv_m)).get(qm[k], qm[k + 1]);
+          (Two(root[h][k], root[h][k + 1]) * Two(inv_v, inv_v)).get(qv[k], qv[k + 1]);
+        }
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          g[k] = e + k < left ? grad[e + k] : cx::Elem<T>::from_f(0.f);
-          if (sizeof(T) == 4 && e + k < left) p[k] = cx::Elem<T>::to_f(param[e + k]);
+          const uint32_t bits = cxadam::random_bits((uint32_t)(flat + e + k), a.noise);
+          qm[k] = cut(qm[k], bits & 0xFFFFu);
+          const float q = fmaxf(cut(qv[k], bits >> 16), 0x1p-9f);
+          qv[k] = root[h][k] == 0.f ? 0.f : q;                 // (only the root of zero is zero)
         }
-        memcpy(&in.g[h], g, sizeof(g));
-        in.p[h] = make_float4(p[0], p[1], p[2], p[3]);
-      }
-      if (sizeof(T) != 4) in.p[h] = *reinterpret_cast<const float4*>(a.master + flat + e);
-      if (EIGHT) {
-        in.m8[h] = reinterpret_cast<const uint32_t*>(a.m)[(flat + e) / 4];
-        in.v8[h] = reinterpret_cast<const uint32_t*>(a.v)[(flat + e) / 4];
-      } else {
-        in.m[h] = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(a.m) + flat + e);
-        in.v[h] = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(a.v) + flat + e);
-      }
-    }
-    // the step; what is done with an element is stored at once, but for the states of 8 bits, which wait for their scale
-    float m[2][4], root[2][4], most_m = 0.f, most_v = 0.f;
+        if (!fine) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int e = h * 128 + lane * 4;
-      float g[4], p[4] = {in.p[h].x, in.p[h].y, in.p[h].z, in.p[h].w}, v[4];
-      Raw::to_f(in.g[h], g);
-      if (EIGHT) {
-        unpack4(in.m8[h], m[h]);
-        unpack4(in.v8[h], v);
-#pragma unroll
-        for (int k = 0; k < 4; k += 2) {                     // 4 bits squared: exact
-          const Two r(v[k], v[k + 1]);
-          (r * r).get(v[k], v[k + 1]);
+          for (int k = 0; k < 4; ++k) {
+            if (!(fabsf(m[h][k]) < INFINITY)) qm[k] = NAN;
+            if (!(root[h][k] < INFINITY)) qv[k] = NAN;
+          }
         }
-      } else {
-        const float4 x = in.m[h], y = in.v[h];
-        m[h][0] = x.x, m[h][1] = x.y, m[h][2] = x.z, m[h][3] = x.w;
-        v[0] = y.x, v[1] = y.y, v[2] = y.z, v[3] = y.w;
+        reinterpret_cast<uint32_t*>(a.m)[(flat + e) / 4] = pack4(qm);
+        reinterpret_cast<uint32_t*>(a.v)[(flat + e) / 4] = pack4(qv);
       }
-#pragma unroll
-      for (int k = 0; k < 4; k += 2) {
-        const Two g2(g[k], g[k + 1]);
-        sum_of_products(Two(m[h][k], m[h][k + 1]), Two(keep_m, keep_m), g2, Two(c.ob1, c.ob1), m[h][k], m[h][k + 1]);
-        sum_of_products(Two(v[k], v[k + 1]), Two(keep_v, keep_v), g2 * Two(c.ob2, c.ob2), g2, v[k], v[k + 1]);
-        const Two m2(m[h][k], m[h][k + 1]);
-        root[h][k] = sqrtf(v[k]);
-        root[h][k + 1] = sqrtf(v[k + 1]);
-        float low0, low1;
-        fma2(Two(root[h][k], root[h][k + 1]), Two(c.norm, c.norm), Two(c.eps, c.eps)).get(low0, low1);
-        fma2(Two(p[k], p[k + 1]), Two(c.decay, c.decay), m2 * Two(-c.rate, -c.rate) * Two(approx_inverse(low0), approx_inverse(low1))).get(p[k], p[k + 1]);
-      }
-      if (EIGHT) {
-        most_m = top3(most_m, m[h][0], top3(m[h][1], m[h][2], m[h][3]));
-        most_v = top3(most_v, v[0], top3(v[1], v[2], v[3]));
-      }
-      if (wide) {
-        if (sizeof(T) == 4) cx::store4(reinterpret_cast<float*>(param) + e, p);
-        else cx::store4(param + e, p);
-      } else {
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          if (e + k < left) param[e + k] = cx::Elem<T>::from_f(p[k]);
-      }
-      if (sizeof(T) != 4) cx::store4(a.master + flat + e, p);
-      if (!EIGHT) {
-        cx::store4(reinterpret_cast<float*>(a.m) + flat + e, m[h]);
-        cx::store4(reinterpret_cast<float*>(a.v) + flat + e, v);
-      }
-    }
-    if (!EIGHT) continue;
-    const uint32_t top_m = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(most_m) & 0x7FFFFFFFu);
-    const uint32_t top_v = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(most_v) & 0x7FFFFFFFu);
-    const uint32_t e_m = top_m >> 23, e_v = cxadam::root_exponent(top_v >> 23);
-    const bool fine = max(top_m, top_v) < 0x7F800000u;       // no element of the block is infinite or no number
-    const float inv_m = __uint_as_float(cxadam::inverse_bits(e_m)), inv_v = __uint_as_float(cxadam::inverse_bits(e_v));
-    if (lane == 0) {
-      a.m_scale[b] = __uint_as_float(cxadam::scale_bits(e_m));
-      a.v_scale[b] = __uint_as_float(cxadam::scale_bits(e_v));
-    }
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int e = h * 128 + lane * 4;
-      float qm[4], qv[4];
-#pragma unroll
-      for (int k = 0; k < 4; k += 2) {
-        (Two(m[h][k], m[h][k + 1]) * Two(inv_m, inv_m)).get(qm[k], qm[k + 1]);
-        (Two(root[h][k], root[h][k + 1]) * Two(inv_v, inv_v)).get(qv[k], qv[k + 1]);
-      }
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const uint32_t bits = cxadam::random_bits((uint32_t)(flat + e + k), a.noise);
-        qm[k] = cut(qm[k], bits & 0xFFFFu);
-        const float q = fmaxf(cut(qv[k], bits >> 16), 0x1p-9f);
-        qv[k] = root[h][k] == 0.f ? 0.f : q;                 // (only the root of zero is zero)
-      }
-      if (!fine) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          if (!(fabsf(m[h][k]) < INFINITY)) qm[k] = NAN;
-          if (!(root[h][k] < INFINITY)) qv[k] = NAN;
-        }
-      }
-      reinterpret_cast<uint32_t*>(a.m)[(flat + e) / 4] = pack4(qm);
-      reinterpret_cast<uint32_t*>(a.v)[(flat + e) / 4] = pack4(qv);
     }
   }
 }
@@ -263,7 +269,10 @@ int launch(const CxAdamW& a, cudaStream_t s) {
   }();
   const int64_t ctas = (a.blocks + kThreads / 32 - 1) / (kThreads / 32);
   const int grid = (int)(ctas < (int64_t)per_sm * cx_sm_count() ? ctas : (int64_t)per_sm * cx_sm_count());
-  adamw_kernel<T, EIGHT><<<grid, kThreads, 0, s>>>(a);
+  constexpr int64_t most = EIGHT ? 512 : 32;
+  int64_t run = (a.blocks + grid - 1) / grid;
+  run = run < most ? (run + 7) / 8 * 8 : most;
+  adamw_kernel<T, EIGHT><<<grid, kThreads, 0, s>>>(a, run);
   cx_note_launch();
   return cx_check_launch("cx_adamw_step");
 }
