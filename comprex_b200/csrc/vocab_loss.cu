@@ -218,7 +218,7 @@ struct Piece {
 // kPieceBytes the one that the model of the products says is fastest.  Backward call of 8192 rows, width 1024, vocabulary
 // 50257 at the power limit, pieces of up to 72 / 144 / 208 / 288 / 424 MB and the whole: 2188 / 2160 / 2115 / 2200 / 2163 /
 // 2255 us (at 1402 / 1250 / 1200 / 1085 / 1085 / 1060 MHz).
-int64_t piece_columns(const CxVocabLoss& l) {
+int64_t search_columns(const CxVocabLoss& l) {
   const int64_t size = l.dtype == CX_F32 ? 4 : 2, whole = (l.vocab + 7) / 8 * 8;
   int64_t most = kPieceBytes / (l.rows * size) / 256 * 256;
   if (most < 256) most = 256;
@@ -226,26 +226,29 @@ int64_t piece_columns(const CxVocabLoss& l) {
   if (l.dtype == CX_F32) return whole < most ? whole : most;
   int64_t best = whole < most ? whole : most;
   double least = 1e30;
-  const int64_t fewest = (l.vocab + most - 1) / most;
-  for (int64_t pieces = fewest; pieces < fewest + 4; ++pieces)
-    for (int64_t more = 0; more < 6; ++more) {
-      int64_t n = ((l.vocab + pieces - 1) / pieces + 255) / 256 * 256 + (more - 2) * 256;
-      if (n > whole) n = whole;
-      if (n < 256 || n > most) continue;
-      double time = 0;
-      const int64_t full = l.vocab / n, rest = l.vocab % n;
-      const Piece a(l, nullptr, 8, nullptr, 8, 0, n, nullptr, 8);
-      time += full * (cx_tensor_product_time(&a.prob, 1) + cx_tensor_product_time(a.both, a.count));
-      if (rest) {
-        const Piece b(l, nullptr, 8, nullptr, 8, 0, rest, nullptr, 8);
-        time += cx_tensor_product_time(&b.prob, 1) + cx_tensor_product_time(b.both, b.count);
-      }
-      if (time < least) {
-        least = time;
-        best = n;
-      }
+  for (int64_t n = most; n >= 256 && n > most / 4; n -= 256) {
+    const int64_t columns = n < whole ? n : whole, full = l.vocab / columns, rest = l.vocab % columns;
+    const Piece a(l, nullptr, 8, nullptr, 8, 0, columns, nullptr, 8);
+    double time = full * (cx_tensor_product_time(&a.prob, 1) + cx_tensor_product_time(a.both, a.count));
+    if (rest) {
+      const Piece b(l, nullptr, 8, nullptr, 8, 0, rest, nullptr, 8);
+      time += cx_tensor_product_time(&b.prob, 1) + cx_tensor_product_time(b.both, b.count);
     }
+    if (time < least) {
+      least = time;
+      best = columns;
+    }
+  }
   return best;
+}
+int64_t piece_columns(const CxVocabLoss& l) {
+  static thread_local int64_t seen[6] = {};            // the sizes asked for last, and the answer
+  const int64_t key[5] = {l.rows, l.vocab, l.dim, l.dtype, (l.dh ? 1 : 0) | (l.dw ? 2 : 0)};
+  if (memcmp(seen, key, sizeof(key)) != 0) {
+    seen[5] = search_columns(l);
+    memcpy(seen, key, sizeof(key));
+  }
+  return seen[5];
 }
 
 int backward(const CxVocabLoss& l, cxprod::Arena& ws, cudaStream_t s) {
