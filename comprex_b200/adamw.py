@@ -183,6 +183,8 @@ class AdamW(torch.optim.Optimizer):
                 loss = closure()
         for g in self.param_groups:
             self._check_settings(g)
+        if self._device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+            raise ComprexError("a step cannot be captured in a CUDA graph: its settings and step count are the launch's own")
         if self._device.type == "cuda" and torch.cuda.current_device() != self._device.index:
             with torch.cuda.device(self._device):
                 self._step()

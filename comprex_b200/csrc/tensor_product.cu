@@ -10,6 +10,8 @@
 // while the clock is 1.9 GHz and 1.3 to 1.4 when the power limit is reached; a slice of smaller tiles about 340 cycles of
 // waits and issues; a launch 4 to 6 us from its start to its first results (tensor memory 0.35, the first copies 0.5, the
 // epilogue 0.7, the end 1).  8192 x 4096 x 1024 48 us, x 4096 175 us (1.57 PFLOP/s), 8192 x 1024 x 4096 50 us.
+#include <atomic>
+
 #include "cx_product.cuh"
 #include "cx_tensor.cuh"
 
@@ -725,8 +727,14 @@ int launch(const Plan& t, int count, cudaStream_t s) {
                            : make_map(&map[2 * i + 1], p.b, p.dtype, p.k, p.n, p.ldb, kDepth);
   }
   if (rc) return rc;
-  static const int ready = (int)cudaFuncSetAttribute(tensor_product_kernel<CG, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes);
-  if (ready) return cx_set_error("cx_product", ready);
+  static std::atomic<uint64_t> ready{0};           // devices that know of the kernel's shared memory
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) dev = 63;
+  if (dev >= 63 || !(ready.load(std::memory_order_relaxed) >> dev & 1)) {
+    const cudaError_t e = cudaFuncSetAttribute(tensor_product_kernel<CG, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes);
+    if (e != cudaSuccess) return cx_set_error("cx_product", (int)e);
+    if (dev < 63) ready.fetch_or(1ull << dev, std::memory_order_relaxed);
+  }
   Plan plan = t;
   const int64_t units = (int64_t)t.job[0].units + t.job[1].units, most = cx_sm_count() / CG, workers = units < most ? units : most;
   share_out(t.job[0].units, t.job[0].slices_per, t.job[1].units, t.job[1].slices_per, workers, &plan.extra, &plan.few, &plan.many);

@@ -268,3 +268,19 @@ def test_refusals(device):
         opt.load_state_dict(cx.AdamW([p], state_bits=8).state_dict())
     opt.step()                   # no gradient anywhere: nothing moves
     assert not p.detach().any()
+
+
+@pytest.mark.gpu
+def test_a_step_is_not_captured():
+    p = torch.nn.Parameter(torch.zeros(300, device="cuda"))
+    p.grad = torch.ones(300, device="cuda")
+    opt = cx.AdamW([p])
+    opt.step()
+    before = p.detach().clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        torch.zeros(1, device="cuda")
+        with pytest.raises(ComprexError):
+            opt.step()
+    opt.step()
+    assert not torch.equal(p.detach(), before)
