@@ -108,18 +108,24 @@ class AdamW(torch.optim.Optimizer):
             a.m_scale, a.v_scale = (state[s + "_scale"].data_ptr() for s in names)
         if "master" in state:
             a.master = state["master"].data_ptr()
-            self.refresh_master()
+            self._take_master()
         # host copies of what the device holds, and pinned buffers to bring it there
         self._now = {"seg_param": torch.zeros(k, dtype=torch.int64), "seg_grad": torch.zeros(k, dtype=torch.int64),
                      "seg_class": torch.zeros(k, dtype=torch.int32)}
         self._collect, self._scalar_type = _lib.host().collect, _lib.host().scalar_type(self._params[0])
+        self._layout = _lib.host().layout(self._params)
         self._ring = {}
         self._classes, self._same = None, False
         self._place()
 
     def _place(self) -> None:
-        """The table of the tensors' addresses."""
-        if _lib.host().addresses(self._params, self._now["seg_param"].data_ptr()):
+        """The table of the tensors' addresses.  A tensor may be another one than at construction, but not another kind: the
+        flat states have its length and its memory order."""
+        changed = _lib.host().addresses(self._params, self._layout, self._now["seg_param"].data_ptr())
+        if changed < 0:
+            raise ComprexError(f"parameter {-1 - changed} is not as it was when the optimizer was made (shape, type, device or memory "
+                               "order): convert or move a model before its optimizer is made")
+        if changed:
             self._upload("seg_param")
 
     def _upload(self, name) -> None:
@@ -152,8 +158,8 @@ class AdamW(torch.optim.Optimizer):
                 g = p.grad
                 if g is None:
                     continue
-                if g.layout != torch.strided or g.size() != p.size():
-                    raise ComprexError("a gradient is sparse or does not have its parameter's shape")
+                if g.layout != torch.strided or g.size() != p.size() or g.device != p.device:
+                    raise ComprexError("a gradient is sparse, on another device or does not have its parameter's shape")
                 if g.dtype is not self._dtype or g.stride() != p.stride():
                     p.grad = torch.empty_strided(p.size(), p.stride(), dtype=self._dtype, device=p.device).copy_(g)
             changed = self._collect(self._params, self._scalar_type, 0, now.data_ptr())
@@ -230,6 +236,11 @@ class AdamW(torch.optim.Optimizer):
     @torch.no_grad()
     def refresh_master(self) -> None:
         """Take the tensors as they are as the 32-bit weights: after they were overwritten from outside."""
+        self._place()
+        self._take_master()
+
+    @torch.no_grad()
+    def _take_master(self) -> None:
         master = self._flat.get("master")
         if master is not None:
             for p, (a, n) in zip(self._params, self.spans()):
@@ -250,6 +261,7 @@ class AdamW(torch.optim.Optimizer):
             raise ComprexError("not a checkpoint of this optimizer")
         if mine["bits"] != self.state_bits or mine["numel"] != self._numel.tolist() or set(mine["flat"]) != set(self._flat):
             raise ComprexError("checkpoint was written for other parameters or another width of states")
+        self._place()
         super().load_state_dict(state_dict)
         for k, t in self._flat.items():
             t.copy_(mine["flat"][k])

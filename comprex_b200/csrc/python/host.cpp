@@ -2,7 +2,7 @@
 // much as the GPU's work:
 //  * collect: the addresses of an optimizer's gradients (161 parameters: 60 us in Python, 3 us here,
 //    next to 110 us of GPU work for the step),
-//  * addresses: those of the tensors themselves,
+//  * layout, addresses: those of the tensors themselves, as long as the tensors are what they were,
 //  * run_vector: the launches of one message of a prepared connection.  Checks of the vector,
 //    descriptors and native calls took 20 us per exchange in Python, the kernels of a 64 k-element
 //    exchange take 15 us,
@@ -13,6 +13,8 @@
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 #include <torch/csrc/autograd/python_variable.h>
+
+#include <vector>
 
 #include "../cx_common.h"
 #include "operators.h"
@@ -30,7 +32,7 @@ bool same_layout(const at::Tensor& a, const at::Tensor& b) {
 }
 
 // collect(params, scalar_type, zeros, out) -> 0: the table at address `out` (one int64 per parameter)
-// already held these addresses, 1: it has changed, 2: some gradient has another element type or
+// already held these addresses, 1: it has changed, 2: some gradient has another element type, device or
 // memory order than its parameter (the table is incomplete).  `zeros` stands in for a missing one.
 PyObject* collect(PyObject*, PyObject* args) {
   PyObject* params;
@@ -51,7 +53,7 @@ PyObject* collect(PyObject*, PyObject* args) {
       const at::Tensor& p = THPVariable_Unpack(o);
       const at::Tensor& g = p.grad();
       if (g.defined()) {
-        if (static_cast<int>(g.scalar_type()) != scalar_type || g.layout() != at::kStrided || !same_layout(g, p))
+        if (static_cast<int>(g.scalar_type()) != scalar_type || g.layout() != at::kStrided || g.device() != p.device() || !same_layout(g, p))
           return PyLong_FromLong(2);
         a = reinterpret_cast<int64_t>(g.data_ptr());
       }
@@ -64,12 +66,62 @@ PyObject* collect(PyObject*, PyObject* args) {
   return PyLong_FromLong(changed);
 }
 
-// addresses(tensors, out) -> whether the table at address `out` (one int64 per tensor) did not hold them already
+// What the flat states of an optimizer go by: element type, device, sizes and strides of each of its tensors.
+void describe(const at::Tensor& t, std::vector<int64_t>& out) {
+  out.push_back(static_cast<int64_t>(t.scalar_type()));
+  out.push_back(static_cast<int64_t>(t.device().type()));
+  out.push_back(t.device().index());
+  out.push_back(t.dim());
+  for (int64_t d = 0; d < t.dim(); ++d) {
+    out.push_back(t.size(d));
+    out.push_back(t.size(d) == 1 ? 0 : t.stride(d));
+  }
+}
+// the end of the description at `d` if it is that of `t`, else NULL; nothing is read from `end` on
+const int64_t* as_described(const at::Tensor& t, const int64_t* d, const int64_t* end) {
+  if (end - d < 4 || t.layout() != at::kStrided || d[0] != static_cast<int64_t>(t.scalar_type()) || d[1] != static_cast<int64_t>(t.device().type()) ||
+      d[2] != t.device().index() || d[3] != t.dim())
+    return nullptr;
+  d += 4;
+  if (end - d < 2 * t.dim()) return nullptr;
+  const auto size = t.sizes(), stride = t.strides();
+  for (size_t i = 0; i < size.size(); ++i, d += 2)
+    if (d[0] != size[i] || (size[i] != 1 && d[1] != stride[i])) return nullptr;
+  return d;
+}
+
+// layout(tensors) -> bytes for `addresses`
+PyObject* layout(PyObject*, PyObject* tensors) {
+  if (!PyList_Check(tensors)) {
+    PyErr_SetString(PyExc_TypeError, "layout: a list of tensors");
+    return nullptr;
+  }
+  try {
+    std::vector<int64_t> all;
+    for (Py_ssize_t i = 0; i < PyList_GET_SIZE(tensors); ++i) {
+      PyObject* o = PyList_GET_ITEM(tensors, i);
+      if (!THPVariable_Check(o)) {
+        PyErr_SetString(PyExc_TypeError, "layout: not a tensor");
+        return nullptr;
+      }
+      describe(THPVariable_Unpack(o), all);
+    }
+    return PyBytes_FromStringAndSize(reinterpret_cast<const char*>(all.data()), static_cast<Py_ssize_t>(all.size() * sizeof(int64_t)));
+  } catch (const std::exception& e) {
+    PyErr_SetString(PyExc_RuntimeError, e.what());
+    return nullptr;
+  }
+}
+
+// addresses(tensors, layout, out) -> 0: the table at address `out` (one int64 per tensor) already held these addresses, 1: it
+// has changed, -1 - i: tensor i is not what `layout` says of it (the table is as it was)
 PyObject* addresses(PyObject*, PyObject* args) {
-  PyObject* tensors;
+  PyObject *tensors, *bytes;
   unsigned long long out;
-  if (!PyArg_ParseTuple(args, "O!K", &PyList_Type, &tensors, &out)) return nullptr;
+  if (!PyArg_ParseTuple(args, "O!SK", &PyList_Type, &tensors, &bytes, &out)) return nullptr;
   int64_t* table = reinterpret_cast<int64_t*>(out);
+  const int64_t* d = reinterpret_cast<const int64_t*>(PyBytes_AS_STRING(bytes));
+  const int64_t* end = d + PyBytes_GET_SIZE(bytes) / static_cast<Py_ssize_t>(sizeof(int64_t));
   bool changed = false;
   const Py_ssize_t n = PyList_GET_SIZE(tensors);
   for (Py_ssize_t i = 0; i < n; ++i) {
@@ -79,15 +131,17 @@ PyObject* addresses(PyObject*, PyObject* args) {
       return nullptr;
     }
     try {
-      const int64_t a = reinterpret_cast<int64_t>(THPVariable_Unpack(o).data_ptr());
-      changed |= table[i] != a;
-      table[i] = a;
-    } catch (const std::exception& e) {
-      PyErr_SetString(PyExc_RuntimeError, e.what());
-      return nullptr;
+      const at::Tensor& t = THPVariable_Unpack(o);
+      d = as_described(t, d, end);
+      if (!d) return PyLong_FromLong(-1 - static_cast<long>(i));
+      changed |= table[i] != reinterpret_cast<int64_t>(t.data_ptr());
+    } catch (const std::exception&) {
+      return PyLong_FromLong(-1 - static_cast<long>(i));
     }
   }
-  return PyBool_FromLong(changed);
+  if (!changed) return PyLong_FromLong(0);
+  for (Py_ssize_t i = 0; i < n; ++i) table[i] = reinterpret_cast<int64_t>(THPVariable_Unpack(PyList_GET_ITEM(tensors, i)).data_ptr());
+  return PyLong_FromLong(1);
 }
 
 int element_code(const at::Tensor& t) {
@@ -210,6 +264,7 @@ PyObject* scalar_type(PyObject*, PyObject* o) {
 }
 
 PyMethodDef methods[] = {{"collect", collect, METH_VARARGS, nullptr},
+                         {"layout", layout, METH_O, nullptr},
                          {"addresses", addresses, METH_VARARGS, nullptr},
                          {"run_vector", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(run_vector)),
                           METH_FASTCALL, nullptr},

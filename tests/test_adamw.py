@@ -284,3 +284,62 @@ def test_a_step_is_not_captured():
             opt.step()
     opt.step()
     assert not torch.equal(p.detach(), before)
+
+
+def _replaced(p, how):
+    """``p.data`` as another tensor than the one that the optimizer was made for, with a gradient that fits it."""
+    if how == "shorter":
+        p.data = torch.zeros(4, 2, 2, 2, dtype=p.dtype, device=p.device)
+    elif how == "longer":
+        p.data = torch.zeros(4, 3, 2, 8, dtype=p.dtype, device=p.device)
+    elif how == "shape":
+        p.data = p.data.reshape(3, 4, 2, 2).clone()
+    elif how == "order":
+        p.data = p.data.contiguous(memory_format=torch.channels_last)
+    elif how == "dimensions":
+        p.data = p.data.reshape(48).clone()
+    p.grad = torch.ones_like(p)
+
+
+@pytest.mark.parametrize("how", ["shorter", "longer", "shape", "order", "dimensions"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_replaced_tensor_is_refused(device, dtype, how):
+    """Length and order of the flat states are those of construction: a step over another tensor would leave it, or mix it up."""
+    p = torch.nn.Parameter(torch.randn(4, 3, 2, 2, generator=torch.Generator().manual_seed(0)).to(device, dtype))
+    opt = cx.AdamW([p], lr=0.1)
+    was = p.data
+    held = {k: t.clone() for k, t in opt.flat_state().items()}
+    _replaced(p, how)
+    before = p.detach().clone()
+    for call in (opt.step, opt.refresh_master, lambda: opt.load_state_dict(cx.AdamW([torch.nn.Parameter(was.clone())]).state_dict())):
+        with pytest.raises(ComprexError, match="as it was"):
+            call()
+    assert torch.equal(p.detach(), before)
+    assert all(torch.equal(t, opt.flat_state()[k]) for k, t in held.items())
+    # the tensor that it was made for, or another one like it, steps
+    p.data = was.clone()
+    p.grad = torch.ones_like(p)
+    opt.step()
+    assert not torch.equal(p.detach(), was)
+
+
+def test_sizes_of_one_have_no_order(device):
+    """Strides of dimensions of size 1 say nothing: converting such a tensor changes only them."""
+    p = torch.nn.Parameter(torch.zeros(4, 3, 1, 1, device=device))
+    opt = cx.AdamW([p], lr=0.1)
+    p.data = p.data.as_strided(p.size(), (3, 1, 3, 3))
+    p.grad = torch.ones_like(p)
+    opt.step()
+    assert (p.detach() < 0).all()
+
+
+@pytest.mark.gpu
+def test_a_module_that_moved_is_refused():
+    for there, back in (("cpu", "cuda"), ("cuda", "cpu")):
+        m = torch.nn.Linear(8, 8).to(there)
+        opt = cx.AdamW(m.parameters(), lr=0.1)
+        m.to(back)
+        for p in m.parameters():
+            p.grad = torch.ones_like(p)
+        with pytest.raises(ComprexError, match="as it was"):
+            opt.step()
