@@ -19,7 +19,8 @@ parameters (:meth:`AdamW.flat_state`).  With ``state_bits=8`` each block of 256 
 ``exp_avg_rms``, the square root of the second moment, as ``float8_e4m3fn`` times a power of two: 2.03 bytes an
 element instead of 8.  They are rounded at random (up as often as what is cut off is part of a step), because a moving
 average with a beta near one would never leave its value under rounding to nearest; the random bits are a hash of the
-element's place, the step and ``seed``, so a run can be repeated bit for bit and does not depend on the launch.  A
+element's place, the number of the optimizer's step and ``seed``, so a run can be repeated bit for bit and does not depend on the
+launch.  A
 gradient that is no number spoils its own element, and the 8-bit states of its block.
 """
 from __future__ import annotations
@@ -98,6 +99,7 @@ class AdamW(torch.optim.Optimizer):
                 state[s + "_scale"] = torch.zeros(nblk, dtype=torch.float32, device=dev)
         self._flat = state
         self._steps = np.zeros(k, dtype=np.int64)
+        self._turns = 0                       # steps that moved any tensor: what the random bits go by
         a = self._args = _lib.AdamW()
         for name, t in self._lay.items():
             setattr(a, name, t.data_ptr())
@@ -220,8 +222,9 @@ class AdamW(torch.optim.Optimizer):
             c.decay = 1.0 - float(g["lr"]) * float(g["weight_decay"])
             c.b1, c.ob1, c.b2, c.ob2 = b1, 1.0 - b1, b2, 1.0 - b2
             c.rate, c.norm, c.eps = float(g["lr"]) / (1.0 - b1 ** t), 1.0 / math.sqrt(1.0 - b2 ** t), g["eps"]
+        self._turns += bool(self._has.any())
         lib = _lib.load()
-        a.noise = lib.cx_adamw_noise((self.seed + int(self._steps.max())) & 0xFFFFFFFF)
+        a.noise = lib.cx_adamw_noise((self.seed + self._turns) & 0xFFFFFFFF)
         _lib.check(lib.cx_adamw_step(self._dev, C.byref(a), _lib.stream_ptr(self._device)), "cx_adamw_step")
 
     def flat_state(self) -> dict:
@@ -250,7 +253,7 @@ class AdamW(torch.optim.Optimizer):
     def state_dict(self):
         sd = super().state_dict()
         sd["comprex_adamw"] = {"version": 1, "bits": self.state_bits, "seed": self.seed, "numel": self._numel.tolist(),
-                               "steps": self._steps.tolist(), "flat": {k: t.detach().cpu().clone() for k, t in self._flat.items()}}
+                               "steps": self._steps.tolist(), "turns": self._turns, "flat": {k: t.detach().cpu().clone() for k, t in self._flat.items()}}
         return sd
 
     @torch.no_grad()
@@ -267,6 +270,7 @@ class AdamW(torch.optim.Optimizer):
             t.copy_(mine["flat"][k])
         self.seed = int(mine["seed"])
         self._steps = np.array(mine["steps"], dtype=np.int64)
+        self._turns = int(mine.get("turns", max(mine["steps"])))
         self._classes = None
         if "master" in self._flat:
             for p, (a, n) in zip(self._params, self.spans()):

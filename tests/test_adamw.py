@@ -343,3 +343,57 @@ def test_a_module_that_moved_is_refused():
             p.grad = torch.ones_like(p)
         with pytest.raises(ComprexError, match="as it was"):
             opt.step()
+
+
+def test_rounding_goes_on_while_another_tensor_rests(device):
+    """A tensor with more steps that gets no gradient any more: the others' random bits are new ones at every step all the same, so
+    their moments follow (bounds as in the test of one tensor)."""
+    n = 4096
+    p, rests = (torch.nn.Parameter(torch.zeros(n, device=device)) for _ in range(2))
+    opt = cx.AdamW([p, rests], state_bits=8, lr=0.0, betas=(0.9, 0.98), weight_decay=0.0)
+    rests.grad = torch.ones(n, device=device)
+    for _ in range(200):
+        opt.step()
+    rests.grad = None
+    p.grad = torch.ones(n, device=device)
+    opt.step()
+    p.grad = torch.full((n,), 0.25, device=device)
+    p.grad[::256] = 1.0
+    steps = 60
+    for _ in range(steps):
+        opt.step()
+    keep = torch.arange(n) % 256 != 0
+    got = (_decoded(opt, "exp_avg_rms")[0][keep] ** 2).mean().item()
+    exact = 0.02 * 0.98 ** steps + 0.0625 * (1 - 0.98 ** steps)
+    assert exact * 0.98 <= got <= exact * (1 + steps * 2.0 ** -8 * 1.05)
+    # the first moment is near 0.25, in steps of 2^-5 of it at most 2^-3 wide; independent roundings, forgotten with 0.9 a step, have a
+    # standard deviation below half a step / sqrt(1 - 0.81) each; their mean over n elements within five of its own
+    exact = 0.1 * 0.9 ** steps + 0.25 * (1 - 0.9 ** steps)
+    assert abs(_decoded(opt, "exp_avg")[0][keep].mean().item() - exact) <= 5 * (0.25 / 8 / 2 / (1 - 0.81) ** 0.5) / keep.sum().item() ** 0.5 + 0.25 * steps * 2.0 ** -16
+
+
+def test_a_checkpoint_keeps_the_rounding(device):
+    """The steps that make the random bits are the optimizer's own, whichever tensors took them."""
+    def make():
+        params = _params(torch.bfloat16, device, [700, 300])
+        return params, cx.AdamW(params, state_bits=8, seed=1, **HYPER)
+
+    def run(opt, params, steps):
+        for t in steps:
+            _set_grads(params, seed=t)
+            params[t % 2].grad = None
+            opt.step()
+    a, whole = make()
+    run(whole, a, range(6))
+    b, part = make()
+    run(part, b, range(3))
+    c, other = make()
+    other.load_state_dict(part.state_dict())
+    run(other, c, range(3, 6))
+    assert all(torch.equal(x, y) for x, y in zip(a, c))
+    for k, t in whole.flat_state().items():
+        assert torch.equal(t.view(torch.uint8), other.flat_state()[k].view(torch.uint8)), k
+    # a file without the number of steps: that of the tensor with the most
+    old = part.state_dict()
+    del old["comprex_adamw"]["turns"]
+    other.load_state_dict(old)
