@@ -226,6 +226,7 @@ class AdamW(torch.optim.Optimizer):
         lib = _lib.load()
         a.noise = lib.cx_adamw_noise((self.seed + self._turns) & 0xFFFFFFFF)
         _lib.check(lib.cx_adamw_step(self._dev, C.byref(a), _lib.stream_ptr(self._device)), "cx_adamw_step")
+        _lib.host().stepped(self._params, self._now["seg_grad"].data_ptr())
 
     def flat_state(self) -> dict:
         """The buffers that hold the states of all tensors (not copies): ``master`` for 16-bit tensors, ``exp_avg`` and

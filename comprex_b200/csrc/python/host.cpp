@@ -3,6 +3,7 @@
 //  * collect: the addresses of an optimizer's gradients (161 parameters: 60 us in Python, 3 us here,
 //    next to 110 us of GPU work for the step),
 //  * layout, addresses: those of the tensors themselves, as long as the tensors are what they were,
+//  * stepped: tells autograd which tensors have been written,
 //  * run_vector: the launches of one message of a prepared connection.  Checks of the vector,
 //    descriptors and native calls took 20 us per exchange in Python, the kernels of a 64 k-element
 //    exchange take 15 us,
@@ -144,6 +145,24 @@ PyObject* addresses(PyObject*, PyObject* args) {
   return PyLong_FromLong(1);
 }
 
+// stepped(tensors, table): those with an address at `table` (one int64 per tensor, 0: none) have been written in place
+PyObject* stepped(PyObject*, PyObject* args) {
+  PyObject* tensors;
+  unsigned long long at;
+  if (!PyArg_ParseTuple(args, "O!K", &PyList_Type, &tensors, &at)) return nullptr;
+  const int64_t* table = reinterpret_cast<const int64_t*>(at);
+  for (Py_ssize_t i = 0; i < PyList_GET_SIZE(tensors); ++i) {
+    PyObject* o = PyList_GET_ITEM(tensors, i);
+    if (!THPVariable_Check(o)) {
+      PyErr_SetString(PyExc_TypeError, "stepped: not a tensor");
+      return nullptr;
+    }
+    const at::Tensor& t = THPVariable_Unpack(o);
+    if (table[i] && !t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+  }
+  Py_RETURN_NONE;
+}
+
 int element_code(const at::Tensor& t) {
   switch (t.scalar_type()) {
     case at::kFloat: return CX_F32;
@@ -266,6 +285,7 @@ PyObject* scalar_type(PyObject*, PyObject* o) {
 PyMethodDef methods[] = {{"collect", collect, METH_VARARGS, nullptr},
                          {"layout", layout, METH_O, nullptr},
                          {"addresses", addresses, METH_VARARGS, nullptr},
+                         {"stepped", stepped, METH_VARARGS, nullptr},
                          {"run_vector", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(run_vector)),
                           METH_FASTCALL, nullptr},
                          {"install", install, METH_O, nullptr},

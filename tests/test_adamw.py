@@ -397,3 +397,20 @@ def test_a_checkpoint_keeps_the_rounding(device):
     old = part.state_dict()
     del old["comprex_adamw"]["turns"]
     other.load_state_dict(old)
+
+
+def test_a_graph_from_before_the_step_is_refused(device):
+    """A step changes tensors in place, as autograd must know: a graph that still holds them cannot be gone back through."""
+    w, b = (torch.nn.Parameter(torch.ones(*s, device=device)) for s in ((3, 5), (3,)))
+    opt = cx.AdamW([w, b], lr=0.1)
+    x = torch.ones(2, 5, device=device, requires_grad=True)
+    y = cx.linear(x, w, b).square().sum()
+    y.backward(retain_graph=True)
+    b.grad = None
+    versions = w._version, b._version
+    opt.step()
+    assert w._version > versions[0] and b._version == versions[1]       # only what has stepped
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    opt.zero_grad()
+    cx.linear(x, w, b).sum().backward()                                 # a new graph is as good as any
