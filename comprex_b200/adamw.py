@@ -36,6 +36,7 @@ from ._lib import ComprexError
 from .optim import _dense_layout
 
 _BLOCK = 256
+_ONE_STEP = np.array([[0], [1]])
 
 
 class AdamW(torch.optim.Optimizer):
@@ -172,16 +173,16 @@ class AdamW(torch.optim.Optimizer):
             self._upload("seg_grad")
         return bool(changed)
 
-    def _set_classes(self) -> None:
-        """Tensors with the same settings and step count share a row of settings."""
-        pair, of = np.unique(np.stack((self._group, self._steps)), axis=1, return_inverse=True)
+    def _make_classes(self, steps):
+        """Tensors with the same settings and step count share a row of settings: (group, steps) of the rows."""
+        pair, of = np.unique(np.stack((self._group, steps)), axis=1, return_inverse=True)
         if pair.shape[1] > len(self._args.cls):
             raise ComprexError(f"more than {len(self._args.cls)} different settings and step counts")
-        self._classes = pair
         of = torch.from_numpy(of.reshape(-1).astype(np.int32))
         if not torch.equal(of, self._now["seg_class"]):
             self._now["seg_class"].copy_(of)
             self._upload("seg_class")
+        return pair
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -208,24 +209,23 @@ class AdamW(torch.optim.Optimizer):
             self._has = has
             self._classes = None
         a = self._args
+        steps = self._steps + self._has
         if self._same and self._classes is not None:
-            # all tensors step: the classes stay what they are, one step further
-            self._steps += 1
-            self._classes[1] += 1
+            classes = self._classes + _ONE_STEP          # all tensors step: the classes stay what they are, one step further
         else:
-            self._steps += self._has
-            self._set_classes()
-        for i, (group, t) in enumerate(self._classes.T.tolist()):
+            classes = self._make_classes(steps)
+        for i, (group, t) in enumerate(classes.T.tolist()):
             g, c = self.param_groups[group], a.cls[i]
             b1, b2 = g["betas"]
             t = max(t, 1)                     # a class that has never stepped has no tensor with a gradient
             c.decay = 1.0 - float(g["lr"]) * float(g["weight_decay"])
             c.b1, c.ob1, c.b2, c.ob2 = b1, 1.0 - b1, b2, 1.0 - b2
             c.rate, c.norm, c.eps = float(g["lr"]) / (1.0 - b1 ** t), 1.0 / math.sqrt(1.0 - b2 ** t), g["eps"]
-        self._turns += bool(self._has.any())
+        turns = self._turns + bool(self._has.any())
         lib = _lib.load()
-        a.noise = lib.cx_adamw_noise((self.seed + self._turns) & 0xFFFFFFFF)
+        a.noise = lib.cx_adamw_noise((self.seed + turns) & 0xFFFFFFFF)
         _lib.check(lib.cx_adamw_step(self._dev, C.byref(a), _lib.stream_ptr(self._device)), "cx_adamw_step")
+        self._steps, self._classes, self._turns = steps, classes, turns          # a step that was refused does not count
         _lib.host().stepped(self._params, self._now["seg_grad"].data_ptr())
 
     def flat_state(self) -> dict:

@@ -414,3 +414,32 @@ def test_a_graph_from_before_the_step_is_refused(device):
         y.backward()
     opt.zero_grad()
     cx.linear(x, w, b).sum().backward()                                 # a new graph is as good as any
+
+
+def test_a_step_that_failed_does_not_count(device, monkeypatch):
+    """Neither the tensors' step counts nor the optimizer's own move before the launch is out."""
+    from comprex_b200 import _lib
+    lib = _lib.load()
+
+    class Failing:
+        def __getattr__(self, name):
+            return (lambda *a: -1) if name == "cx_adamw_step" else getattr(lib, name)
+    params = _params(torch.bfloat16, device, [300, 5, 700])
+    twin = _params(torch.bfloat16, device, [300, 5, 700])
+    opt, clean = (cx.AdamW(x, state_bits=8, **HYPER) for x in (params, twin))
+    for turn, missing in enumerate([(), (1,), (), (0, 2), ()]):
+        for x in (params, twin):
+            _set_grads(x, seed=turn)
+            for i in missing:
+                x[i].grad = None
+        with monkeypatch.context() as m:
+            m.setattr(_lib, "load", lambda: Failing())
+            for _ in range(2):
+                with pytest.raises(ComprexError):
+                    opt.step()
+        opt.step()
+        clean.step()
+    assert all(torch.equal(a, b) for a, b in zip(params, twin))
+    for k, t in clean.flat_state().items():
+        assert torch.equal(t.view(torch.uint8), opt.flat_state()[k].view(torch.uint8)), k
+    assert opt.state_dict()["comprex_adamw"]["steps"] == clean.state_dict()["comprex_adamw"]["steps"] == [4, 4, 4]
