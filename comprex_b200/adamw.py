@@ -133,6 +133,13 @@ class AdamW(torch.optim.Optimizer):
 
     def _upload(self, name) -> None:
         """Table ``name`` to the device, in stream order and without waiting for it."""
+        try:
+            self._send(name)
+        except BaseException:
+            self._now[name].fill_(-1)         # not what the device holds: the next step sends it
+            raise
+
+    def _send(self, name) -> None:
         src = self._now[name]
         if self._device.type != "cuda":
             self._lay[name].copy_(src)

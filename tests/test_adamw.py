@@ -443,3 +443,29 @@ def test_a_step_that_failed_does_not_count(device, monkeypatch):
     for k, t in clean.flat_state().items():
         assert torch.equal(t.view(torch.uint8), opt.flat_state()[k].view(torch.uint8)), k
     assert opt.state_dict()["comprex_adamw"]["steps"] == clean.state_dict()["comprex_adamw"]["steps"] == [4, 4, 4]
+
+
+def test_a_table_that_was_not_brought_over_is_sent_again(device):
+    """Addresses that the device has not got are not taken for known: it would go on with the old ones."""
+    class Broken:
+        def copy_(self, *args, **kwargs):
+            raise RuntimeError("no memory")
+    params = _params(torch.float32, device, [300, 5, 700])
+    twin = _params(torch.float32, device, [300, 5, 700])
+    opt, clean = (cx.AdamW(x, **HYPER) for x in (params, twin))
+    held = []
+    for turn, name in enumerate(["seg_param", "seg_grad", "seg_class"]):
+        for x in (params, twin):
+            _set_grads(x, seed=turn)
+            if name == "seg_param":
+                held.append(x[0].data)
+                x[0].data = x[0].data.clone()
+            if name == "seg_class":
+                x[1].grad = None
+        table, opt._lay[name] = opt._lay[name], Broken()
+        with pytest.raises(RuntimeError, match="no memory"):
+            opt.step()
+        opt._lay[name] = table
+        opt.step()
+        clean.step()
+        assert all(torch.equal(a, b) for a, b in zip(params, twin)), name
