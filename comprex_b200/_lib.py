@@ -103,7 +103,7 @@ class AdamW(C.Structure):
     _fields_ = ([(n, C.c_void_p) for n in ("blk_seg", "seg_blk", "seg_len", "seg_param", "seg_grad", "seg_class", "master", "m",
                                            "v", "m_scale", "v_scale")]
                 + [("blocks", C.c_int64), ("segs", C.c_int32), ("dtype", C.c_int32), ("bits", C.c_int32),
-                   ("noise", C.c_uint32), ("cls", AdamWClass * 64)])
+                   ("noise", C.c_uint32), ("first_class", C.c_int32), ("pad", C.c_int32), ("cls", AdamWClass * 64)])
 
 
 ACTIVATIONS = {None: 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}

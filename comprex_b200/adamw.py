@@ -181,13 +181,13 @@ class AdamW(torch.optim.Optimizer):
         return bool(changed)
 
     def _make_classes(self, steps):
-        """Tensors with the same settings and step count share a row of settings: (group, steps) of the rows."""
-        pair, of = np.unique(np.stack((self._group, steps)), axis=1, return_inverse=True)
-        if pair.shape[1] > len(self._args.cls):
-            raise ComprexError(f"more than {len(self._args.cls)} different settings and step counts")
-        of = torch.from_numpy(of.reshape(-1).astype(np.int32))
-        if not torch.equal(of, self._now["seg_class"]):
-            self._now["seg_class"].copy_(of)
+        """Tensors that step with the same settings and step count share a row of settings: (group, steps) of the rows."""
+        pair, of = np.unique(np.stack((self._group, steps))[:, self._has], axis=1, return_inverse=True)
+        table = np.full(len(steps), -1, dtype=np.int32)
+        table[self._has] = of.reshape(-1)
+        table = torch.from_numpy(table)
+        if not torch.equal(table, self._now["seg_class"]):
+            self._now["seg_class"].copy_(table)
             self._upload("seg_class")
         return pair
 
@@ -221,17 +221,18 @@ class AdamW(torch.optim.Optimizer):
             classes = self._classes + _ONE_STEP          # all tensors step: the classes stay what they are, one step further
         else:
             classes = self._make_classes(steps)
-        for i, (group, t) in enumerate(classes.T.tolist()):
-            g, c = self.param_groups[group], a.cls[i]
-            b1, b2 = g["betas"]
-            t = max(t, 1)                     # a class that has never stepped has no tensor with a gradient
-            c.decay = 1.0 - float(g["lr"]) * float(g["weight_decay"])
-            c.b1, c.ob1, c.b2, c.ob2 = b1, 1.0 - b1, b2, 1.0 - b2
-            c.rate, c.norm, c.eps = float(g["lr"]) / (1.0 - b1 ** t), 1.0 / math.sqrt(1.0 - b2 ** t), g["eps"]
         turns = self._turns + bool(self._has.any())
         lib = _lib.load()
         a.noise = lib.cx_adamw_noise((self.seed + turns) & 0xFFFFFFFF)
-        _lib.check(lib.cx_adamw_step(self._dev, C.byref(a), _lib.stream_ptr(self._device)), "cx_adamw_step")
+        rows, stream = classes.T.tolist(), _lib.stream_ptr(self._device)
+        for a.first_class in range(0, len(rows), len(a.cls)):        # one launch, where there are more rows than it holds more
+            for c, (group, t) in zip(a.cls, rows[a.first_class:]):
+                g = self.param_groups[group]
+                b1, b2 = g["betas"]
+                c.decay = 1.0 - float(g["lr"]) * float(g["weight_decay"])
+                c.b1, c.ob1, c.b2, c.ob2 = b1, 1.0 - b1, b2, 1.0 - b2
+                c.rate, c.norm, c.eps = float(g["lr"]) / (1.0 - b1 ** t), 1.0 / math.sqrt(1.0 - b2 ** t), g["eps"]
+            _lib.check(lib.cx_adamw_step(self._dev, C.byref(a), stream), "cx_adamw_step")
         self._steps, self._classes, self._turns = steps, classes, turns          # a step that was refused does not count
         _lib.host().stepped(self._params, self._now["seg_grad"].data_ptr())
 

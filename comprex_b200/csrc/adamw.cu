@@ -118,7 +118,8 @@ __global__ void __launch_bounds__(kThreads, EIGHT ? 4 : 2) adamw_kernel(const __
         param0 = reinterpret_cast<T*>(a.seg_param[seg]);
         first = a.seg_blk[seg];
         len = a.seg_len[seg];
-        cls = a.seg_class[seg];
+        cls = a.seg_class[seg] - a.first_class;
+        if ((uint32_t)cls >= CX_ADAMW_CLASSES) grad0 = nullptr;      // its settings are another launch's
         const char* base = part == 0 ? reinterpret_cast<const char*>(grad0) - first * per
                            : part == 1 ? (sizeof(T) == 4 ? reinterpret_cast<const char*>(param0) - first * per : reinterpret_cast<const char*>(a.master))
                            : reinterpret_cast<const char*>(part == 2 ? a.m : a.v);

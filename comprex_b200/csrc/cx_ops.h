@@ -27,7 +27,7 @@ typedef struct CxAdamW {
   const int64_t* seg_len;      /* [segs] its elements */
   void* const* seg_param;      /* [segs] the tensors */
   const void* const* seg_grad; /* [segs] and their gradients, of the same type; NULL: the tensor is left as it is */
-  const int32_t* seg_class;    /* [segs] index into cls */
+  const int32_t* seg_class;    /* [segs] row of settings; those of this call are first_class + index into cls */
   float* master;               /* flat 32-bit weights behind 16-bit tensors; NULL for tensors of 32 bits */
   void* m;                     /* flat first moments: float, or e4m3 with 8 bits */
   void* v;                     /* flat second moments: float, or with 8 bits e4m3 of their square roots */
@@ -38,6 +38,8 @@ typedef struct CxAdamW {
   int32_t dtype;               /* CX_F32, CX_BF16, CX_F16 */
   int32_t bits;                /* 32 or 8 */
   uint32_t noise;              /* of this step: cx_adamw_noise(seed + step) */
+  int32_t first_class;         /* tensors of other rows are left as they are: more rows are more calls */
+  int32_t pad;
   CxAdamWClass cls[CX_ADAMW_CLASSES];
 } CxAdamW;
 

@@ -58,7 +58,7 @@ uint32_t cx_adamw_noise(uint32_t number) { return cxadam::mix(number); }
 int cx_adamw_step(int dev, const CxAdamW* a, void* stream) {
   if (!a || !type_ok(a->dtype)) return cx_set_error("cx_adamw_step: bad element type", 0);
   if (a->bits != 8 && a->bits != 32) return cx_set_error("cx_adamw_step: states have 8 or 32 bits", 0);
-  if (a->blocks < 0 || a->segs < 0) return cx_set_error("cx_adamw_step: negative size", 0);
+  if (a->blocks < 0 || a->segs < 0 || a->first_class < 0) return cx_set_error("cx_adamw_step: negative size", 0);
   if (a->blocks == 0) return 0;
   if (!a->blk_seg || !a->seg_blk || !a->seg_len || !a->seg_param || !a->seg_grad || !a->seg_class || !a->m || !a->v ||
       (a->bits == 8 && (!a->m_scale || !a->v_scale)) || (a->dtype != CX_F32 && !a->master))

@@ -50,8 +50,9 @@ int cx_adamw_step_host(const CxAdamW* a) {
   for (int64_t b = 0; b < a->blocks; ++b) {
     const int32_t seg = a->blk_seg[b];
     const void* grad = a->seg_grad[seg];
-    if (!grad) continue;
-    const CxAdamWClass& c = a->cls[a->seg_class[seg]];
+    const uint32_t row = (uint32_t)(a->seg_class[seg] - a->first_class);
+    if (!grad || row >= CX_ADAMW_CLASSES) continue;      // (of another call)
+    const CxAdamWClass& c = a->cls[row];
     const int64_t at = (b - a->seg_blk[seg]) * CX_ADAMW_BLOCK, flat = b * CX_ADAMW_BLOCK;
     const int left = (int)std::min<int64_t>(CX_ADAMW_BLOCK, a->seg_len[seg] - at);
     uint32_t top_m = 0, top_v = 0;

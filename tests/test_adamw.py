@@ -469,3 +469,48 @@ def test_a_table_that_was_not_brought_over_is_sent_again(device):
         opt.step()
         clean.step()
         assert all(torch.equal(a, b) for a, b in zip(params, twin)), name
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_every_tensor_its_own_step_count(device, bits):
+    """More step counts than fit into one launch, and tensors that rest: as each tensor would step alone."""
+    k = 150
+    params = _params(torch.bfloat16, device, [40 + 7 * i for i in range(k)])
+    opt = cx.AdamW(params, state_bits=bits, seed=2, **HYPER)
+    launches = []
+    for turn in range(k + 2):
+        _set_grads(params, seed=turn)
+        for i, p in enumerate(params):
+            if i > turn:                          # tensor i steps from turn i on; at last there are 150 counts
+                p.grad = None
+        if turn < k - 3:
+            opt._steps[:turn + 1] += 1            # (quickly: as if they had stepped)
+            opt._classes = None
+            continue
+        counts = opt._steps.copy()
+        before = cx.launch_count()
+        exact = []
+        held = (_decoded(opt, "exp_avg"), [r * r for r in _decoded(opt, "exp_avg_rms")]) if bits == 8 else \
+            tuple([opt.flat_state()[s][a:a + n].double().cpu() for a, n in opt.spans()] for s in ("exp_avg", "exp_avg_sq"))
+        for i, (w, p) in enumerate(zip(_weights(opt, params), params)):
+            exact.append(w if p.grad is None else _formula(w, held[0][i], held[1][i], p.grad.double().cpu(), int(counts[i]) + 1, **HYPER)[0])
+        opt.step()
+        launches.append(cx.launch_count() - before)
+        for got, w in zip(_weights(opt, params), exact):
+            assert (got - w).abs().max() <= EPS32 * (2 * w.abs().max() + 10 * HYPER["lr"] * 8) + 1e-7
+    assert opt.state_dict()["comprex_adamw"]["steps"] == [k + 2 - i for i in range(k)]
+    if device == "cuda":
+        assert launches[-1] == 3                  # 64 rows of settings each
+
+
+def test_settings_of_tensors_that_rest_take_no_row(device):
+    params = _params(torch.float32, device, [20] * 100)
+    opt = cx.AdamW(params, **HYPER)
+    for i, p in enumerate(params):
+        for q in params:
+            q.grad = None
+        p.grad = torch.ones_like(p)
+        before = cx.launch_count()
+        opt.step()
+        assert device != "cuda" or cx.launch_count() - before == 1
+    assert opt.state_dict()["comprex_adamw"]["steps"] == [1] * 100
