@@ -60,8 +60,8 @@ class AdamW(torch.optim.Optimizer):
         for p in self._params:
             if p.dtype != self._dtype or p.device != self._device:
                 raise ComprexError("all parameters must share one dtype and live on one device")
-            if p.layout != torch.strided or not _dense_layout(p):
-                raise ComprexError("a parameter has gaps in memory")
+            if p.layout != torch.strided or not _dense_layout(p) or p.is_neg():
+                raise ComprexError("a parameter has gaps in memory, or its sign only noted")
         self._lay_out()
 
     @staticmethod
@@ -170,7 +170,7 @@ class AdamW(torch.optim.Optimizer):
                     continue
                 if g.layout != torch.strided or g.size() != p.size() or g.device != p.device:
                     raise ComprexError("a gradient is sparse, on another device or does not have its parameter's shape")
-                if g.dtype is not self._dtype or g.stride() != p.stride():
+                if g.dtype is not self._dtype or g.stride() != p.stride() or g.is_neg():
                     p.grad = torch.empty_strided(p.size(), p.stride(), dtype=self._dtype, device=p.device).copy_(g)
             changed = self._collect(self._params, self._scalar_type, 0, now.data_ptr())
             if changed == 2:

@@ -33,8 +33,8 @@ bool same_layout(const at::Tensor& a, const at::Tensor& b) {
 }
 
 // collect(params, scalar_type, zeros, out) -> 0: the table at address `out` (one int64 per parameter)
-// already held these addresses, 1: it has changed, 2: some gradient has another element type, device or
-// memory order than its parameter (the table is incomplete).  `zeros` stands in for a missing one.
+// already held these addresses, 1: it has changed, 2: some gradient has another element type, device,
+// memory order or sign convention than its parameter (the table is incomplete).  `zeros` stands in for a missing one.
 PyObject* collect(PyObject*, PyObject* args) {
   PyObject* params;
   int scalar_type;
@@ -54,7 +54,7 @@ PyObject* collect(PyObject*, PyObject* args) {
       const at::Tensor& p = THPVariable_Unpack(o);
       const at::Tensor& g = p.grad();
       if (g.defined()) {
-        if (static_cast<int>(g.scalar_type()) != scalar_type || g.layout() != at::kStrided || g.device() != p.device() || !same_layout(g, p))
+        if (static_cast<int>(g.scalar_type()) != scalar_type || g.layout() != at::kStrided || g.device() != p.device() || g.is_neg() || !same_layout(g, p))
           return PyLong_FromLong(2);
         a = reinterpret_cast<int64_t>(g.data_ptr());
       }
@@ -80,7 +80,7 @@ void describe(const at::Tensor& t, std::vector<int64_t>& out) {
 }
 // the end of the description at `d` if it is that of `t`, else NULL; nothing is read from `end` on
 const int64_t* as_described(const at::Tensor& t, const int64_t* d, const int64_t* end) {
-  if (end - d < 4 || t.layout() != at::kStrided || d[0] != static_cast<int64_t>(t.scalar_type()) || d[1] != static_cast<int64_t>(t.device().type()) ||
+  if (end - d < 4 || t.layout() != at::kStrided || t.is_neg() || d[0] != static_cast<int64_t>(t.scalar_type()) || d[1] != static_cast<int64_t>(t.device().type()) ||
       d[2] != t.device().index() || d[3] != t.dim())
     return nullptr;
   d += 4;

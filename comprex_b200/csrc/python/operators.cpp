@@ -69,9 +69,9 @@ void* stream_of(const Tensor& t) {
   return c10::impl::VirtualGuardImpl(c10::DeviceType::CUDA).getStream(t.device()).native_handle();
 }
 
-// `t` as a matrix of rows of `cols` consecutive elements that do not overlap: a view where that can be
+// `t` as a matrix of rows of `cols` consecutive elements that do not overlap, with their signs in memory: a view where that can be
 Tensor rows_of(const Tensor& t, int64_t cols) {
-  Tensor m = t.dim() == 2 ? t : t.reshape({-1, cols});
+  Tensor m = (t.dim() == 2 ? t : t.reshape({-1, cols})).resolve_neg();
   if ((m.size(0) > 1 && m.stride(0) < cols) || (cols > 1 && m.stride(1) != 1)) m = m.contiguous();
   return m;
 }
@@ -138,7 +138,7 @@ Tensor linear_forward(const Tensor& x, const Tensor& w, const Maybe& bias, int a
     return y;
   }
   const c10::OptionalDeviceGuard guard(x.is_cuda() ? std::make_optional(x.device()) : std::nullopt);
-  const Tensor xm = rows_of(x, inner), wm = rows_of(w, inner), b = bias ? bias->contiguous() : Tensor(), r = residual ? rows_of(*residual, outer) : Tensor();
+  const Tensor xm = rows_of(x, inner), wm = rows_of(w, inner), b = bias ? bias->resolve_neg().contiguous() : Tensor(), r = residual ? rows_of(*residual, outer) : Tensor();
   CxLinear d = describe(xm, wm, act);
   if (bias) d.bias = b.data_ptr();
   if (residual) {
@@ -226,7 +226,7 @@ CxVocabLoss describe(const Tensor& hm, const Tensor& wm, const Tensor& tm, int64
 
 Tensor loss_forward(const Tensor& h, const Tensor& w, const Tensor& targets, int64_t ignore, int reduction, Tensor& tm, Tensor& lse, Tensor& count) {
   const c10::OptionalDeviceGuard guard(h.is_cuda() ? std::make_optional(h.device()) : std::nullopt);
-  tm = targets.reshape({-1}).contiguous();
+  tm = targets.reshape({-1}).resolve_neg().contiguous();
   const auto f32 = h.options().dtype(at::kFloat);
   Tensor loss = reduction == CX_REDUCE_NONE ? at::empty(targets.sizes(), f32) : at::empty({}, f32);
   lse = at::empty({tm.numel()}, f32);
@@ -265,7 +265,7 @@ struct LossFn : torch::autograd::Function<LossFn> {
       const c10::OptionalDeviceGuard guard(h.is_cuda() ? std::make_optional(h.device()) : std::nullopt);
       const Tensor hm = rows_of(h, w.size(1)), wm = rows_of(w, w.size(1));
       CxVocabLoss d = describe(hm, wm, tm, ctx->saved_data["ignore"].toInt(), (int)ctx->saved_data["reduction"].toInt(), saved[3], saved[4]);
-      Tensor g = grads[0].to(at::kFloat);
+      Tensor g = grads[0].to(at::kFloat).resolve_neg();
       if (g.dim() > 1) g = g.reshape({-1});
       d.grad = g.data_ptr<float>();
       d.grad_stride = g.dim() ? g.stride(0) : 0;

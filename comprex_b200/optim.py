@@ -176,7 +176,7 @@ class _FoldTable:
             self.now.fill_(-1)                    # incomplete, and not what the device holds, should this raise
             for p in self.params:
                 g = p.grad
-                if g is not None and (g.dtype is not self.dtype or g.stride() != p.stride()):
+                if g is not None and (g.dtype is not self.dtype or g.stride() != p.stride() or g.is_neg()):
                     p.grad = torch.empty_strided(p.size(), p.stride(), dtype=self.dtype, device=p.device).copy_(g)
             changed = self._collect(self.params, self.scalar_type, zeros.data_ptr(), self.now.data_ptr())
             if changed == 2:

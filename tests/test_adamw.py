@@ -514,3 +514,16 @@ def test_settings_of_tensors_that_rest_take_no_row(device):
         opt.step()
         assert device != "cuda" or cx.launch_count() - before == 1
     assert opt.state_dict()["comprex_adamw"]["steps"] == [1] * 100
+
+
+def test_the_negative_bit(device):
+    """A gradient whose sign is only noted is one with that sign; a tensor of that kind is not one to step."""
+    p, q = (torch.nn.Parameter(torch.ones(300, device=device)) for _ in range(2))
+    g = torch.linspace(-1, 1, 300, device=device)
+    p.grad, q.grad = torch._neg_view(g), -g
+    cx.AdamW([p], lr=0.1).step()
+    cx.AdamW([q], lr=0.1).step()
+    assert torch.equal(p, q)
+    noted = torch._neg_view(torch.ones(300, device=device)).requires_grad_()
+    with pytest.raises(ComprexError):
+        cx.AdamW([noted])

@@ -179,3 +179,17 @@ def test_refusals(device):
         cx.linear(x.double(), w.double())
     with pytest.raises(ComprexError):
         cx.linear(x, w[:, :0].expand(24, 0))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_the_negative_bit(device, dtype):
+    """A tensor whose sign is only noted (an imaginary part of a conjugate, say) counts with its sign."""
+    x, w, b, r, g = _inputs(9, 24, 16, dtype, device)
+    y = cx.linear(-x, -w, -b, activation="silu", residual=-r)
+    noted = [torch._neg_view(t) for t in (x, w, b, r)]
+    assert torch.equal(cx.linear(noted[0], noted[1], noted[2], activation="silu", residual=noted[3]), y)
+    grads = []
+    for s, up in ((lambda t: -t, -g), (torch._neg_view, torch._neg_view(g))):
+        leaves = [s(t.clone()).detach().requires_grad_() for t in (x, w, b, r)]
+        grads.append(torch.autograd.grad(cx.linear(*leaves[:3], activation="silu", residual=leaves[3]), leaves, up))
+    assert all(torch.equal(p.resolve_neg(), q.resolve_neg()) for p, q in zip(*grads))

@@ -1021,3 +1021,18 @@ def test_thresholds_of_short_folded_buckets(dtype, ratio):
                 folded = folded + rests[:b.end - b.start]
             assert float(b.ar._comp.thr) == ref_threshold_topk(folded, ratio), (step, b.start)
     env.close()
+
+
+def test_a_gradient_with_the_negative_bit(device):
+    """A gradient whose sign is only noted is one with that sign."""
+    out = []
+    for noted in (False, True):
+        env = cx.GaspiEnvironment(8 << 20, device=device)
+        p = torch.nn.Parameter(torch.ones(300, device=device))
+        opt = ComprexOptimizer([p], env, lr=0.1, momentum=0.9)
+        g = torch.linspace(-1, 1, 300, device=device)
+        p.grad = torch._neg_view(g) if noted else -g
+        opt.step()
+        out.append(p.detach().clone())
+        env.close()
+    assert torch.equal(*out)

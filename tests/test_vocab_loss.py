@@ -207,3 +207,18 @@ def test_refusals(device):
                 dict(weight=w[0]), dict(hidden=h.double(), weight=w.double())):
         with pytest.raises(ComprexError):
             cx.linear_cross_entropy(**(dict(hidden=h, weight=w, targets=t) | bad))
+
+
+@pytest.mark.parametrize("which", [0, 1, 2])
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_the_negative_bit(device, reduction, which):
+    """A tensor whose sign is only noted counts with its sign, the gradient that comes in, too."""
+    h, w, t, g = _inputs(20, 90, 16, torch.bfloat16, device)
+    if reduction != "none":
+        g = g[0]
+    got = []
+    for s in (torch.neg, torch._neg_view):
+        leaves = [(s(x.clone()) if i == which else x.clone()).detach().requires_grad_() for i, x in enumerate((h, w))]
+        loss = cx.linear_cross_entropy(*leaves, t, reduction=reduction)
+        got.append([loss, *torch.autograd.grad(loss, leaves, s(g) if which == 2 else g)])
+    assert all(torch.equal(p.resolve_neg(), q.resolve_neg()) for p, q in zip(*got))
