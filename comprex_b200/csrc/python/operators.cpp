@@ -87,6 +87,11 @@ Tensor workspace(D& d, const Tensor& like, int64_t bytes) {
   return ws;
 }
 
+// There is no forward-mode derivative: a tangent would be lost in silence.
+void no_tangent(const Tensor& t, const char* name) {
+  if (t._fw_grad(0).defined()) refuse(name, " has a forward-mode tangent, and this operator no forward-mode derivative");
+}
+
 // Gradients that are computed here cannot be differentiated again: asking for it is an error of that second pass.
 variable_list once(variable_list&& grads) {
   if (!at::GradMode::is_enabled()) return std::move(grads);
@@ -172,6 +177,7 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
       const int64_t act = ctx->saved_data["act"].toInt(), inputs = ctx->saved_data["inputs"].toInt();
       variable_list out(5);
       if (!grad.defined()) return out;
+      no_tangent(grad, "the gradient");
       const bool bias = inputs & 1, residual = inputs & 2;
       const bool need_b = bias && ctx->needs_input_grad(2), need_r = residual && ctx->needs_input_grad(bias ? 3 : 2);
       const int64_t outer = w.size(0), inner = w.size(1);
@@ -255,6 +261,7 @@ struct LossFn : torch::autograd::Function<LossFn> {
       const Tensor &h = saved[0], &w = saved[1], &tm = saved[2];
       variable_list out(5);
       if (!grads[0].defined()) return out;
+      no_tangent(grads[0], "the gradient");
       const at::AutoDispatchBelowADInplaceOrView below;
       if (ctx->needs_input_grad(0)) out[0] = at::empty(h.sizes(), h.options());
       if (ctx->needs_input_grad(1)) out[1] = at::empty(w.sizes(), w.options());
@@ -286,6 +293,7 @@ const Tensor& tensor(PyObject* o, const char* name, const Tensor* like) {
   if (t.layout() != at::kStrided) refuse(name, " must be a strided tensor");
   if (!like && !t.is_cuda() && !t.is_cpu()) refuse("tensors on ", t.device(), " are not supported");
   if (like && t.device() != like->device()) refuse(name, " is on ", t.device(), ", not on ", like->device());
+  no_tangent(t, name);
   return t;
 }
 const Tensor& same_type(const Tensor& t, const char* name, const Tensor& like) {

@@ -193,3 +193,17 @@ def test_the_negative_bit(device, dtype):
         leaves = [s(t.clone()).detach().requires_grad_() for t in (x, w, b, r)]
         grads.append(torch.autograd.grad(cx.linear(*leaves[:3], activation="silu", residual=leaves[3]), leaves, up))
     assert all(torch.equal(p.resolve_neg(), q.resolve_neg()) for p, q in zip(*grads))
+
+
+def test_forward_mode_is_refused(device):
+    """A tangent is not dropped in silence: there is no forward-mode derivative."""
+    x, w, b, r, g = _inputs(4, 16, 24, torch.float32, device)
+    with torch.autograd.forward_ad.dual_level():
+        for i in range(4):
+            args = [torch.autograd.forward_ad.make_dual(t, torch.ones_like(t)) if i == j else t for j, t in enumerate((x, w, b, r))]
+            with pytest.raises(ComprexError, match="forward-mode"):
+                cx.linear(*args[:3], residual=args[3])
+        leaf = x.clone().requires_grad_()
+        up = torch.autograd.forward_ad.make_dual(g, torch.ones_like(g))
+        with pytest.raises(ComprexError, match="forward-mode"):
+            torch.autograd.grad(cx.linear(leaf, w, b), leaf, up)

@@ -222,3 +222,17 @@ def test_the_negative_bit(device, reduction, which):
         loss = cx.linear_cross_entropy(*leaves, t, reduction=reduction)
         got.append([loss, *torch.autograd.grad(loss, leaves, s(g) if which == 2 else g)])
     assert all(torch.equal(p.resolve_neg(), q.resolve_neg()) for p, q in zip(*got))
+
+
+def test_forward_mode_is_refused(device):
+    """A tangent is not dropped in silence: there is no forward-mode derivative."""
+    h, w, t, g = _inputs(8, 30, 16, torch.float32, device)
+    with torch.autograd.forward_ad.dual_level():
+        for i in range(2):
+            args = [torch.autograd.forward_ad.make_dual(x, torch.ones_like(x)) if i == j else x for j, x in enumerate((h, w))]
+            with pytest.raises(ComprexError, match="forward-mode"):
+                cx.linear_cross_entropy(*args, t)
+        leaf = h.clone().requires_grad_()
+        up = torch.autograd.forward_ad.make_dual(g, torch.ones_like(g))
+        with pytest.raises(ComprexError, match="forward-mode"):
+            torch.autograd.grad(cx.linear_cross_entropy(leaf, w, t, reduction="none"), leaf, up)
