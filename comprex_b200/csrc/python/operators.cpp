@@ -7,11 +7,13 @@
 #include <Python.h>
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/core/impl/VirtualGuardImpl.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include <sstream>
 
@@ -87,6 +89,14 @@ Tensor workspace(D& d, const Tensor& like, int64_t bytes) {
   return ws;
 }
 
+// A trace sees the outputs being allocated and not the kernels that fill them: what it plays back would be memory that nobody
+// wrote.  (torch.compile leaves a call to these functions out of its graphs.)
+void not_traced() {
+  using c10::impl::TorchDispatchModeKey;
+  if (torch::jit::tracer::isTracing() || c10::impl::TorchDispatchModeTLS::get_mode(TorchDispatchModeKey::PROXY))
+    refuse("this operator cannot be put into a trace");
+}
+
 // There is no forward-mode derivative: a tangent would be lost in silence.
 void no_tangent(const Tensor& t, const char* name) {
   if (t._fw_grad(0).defined()) refuse(name, " has a forward-mode tangent, and this operator no forward-mode derivative");
@@ -107,6 +117,7 @@ variable_list once(variable_list&& grads) {
 template <typename F>
 variable_list in_backward(const F& f) {
   try {
+    not_traced();
     return once(f());
   } catch (const Refused& r) {          // the engine may have called from a thread of its own
     const PyGILState_STATE gil = PyGILState_Ensure();
@@ -291,6 +302,7 @@ const Tensor& tensor(PyObject* o, const char* name, const Tensor* like) {
   if (!THPVariable_Check(o)) refuse(name, " must be a strided tensor");
   const Tensor& t = THPVariable_Unpack(o);
   if (t.layout() != at::kStrided) refuse(name, " must be a strided tensor");
+  if (!like) not_traced();
   if (!like && !t.is_cuda() && !t.is_cpu()) refuse("tensors on ", t.device(), " are not supported");
   if (like && t.device() != like->device()) refuse(name, " is on ", t.device(), ", not on ", like->device());
   no_tangent(t, name);

@@ -207,3 +207,23 @@ def test_forward_mode_is_refused(device):
         up = torch.autograd.forward_ad.make_dual(g, torch.ones_like(g))
         with pytest.raises(ComprexError, match="forward-mode"):
             torch.autograd.grad(cx.linear(leaf, w, b), leaf, up)
+
+
+def test_tracing_is_refused(device):
+    """A trace sees outputs being allocated, and no kernel: what it plays back would be memory that nobody wrote."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    x, w, _, _, _ = _inputs(4, 16, 24, torch.float32, device)
+    h, t = x[:, :16], torch.zeros(4, dtype=torch.int64, device=device)
+    for f in (lambda a: cx.linear(a, w), lambda a: cx.linear_cross_entropy(a, w, t)):
+        with pytest.raises(ComprexError, match="trace"):
+            torch.jit.trace(f, (h,), check_trace=False)
+        with pytest.raises(ComprexError, match="trace"):
+            make_fx(f)(h)
+    assert torch.isfinite(cx.linear(x, w)).all()
+
+    def back(a):
+        return torch.autograd.grad(y, leaf, a)[0]
+    leaf = x.clone().requires_grad_()
+    y = cx.linear(leaf, w)
+    with pytest.raises(ComprexError, match="trace"):
+        make_fx(back)(torch.ones_like(y))
