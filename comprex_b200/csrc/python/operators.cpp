@@ -97,9 +97,27 @@ void not_traced() {
     refuse("this operator cannot be put into a trace");
 }
 
+// Fake tensors, those that a transform (vmap, grad) has wrapped and subclasses that dispatch in Python have no memory that the
+// kernels could read, and under such a mode the outputs would have none either.
+void has_memory(const Tensor& t, const char* name) {
+  using c10::DispatchKey;
+  using c10::impl::TorchDispatchModeKey;
+  using c10::impl::TorchDispatchModeTLS;
+  const c10::DispatchKeySet keys = t.key_set();
+  if (TorchDispatchModeTLS::get_mode(TorchDispatchModeKey::FAKE) || TorchDispatchModeTLS::get_mode(TorchDispatchModeKey::FUNCTIONAL) ||
+      keys.has(DispatchKey::Python) || keys.has(DispatchKey::FuncTorchBatched) || keys.has(DispatchKey::FuncTorchGradWrapper) ||
+      keys.has(DispatchKey::Functionalize) || keys.has(DispatchKey::ZeroTensor) || !t.has_storage())
+    refuse(name, " has no memory of its own (a fake or wrapped tensor, or one under such a mode)");
+}
+
 // There is no forward-mode derivative: a tangent would be lost in silence.
 void no_tangent(const Tensor& t, const char* name) {
   if (t._fw_grad(0).defined()) refuse(name, " has a forward-mode tangent, and this operator no forward-mode derivative");
+}
+
+// a gradient of zeros that autograd has not written down, written down
+Tensor written(const Tensor& t) {
+  return t.defined() && t._is_zerotensor() ? at::zeros(t.sizes(), t.options()) : t;
 }
 
 // Gradients that are computed here cannot be differentiated again: asking for it is an error of that second pass.
@@ -184,10 +202,11 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     return in_backward([&]() -> variable_list {
       const variable_list saved = ctx->get_saved_variables();
-      const Tensor &x = saved[0], &w = saved[1], &pre = saved[2], &grad = grads[0];
+      const Tensor &x = saved[0], &w = saved[1], &pre = saved[2], grad = written(grads[0]);
       const int64_t act = ctx->saved_data["act"].toInt(), inputs = ctx->saved_data["inputs"].toInt();
       variable_list out(5);
       if (!grad.defined()) return out;
+      has_memory(grad, "the gradient");
       no_tangent(grad, "the gradient");
       const bool bias = inputs & 1, residual = inputs & 2;
       const bool need_b = bias && ctx->needs_input_grad(2), need_r = residual && ctx->needs_input_grad(bias ? 3 : 2);
@@ -270,8 +289,10 @@ struct LossFn : torch::autograd::Function<LossFn> {
     return in_backward([&]() -> variable_list {
       const variable_list saved = ctx->get_saved_variables();
       const Tensor &h = saved[0], &w = saved[1], &tm = saved[2];
+      grads[0] = written(grads[0]);
       variable_list out(5);
       if (!grads[0].defined()) return out;
+      has_memory(grads[0], "the gradient");
       no_tangent(grads[0], "the gradient");
       const at::AutoDispatchBelowADInplaceOrView below;
       if (ctx->needs_input_grad(0)) out[0] = at::empty(h.sizes(), h.options());
@@ -305,6 +326,7 @@ const Tensor& tensor(PyObject* o, const char* name, const Tensor* like) {
   if (!like) not_traced();
   if (!like && !t.is_cuda() && !t.is_cpu()) refuse("tensors on ", t.device(), " are not supported");
   if (like && t.device() != like->device()) refuse(name, " is on ", t.device(), ", not on ", like->device());
+  has_memory(t, name);
   no_tangent(t, name);
   return t;
 }

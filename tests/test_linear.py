@@ -227,3 +227,54 @@ def test_tracing_is_refused(device):
     y = cx.linear(leaf, w)
     with pytest.raises(ComprexError, match="trace"):
         make_fx(back)(torch.ones_like(y))
+
+
+def _without_memory(device):
+    """Tensors that have no memory of their own to read, and how a call meets them."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    x, w, b, r, g = _inputs(4, 16, 16, torch.float32, device)
+    t = torch.zeros(4, dtype=torch.int64, device=device)
+    mode = FakeTensorMode()
+
+    def faked(call):
+        def f():
+            with mode:
+                call(*(mode.from_tensor(v) for v in (x, w, t)))
+        return f
+
+    def in_the_mode(call):
+        def f():
+            with mode:
+                call(x, w, t)
+        return f
+
+    def zero(call):
+        return lambda: call(torch._efficientzerotensor((4, 16), device=device), w, t)
+
+    def mapped(call):
+        return lambda: torch.vmap(lambda a: call(a[None], w, t[:1]))(x)
+
+    def differentiated(call):
+        return lambda: torch.func.grad(lambda a: call(a, w, t).sum())(x)
+    return [k(call) for k in (faked, in_the_mode, zero, mapped, differentiated)
+            for call in (lambda a, c, i: cx.linear(a, c), lambda a, c, i: cx.linear(x, c, residual=a),
+                         lambda a, c, i: cx.linear_cross_entropy(a, c, i))]
+
+
+@pytest.mark.parametrize("which", range(15))
+def test_tensors_without_memory_are_refused(device, which):
+    with pytest.raises(ComprexError):
+        _without_memory(device)[which]()
+
+
+def test_backward_without_memory_is_refused(device):
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    x, w, _, _, _ = _inputs(4, 16, 16, torch.float32, device)
+    leaf = x.clone().requires_grad_()
+    t = torch.zeros(4, dtype=torch.int64, device=device)
+    for y in (cx.linear(leaf, w), cx.linear_cross_entropy(leaf, w, t, reduction="none")):
+        with pytest.raises(ComprexError), FakeTensorMode(allow_non_fake_inputs=True):
+            torch.autograd.grad(y, leaf, torch.ones(y.shape, device=device), retain_graph=True)
+        # no gradient at all, without memory for it
+        got, = torch.autograd.grad(y, leaf, torch._efficientzerotensor(tuple(y.shape), device=device))
+        assert not got.any()
