@@ -60,8 +60,8 @@ class AdamW(torch.optim.Optimizer):
         for p in self._params:
             if p.dtype != self._dtype or p.device != self._device:
                 raise ComprexError("all parameters must share one dtype and live on one device")
-            if p.layout != torch.strided or not _dense_layout(p) or p.is_neg():
-                raise ComprexError("a parameter has gaps in memory, or its sign only noted")
+            if p.layout != torch.strided or not _dense_layout(p):
+                raise ComprexError("a parameter has gaps in memory")
         self._lay_out()
 
     @staticmethod
@@ -76,6 +76,9 @@ class AdamW(torch.optim.Optimizer):
         super().add_param_group(param_group)
 
     def _lay_out(self) -> None:
+        self._layout = _lib.host().layout(self._params)
+        if self._layout is None:
+            raise ComprexError("a parameter has no memory of its own (a fake or wrapped tensor, a sign that is only noted)")
         dev = self._device
         numel = np.array([p.numel() for p in self._params], dtype=np.int64)
         blocks = -(-numel // _BLOCK)
@@ -116,7 +119,6 @@ class AdamW(torch.optim.Optimizer):
         self._now = {"seg_param": torch.zeros(k, dtype=torch.int64), "seg_grad": torch.zeros(k, dtype=torch.int64),
                      "seg_class": torch.zeros(k, dtype=torch.int32)}
         self._collect, self._scalar_type = _lib.host().collect, _lib.host().scalar_type(self._params[0])
-        self._layout = _lib.host().layout(self._params)
         self._ring = {}
         self._classes, self._same = None, False
         self._place()
@@ -170,12 +172,12 @@ class AdamW(torch.optim.Optimizer):
                     continue
                 if g.layout != torch.strided or g.size() != p.size() or g.device != p.device:
                     raise ComprexError("a gradient is sparse, on another device or does not have its parameter's shape")
-                if g.dtype is not self._dtype or g.stride() != p.stride() or g.is_neg():
+                if g.dtype is not self._dtype or g.stride() != p.stride() or g.is_neg() or g._is_zerotensor():
                     p.grad = torch.empty_strided(p.size(), p.stride(), dtype=self._dtype, device=p.device).copy_(g)
             changed = self._collect(self._params, self._scalar_type, 0, now.data_ptr())
             if changed == 2:
                 now.fill_(-1)
-                raise ComprexError("a gradient does not have its parameter's shape")
+                raise ComprexError("a gradient does not have its parameter's shape, or no memory of its own")
         if changed:
             self._upload("seg_grad")
         return bool(changed)

@@ -13,6 +13,7 @@
 // says what is wrong with it.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <vector>
@@ -32,9 +33,17 @@ bool same_layout(const at::Tensor& a, const at::Tensor& b) {
   return true;
 }
 
+// Whether the elements lie in memory as strides say.  (Fake tensors, wrapped ones, zeros that are not written down and signs that
+// are only noted do not.)
+bool plain(const at::Tensor& t) {
+  const c10::DispatchKeySet keys = t.key_set();
+  return t.layout() == at::kStrided && t.has_storage() && !t.is_neg() && !keys.has(c10::DispatchKey::Python) &&
+         !keys.has(c10::DispatchKey::ZeroTensor) && !keys.has(c10::DispatchKey::Functionalize);
+}
+
 // collect(params, scalar_type, zeros, out) -> 0: the table at address `out` (one int64 per parameter)
-// already held these addresses, 1: it has changed, 2: some gradient has another element type, device,
-// memory order or sign convention than its parameter (the table is incomplete).  `zeros` stands in for a missing one.
+// already held these addresses, 1: it has changed, 2: some gradient has another element type, device
+// or memory order than its parameter, or no plain memory (the table is incomplete).  `zeros` stands in for a missing one.
 PyObject* collect(PyObject*, PyObject* args) {
   PyObject* params;
   int scalar_type;
@@ -54,7 +63,7 @@ PyObject* collect(PyObject*, PyObject* args) {
       const at::Tensor& p = THPVariable_Unpack(o);
       const at::Tensor& g = p.grad();
       if (g.defined()) {
-        if (static_cast<int>(g.scalar_type()) != scalar_type || g.layout() != at::kStrided || g.device() != p.device() || g.is_neg() || !same_layout(g, p))
+        if (static_cast<int>(g.scalar_type()) != scalar_type || !plain(g) || g.device() != p.device() || !same_layout(g, p))
           return PyLong_FromLong(2);
         a = reinterpret_cast<int64_t>(g.data_ptr());
       }
@@ -80,7 +89,7 @@ void describe(const at::Tensor& t, std::vector<int64_t>& out) {
 }
 // the end of the description at `d` if it is that of `t`, else NULL; nothing is read from `end` on
 const int64_t* as_described(const at::Tensor& t, const int64_t* d, const int64_t* end) {
-  if (end - d < 4 || t.layout() != at::kStrided || t.is_neg() || d[0] != static_cast<int64_t>(t.scalar_type()) || d[1] != static_cast<int64_t>(t.device().type()) ||
+  if (end - d < 4 || !plain(t) || d[0] != static_cast<int64_t>(t.scalar_type()) || d[1] != static_cast<int64_t>(t.device().type()) ||
       d[2] != t.device().index() || d[3] != t.dim())
     return nullptr;
   d += 4;
@@ -91,7 +100,7 @@ const int64_t* as_described(const at::Tensor& t, const int64_t* d, const int64_t
   return d;
 }
 
-// layout(tensors) -> bytes for `addresses`
+// layout(tensors) -> bytes for `addresses`; None where one has no plain memory, or what is made now would not have any
 PyObject* layout(PyObject*, PyObject* tensors) {
   if (!PyList_Check(tensors)) {
     PyErr_SetString(PyExc_TypeError, "layout: a list of tensors");
@@ -99,12 +108,14 @@ PyObject* layout(PyObject*, PyObject* tensors) {
   }
   try {
     std::vector<int64_t> all;
+    if (c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::FAKE)) Py_RETURN_NONE;
     for (Py_ssize_t i = 0; i < PyList_GET_SIZE(tensors); ++i) {
       PyObject* o = PyList_GET_ITEM(tensors, i);
       if (!THPVariable_Check(o)) {
         PyErr_SetString(PyExc_TypeError, "layout: not a tensor");
         return nullptr;
       }
+      if (!plain(THPVariable_Unpack(o))) Py_RETURN_NONE;
       describe(THPVariable_Unpack(o), all);
     }
     return PyBytes_FromStringAndSize(reinterpret_cast<const char*>(all.data()), static_cast<Py_ssize_t>(all.size() * sizeof(int64_t)));

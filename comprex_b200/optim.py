@@ -176,12 +176,13 @@ class _FoldTable:
             self.now.fill_(-1)                    # incomplete, and not what the device holds, should this raise
             for p in self.params:
                 g = p.grad
-                if g is not None and (g.dtype is not self.dtype or g.stride() != p.stride() or g.is_neg()):
+                if g is not None and (g.dtype is not self.dtype or g.stride() != p.stride() or g.is_neg()
+                                      or g._is_zerotensor()):
                     p.grad = torch.empty_strided(p.size(), p.stride(), dtype=self.dtype, device=p.device).copy_(g)
             changed = self._collect(self.params, self.scalar_type, zeros.data_ptr(), self.now.data_ptr())
             if changed == 2:
                 self.now.fill_(-1)
-                raise ComprexError("a gradient does not have its parameter's shape")
+                raise ComprexError("a gradient does not have its parameter's shape, or no memory of its own")
         if not changed:
             return
         if not self.cuda:

@@ -527,3 +527,24 @@ def test_the_negative_bit(device):
     noted = torch._neg_view(torch.ones(300, device=device)).requires_grad_()
     with pytest.raises(ComprexError):
         cx.AdamW([noted])
+
+
+def test_tensors_without_memory_are_refused(device):
+    """Fake tensors have no memory to step, or to read a gradient from; a gradient of zeros that is not written down is one."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    real, mode = torch.nn.Parameter(torch.zeros(300, device=device)), FakeTensorMode()
+    with mode:
+        with pytest.raises(ComprexError):
+            cx.AdamW([torch.nn.Parameter(torch.zeros(300, device=device))])
+        with pytest.raises(ComprexError):
+            cx.AdamW([real])
+    opt = cx.AdamW([real], lr=0.1)
+    with mode:
+        real.grad = torch.ones(300, device=device)
+    with pytest.raises(ComprexError):
+        opt.step()
+    assert not real.detach().any()
+    real.grad = None
+    real.grad = torch._efficientzerotensor((300,), device=device)
+    opt.step()
+    assert not real.detach().any() and opt.state_dict()["comprex_adamw"]["steps"] == [1]
