@@ -260,10 +260,14 @@ class AdamW(torch.optim.Optimizer):
             for p, (a, n) in zip(self._params, self.spans()):
                 master[a:a + n].as_strided(p.size(), p.stride()).copy_(p)
 
+    def _shapes(self) -> list:
+        """Sizes and memory orders of the tensors (strides of dimensions of size 1 say nothing)."""
+        return [[list(p.size()), [s if n != 1 else 0 for n, s in zip(p.size(), p.stride())]] for p in self._params]
+
     # ---- checkpoint ------------------------------------------------------------------------------------------------
     def state_dict(self):
         sd = super().state_dict()
-        sd["comprex_adamw"] = {"version": 1, "bits": self.state_bits, "seed": self.seed, "numel": self._numel.tolist(),
+        sd["comprex_adamw"] = {"version": 1, "bits": self.state_bits, "seed": self.seed, "numel": self._numel.tolist(), "shapes": self._shapes(),
                                "steps": self._steps.tolist(), "turns": self._turns, "flat": {k: t.detach().cpu().clone() for k, t in self._flat.items()}}
         return sd
 
@@ -276,6 +280,8 @@ class AdamW(torch.optim.Optimizer):
         if mine["bits"] != self.state_bits or mine["numel"] != self._numel.tolist() or set(mine["flat"]) != set(self._flat):
             raise ComprexError("checkpoint was written for other parameters or another width of states")
         self._place()
+        if mine.get("shapes", self._shapes()) != self._shapes():
+            raise ComprexError("checkpoint was written for tensors of other shapes or in another memory order")
         super().load_state_dict(state_dict)
         for k, t in self._flat.items():
             t.copy_(mine["flat"][k])

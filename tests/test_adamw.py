@@ -548,3 +548,30 @@ def test_tensors_without_memory_are_refused(device):
     real.grad = torch._efficientzerotensor((300,), device=device)
     opt.step()
     assert not real.detach().any() and opt.state_dict()["comprex_adamw"]["steps"] == [1]
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_a_checkpoint_of_another_order_is_refused(device, bits):
+    """The flat states are in the tensors' memory order: read in another one they would belong to other elements."""
+    def make(order):
+        p = torch.nn.Parameter(torch.randn(4, 3, 2, 2, generator=torch.Generator().manual_seed(0)).to(device, torch.bfloat16))
+        p.data = order(p.data)
+        opt = cx.AdamW([p], lr=0.1, state_bits=bits)
+        p.grad = torch.ones_like(p)
+        opt.step()
+        return p, opt
+    orders = [lambda t: t, lambda t: t.contiguous(memory_format=torch.channels_last), lambda t: t.reshape(3, 4, 2, 2), lambda t: t.reshape(12, 4)]
+    for i, there in enumerate(orders):
+        p, opt = make(there)
+        before = p.detach().clone()
+        for j, here in enumerate(orders):
+            saved = make(here)[1].state_dict()
+            if i == j:
+                opt.load_state_dict(saved)
+                continue
+            with pytest.raises(ComprexError, match="order"):
+                opt.load_state_dict(saved)
+            assert torch.equal(p.detach(), before)
+        # a file that does not say: taken to be in the tensors' order, as it was
+        del saved["comprex_adamw"]["shapes"]
+        opt.load_state_dict(saved)
