@@ -15,7 +15,7 @@ Tensors of 16 bits have 32-bit weights behind them, which take the step; the ten
 parameter group has its own settings and every tensor its own step count: a tensor without a gradient is left alone.
 
 States live in flat buffers in which tensor ``i`` starts at a multiple of 256 elements, in the order of the
-parameters (:meth:`AdamW.flat_state`).  With ``state_bits=8`` each block of 256 elements keeps ``exp_avg`` and
+parameters (:meth:`AdamW.flat_state`).  A tensor that is frozen has none; with its first gradient the buffers are laid out anew.  With ``state_bits=8`` each block of 256 elements keeps ``exp_avg`` and
 ``exp_avg_rms``, the square root of the second moment, as ``float8_e4m3fn`` times a power of two: 2.03 bytes an
 element instead of 8.  They are rounded at random (up as often as what is cut off is part of a step), because a moving
 average with a beta near one would never leave its value under rounding to nearest; the random bits are a hash of the
@@ -48,21 +48,56 @@ class AdamW(torch.optim.Optimizer):
         self._check_settings(dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
         self.state_bits, self.seed = int(state_bits), int(seed)
-        self._params = [p for g in self.param_groups for p in g["params"] if p.requires_grad]
-        if not self._params:
+        chosen = [p for g in self.param_groups for p in g["params"] if p.requires_grad]
+        if not chosen:
             raise ValueError("optimizer got an empty parameter list")
-        self._group = np.array([i for i, g in enumerate(self.param_groups) for p in g["params"] if p.requires_grad])
-        first = self._params[0]
+        first = chosen[0]
         self._dtype, self._device = first.dtype, first.device
         self._code, self._dev = _lib.dtype_code(first.dtype), _lib.dev_code(first)
         if first.device.type not in ("cuda", "cpu"):
             raise ComprexError(f"parameters on {first.device} are not supported")
-        for p in self._params:
+        self._take(chosen)
+
+    def _take(self, chosen) -> None:
+        """Lay out the flat states for these tensors, in the order of the parameters; the others rest until they get a gradient."""
+        ids = {id(p) for p in chosen}
+        every = [(i, group, p) for i, (group, p) in enumerate((j, p) for j, g in enumerate(self.param_groups) for p in g["params"])]
+        mine = [e for e in every if id(e[2]) in ids]
+        for _, _, p in mine:
             if p.dtype != self._dtype or p.device != self._device:
                 raise ComprexError("all parameters must share one dtype and live on one device")
             if p.layout != torch.strided or not _dense_layout(p):
                 raise ComprexError("a parameter has gaps in memory")
-        self._lay_out()
+        kept = dict(self.__dict__)
+        try:
+            self._index, group, self._params = (list(x) for x in zip(*mine))
+            self._group, self._frozen = np.array(group), [p for _, _, p in every if id(p) not in ids]
+            self._lay_out()
+        except BaseException:
+            self.__dict__.clear()
+            self.__dict__.update(kept)
+            raise
+
+    @torch.no_grad()
+    def _take_too(self, more) -> None:
+        """Lay the flat states out anew with tensors that had none; what is there is copied into its new place."""
+        self._place()
+        kept = dict(self.__dict__)
+        try:
+            self._take(self._params + more)
+            at = {id(p): i for i, p in enumerate(self._params)}
+            for i, (p, first) in enumerate(zip(kept["_params"], kept["_first"])):
+                j = at[id(p)]
+                blocks, to = int(kept["_first"][i + 1] - first), int(self._first[j])
+                for name, old in kept["_flat"].items():
+                    per = 1 if name.endswith("_scale") else _BLOCK
+                    self._flat[name][to * per:(to + blocks) * per].copy_(old[int(first) * per:(int(first) + blocks) * per])
+                self._steps[j] = kept["_steps"][i]
+            self._turns = kept["_turns"]
+        except BaseException:
+            self.__dict__.clear()
+            self.__dict__.update(kept)
+            raise
 
     @staticmethod
     def _check_settings(group):
@@ -211,6 +246,10 @@ class AdamW(torch.optim.Optimizer):
         return loss
 
     def _step(self) -> None:
+        if self._frozen:
+            thawed = [p for p in self._frozen if p.grad is not None]
+            if thawed:
+                self._take_too(thawed)
         self._place()
         if self._grads() or self._classes is None:
             has = (self._now["seg_grad"] != 0).numpy()
@@ -260,15 +299,16 @@ class AdamW(torch.optim.Optimizer):
             for p, (a, n) in zip(self._params, self.spans()):
                 master[a:a + n].as_strided(p.size(), p.stride()).copy_(p)
 
-    def _shapes(self) -> list:
-        """Sizes and memory orders of the tensors (strides of dimensions of size 1 say nothing)."""
-        return [[list(p.size()), [s if n != 1 else 0 for n, s in zip(p.size(), p.stride())]] for p in self._params]
+    @staticmethod
+    def _shape(p) -> list:
+        """Size and memory order of a tensor (strides of dimensions of size 1 say nothing)."""
+        return [list(p.size()), [s if n != 1 else 0 for n, s in zip(p.size(), p.stride())]]
 
     # ---- checkpoint ------------------------------------------------------------------------------------------------
     def state_dict(self):
         sd = super().state_dict()
-        sd["comprex_adamw"] = {"version": 1, "bits": self.state_bits, "seed": self.seed, "numel": self._numel.tolist(), "shapes": self._shapes(),
-                               "steps": self._steps.tolist(), "turns": self._turns, "flat": {k: t.detach().cpu().clone() for k, t in self._flat.items()}}
+        sd["comprex_adamw"] = {"version": 1, "bits": self.state_bits, "seed": self.seed, "numel": self._numel.tolist(), "shapes": [self._shape(p) for p in self._params],
+                               "index": list(self._index), "steps": self._steps.tolist(), "turns": self._turns, "flat": {k: t.detach().cpu().clone() for k, t in self._flat.items()}}
         return sd
 
     @torch.no_grad()
@@ -277,12 +317,16 @@ class AdamW(torch.optim.Optimizer):
         mine = state_dict.pop("comprex_adamw", None)
         if mine is None:
             raise ComprexError("not a checkpoint of this optimizer")
-        if mine["bits"] != self.state_bits or mine["numel"] != self._numel.tolist() or set(mine["flat"]) != set(self._flat):
-            raise ComprexError("checkpoint was written for other parameters or another width of states")
         self._place()
-        if mine.get("shapes", self._shapes()) != self._shapes():
+        every, index = [p for g in self.param_groups for p in g["params"]], list(mine.get("index", self._index))
+        there = [every[i] for i in index if i < len(every)]
+        if mine["bits"] != self.state_bits or mine["numel"] != [p.numel() for p in there] or set(mine["flat"]) != set(self._flat):
+            raise ComprexError("checkpoint was written for other parameters or another width of states")
+        if "shapes" in mine and mine["shapes"] != [self._shape(p) for p in there]:
             raise ComprexError("checkpoint was written for tensors of other shapes or in another memory order")
         super().load_state_dict(state_dict)
+        if index != self._index:              # tensors were unfrozen there and not here, or the other way round
+            self._take(there)
         for k, t in self._flat.items():
             t.copy_(mine["flat"][k])
         self.seed = int(mine["seed"])

@@ -575,3 +575,71 @@ def test_a_checkpoint_of_another_order_is_refused(device, bits):
         # a file that does not say: taken to be in the tensors' order, as it was
         del saved["comprex_adamw"]["shapes"]
         opt.load_state_dict(saved)
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_tensor_unfrozen_later_steps(device, dtype, bits):
+    """Frozen when the optimizer is made, stepped from its first gradient on; the others go on as if nothing had happened."""
+    sizes = [300, 5, 700, 1000]
+    params = _params(dtype, device, sizes)
+    for i in (0, 2):
+        params[i].requires_grad_(False)
+    opt = cx.AdamW([{"params": params[:2], "lr": 0.02}, {"params": params[2:]}], state_bits=bits, **HYPER)
+    assert len(opt.spans()) == 2
+    held = opt.flat_state()
+    hyper = [HYPER | {"lr": 0.02}] * 2 + [HYPER] * 2
+    saved = None
+    for turn in range(6):
+        live = [i for i in range(4) if i in (1, 3) or (i == 2 and turn >= 2) or (i == 0 and turn >= 4)]
+        grads = [(torch.randn(n, generator=torch.Generator().manual_seed(10 * turn + i)) * 1e-2).to(dtype).to(device) for i, n in enumerate(sizes)]
+        for i, p in enumerate(params):
+            p.requires_grad_(i in live)
+            p.grad = grads[i].clone() if i in live else None
+        index = {id(p): j for j, p in enumerate(opt._params)}
+        names = ("exp_avg", "exp_avg_rms") if bits == 8 else ("exp_avg", "exp_avg_sq")
+        was = [_decoded(opt, n) if bits == 8 else [opt.flat_state()[n][a:a + k].double().cpu() for a, k in opt.spans()] for n in names]
+        weights = _weights(opt, opt._params)
+        want, count = {}, opt.state_dict()["comprex_adamw"]["steps"]
+        for i in live:
+            j = index.get(id(params[i]))
+            zero = torch.zeros(sizes[i], dtype=torch.float64)
+            w, m, v, t = (params[i].detach().double().cpu(), zero, zero, 0) if j is None else (weights[j], was[0][j], was[1][j], count[j])
+            want[i] = _formula(w, m, v * v if bits == 8 else v, grads[i].double().cpu(), t + 1, **hyper[i])[0]
+        frozen = {i: params[i].detach().clone() for i in range(4) if i not in live}
+        opt.step()
+        got = dict(zip((id(p) for p in opt._params), _weights(opt, opt._params)))
+        for i, w in want.items():
+            assert (got[id(params[i])] - w).abs().max() <= EPS32 * (2 * w.abs().max() + 10 * 0.02 * 8) + 1e-7, (turn, i)
+        assert all(torch.equal(params[i].detach(), w) for i, w in frozen.items())
+        assert len(opt.spans()) == (2 if turn < 2 else 3 if turn < 4 else 4)
+        assert (opt.flat_state()["exp_avg"] is held["exp_avg"]) == (turn < 2)
+        if turn == 2:
+            saved = opt.state_dict(), [p.detach().clone() for p in params]
+    assert opt.state_dict()["comprex_adamw"]["steps"] == [2, 6, 4, 6]
+    # a checkpoint says which tensors it has
+    fresh = [torch.nn.Parameter(w.clone(), requires_grad=i in (1, 3)) for i, w in enumerate(saved[1])]
+    other = cx.AdamW([{"params": fresh[:2]}, {"params": fresh[2:]}], state_bits=bits)
+    other.load_state_dict(saved[0])
+    assert len(other.spans()) == 3 and other.state_dict()["comprex_adamw"]["steps"] == [3, 1, 3]
+    opt.load_state_dict(saved[0])                 # and back, in the run that has gone on
+    for k, t in saved[0]["comprex_adamw"]["flat"].items():
+        assert torch.equal(t.view(torch.uint8), other.flat_state()[k].cpu().view(torch.uint8))
+        assert torch.equal(t.view(torch.uint8), opt.flat_state()[k].cpu().view(torch.uint8))
+
+
+def test_an_unfrozen_tensor_of_another_type_is_refused(device):
+    p = torch.nn.Parameter(torch.ones(30, device=device))
+    q = torch.nn.Parameter(torch.ones(30, device=device, dtype=torch.bfloat16), requires_grad=False)
+    opt = cx.AdamW([p, q], lr=0.1)
+    p.grad = torch.ones_like(p)
+    opt.step()
+    q.requires_grad_()
+    q.grad = torch.ones_like(q)
+    before = p.detach().clone()
+    with pytest.raises(ComprexError):
+        opt.step()
+    assert torch.equal(p.detach(), before) and len(opt.spans()) == 1
+    q.grad = None
+    opt.step()
+    assert opt.state_dict()["comprex_adamw"]["steps"] == [2]
