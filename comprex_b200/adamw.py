@@ -51,15 +51,15 @@ class AdamW(torch.optim.Optimizer):
         chosen = [p for g in self.param_groups for p in g["params"] if p.requires_grad]
         if not chosen:
             raise ValueError("optimizer got an empty parameter list")
+        self._take(chosen)
+
+    def _take(self, chosen) -> None:
+        """Lay out the flat states for these tensors, in the order of the parameters; the others rest until they get a gradient."""
         first = chosen[0]
         self._dtype, self._device = first.dtype, first.device
         self._code, self._dev = _lib.dtype_code(first.dtype), _lib.dev_code(first)
         if first.device.type not in ("cuda", "cpu"):
             raise ComprexError(f"parameters on {first.device} are not supported")
-        self._take(chosen)
-
-    def _take(self, chosen) -> None:
-        """Lay out the flat states for these tensors, in the order of the parameters; the others rest until they get a gradient."""
         ids = {id(p) for p in chosen}
         every = [(i, group, p) for i, (group, p) in enumerate((j, p) for j, g in enumerate(self.param_groups) for p in g["params"])]
         mine = [e for e in every if id(e[2]) in ids]
@@ -303,6 +303,30 @@ class AdamW(torch.optim.Optimizer):
     def _shape(p) -> list:
         """Size and memory order of a tensor (strides of dimensions of size 1 say nothing)."""
         return [list(p.size()), [s if n != 1 else 0 for n, s in zip(p.size(), p.stride())]]
+
+    # ---- copies: the tables and buffers are made anew, with what is in them --------------------------------------------
+    def __getstate__(self):
+        return super().__getstate__() | {"comprex_adamw": {
+            "bits": self.state_bits, "seed": self.seed, "index": self._index, "shapes": [self._shape(p) for p in self._params],
+            "steps": self._steps, "turns": self._turns,
+            "flat": {k: t.view(torch.uint8) if t.itemsize == 1 else t for k, t in self._flat.items()}}}     # (pickle knows no e4m3)
+
+    def __setstate__(self, state):
+        state = dict(state)
+        mine = state.pop("comprex_adamw", None)
+        super().__setstate__(state)
+        if mine is None:                      # (of load_state_dict: settings alone)
+            return
+        self.state_bits, self.seed = mine["bits"], mine["seed"]
+        every = [p for g in self.param_groups for p in g["params"]]
+        self._take([every[i] for i in mine["index"]])
+        if mine["shapes"] != [self._shape(p) for p in self._params]:
+            raise ComprexError("the copied tensors have other shapes or another memory order")
+        with torch.no_grad():
+            for k, t in self._flat.items():
+                t.view(mine["flat"][k].dtype).copy_(mine["flat"][k])
+        self._steps[:] = mine["steps"]
+        self._turns = mine["turns"]
 
     # ---- checkpoint ------------------------------------------------------------------------------------------------
     def state_dict(self):

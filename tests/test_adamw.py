@@ -643,3 +643,43 @@ def test_an_unfrozen_tensor_of_another_type_is_refused(device):
     q.grad = None
     opt.step()
     assert opt.state_dict()["comprex_adamw"]["steps"] == [2]
+
+
+@pytest.mark.parametrize("how", ["deepcopy", "pickle", "torch.save"])
+@pytest.mark.parametrize("bits", [8, 32])
+def test_copies_step_on(device, bits, how):
+    """A copy, with the model or alone, goes on as the optimizer itself does, and neither disturbs the other."""
+    import copy
+    import io
+    import pickle
+    params = torch.nn.ParameterList(_params(torch.bfloat16, device, [300, 5, 700]))
+    params.append(torch.nn.Parameter(torch.randn(4, 3, 2, 2).to(device, torch.bfloat16).contiguous(memory_format=torch.channels_last)))
+    params[1].requires_grad_(False)
+    opt = cx.AdamW(params, state_bits=bits, seed=4, **HYPER)
+
+    def run(o, ps, turns):
+        for t in turns:
+            gen = torch.Generator().manual_seed(t)
+            for i, p in enumerate(ps):
+                g = (torch.randn(p.size(), generator=gen) * 1e-2).to(p.dtype).to(device)
+                p.grad = None if i == 1 and t < 4 else torch.empty_like(p, requires_grad=False).copy_(g)
+            o.step()
+    run(opt, params, range(3))
+    if how == "deepcopy":
+        twins, other = copy.deepcopy((params, opt))
+    elif how == "pickle":
+        twins, other = pickle.loads(pickle.dumps((params, opt)))
+    else:
+        file = io.BytesIO()
+        torch.save((params, opt), file)
+        file.seek(0)
+        twins, other = torch.load(file, weights_only=False)
+    assert all(p is q for p, q in zip(other._params, [twins[0], twins[2], twins[3]]))
+    before = [p.detach().clone() for p in params]
+    run(other, twins, range(3, 6))
+    assert all(torch.equal(p, q) for p, q in zip(params, before))
+    run(opt, params, range(3, 6))
+    assert all(torch.equal(p, q) for p, q in zip(params, twins))
+    assert other.state_dict()["comprex_adamw"]["steps"] == [6, 2, 6, 6]
+    for k, t in opt.flat_state().items():
+        assert torch.equal(t.view(torch.uint8), other.flat_state()[k].view(torch.uint8)), k
