@@ -12,7 +12,7 @@
 // limit, forward and backward 2.7 ms (1.23 PFLOP/s with the logits counted twice).
 //
 // P in 16 bits: a probability of a large vocabulary times the 1 / rows of a mean is below what fp16 can hold, so P is
-// stored times a power of two that brings the largest |g_r| to [2^13, 2^14), and both products take it out at the end.
+// stored times a power of two that brings the largest finite |g_r| to [2^13, 2^14), and both products take it out at the end.
 #include "cx_product.cuh"
 
 namespace {
@@ -139,7 +139,10 @@ __global__ void __launch_bounds__(1024) factor_kernel(const __grid_constant__ Fa
     if (threadIdx.x == 0) s_top = 0;
     __syncthreads();
 #pragma unroll 4
-    for (int64_t r = threadIdx.x; r < f.rows; r += 1024) top = max(top, __float_as_uint(row_grad(f, r)) & 0x7FFFFFFFu);
+    for (int64_t r = threadIdx.x; r < f.rows; r += 1024) {
+      const uint32_t bits = __float_as_uint(row_grad(f, r)) & 0x7FFFFFFFu;
+      top = max(top, bits < 0x7F800000u ? bits : 0u);      // a gradient that is infinite or no number is its row's own matter
+    }
     top = __reduce_max_sync(0xFFFFFFFFu, top);
     if ((threadIdx.x & 31) == 0) atomicMax(&s_top, top);
     __syncthreads();

@@ -236,3 +236,19 @@ def test_forward_mode_is_refused(device):
         up = torch.autograd.forward_ad.make_dual(g, torch.ones_like(g))
         with pytest.raises(ComprexError, match="forward-mode"):
             torch.autograd.grad(cx.linear_cross_entropy(leaf, w, t, reduction="none"), leaf, up)
+
+
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_a_bad_gradient_stays_with_its_row(device, dtype, bad):
+    """A row whose upstream gradient is no number does not change what the other rows are scaled by."""
+    h, w, t, g = _inputs(40, 200, 32, dtype, device, ignored=0.0)
+    h.requires_grad_()
+    got = []
+    for value in (0.0, bad):
+        up = g.clone()
+        up[7] = value
+        got.append(torch.autograd.grad(cx.linear_cross_entropy(h, w, t, reduction="none"), (h,), up)[0])
+    keep = torch.arange(40, device=device) != 7
+    assert got[0][keep].abs().amin(1).min() > 0 and torch.equal(got[0][keep], got[1][keep])
+    assert not got[0][7].any() and not torch.isfinite(got[1][7]).any()
