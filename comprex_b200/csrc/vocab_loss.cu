@@ -13,6 +13,9 @@
 //
 // P in 16 bits: a probability of a large vocabulary times the 1 / rows of a mean is below what fp16 can hold, so P is
 // stored times a power of two that brings the largest finite |g_r| to [2^13, 2^14), and both products take it out at the end.
+// One power for all rows, since dw adds rows up.  What it costs in fp16 where rows are weighted far apart: dh of a row at 2^-16 /
+// 2^-20 / 2^-24 / 2^-28 of the largest g is 2.6e-4 / 5.4e-4 / 6e-3 / 4e-2 of itself off (2.4e-4 at the largest, of which its own
+// rounding is 2.0e-4; 50257 words).  Such rows count for less in dw than its rounding, and 2^-30 is the whole range of fp16.
 #include "cx_product.cuh"
 
 namespace {

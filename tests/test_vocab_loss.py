@@ -252,3 +252,22 @@ def test_a_bad_gradient_stays_with_its_row(device, dtype, bad):
     keep = torch.arange(40, device=device) != 7
     assert got[0][keep].abs().amin(1).min() > 0 and torch.equal(got[0][keep], got[1][keep])
     assert not got[0][7].any() and not torch.isfinite(got[1][7]).any()
+
+
+@pytest.mark.parametrize("far", [8, 20, 30])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_gradients_far_apart(device, dtype, far):
+    """Rows whose upstream gradients are up to 2^-30 of the largest.  In fp16 the probabilities share one power of two, so a small row's
+    are off by up to 2^-25 of 2^-12 of the largest gradient each, as the elementwise bounds say; in the row's own measure that is nothing
+    down to 2^-16 (there within three roundings of the result)."""
+    h, w, t, g = _inputs(90, 700, 48, dtype, device, ignored=0.0)
+    g = torch.exp2(-torch.arange(90, device=device) * (far / 89.0)) * (2.0 ** 12 if dtype == torch.float16 else 1.0)
+    h.requires_grad_(), w.requires_grad_()
+    loss = cx.linear_cross_entropy(h, w, t, reduction="none")
+    dh, dw = torch.autograd.grad(loss, (h, w), g)
+    _check(h.detach(), w.detach(), t, g, "none", loss, dh, dw)
+    p = torch.softmax(h.detach().double() @ w.detach().double().T, 1)
+    p[torch.arange(90), t] -= 1
+    want = (p * g.double()[:, None]) @ w.detach().double()
+    near = g >= 2.0 ** -16 * g[0]
+    assert ((dh.double() - want).norm(dim=1) <= (3 * UNIT[dtype] + 2.0 ** -18) * want.norm(dim=1))[near].all()
