@@ -103,14 +103,29 @@ __device__ __forceinline__ float inverse(float x) {
   return y;
 }
 
-// Activations in terms of u = x w^T + b.  gelu_tanh(u) = u / (1 + exp(-2 z)), z = sqrt(2 / pi) (u + 0.044715 u^3): the
-// same function as u / 2 (1 + tanh z), with one exponential.  Power of two and reciprocal are the hardware's (about 2
-// units of 2^-23): three bits below what the result is rounded to in 16 bits, and inside the sums' own error in 32.
+// Activations in terms of u = x w^T + b.  gelu_tanh(u) = u sigmoid(2 z), z = sqrt(2 / pi) (u + 0.044715 u^3): the same
+// function as u / 2 (1 + tanh z), with one exponential and without the sum's cancellation.
+//
+// For results of 16 bits power of two and reciprocal are the hardware's: each is about 2 units of 2^-23 off, the argument's
+// rounding 1.44 |2 z| more of 2^-24 (z = -40: 5e-6 of the result, which is rounded to 2^-9 or 2^-12 of itself), and a gate below
+// 2^-126 is 0.  Results of 32 bits take expf of an argument that is rounded once, and a true quotient.
 constexpr float kGelu = 1.5957691216057308f;       // 2 sqrt(2 / pi)
-__device__ __forceinline__ float sigmoid(float z) { return inverse(1.f + pow2(-kLog2e * z)); }
-__device__ __forceinline__ float gelu_gate(float u) { return inverse(1.f + pow2(u * __fmaf_rn(u * u, -0.044715f * kGelu * kLog2e, -kGelu * kLog2e))); }
-template <int N>
+__device__ __forceinline__ float sigmoid_full(float z) {
+  const float t = expf(-fabsf(z));
+  return (z >= 0.f ? 1.f : t) / (1.f + t);
+}
+template <bool FULL>
+__device__ __forceinline__ float sigmoid(float z) {
+  return FULL ? sigmoid_full(z) : inverse(1.f + pow2(-kLog2e * z));
+}
+template <bool FULL>
+__device__ __forceinline__ float gelu_gate(float u) {
+  return FULL ? sigmoid_full(u * __fmaf_rn(u * u, 0.044715f * kGelu, kGelu)) : inverse(1.f + pow2(u * __fmaf_rn(u * u, -0.044715f * kGelu * kLog2e, -kGelu * kLog2e)));
+}
+// T: of the results
+template <typename T, int N>
 __device__ __forceinline__ void activate(float (&v)[N], int act) {
+  constexpr bool full = sizeof(T) == 4;
   if (act == CX_ACT_RELU) {
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = v[i] > 0.f || v[i] != v[i] ? v[i] : 0.f;
@@ -119,22 +134,26 @@ __device__ __forceinline__ void activate(float (&v)[N], int act) {
     for (int i = 0; i < N; ++i) v[i] = 0.5f * v[i] * (1.f + erff(v[i] * 0.70710678118654752f));
   } else if (act == CX_ACT_GELU_TANH) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] *= gelu_gate(v[i]);
+    for (int i = 0; i < N; ++i) v[i] *= gelu_gate<full>(v[i]);
   } else if (act == CX_ACT_SILU) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] *= sigmoid(v[i]);
+    for (int i = 0; i < N; ++i) v[i] *= sigmoid<full>(v[i]);
   }
 }
-template <int ACT>
+template <typename T, int ACT>
 __device__ __forceinline__ float slope(float u) {
+  constexpr bool full = sizeof(T) == 4;
   if (ACT == CX_ACT_RELU) return u > 0.f ? 1.f : 0.f;
-  if (ACT == CX_ACT_GELU) return 0.5f * (1.f + erff(u * 0.70710678118654752f)) + u * 0.39894228040143268f * pow2(-0.5f * kLog2e * u * u);
+  if (ACT == CX_ACT_GELU) {
+    const float bell = full ? expf(-0.5f * u * u) : pow2(-0.5f * kLog2e * u * u);
+    return 0.5f * (1.f + erff(u * 0.70710678118654752f)) + u * 0.39894228040143268f * bell;
+  }
   if (ACT == CX_ACT_GELU_TANH) {
-    const float q = gelu_gate(u);
+    const float q = gelu_gate<full>(u);
     return q + u * q * (1.f - q) * kGelu * __fmaf_rn(u * u, 0.134145f, 1.f);
   }
   if (ACT == CX_ACT_SILU) {
-    const float q = sigmoid(u);
+    const float q = sigmoid<full>(u);
     return q * __fmaf_rn(u, 1.f - q, 1.f);
   }
   return 1.f;

@@ -82,7 +82,7 @@ __global__ void __launch_bounds__(kThreads) du_kernel(const __grid_constant__ Du
       if (act) u[j].get(y);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        if (act) x[i] *= cxprod::slope<ACT>(y[i]);
+        if (act) x[i] *= cxprod::slope<T, ACT>(y[i]);
         sum[i] += x[i];                                   // (zero from `left` on)
       }
       if (d.du) cxprod::store8(reinterpret_cast<T*>(d.du) + r * d.ldd + c, left == 8 && d.wide_out, left, x);
@@ -242,7 +242,7 @@ __global__ void __launch_bounds__(kThreads) few_rows_kernel(const __grid_constan
     using E = cx::Elem<T>;
     if (d.bias) v[0] += E::to_f(reinterpret_cast<const T*>(d.bias)[c]);
     if (d.pre) reinterpret_cast<T*>(d.pre)[r * d.ldpre + c] = E::from_f(v[0]);
-    cxprod::activate(v, d.act);
+    cxprod::activate<T>(v, d.act);
     if (d.residual) v[0] += E::to_f(reinterpret_cast<const T*>(d.residual)[r * d.ldr + c]);
     reinterpret_cast<T*>(d.y)[r * d.outer + c] = E::from_f(v[0]);
   }

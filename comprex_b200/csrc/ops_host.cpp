@@ -106,8 +106,12 @@ int cx_adamw_step_host(const CxAdamW* a) {
 // ---- linear -----------------------------------------------------------------------------------------------------
 namespace {
 
+float sigmoid_host(float z) {
+  const float t = expf(-fabsf(z));
+  return (z >= 0.f ? 1.f : t) / (1.f + t);
+}
 float act_host(float u, int act, float* slope) {
-  const float k = 0.79788456080286536f;
+  const float k = 1.5957691216057308f;      // 2 sqrt(2 / pi)
   switch (act) {
     case CX_ACT_RELU:
       *slope = u > 0.f ? 1.f : 0.f;
@@ -118,12 +122,12 @@ float act_host(float u, int act, float* slope) {
       return u * cdf;
     }
     case CX_ACT_GELU_TANH: {
-      const float t = tanhf(k * (u + 0.044715f * u * u * u));
-      *slope = 0.5f * (1.f + t) + 0.5f * u * (1.f - t * t) * k * (1.f + 0.134145f * u * u);
-      return 0.5f * u * (1.f + t);
+      const float q = sigmoid_host(u * (0.044715f * k * (u * u) + k));
+      *slope = q + u * q * (1.f - q) * k * (0.134145f * (u * u) + 1.f);
+      return u * q;
     }
     case CX_ACT_SILU: {
-      const float q = 1.f / (1.f + expf(-u));
+      const float q = sigmoid_host(u);
       *slope = q * (1.f + u * (1.f - q));
       return u * q;
     }

@@ -23,7 +23,7 @@ __device__ __forceinline__ void finish(const CxProduct& p, int64_t row, int64_t 
   if (p.bias) v += reinterpret_cast<const float*>(p.bias)[col];
   if (p.pre) reinterpret_cast<float*>(p.pre)[row * p.ldpre + col] = v;
   float one[1] = {v};
-  cxprod::activate(one, p.act);
+  cxprod::activate<float>(one, p.act);
   v = one[0];
   if (p.residual) v += reinterpret_cast<const float*>(p.residual)[row * p.ldr + col];
   reinterpret_cast<float*>(p.out)[row * p.ldo + col] = v;

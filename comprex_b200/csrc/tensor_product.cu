@@ -326,7 +326,7 @@ __device__ __forceinline__ void finish_linear(const Job& t, int64_t row, int64_t
       v[4 * i + 3] = __fmaf_rn(v[4 * i + 3], to.scale, b.w);
     }
     if (to.pre && in) store_row(to.pre + c, to.wide_pre, have, v);
-    cxprod::activate(v, to.act);
+    cxprod::activate<T>(v, to.act);
     if (ahead) {
 #pragma unroll
       for (int i = 0; i < 32; ++i) v[i] += cx::Elem<T>::to_f(reinterpret_cast<const T*>(next)[i]);
@@ -534,7 +534,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_splits_kernel(const __grid_
   for (int k = 0; k < 8; ++k) v[k] *= to.scale;
   if (to.bias) add_row(to.bias, to.wide_bias, to.left, v);
   if (to.pre) store_row(to.pre, to.wide_pre, to.left, v);
-  cxprod::activate(v, to.act);
+  cxprod::activate<T>(v, to.act);
   if (to.residual) add_row(to.residual, to.wide_res, to.left, v);
   store_row(to.out, to.wide_out, to.left, v);
 }

@@ -278,3 +278,33 @@ def test_backward_without_memory_is_refused(device):
         # no gradient at all, without memory for it
         got, = torch.autograd.grad(y, leaf, torch._efficientzerotensor(tuple(y.shape), device=device))
         assert not got.any()
+
+
+@pytest.mark.parametrize("rows", [1, 300])
+def test_activations_in_32_bits_to_their_ends(device, rows):
+    """float32 values and slopes relative to themselves, down to where they leave the normal numbers: an exponential of an exact
+    argument is good to a few units of 2^-24, one of a rounded argument y to |y| more of them."""
+    f = torch.nn.functional
+    u = torch.cat((torch.linspace(-100, 100, 4001), torch.linspace(-6, 6, 999), torch.tensor([-1e-30, 0.0, 1e-30, -1e30, 1e30])))
+    u = u.double().float()
+    u64 = u.double().requires_grad_()
+    x = torch.ones(rows, 1, device=device).requires_grad_()
+    w = u[:, None].to(device)
+    z2 = 2 * 0.7978845608028654 * (u64.detach() + 0.044715 * u64.detach() ** 3)
+    for act, value, off in (("silu", u64 * torch.sigmoid(u64), 8.0),
+                            # u (1 + tanh z) / 2 = u sigmoid(2 z), without the sum's cancellation; the argument has six roundings
+                            ("gelu_tanh", u64 * torch.sigmoid(2 * 0.7978845608028654 * (u64 + 0.044715 * u64 ** 3)), 8.0 + 6 * z2.abs())):
+        slope, = torch.autograd.grad(value.sum(), u64, retain_graph=True)
+        y = cx.linear(x, w, activation=act)
+        # one output of one row at a time: dx is its slope times u, so take the bias's gradient
+        b = torch.zeros(u.numel(), device=device).requires_grad_()
+        db, = torch.autograd.grad(cx.linear(x[:1].detach(), w, b, activation=act), b, torch.ones(1, u.numel(), device=device))
+        value = value.detach()
+        off = torch.as_tensor(off) * 2.0 ** -24
+        assert ((y.detach().double().cpu() - value).abs() <= off * value.abs() + 1e-36).all(), act
+        # the slope is a sum of two terms that cancel: relative to both
+        gate = torch.sigmoid(u64.detach() if act == "silu" else z2)
+        inner = u64.detach() if act == "silu" else z2 + 2 * 2 * 0.7978845608028654 * 0.044715 * u64.detach() ** 3
+        terms = gate + (inner * gate * (1 - gate)).abs()
+        finite = u64.detach().abs() < 1e18            # (beyond, the cube leaves 32 bits, here as anywhere)
+        assert ((db.double().cpu() - slope).abs() <= 3 * off * terms + 1e-36)[finite].all(), act
