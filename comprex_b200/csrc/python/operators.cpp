@@ -6,6 +6,7 @@
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 #include <ATen/ATen.h>
+#include <ATen/autocast_mode.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/core/impl/VirtualGuardImpl.h>
@@ -335,6 +336,26 @@ const Tensor& same_type(const Tensor& t, const char* name, const Tensor& like) {
   return t;
 }
 
+// The type that torch's own product would be in here: autocast's, where that is on and `x` is cast; else the tensor's.
+at::ScalarType product_type(const Tensor& x) {
+  const auto device = x.device().type();
+  const bool cast = at::autocast::is_autocast_enabled(device) && x.is_floating_point() && x.scalar_type() != at::kDouble;
+  return cast ? at::autocast::get_autocast_dtype(device) : x.scalar_type();
+}
+// ... and an operand in it, by autocast's rules and through its cache of weights
+Tensor in_type(const Tensor& t, at::ScalarType type) {
+  return at::autocast::is_autocast_enabled(t.device().type()) ? at::autocast::cached_cast(type, t, t.device().type()) : t;
+}
+
+void out_of_memory(const c10::OutOfMemoryError& e) {
+  PyObject* torch = PyImport_ImportModule("torch");
+  PyObject* kind = torch ? PyObject_GetAttrString(torch, "OutOfMemoryError") : nullptr;
+  PyErr_Clear();
+  PyErr_SetString(kind ? kind : PyExc_MemoryError, e.what_without_backtrace());
+  Py_XDECREF(kind);
+  Py_XDECREF(torch);
+}
+
 template <typename F>
 PyObject* guarded(const F& f) {
   try {
@@ -352,12 +373,7 @@ PyObject* guarded(const F& f) {
   } catch (python_error& e) {
     e.restore();
   } catch (const c10::OutOfMemoryError& e) {
-    PyObject* torch = PyImport_ImportModule("torch");
-    PyObject* kind = torch ? PyObject_GetAttrString(torch, "OutOfMemoryError") : nullptr;
-    PyErr_Clear();
-    PyErr_SetString(kind ? kind : PyExc_MemoryError, e.what_without_backtrace());
-    Py_XDECREF(kind);
-    Py_XDECREF(torch);
+    out_of_memory(e);
   } catch (const std::exception& e) {
     PyErr_SetString(PyExc_RuntimeError, e.what());
   }
@@ -376,12 +392,19 @@ PyObject* cx_py_linear(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   if (PyErr_Occurred()) return nullptr;
   Tensor x, w;
   Maybe bias, residual;
+  bool apart = false;          // the residual is added to the result, in the type that torch adds the two in
   try {
-    x = tensor(a[0], "x", nullptr);
+    const Tensor& given = tensor(a[0], "x", nullptr);
+    const at::ScalarType type = product_type(given);
+    x = in_type(given, type);
     code_of(x);
-    w = same_type(tensor(a[1], "weight", &x), "weight", x);
-    if (a[2] != Py_None) bias = same_type(tensor(a[2], "bias", &x), "bias", x);
-    if (a[4] != Py_None) residual = same_type(tensor(a[4], "residual", &x), "residual", x);
+    w = same_type(in_type(tensor(a[1], "weight", &x), type), "weight", x);
+    if (a[2] != Py_None) bias = same_type(in_type(tensor(a[2], "bias", &x), type), "bias", x);
+    if (a[4] != Py_None) {
+      residual = tensor(a[4], "residual", &x);
+      if (at::autocast::is_autocast_enabled(x.device().type()) && residual->scalar_type() != type) apart = true;       // (autocast leaves sums as they are)
+      else residual = same_type(*residual, "residual", x);
+    }
     if (w.dim() != 2 || x.dim() < 1 || x.size(-1) != w.size(1) || !w.numel()) refuse("x ", shape_of(x), " does not fit weight ", shape_of(w));
     if (bias && (bias->dim() != 1 || bias->size(0) != w.size(0))) refuse("bias ", shape_of(*bias), " does not fit weight ", shape_of(w));
     if (residual) {
@@ -392,13 +415,24 @@ PyObject* cx_py_linear(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   } catch (const Refused& r) {
     PyErr_SetString(native.error, r.why.c_str());
     return nullptr;
+  } catch (const c10::OutOfMemoryError& e) {
+    out_of_memory(e);
+    return nullptr;
   } catch (const std::exception& e) {
     PyErr_SetString(native.error, e.what());
     return nullptr;
   }
+  Tensor more;
+  if (apart) {
+    more = *residual;
+    residual.reset();
+  }
   const bool train = at::GradMode::is_enabled() &&
                      (x.requires_grad() || w.requires_grad() || (bias && bias->requires_grad()) || (residual && residual->requires_grad()));
-  return guarded([&] { return train ? LinearFn::apply(x, w, bias, (int64_t)act, residual) : linear_forward(x, w, bias, (int)act, residual, nullptr); });
+  return guarded([&] {
+    const Tensor y = train ? LinearFn::apply(x, w, bias, (int64_t)act, residual) : linear_forward(x, w, bias, (int)act, residual, nullptr);
+    return apart ? y + more : y;
+  });
 }
 
 // vocab_loss(hidden, weight, targets, ignore_index, reduction); reduction: CX_REDUCE_*
@@ -412,15 +446,20 @@ PyObject* cx_py_vocab_loss(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   if (PyErr_Occurred()) return nullptr;
   Tensor h, w, targets;
   try {
-    h = tensor(a[0], "hidden", nullptr);
+    const Tensor& given = tensor(a[0], "hidden", nullptr);
+    const at::ScalarType type = product_type(given);
+    h = in_type(given, type);
     code_of(h);
-    w = same_type(tensor(a[1], "weight", &h), "weight", h);
+    w = same_type(in_type(tensor(a[1], "weight", &h), type), "weight", h);
     targets = tensor(a[2], "targets", &h);
     if (targets.scalar_type() != at::kLong) refuse("targets must be int64, not ", targets.scalar_type());
     if (w.dim() != 2 || !w.numel() || h.dim() < 1 || h.size(-1) != w.size(1)) refuse("hidden ", shape_of(h), " does not fit weight ", shape_of(w));
     if (targets.sizes() != h.sizes().slice(0, h.dim() - 1)) refuse("targets ", shape_of(targets), " do not fit hidden ", shape_of(h));
   } catch (const Refused& r) {
     PyErr_SetString(native.error, r.why.c_str());
+    return nullptr;
+  } catch (const c10::OutOfMemoryError& e) {
+    out_of_memory(e);
     return nullptr;
   } catch (const std::exception& e) {
     PyErr_SetString(native.error, e.what());

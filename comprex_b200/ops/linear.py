@@ -16,8 +16,10 @@ def linear(x, weight, bias=None, *, activation=None, residual=None):
     ``x`` [..., inner], ``weight`` [outer, inner], ``bias`` [outer], ``residual`` [..., outer]: float32, bfloat16 or
     float16, all of one type and on one device (CUDA, or the host).  Rows may lie apart in memory; other orders are
     copied.  ``activation``: None, ``"relu"``, ``"gelu"``, ``"gelu_tanh"`` or ``"silu"``.  Gradients reach ``x``,
-    ``weight``, ``bias`` and ``residual``, once: they cannot be differentiated again.  Products of 16-bit operands run on the
-    tensor cores, of float32 on the CUDA cores; the host's are plain loops, for ranks without a GPU and for tests."""
+    ``weight``, ``bias`` and ``residual``, once: they cannot be differentiated again.  Under ``torch.autocast`` the operands
+    are cast as torch's own product casts them, and a residual of another type is added to the result.  Products of 16-bit
+    operands run on the tensor cores, of float32 on the CUDA cores; the host's are plain loops, for ranks without a GPU and for
+    tests."""
     try:
         act = _lib.ACTIVATIONS[activation]
     except (KeyError, TypeError):

@@ -19,7 +19,7 @@ def linear_cross_entropy(hidden, weight, targets, *, ignore_index=-100, reductio
     ``hidden`` [..., dim] and ``weight`` [vocab, dim]: float32, bfloat16 or float16, of one type and on one device;
     ``targets`` [...]: int64.  Rows whose target is ``ignore_index`` have loss 0 and no gradient; the mean is over the
     others, and NaN (with zero gradients) where there are none.  A target outside the vocabulary makes its row's loss
-    and gradients NaN.  The loss is float32: a scalar, or with ``reduction="none"`` of the shape of ``targets``."""
+    and gradients NaN.  Under ``torch.autocast`` the product is in autocast's type.  The loss is float32: a scalar, or with ``reduction="none"`` of the shape of ``targets``."""
     try:
         code = _lib.REDUCTIONS[reduction]
     except (KeyError, TypeError):

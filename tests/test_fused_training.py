@@ -150,3 +150,21 @@ def test_operands_of_another_stream():
         got = torch.autograd.grad(cx.linear_cross_entropy(a, b, t), (a, b))
     torch.cuda.current_stream().wait_stream(side)
     assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
+def test_gpt2_under_autocast(device):
+    """The model with and without the operators, weights in 32 bits: the same types, and the same numbers but for bf16 roundings."""
+    plain, fused = _models(device)
+    idx = torch.randint(0, 257, (2, 33), generator=torch.Generator().manual_seed(1)).to(device)
+    losses, logits = [], []
+    for m in (plain, fused):
+        with torch.autocast(device, dtype=torch.bfloat16):
+            losses.append(m(idx[:, :-1], idx[:, 1:].contiguous()))
+            logits.append(m(idx))
+        losses[-1].backward()
+    assert losses[0].dtype == losses[1].dtype and logits[0].dtype == logits[1].dtype
+    # logits of a tiny model near zero: rounded to 2^-9 of themselves in both, and so are the activations before them
+    assert abs(losses[0].item() - losses[1].item()) <= 2.0 ** -8 * losses[0].item()
+    assert (logits[0] - logits[1]).norm() <= 2.0 ** -5 * logits[0].norm()
+    for (name, p), q in zip(plain.named_parameters(), fused.parameters()):
+        assert q.grad.dtype == torch.float32 and (p.grad - q.grad).norm() <= 2.0 ** -4 * p.grad.norm() + 1e-6, name

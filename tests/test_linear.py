@@ -308,3 +308,25 @@ def test_activations_in_32_bits_to_their_ends(device, rows):
         terms = gate + (inner * gate * (1 - gate)).abs()
         finite = u64.detach().abs() < 1e18            # (beyond, the cube leaves 32 bits, here as anywhere)
         assert ((db.double().cpu() - slope).abs() <= 3 * off * terms + 1e-36)[finite].all(), act
+
+
+@pytest.mark.parametrize("low", [torch.bfloat16, torch.float16])
+def test_autocast(device, low):
+    """Products are in autocast's type, as torch's; what is added to them keeps its own."""
+    x, w, b, r, _ = _inputs(20, 32, 24, torch.float32, device)
+    leaves = [t.clone().requires_grad_() for t in (x, w, b, r)]
+    cast = [t.clone().to(low).requires_grad_() for t in (x, w, b)]
+    with torch.autocast(device, dtype=low):
+        y = cx.linear(*leaves[:3], activation="silu", residual=leaves[3])
+        z = cx.linear(*leaves[:3], activation="silu", residual=leaves[3].to(low))
+        assert cx.linear(x, w).dtype == torch.nn.functional.linear(x, w).dtype == low
+    assert y.dtype == torch.float32 and z.dtype == low
+    inner = cx.linear(*cast, activation="silu")
+    assert torch.equal(y, inner + r) and torch.equal(z, cx.linear(*cast, activation="silu", residual=r.to(low)))
+    g = torch.randn(20, 24, generator=torch.Generator().manual_seed(2)).to(device)
+    got, want = torch.autograd.grad(y, leaves, g), torch.autograd.grad(inner, cast, g.to(low))
+    assert all(p.dtype == torch.float32 and torch.equal(p, q.float()) for p, q in zip(got, want)) and torch.equal(got[3], g)
+    with torch.autocast(device, enabled=False):
+        assert cx.linear(x, w).dtype == torch.float32
+    with torch.autocast(device, dtype=low), pytest.raises(ComprexError):
+        cx.linear(x.double(), w.double())

@@ -271,3 +271,14 @@ def test_gradients_far_apart(device, dtype, far):
     want = (p * g.double()[:, None]) @ w.detach().double()
     near = g >= 2.0 ** -16 * g[0]
     assert ((dh.double() - want).norm(dim=1) <= (3 * UNIT[dtype] + 2.0 ** -18) * want.norm(dim=1))[near].all()
+
+
+def test_autocast(device):
+    """The product is in autocast's type, as torch's; the loss in 32 bits as ever."""
+    h, w, t, _ = _inputs(20, 90, 16, torch.float32, device)
+    leaves, cast = [x.clone().requires_grad_() for x in (h, w)], [x.bfloat16().requires_grad_() for x in (h, w)]
+    with torch.autocast(device, dtype=torch.bfloat16):
+        loss = cx.linear_cross_entropy(*leaves, t)
+    want = cx.linear_cross_entropy(*cast, t)
+    assert loss.dtype == torch.float32 and torch.equal(loss, want)
+    assert all(torch.equal(p, q.float()) for p, q in zip(torch.autograd.grad(loss, leaves), torch.autograd.grad(want, cast)))
