@@ -16,7 +16,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 
-#include <sstream>
+#include <string>
 
 #include "../cx_ops.h"
 #include "operators.h"
@@ -48,11 +48,16 @@ std::string shape_of(const Tensor& t) {
   for (int64_t i = 0; i < t.dim(); ++i) s += (i ? ", " : "") + std::to_string(t.size(i));
   return s + ")";
 }
+// (No streams: a number put into one ended the process, with torch's and this library's C++ runtimes in it side by side.)
+std::string text(const char* s) { return s; }
+std::string text(const std::string& s) { return s; }
+std::string text(int64_t n) { return std::to_string(n); }
+std::string text(int n) { return std::to_string(n); }
+std::string text(at::ScalarType t) { return c10::toString(t); }
+std::string text(const c10::Device& d) { return d.str(); }
 template <typename... A>
 [[noreturn]] void refuse(const A&... parts) {
-  std::ostringstream s;
-  (s << ... << parts);
-  throw Refused{s.str()};
+  throw Refused{(std::string() + ... + text(parts))};
 }
 void done(int rc, const char* what) {
   if (rc) refuse(what, " failed: ", native.last_error(), " (rc=", rc, ")");

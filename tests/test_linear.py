@@ -330,3 +330,42 @@ def test_autocast(device, low):
         assert cx.linear(x, w).dtype == torch.float32
     with torch.autocast(device, dtype=low), pytest.raises(ComprexError):
         cx.linear(x.double(), w.double())
+
+
+def _with_failing_calls(names, f):
+    """``f()`` while these native calls return an error."""
+    import ctypes as C
+    from comprex_b200 import _lib
+    lib, host = _lib.load(), _lib.host()
+    every = ("cx_linear_workspace_bytes", "cx_linear_forward", "cx_linear_backward", "cx_vocab_loss_workspace_bytes", "cx_vocab_loss_forward",
+             "cx_vocab_loss_backward", "cx_last_error")
+    fails = C.CFUNCTYPE(C.c_int, C.c_int, C.c_void_p, C.c_void_p)(lambda *a: -7)
+    address = [C.cast(fails if n in names else getattr(lib, n), C.c_void_p).value for n in every]
+    try:
+        host.bind_operators(ComprexError, *address)
+        f()
+    finally:
+        host.bind_operators(ComprexError, *(C.cast(getattr(lib, n), C.c_void_p).value for n in every))
+
+
+def test_errors_of_native_calls(device):
+    """A call that fails below is the package's error, forward, in a training step and in its backward pass."""
+    x, w, _, _, g = _inputs(4, 16, 24, torch.float32, device)
+    t = torch.zeros(4, dtype=torch.int64, device=device)
+    leaf = x.clone().requires_grad_()
+    calls = [lambda a: cx.linear(a, w, activation="silu"), lambda a: cx.linear_cross_entropy(a, w, t, reduction="none")]
+
+    def forward():
+        for f in calls:
+            for a in (x, leaf):
+                with pytest.raises(ComprexError, match=r"forward failed: .*\(rc=-7\)"):
+                    f(a)
+    _with_failing_calls(("cx_linear_forward", "cx_vocab_loss_forward"), forward)
+
+    def backward():
+        for f in calls:
+            y = f(leaf)
+            with pytest.raises(ComprexError, match=r"backward failed: .*\(rc=-7\)"):
+                torch.autograd.grad(y.sum(), leaf)
+    _with_failing_calls(("cx_linear_backward", "cx_vocab_loss_backward"), backward)
+    assert torch.isfinite(torch.autograd.grad(calls[0](leaf).sum(), leaf)[0]).all()
