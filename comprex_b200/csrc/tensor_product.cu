@@ -11,6 +11,7 @@
 // waits and issues; a launch 4 to 6 us from its start to its first results (tensor memory 0.35, the first copies 0.5, the
 // epilogue 0.7, the end 1).  8192 x 4096 x 1024 48 us, x 4096 175 us (1.57 PFLOP/s), 8192 x 1024 x 4096 50 us.
 #include <atomic>
+#include <mutex>
 
 #include "cx_product.cuh"
 #include "cx_tensor.cuh"
@@ -598,17 +599,40 @@ int make_map(CUtensorMap* map, const void* base, int dtype, int64_t rows, int64_
   return 0;
 }
 
-// a word that kernels set and the host reads
-uint32_t* status_word(bool host) {
-  static uint32_t* word = [] {
-    void* p = nullptr;
-    if (cudaHostAlloc(&p, 64, cudaHostAllocMapped | cudaHostAllocPortable) != cudaSuccess) return static_cast<uint32_t*>(nullptr);
-    *static_cast<uint32_t*>(p) = 0;
-    return static_cast<uint32_t*>(p);
-  }();
-  if (host || !word) return word;
+// A word of the current device that its kernels set and the host reads: `host`, and where they find it.  Made at the device's
+// first product, which may be under a stream's capture: allocating is not part of what is captured.
+struct Word {
+  uint32_t* host;
+  uint32_t* device;
+};
+Word status_word() {
+  constexpr int kDevices = 64;
+  static std::atomic<uint32_t*> words[kDevices];
+  static std::mutex making;
+  int dev = 0;
+  Word w = {nullptr, nullptr};
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kDevices) return w;
+  uint32_t* at = words[dev].load(std::memory_order_acquire);
+  if (!at) {
+    const std::lock_guard<std::mutex> lock(making);
+    at = words[dev].load(std::memory_order_acquire);
+    if (!at) {
+      cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+      if (cudaThreadExchangeStreamCaptureMode(&mode) != cudaSuccess) return w;
+      void* p = nullptr;
+      const cudaError_t e = cudaHostAlloc(&p, 64, cudaHostAllocMapped | cudaHostAllocPortable);
+      cudaThreadExchangeStreamCaptureMode(&mode);
+      if (e != cudaSuccess) return w;
+      at = static_cast<uint32_t*>(p);
+      *at = 0;
+      words[dev].store(at, std::memory_order_release);
+    }
+  }
   void* d = nullptr;
-  return cudaHostGetDevicePointer(&d, word, 0) == cudaSuccess ? static_cast<uint32_t*>(d) : nullptr;
+  if (cudaHostGetDevicePointer(&d, at, 0) != cudaSuccess) return w;
+  w.host = at;
+  w.device = static_cast<uint32_t*>(d);
+  return w;
 }
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -817,13 +841,13 @@ int cx_tensor_product(CxProduct* p, int count, cxprod::Arena& ws, cudaStream_t s
   if (!ws.base) return 0;
   if (!ws.ok()) return cx_set_error("cx_product: workspace too small", 0);
   if (units > 0x3FFFFFFF) return cx_set_error("cx_product: too many tiles", 0);
-  uint32_t* said = status_word(true);
-  if (!said) return cx_set_error("cx_product: no pinned memory for the status word", 0);
-  if (*reinterpret_cast<volatile uint32_t*>(said)) {
-    *reinterpret_cast<volatile uint32_t*>(said) = 0;
-    return cx_set_error("cx_product: an earlier product gave up waiting, its results are not valid", 0);
+  const Word said = status_word();
+  if (!said.host) return cx_set_error("cx_product: no pinned memory for the status word", 0);
+  if (*reinterpret_cast<volatile uint32_t*>(said.host)) {
+    *reinterpret_cast<volatile uint32_t*>(said.host) = 0;
+    return cx_set_error("cx_product: an earlier product of this device gave up waiting, its results are not valid", 0);
   }
-  t.status = status_word(false);
+  t.status = said.device;
   const int rc = c.cg == 2 ? launch<2, 256>(t, count, s) : c.bn == 128 ? launch<1, 128>(t, count, s) : launch<1, 64>(t, count, s);
   if (rc) return rc;
   if (most) {

@@ -168,3 +168,31 @@ def test_gpt2_under_autocast(device):
     assert (logits[0] - logits[1]).norm() <= 2.0 ** -5 * logits[0].norm()
     for (name, p), q in zip(plain.named_parameters(), fused.parameters()):
         assert q.grad.dtype == torch.float32 and (p.grad - q.grad).norm() <= 2.0 ** -4 * p.grad.norm() + 1e-6, name
+
+
+FIRST_IN_A_GRAPH = """
+import torch
+import comprex_b200 as cx
+torch.manual_seed(0)
+x, w, v = (torch.randn(*s, device="cuda").bfloat16() for s in ((200, 64), (128, 64), (1000, 128)))
+t = torch.randint(0, 1000, (200,), device="cuda")
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.no_grad(), torch.cuda.graph(graph):
+    h = cx.linear(x, w)
+    loss = cx.linear_cross_entropy(h, v, t)
+graph.replay()
+got = h.clone(), loss.clone()
+with torch.no_grad():
+    h = cx.linear(x, w)
+    loss = cx.linear_cross_entropy(h, v, t)
+assert torch.equal(got[0], h) and torch.equal(got[1], loss) and torch.isfinite(loss)
+print("the same")
+"""
+
+
+@pytest.mark.gpu
+def test_the_first_product_of_a_process_in_a_cuda_graph():
+    """What a process sets up once is set up under a capture, too."""
+    res = subprocess.run([sys.executable, "-c", FIRST_IN_A_GRAPH], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert res.returncode == 0 and "the same" in res.stdout, res.stdout + res.stderr
