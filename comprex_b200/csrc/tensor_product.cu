@@ -5,6 +5,7 @@
 // instructions, whose sums stay in tensor memory, and eight warps take finished sums from there: the tensor memory holds
 // two tiles, so the matrix instructions of a tile run under the epilogue of the tile before.  Each layout of the operands
 // is read as it lies: consecutive along k or along m and n is a bit of the instruction and another shape of the copy.
+// Every wait is bounded: where one runs out, the tiles that did not come are filled with NaN and a word is set for the host.
 //
 // What bounds it: a pair's slice of 256 x 256 x 64 is 512 cycles of matrix instructions and 64 KB from L2, at 2.3 PFLOP/s
 // while the clock is 1.9 GHz and 1.3 to 1.4 when the power limit is reached; a slice of smaller tiles about 340 cycles of
@@ -357,6 +358,30 @@ __device__ __forceinline__ void finish_part(const Job& t, const Unit& u, int hal
   finish_linear<T, WIDTH>(t, row, col0, tmem, bias);
 }
 
+// What a finishing warp leaves of its part of a tile when the sums never came: no numbers, so that nothing that follows can take
+// the call for a valid one.  (The host learns of it at the device's next product.)
+template <int WIDTH>
+__device__ __noinline__ void spoil_part(const Job& t, const Unit& u, int half, int64_t row, int64_t col0) {
+  const CxProduct& p = t.p;
+  if (row >= p.m || col0 >= p.n) return;
+  const int left = (int)min((int64_t)WIDTH, p.n - col0);
+  if (p.mode == kStats) {
+    p.part[(2ll * u.tn + half) * p.m + row] = make_float2(-INFINITY, NAN);
+    return;
+  }
+  float* sums = t.partial ? t.partial + ((int64_t)u.split * p.m + row) * t.part_ld + col0 : p.mode == kSums ? p.addend + row * p.ldadd + col0 : nullptr;
+  uint16_t* out = reinterpret_cast<uint16_t*>(p.out) + row * p.ldo + col0;
+  uint16_t* pre = p.mode == kOut && p.pre ? reinterpret_cast<uint16_t*>(p.pre) + row * p.ldpre + col0 : nullptr;
+  for (int i = 0; i < left; ++i) {
+    if (sums) {
+      sums[i] = NAN;
+    } else {
+      out[i] = 0x7FFF;                 // no number in bf16 and in fp16
+      if (pre) pre[i] = 0x7FFF;
+    }
+  }
+}
+
 template <int CG, int BN>
 __global__ void __launch_bounds__(kThreads, 1)
 tensor_product_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_constant__ CUtensorMap map_b0,
@@ -505,6 +530,12 @@ tensor_product_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_c
       cxt::fence_before_sync();
       __syncwarp();
       if (lane == 0) cxt::arrive_cluster(taken + 8 * (turn & 1));
+    }
+    if (gave_up) {                       // this unit's sums, and those of all that would have followed
+      for (; w.more(); w.next()) {
+        const Unit left = unit_of(t.job[w.job], w.u);
+        spoil_part<BN / 2>(t.job[w.job], left, half, (int64_t)(left.tm * CG + (int)rank) * 128 + quarter * 32 + lane, (int64_t)left.tn * BN + half * (BN / 2));
+      }
     }
   }
   if (gave_up) *reinterpret_cast<volatile uint32_t*>(t.status) = CX_ST_TIMEOUT;
