@@ -822,6 +822,8 @@ int cx_tensor_product(CxProduct* p, int count, cxprod::Arena& ws, cudaStream_t s
   Spread spread = {};
   int spreads = 0;
   int64_t most = 0, units = 0, spread_rows = 0;
+  for (int i = 0; i < count; ++i) units += ceil_div(p[i].m, 128 * c.cg) * ceil_div(p[i].n, c.bn) * c.splits[i];       // (at least as many)
+  if (units > 0x3FFFFFFF) return cx_set_error("cx_product: too many tiles", 0);
   // the longer units first
   const bool swap = count == 2 && ceil_div(ceil_div(p[0].k, kDepth), c.splits[0]) < ceil_div(ceil_div(p[1].k, kDepth), c.splits[1]);
   for (int i = 0; i < count; ++i) {
@@ -832,7 +834,6 @@ int cx_tensor_product(CxProduct* p, int count, cxprod::Arena& ws, cudaStream_t s
     job.slices = (int)ceil_div(q.k, kDepth);
     job.slices_per = (int)ceil_div(job.slices, c.splits[from]);
     job.splits = (int)ceil_div(job.slices, job.slices_per);
-    units += tm * tn * job.splits;
     job.tiles_m = (int)tm;
     job.tiles_n = (int)tn;
     job.units = (int)(tm * tn * job.splits);
@@ -871,7 +872,6 @@ int cx_tensor_product(CxProduct* p, int count, cxprod::Arena& ws, cudaStream_t s
   }
   if (!ws.base) return 0;
   if (!ws.ok()) return cx_set_error("cx_product: workspace too small", 0);
-  if (units > 0x3FFFFFFF) return cx_set_error("cx_product: too many tiles", 0);
   const Word said = status_word();
   if (!said.host) return cx_set_error("cx_product: no pinned memory for the status word", 0);
   if (*reinterpret_cast<volatile uint32_t*>(said.host)) {

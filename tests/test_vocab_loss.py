@@ -282,3 +282,25 @@ def test_autocast(device):
     want = cx.linear_cross_entropy(*cast, t)
     assert loss.dtype == torch.float32 and torch.equal(loss, want)
     assert all(torch.equal(p, q.float()) for p, q in zip(torch.autograd.grad(loss, leaves), torch.autograd.grad(want, cast)))
+
+
+def test_sizes_beyond_the_tiles_are_refused():
+    """As many tiles as 32 bits count once round: an error of the call (in a process of its own), not of the arithmetic."""
+    import os
+    import subprocess
+    import sys
+    code = """
+import ctypes as C
+from comprex_b200 import _lib
+lib, l = _lib.load(), _lib.VocabLoss()
+l.rows, l.vocab, l.dim, l.ldh, l.ldw, l.dtype = 1 << 25, 1 << 23, 8, 8, 8, 1
+for name in ("h", "w", "targets", "loss", "lse", "count", "grad", "dh", "dw"):
+    setattr(l, name, 1 << 20)
+for back in (0, 1):
+    assert lib.cx_vocab_loss_workspace_bytes(1, C.byref(l), back) > 0
+    print(lib.cx_last_error().decode())
+"""
+    assert code.count("l.dtype") == 1
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    res = subprocess.run([sys.executable, "-c", code], cwd=root, env=dict(os.environ, CUDA_VISIBLE_DEVICES=""), capture_output=True, text=True, timeout=200)
+    assert res.returncode == 0 and "too many tiles" in res.stdout, res
