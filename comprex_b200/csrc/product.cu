@@ -32,7 +32,9 @@ __device__ __forceinline__ void finish(const CxProduct& p, int64_t row, int64_t 
 __global__ void __launch_bounds__(kThreads) product_kernel(const __grid_constant__ CxProduct p) {
   __shared__ float sa[kDepth][kTile + 1], sb[kDepth][kTile + 1];
   __shared__ float2 stat[kTile][16];
-  const int64_t row0 = (int64_t)blockIdx.x * kTile, col0 = (int64_t)blockIdx.y * kTile;
+  // neighbouring blocks have the same columns; one dimension, since a grid's second one ends at 65535
+  const uint32_t tiles_m = (uint32_t)((p.m + kTile - 1) / kTile), tile_n = blockIdx.x / tiles_m;
+  const int64_t row0 = (int64_t)(blockIdx.x - tile_n * tiles_m) * kTile, col0 = (int64_t)tile_n * kTile;
   const int tr = threadIdx.x / 16, tc = threadIdx.x % 16;
   const float* a = reinterpret_cast<const float*>(p.a);
   const float* b = reinterpret_cast<const float*>(p.b);
@@ -101,7 +103,7 @@ __global__ void __launch_bounds__(kThreads) product_kernel(const __grid_constant
       const float2 s = stat[threadIdx.x][j];
       if (s.x != -INFINITY) sum += s.y * exp2f((s.x - top) * cxprod::kLog2e);
     }
-    p.part[(int64_t)blockIdx.y * p.m + row0 + threadIdx.x] = make_float2(top, sum);
+    p.part[(int64_t)tile_n * p.m + row0 + threadIdx.x] = make_float2(top, sum);
   }
 }
 
@@ -151,8 +153,9 @@ int cx_product(CxProduct* p, int count, cxprod::Arena& ws, cudaStream_t s) {
   if (!ws.base) return 0;
   if (!ws.ok()) return cx_set_error("cx_product: workspace too small", 0);
   for (int i = 0; i < count; ++i) {
-    const dim3 grid((unsigned)((p[i].m + kTile - 1) / kTile), (unsigned)((p[i].n + kTile - 1) / kTile));
-    product_kernel<<<grid, kThreads, 0, s>>>(p[i]);
+    const int64_t tiles = ((p[i].m + kTile - 1) / kTile) * ((p[i].n + kTile - 1) / kTile);
+    if (tiles > 0x7FFFFFFF) return cx_set_error("cx_product: too many tiles", 0);
+    product_kernel<<<(unsigned)tiles, kThreads, 0, s>>>(p[i]);
     cx_note_launch();
   }
   return cx_check_launch("cx_product");

@@ -369,3 +369,11 @@ def test_errors_of_native_calls(device):
                 torch.autograd.grad(y.sum(), leaf)
     _with_failing_calls(("cx_linear_backward", "cx_vocab_loss_backward"), backward)
     assert torch.isfinite(torch.autograd.grad(calls[0](leaf).sum(), leaf)[0]).all()
+
+
+def test_many_outputs_in_32_bits(device):
+    """More tiles of columns than a grid's second dimension has."""
+    n = 64 * 65535 + 70
+    x = torch.tensor([[0.5], [-2.0], [3.0], [1.0], [0.25]], device=device)
+    w = torch.arange(n, dtype=torch.float32, device=device)[:, None]
+    assert torch.equal(cx.linear(x, w), x * w.T)

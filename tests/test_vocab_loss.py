@@ -304,3 +304,19 @@ for back in (0, 1):
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     res = subprocess.run([sys.executable, "-c", code], cwd=root, env=dict(os.environ, CUDA_VISIBLE_DEVICES=""), capture_output=True, text=True, timeout=200)
     assert res.returncode == 0 and "too many tiles" in res.stdout, res
+
+
+@pytest.mark.gpu
+def test_many_words_in_32_bits():
+    """More tiles of the vocabulary than a grid's second dimension has."""
+    vocab = 64 * 65535 + 70
+    h = torch.ones(3, 1, device="cuda", requires_grad=True)
+    w = torch.zeros(vocab, 1, device="cuda", requires_grad=True)
+    t = torch.tensor([0, vocab - 1, 77], device="cuda")
+    loss = cx.linear_cross_entropy(h, w, t, reduction="none")
+    # a sum of `vocab` equal terms over tiles: its roundings are below 2^-20 of it
+    assert (loss - math.log(vocab)).abs().max() <= 2.0 ** -20 * (1 + math.log(vocab))
+    dw, = torch.autograd.grad(loss.sum(), (w,))
+    want = torch.full((vocab, 1), 3.0 / vocab, device="cuda", dtype=torch.float64)
+    want[t] -= 1.0
+    assert ((dw.double() - want).abs() <= 2.0 ** -18 * want.abs()).all()
