@@ -143,12 +143,10 @@ std::vector<float> widen(int dtype, const void* p, int64_t rows, int64_t cols, i
     for (int64_t c = 0; c < cols; ++c) out[(size_t)(r * cols + c)] = load_elem(dtype, p, r * ld + c);
   return out;
 }
-// out[c] += sum over i of a[i] b[i][c]
+// out[c] += sum over i of a[i] b[i][c]  (also where a[i] is zero: b may be no number)
 void add_product(const float* a, const float* b, float* out, int64_t inner, int64_t cols) {
-  for (int64_t i = 0; i < inner; ++i) {
-    if (a[i] == 0.f) continue;
+  for (int64_t i = 0; i < inner; ++i)
     for (int64_t c = 0; c < cols; ++c) out[c] += a[i] * b[i * cols + c];
-  }
 }
 float dot(const float* a, const float* b, int64_t n) {
   float sum = 0.f;

@@ -377,3 +377,15 @@ def test_many_outputs_in_32_bits(device):
     x = torch.tensor([[0.5], [-2.0], [3.0], [1.0], [0.25]], device=device)
     w = torch.arange(n, dtype=torch.float32, device=device)[:, None]
     assert torch.equal(cx.linear(x, w), x * w.T)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_zeros_times_what_is_no_number(device, dtype):
+    """Gradients are sums of products: zero times infinity is no number on either back end, as in torch."""
+    x, w, _, _, g = _inputs(6, 16, 24, dtype, device)
+    g[2], g[:, 5] = 0.0, 0.0
+    x[2, 3], x[4, 1], w[5, 2], w[7, 9] = float("inf"), float("nan"), float("inf"), float("nan")
+    leaves = [t.clone().requires_grad_() for t in (x, w)]
+    got = torch.autograd.grad(cx.linear(*leaves), leaves, g)
+    want = g.float() @ w.float(), g.float().T @ x.float()
+    assert all(torch.equal(torch.isnan(a), torch.isnan(b)) for a, b in zip(got, want))
