@@ -161,7 +161,7 @@ int du_pass(Du& d, void* dbias, cudaStream_t s) {
 // Bound by reading w, and at these sizes by latency: every weight is used once per row, so the tensor cores have nothing to
 // do.  A warp has four rows of w and a share of k, 256 elements at a time, all loads of a turn under way at once; `share`
 // warps of a block join their sums in a fixed order, and one thread per result does the rest.
-constexpr int kFewRows = 16, kFewColumns = 4, kWarps = kThreads / 32;
+constexpr int kFewColumns = 4, kWarps = kThreads / 32;
 
 struct Few {
   const void* x;
@@ -271,7 +271,10 @@ int few_rows(const CxLinear& l, cudaStream_t s) {
 
 // Both calls also run without a workspace: they launch nothing then and count the bytes that they need.
 int forward(const CxLinear& l, cxprod::Arena& ws, cudaStream_t s) {
-  if (l.rows <= 2 || (l.rows <= 4 && l.outer * l.inner <= (8 << 20))) {
+  // On the CUDA cores up to two rows, and up to four where w is small or of 32 bits, which the tensor cores do not multiply.  Weights
+  // from memory, one row, then four; here / as tiles, us: bf16 1024 x 1024 3.5 / 5.4, 4.3 / 5.5; 2048 x 4096 5.5 / 10.0, 10.7 / 10.1;
+  // 4096 x 4096 9.6 / 12.6, 15.7 / 12.8 (two rows 13.6 / 12.7); float32 1024 x 1024 3.6 / 102, 4.9 / 105; 4096 x 4096 11.7 / 425, 17.2 / 428.
+  if (l.rows <= 2 || (l.rows <= 4 && (l.dtype == CX_F32 || l.outer * l.inner <= (8 << 20)))) {
     if (!ws.base) return 0;
     return l.dtype == CX_F32 ? few_rows<float>(l, s) : l.dtype == CX_BF16 ? few_rows<__nv_bfloat16>(l, s) : few_rows<__half>(l, s);
   }
