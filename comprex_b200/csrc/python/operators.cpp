@@ -138,6 +138,19 @@ variable_list once(variable_list&& grads) {
   return (*stop)(std::move(grads));
 }
 
+// A saved tensor as it was saved, in rows without gaps: hooks may have kept it somewhere else, and must bring it back.
+Tensor kept(const Tensor& t, const char* name, const Tensor& like, at::ScalarType type, at::IntArrayRef sizes) {
+  if (!t.defined() || t.layout() != at::kStrided || t.device() != like.device() || t.scalar_type() != type || t.sizes() != sizes)
+    refuse("the saved ", name, " has come back as another tensor");
+  has_memory(t, name);
+  return t.resolve_neg().contiguous();
+}
+// ... and a saved operand, whose rows may lie apart
+void came_back(const Tensor& t, const char* name, const Tensor& like, at::ScalarType type, bool fits) {
+  if (!fits || t.layout() != at::kStrided || t.device() != like.device() || t.scalar_type() != type) refuse("the saved ", name, " has come back as another tensor");
+  has_memory(t, name);
+}
+
 template <typename F>
 variable_list in_backward(const F& f) {
   try {
@@ -168,6 +181,8 @@ CxLinear describe(const Tensor& xm, const Tensor& wm, int act) {
   return d;
 }
 
+int64_t pre_columns(int64_t outer) { return (outer + 15) / 16 * 16; }
+
 Tensor linear_forward(const Tensor& x, const Tensor& w, const Maybe& bias, int act, const Maybe& residual, Tensor* pre) {
   const int64_t outer = w.size(0), inner = w.size(1);
   std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
@@ -187,7 +202,7 @@ Tensor linear_forward(const Tensor& x, const Tensor& w, const Maybe& bias, int a
   }
   d.y = y.data_ptr();
   if (pre) {                                  // kept for the backward call, in aligned rows
-    d.ldpre = (outer + 15) / 16 * 16;
+    d.ldpre = pre_columns(outer);
     *pre = at::empty({d.rows, d.ldpre}, x.options());
     d.pre = pre->data_ptr();
   }
@@ -208,12 +223,14 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     return in_backward([&]() -> variable_list {
       const variable_list saved = ctx->get_saved_variables();
-      const Tensor &x = saved[0], &w = saved[1], &pre = saved[2], grad = written(grads[0]);
+      const Tensor &x = saved[0], &w = saved[1], grad = written(grads[0]);
       const int64_t act = ctx->saved_data["act"].toInt(), inputs = ctx->saved_data["inputs"].toInt();
       variable_list out(5);
       if (!grad.defined()) return out;
       has_memory(grad, "the gradient");
       no_tangent(grad, "the gradient");
+      came_back(w, "weight", grad, grad.scalar_type(), w.dim() == 2 && w.size(0) == grad.size(-1));
+      came_back(x, "x", grad, grad.scalar_type(), x.dim() == grad.dim() && x.size(-1) == w.size(1) && x.sizes().slice(0, x.dim() - 1) == grad.sizes().slice(0, x.dim() - 1));
       const bool bias = inputs & 1, residual = inputs & 2;
       const bool need_b = bias && ctx->needs_input_grad(2), need_r = residual && ctx->needs_input_grad(bias ? 3 : 2);
       const int64_t outer = w.size(0), inner = w.size(1);
@@ -233,9 +250,11 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
       CxLinear d = describe(xm, wm, (int)act);
       d.grad = gm.data_ptr();
       d.ldg = ld_of(gm);
-      if (pre.defined()) {
+      Tensor pre;
+      if (act != CX_ACT_NONE) {
+        d.ldpre = pre_columns(outer);
+        pre = kept(saved[2], "u", grad, grad.scalar_type(), {d.rows, d.ldpre});
         d.pre = pre.data_ptr();
-        d.ldpre = pre.size(1);
       }
       if (out[0].defined()) d.dx = out[0].data_ptr();
       if (out[1].defined()) d.dw = out[1].data_ptr();
@@ -288,18 +307,27 @@ struct LossFn : torch::autograd::Function<LossFn> {
     Tensor loss = loss_forward(h, w, targets, ignore, (int)reduction, tm, lse, count);
     ctx->saved_data["ignore"] = ignore;
     ctx->saved_data["reduction"] = reduction;
+    ctx->saved_data["rows"] = tm.numel();
+    ctx->saved_data["type"] = static_cast<int64_t>(h.scalar_type());
     ctx->save_for_backward({h, w, tm, lse, count});
     return loss;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     return in_backward([&]() -> variable_list {
       const variable_list saved = ctx->get_saved_variables();
-      const Tensor &h = saved[0], &w = saved[1], &tm = saved[2];
+      const Tensor &h = saved[0], &w = saved[1];
       grads[0] = written(grads[0]);
       variable_list out(5);
       if (!grads[0].defined()) return out;
       has_memory(grads[0], "the gradient");
       no_tangent(grads[0], "the gradient");
+      const int64_t rows = ctx->saved_data["rows"].toInt();
+      const int reduction = (int)ctx->saved_data["reduction"].toInt();
+      const auto type = static_cast<at::ScalarType>(ctx->saved_data["type"].toInt());
+      came_back(w, "weight", grads[0], type, w.dim() == 2 && w.numel());
+      came_back(h, "hidden", grads[0], type, h.dim() >= 1 && h.size(-1) == w.size(1) && h.numel() == rows * w.size(1));
+      const Tensor tm = kept(saved[2], "targets", grads[0], at::kLong, {rows}), lse = kept(saved[3], "sums", grads[0], at::kFloat, {rows}),
+                   count = kept(saved[4], "count", grads[0], at::kFloat, {1});
       const at::AutoDispatchBelowADInplaceOrView below;
       if (ctx->needs_input_grad(0)) out[0] = at::empty(h.sizes(), h.options());
       if (ctx->needs_input_grad(1)) out[1] = at::empty(w.sizes(), w.options());
@@ -309,7 +337,7 @@ struct LossFn : torch::autograd::Function<LossFn> {
       }
       const c10::OptionalDeviceGuard guard(h.is_cuda() ? std::make_optional(h.device()) : std::nullopt);
       const Tensor hm = rows_of(h, w.size(1)), wm = rows_of(w, w.size(1));
-      CxVocabLoss d = describe(hm, wm, tm, ctx->saved_data["ignore"].toInt(), (int)ctx->saved_data["reduction"].toInt(), saved[3], saved[4]);
+      CxVocabLoss d = describe(hm, wm, tm, ctx->saved_data["ignore"].toInt(), reduction, lse, count);
       Tensor g = grads[0].to(at::kFloat).resolve_neg();
       if (g.dim() > 1) g = g.reshape({-1});
       d.grad = g.data_ptr<float>();

@@ -389,3 +389,42 @@ def test_zeros_times_what_is_no_number(device, dtype):
     got = torch.autograd.grad(cx.linear(*leaves), leaves, g)
     want = g.float() @ w.float(), g.float().T @ x.float()
     assert all(torch.equal(torch.isnan(a), torch.isnan(b)) for a, b in zip(got, want))
+
+
+def test_saved_tensors_that_come_back_changed(device):
+    """Hooks may keep what is saved in another order; what comes back as something else is refused, not read as if it were the same."""
+    from torch.autograd.graph import saved_tensors_hooks
+    x, w, b, _, g = _inputs(6, 32, 24, torch.bfloat16, device)
+    t = torch.arange(6, device=device)
+    leaves = [v.requires_grad_() for v in (x, w, b)]
+    calls = [lambda: cx.linear(*leaves, activation="gelu"), lambda: cx.linear(*leaves),
+             lambda: cx.linear_cross_entropy(x, w, t, reduction="none")]
+    for f in calls:
+        y = f()
+        up = torch.ones_like(y)
+        want = torch.autograd.grad(y, leaves, up, allow_unused=True)
+
+        def spread(v):                         # the same numbers, further apart
+            return torch.stack((v, v), -1)[..., 0]
+        with saved_tensors_hooks(lambda v: v, spread):
+            y = f()
+        got = torch.autograd.grad(y, leaves, up, allow_unused=True)
+        assert all(p is None or torch.equal(p, q) for p, q in zip(got, want))
+        for other in (lambda v: v[:2], lambda v: v.double(), lambda v: v[None], lambda v: v.float() + 0, lambda v: v.to("cpu") if v.is_cuda else v[..., :1]):
+            n = 0
+
+            def one(v, which):
+                nonlocal n
+                n += 1
+                return other(v) if n - 1 == which else v
+            for which in range(5):
+                n = 0
+                with saved_tensors_hooks(lambda v: v, lambda v: one(v, which)):
+                    y = f()
+                changed = False
+                try:
+                    got = torch.autograd.grad(y, leaves, up, allow_unused=True)
+                except (ComprexError, RuntimeError):
+                    changed = True
+                # either refused, or what came back was the same after all (nothing left to change, a number in float32 already)
+                assert changed or all(p is None or torch.equal(p, q) for p, q in zip(got, want)), which
