@@ -287,7 +287,7 @@ bool cx_pdl_enabled();   // COMPREX_PDL != 0 (read once)
 // threshold of the next message, the norms of the next step) waits at its own start, and its launch
 // is over when it may go on.  A receive kernel, however, does not wait at its start when its sender is
 // in front of it, so it has to know what is: senders note "not early"; every other kernel that triggers
-// before it is done with its operands notes "early" (receive kernels, thresholds, norms, dense updates),
+// before it is done with its operands notes "early" (receive kernels, thresholds, norms, dense updates, products),
 // and cx_front_wait says how the kernel about to be launched must wait.  The notes know this library's
 // kernels alone: a kernel of the program's own that was queued behind the sender may be at work on the
 // receiver's vectors (and let the receiver in early), so without waiting the receiver may only poll and

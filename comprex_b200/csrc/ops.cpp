@@ -5,6 +5,7 @@
 #include "cx_ops.h"
 
 int cx_set_error(const char* where, int cuda_err);
+void cx_note_stream(const void* stream, bool early);
 int cx_adamw_step_cuda(const CxAdamW*, void*);
 int cx_adamw_step_host(const CxAdamW*);
 int64_t cx_linear_workspace_bytes_cuda(const CxLinear*, int);
@@ -29,6 +30,12 @@ int on_host(F f, const D* d) {
   } catch (const std::exception& e) {
     return cx_set_error(e.what(), 0);
   }
+}
+
+// The products' kernels let the kernel behind them in at their start: a receive kernel that comes next waits first.
+void* noted(void* stream) {
+  cx_note_stream(stream, true);
+  return stream;
 }
 
 constexpr int64_t kMost = 0x7FFFFF00;      // rows, columns and entries of the vocabulary: 32-bit coordinates
@@ -75,7 +82,7 @@ int cx_linear_forward(int dev, const CxLinear* l, void* stream) {
   if (!l->x || !l->w || !l->y) return cx_set_error("cx_linear_forward: an operand is missing", 0);
   if (l->ldx < l->inner || l->ldw < l->inner || (l->residual && l->ldr < l->outer) || (l->pre && l->ldpre < l->outer))
     return cx_set_error("cx_linear_forward: rows overlap", 0);
-  return dev == CX_DEV_CUDA ? cx_linear_forward_cuda(l, stream) : on_host(cx_linear_forward_host, l);
+  return dev == CX_DEV_CUDA ? cx_linear_forward_cuda(l, noted(stream)) : on_host(cx_linear_forward_host, l);
 }
 
 int cx_linear_backward(int dev, const CxLinear* l, void* stream) {
@@ -84,7 +91,7 @@ int cx_linear_backward(int dev, const CxLinear* l, void* stream) {
     return cx_set_error("cx_linear_backward: an operand is missing", 0);
   if (l->ldg < l->outer || (l->act != CX_ACT_NONE && l->ldpre < l->outer) || (l->dw && l->ldx < l->inner) || (l->dx && l->ldw < l->inner))
     return cx_set_error("cx_linear_backward: rows overlap", 0);
-  return dev == CX_DEV_CUDA ? cx_linear_backward_cuda(l, stream) : on_host(cx_linear_backward_host, l);
+  return dev == CX_DEV_CUDA ? cx_linear_backward_cuda(l, noted(stream)) : on_host(cx_linear_backward_host, l);
 }
 
 int64_t cx_vocab_loss_workspace_bytes(int dev, const CxVocabLoss* l, int backward) {
@@ -94,14 +101,14 @@ int64_t cx_vocab_loss_workspace_bytes(int dev, const CxVocabLoss* l, int backwar
 int cx_vocab_loss_forward(int dev, const CxVocabLoss* l, void* stream) {
   if (const char* why = wrong(l)) return cx_set_error(why, 0);
   if (!l->loss) return cx_set_error("cx_vocab_loss_forward: an operand is missing", 0);
-  return dev == CX_DEV_CUDA ? cx_vocab_loss_forward_cuda(l, stream) : on_host(cx_vocab_loss_forward_host, l);
+  return dev == CX_DEV_CUDA ? cx_vocab_loss_forward_cuda(l, noted(stream)) : on_host(cx_vocab_loss_forward_host, l);
 }
 
 int cx_vocab_loss_backward(int dev, const CxVocabLoss* l, void* stream) {
   if (const char* why = wrong(l)) return cx_set_error(why, 0);
   if (!l->grad) return cx_set_error("cx_vocab_loss_backward: an operand is missing", 0);
   if (!l->dh && !l->dw) return 0;
-  return dev == CX_DEV_CUDA ? cx_vocab_loss_backward_cuda(l, stream) : on_host(cx_vocab_loss_backward_host, l);
+  return dev == CX_DEV_CUDA ? cx_vocab_loss_backward_cuda(l, noted(stream)) : on_host(cx_vocab_loss_backward_host, l);
 }
 
 int64_t cx_ops_sizeof(int what) {

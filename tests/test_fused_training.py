@@ -196,3 +196,37 @@ def test_the_first_product_of_a_process_in_a_cuda_graph():
     """What a process sets up once is set up under a capture, too."""
     res = subprocess.run([sys.executable, "-c", FIRST_IN_A_GRAPH], cwd=ROOT, capture_output=True, text=True, timeout=300)
     assert res.returncode == 0 and "the same" in res.stdout, res.stdout + res.stderr
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["pairs", "rle", "dense"])
+@pytest.mark.parametrize("rows", [1, 64, 1024])
+def test_operators_between_send_and_receive(kind, rows):
+    """The receiver's vector is what a product of this package has just written (its kernels let the kernel behind in early): small
+    whole numbers, so everything is exact."""
+    cols = 1024
+    n = rows * cols
+    dtype = torch.bfloat16 if kind != "rle" else torch.float32
+    env = cx.GaspiEnvironment(8 << 20, device="cuda")
+    ex = cx.GaspiEx(env, n, dtype=dtype) if kind == "dense" else cx.Comprex(env, n)
+    if kind != "dense":
+        ex.setThreshold(cx.ThresholdTopK(0.05))
+        ex.setCompressor(cx.CompressorRLE() if kind == "rle" else cx.CompressorIndexPairs())
+    ex.connectTo(0, 0)
+    gen = torch.Generator(device="cuda").manual_seed(rows)
+    held = torch.zeros(n, device="cuda")
+    for _ in range(8):
+        v = torch.randint(-9, 10, (n,), device="cuda", generator=gen).to(dtype)
+        x, w = (torch.randint(-2, 3, (k, 32), device="cuda", generator=gen).to(torch.bfloat16) for k in (rows, cols))
+        want = x.float() @ w.float().T
+        ex.writeRemote(v)
+        out = cx.linear(x, w).view(n)
+        out = out if kind != "rle" else out.float()
+        ex.readRemote_add(out)
+        held += v.float()
+        sent = v.float()
+        if kind != "dense":
+            sent, held = held - ex.getRests(), ex.getRests()
+        assert torch.equal(out.float(), want.view(n) + sent)
+    env.check()
+    env.close()
