@@ -96,24 +96,25 @@ Tensor workspace(D& d, const Tensor& like, int64_t bytes) {
 }
 
 // A trace sees the outputs being allocated and not the kernels that fill them: what it plays back would be memory that nobody
-// wrote.  (torch.compile leaves a call to these functions out of its graphs.)
-void not_traced() {
+// wrote.  (torch.compile leaves a call to these functions out of its graphs.)  Under a mode of fake tensors the outputs would have
+// no memory at all.  Asked once a call.
+void for_real() {
   using c10::impl::TorchDispatchModeKey;
-  if (torch::jit::tracer::isTracing() || c10::impl::TorchDispatchModeTLS::get_mode(TorchDispatchModeKey::PROXY))
-    refuse("this operator cannot be put into a trace");
+  using c10::impl::TorchDispatchModeTLS;
+  if (torch::jit::tracer::isTracing()) refuse("this operator cannot be put into a trace");
+  if (!TorchDispatchModeTLS::any_modes_set()) return;
+  if (TorchDispatchModeTLS::get_mode(TorchDispatchModeKey::PROXY)) refuse("this operator cannot be put into a trace");
+  if (TorchDispatchModeTLS::get_mode(TorchDispatchModeKey::FAKE) || TorchDispatchModeTLS::get_mode(TorchDispatchModeKey::FUNCTIONAL))
+    refuse("what this operator makes would have no memory of its own under this mode");
 }
 
 // Fake tensors, those that a transform (vmap, grad) has wrapped and subclasses that dispatch in Python have no memory that the
-// kernels could read, and under such a mode the outputs would have none either.
+// kernels could read.
 void has_memory(const Tensor& t, const char* name) {
   using c10::DispatchKey;
-  using c10::impl::TorchDispatchModeKey;
-  using c10::impl::TorchDispatchModeTLS;
-  const c10::DispatchKeySet keys = t.key_set();
-  if (TorchDispatchModeTLS::get_mode(TorchDispatchModeKey::FAKE) || TorchDispatchModeTLS::get_mode(TorchDispatchModeKey::FUNCTIONAL) ||
-      keys.has(DispatchKey::Python) || keys.has(DispatchKey::FuncTorchBatched) || keys.has(DispatchKey::FuncTorchGradWrapper) ||
-      keys.has(DispatchKey::Functionalize) || keys.has(DispatchKey::ZeroTensor) || !t.has_storage())
-    refuse(name, " has no memory of its own (a fake or wrapped tensor, or one under such a mode)");
+  constexpr c10::DispatchKeySet without({DispatchKey::Python, DispatchKey::FuncTorchBatched, DispatchKey::FuncTorchGradWrapper,
+                                         DispatchKey::Functionalize, DispatchKey::ZeroTensor});
+  if (t.key_set().has_any(without) || !t.has_storage()) refuse(name, " has no memory of its own (a fake or wrapped tensor)");
 }
 
 // There is no forward-mode derivative: a tangent would be lost in silence.
@@ -154,7 +155,7 @@ void came_back(const Tensor& t, const char* name, const Tensor& like, at::Scalar
 template <typename F>
 variable_list in_backward(const F& f) {
   try {
-    not_traced();
+    for_real();
     return once(f());
   } catch (const Refused& r) {          // the engine may have called from a thread of its own
     const PyGILState_STATE gil = PyGILState_Ensure();
@@ -215,8 +216,7 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Maybe& bias, int64_t act, const Maybe& residual) {
     Tensor pre;
     Tensor y = linear_forward(x, w, bias, (int)act, residual, act != CX_ACT_NONE ? &pre : nullptr);
-    ctx->saved_data["act"] = act;
-    ctx->saved_data["inputs"] = (int64_t)((bias ? 1 : 0) | (residual ? 2 : 0));
+    ctx->saved_data["call"] = std::vector<int64_t>{act, (bias ? 1 : 0) | (residual ? 2 : 0)};
     ctx->save_for_backward({x, w, pre});
     return y;
   }
@@ -224,7 +224,8 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
     return in_backward([&]() -> variable_list {
       const variable_list saved = ctx->get_saved_variables();
       const Tensor &x = saved[0], &w = saved[1], grad = written(grads[0]);
-      const int64_t act = ctx->saved_data["act"].toInt(), inputs = ctx->saved_data["inputs"].toInt();
+      const auto call = ctx->saved_data["call"].toIntVector();
+      const int64_t act = call[0], inputs = call[1];
       variable_list out(5);
       if (!grad.defined()) return out;
       has_memory(grad, "the gradient");
@@ -305,10 +306,7 @@ struct LossFn : torch::autograd::Function<LossFn> {
   static Tensor forward(AutogradContext* ctx, const Tensor& h, const Tensor& w, const Tensor& targets, int64_t ignore, int64_t reduction) {
     Tensor tm, lse, count;
     Tensor loss = loss_forward(h, w, targets, ignore, (int)reduction, tm, lse, count);
-    ctx->saved_data["ignore"] = ignore;
-    ctx->saved_data["reduction"] = reduction;
-    ctx->saved_data["rows"] = tm.numel();
-    ctx->saved_data["type"] = static_cast<int64_t>(h.scalar_type());
+    ctx->saved_data["call"] = std::vector<int64_t>{ignore, reduction, tm.numel(), static_cast<int64_t>(h.scalar_type())};
     ctx->save_for_backward({h, w, tm, lse, count});
     return loss;
   }
@@ -321,9 +319,10 @@ struct LossFn : torch::autograd::Function<LossFn> {
       if (!grads[0].defined()) return out;
       has_memory(grads[0], "the gradient");
       no_tangent(grads[0], "the gradient");
-      const int64_t rows = ctx->saved_data["rows"].toInt();
-      const int reduction = (int)ctx->saved_data["reduction"].toInt();
-      const auto type = static_cast<at::ScalarType>(ctx->saved_data["type"].toInt());
+      const auto call = ctx->saved_data["call"].toIntVector();
+      const int64_t ignore = call[0], rows = call[2];
+      const int reduction = (int)call[1];
+      const auto type = static_cast<at::ScalarType>(call[3]);
       came_back(w, "weight", grads[0], type, w.dim() == 2 && w.numel());
       came_back(h, "hidden", grads[0], type, h.dim() >= 1 && h.size(-1) == w.size(1) && h.numel() == rows * w.size(1));
       const Tensor tm = kept(saved[2], "targets", grads[0], at::kLong, {rows}), lse = kept(saved[3], "sums", grads[0], at::kFloat, {rows}),
@@ -337,7 +336,7 @@ struct LossFn : torch::autograd::Function<LossFn> {
       }
       const c10::OptionalDeviceGuard guard(h.is_cuda() ? std::make_optional(h.device()) : std::nullopt);
       const Tensor hm = rows_of(h, w.size(1)), wm = rows_of(w, w.size(1));
-      CxVocabLoss d = describe(hm, wm, tm, ctx->saved_data["ignore"].toInt(), reduction, lse, count);
+      CxVocabLoss d = describe(hm, wm, tm, ignore, reduction, lse, count);
       Tensor g = grads[0].to(at::kFloat).resolve_neg();
       if (g.dim() > 1) g = g.reshape({-1});
       d.grad = g.data_ptr<float>();
@@ -357,7 +356,7 @@ const Tensor& tensor(PyObject* o, const char* name, const Tensor* like) {
   if (!THPVariable_Check(o)) refuse(name, " must be a strided tensor");
   const Tensor& t = THPVariable_Unpack(o);
   if (t.layout() != at::kStrided) refuse(name, " must be a strided tensor");
-  if (!like) not_traced();
+  if (!like) for_real();
   if (!like && !t.is_cuda() && !t.is_cpu()) refuse("tensors on ", t.device(), " are not supported");
   if (like && t.device() != like->device()) refuse(name, " is on ", t.device(), ", not on ", like->device());
   has_memory(t, name);
@@ -369,16 +368,16 @@ const Tensor& same_type(const Tensor& t, const char* name, const Tensor& like) {
   return t;
 }
 
-// The type that torch's own product would be in here: autocast's, where that is on and `x` is cast; else the tensor's.
-at::ScalarType product_type(const Tensor& x) {
-  const auto device = x.device().type();
-  const bool cast = at::autocast::is_autocast_enabled(device) && x.is_floating_point() && x.scalar_type() != at::kDouble;
-  return cast ? at::autocast::get_autocast_dtype(device) : x.scalar_type();
-}
-// ... and an operand in it, by autocast's rules and through its cache of weights
-Tensor in_type(const Tensor& t, at::ScalarType type) {
-  return at::autocast::is_autocast_enabled(t.device().type()) ? at::autocast::cached_cast(type, t, t.device().type()) : t;
-}
+// The type that torch's own product would be in: autocast's, where that is on and casts such a tensor; else the tensor's.
+struct Cast {
+  bool on;
+  at::ScalarType type;
+  explicit Cast(const Tensor& x) : on(at::autocast::is_autocast_enabled(x.device().type())), type(x.scalar_type()) {
+    if (on && x.is_floating_point() && type != at::kDouble) type = at::autocast::get_autocast_dtype(x.device().type());
+  }
+  // an operand in it, by autocast's rules and through its cache of weights
+  Tensor of(const Tensor& t) const { return on ? at::autocast::cached_cast(type, t, t.device().type()) : t; }
+};
 
 void out_of_memory(const c10::OutOfMemoryError& e) {
   PyObject* torch = PyImport_ImportModule("torch");
@@ -428,14 +427,14 @@ PyObject* cx_py_linear(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   bool apart = false;          // the residual is added to the result, in the type that torch adds the two in
   try {
     const Tensor& given = tensor(a[0], "x", nullptr);
-    const at::ScalarType type = product_type(given);
-    x = in_type(given, type);
+    const Cast cast(given);
+    x = cast.of(given);
     code_of(x);
-    w = same_type(in_type(tensor(a[1], "weight", &x), type), "weight", x);
-    if (a[2] != Py_None) bias = same_type(in_type(tensor(a[2], "bias", &x), type), "bias", x);
+    w = same_type(cast.of(tensor(a[1], "weight", &x)), "weight", x);
+    if (a[2] != Py_None) bias = same_type(cast.of(tensor(a[2], "bias", &x)), "bias", x);
     if (a[4] != Py_None) {
       residual = tensor(a[4], "residual", &x);
-      if (at::autocast::is_autocast_enabled(x.device().type()) && residual->scalar_type() != type) apart = true;       // (autocast leaves sums as they are)
+      if (cast.on && residual->scalar_type() != cast.type) apart = true;       // (autocast leaves sums as they are)
       else residual = same_type(*residual, "residual", x);
     }
     if (w.dim() != 2 || x.dim() < 1 || x.size(-1) != w.size(1) || !w.numel()) refuse("x ", shape_of(x), " does not fit weight ", shape_of(w));
@@ -480,10 +479,10 @@ PyObject* cx_py_vocab_loss(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   Tensor h, w, targets;
   try {
     const Tensor& given = tensor(a[0], "hidden", nullptr);
-    const at::ScalarType type = product_type(given);
-    h = in_type(given, type);
+    const Cast cast(given);
+    h = cast.of(given);
     code_of(h);
-    w = same_type(in_type(tensor(a[1], "weight", &h), type), "weight", h);
+    w = same_type(cast.of(tensor(a[1], "weight", &h)), "weight", h);
     targets = tensor(a[2], "targets", &h);
     if (targets.scalar_type() != at::kLong) refuse("targets must be int64, not ", targets.scalar_type());
     if (w.dim() != 2 || !w.numel() || h.dim() < 1 || h.size(-1) != w.size(1)) refuse("hidden ", shape_of(h), " does not fit weight ", shape_of(w));
