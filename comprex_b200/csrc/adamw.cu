@@ -1,9 +1,8 @@
 // AdamW step over all tensors of a model in one launch, states in 32 bits or in 8 (the mathematics: cx_adamw.h).
 //
 // An element moves its gradient, its 32-bit weight both ways, its 16-bit copy and two states both ways: 16 bytes for a bf16
-// tensor with 8-bit states, 28 with 32-bit ones.  With 32 bits that bounds it (268 M elements bf16 / fp32 1270 / 1248 us, 5.9
-// / 6.0 TB/s); with 8 it is instructions as well, 78 an element, 18 of them the random bits (876 / 829 us, 4.9 / 5.2 TB/s;
-// without the random bits 727 / 706).  One warp takes one block of 256 elements at a time: the block is what shares a scale,
+// tensor with 8-bit states, 28 with 32-bit ones.  With 32 bits that bounds it (268 M elements bf16 / fp32 1146 / 1127 us, 6.6
+// / 6.7 TB/s); with 8 it is instructions as well, 73 an element, 18 of them the random bits (830 / 803 us, 5.2 / 5.3 TB/s).  One warp takes one block of 256 elements at a time: the block is what shares a scale,
 // so its largest values are two warp-wide integer maxima and nothing crosses warps, and a lane's two groups of four
 // consecutive elements make every access of the warp whole lines.  Tensors are found through a table of blocks, so a model of
 // many small tensors is one launch as well.

@@ -10,7 +10,8 @@
 // What bounds it: a pair's slice of 256 x 256 x 64 is 512 cycles of matrix instructions and 64 KB from L2, at 2.3 PFLOP/s
 // while the clock is 1.9 GHz and 1.3 to 1.4 when the power limit is reached; a slice of smaller tiles about 340 cycles of
 // waits and issues; a launch 4 to 6 us from its start to its first results (tensor memory 0.35, the first copies 0.5, the
-// epilogue 0.7, the end 1).  8192 x 4096 x 1024 48 us, x 4096 175 us (1.57 PFLOP/s), 8192 x 1024 x 4096 50 us.
+// epilogue 0.7, the end 1).  8192 x 4096 x 1024 50 us, x 4096 177 us (1.55 PFLOP/s), 8192 x 1024 x 4096 50 us
+// (operands from memory, after a pause).
 #include <atomic>
 #include <mutex>
 
