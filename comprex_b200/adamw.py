@@ -15,13 +15,13 @@ Tensors of 16 bits have 32-bit weights behind them, which take the step; the ten
 parameter group has its own settings and every tensor its own step count: a tensor without a gradient is left alone.
 
 States live in flat buffers in which tensor ``i`` starts at a multiple of 256 elements, in the order of the
-parameters (:meth:`AdamW.flat_state`).  A tensor that is frozen has none; with its first gradient the buffers are laid out anew.  With ``state_bits=8`` each block of 256 elements keeps ``exp_avg`` and
-``exp_avg_rms``, the square root of the second moment, as ``float8_e4m3fn`` times a power of two: 2.03 bytes an
-element instead of 8.  They are rounded at random (up as often as what is cut off is part of a step), because a moving
-average with a beta near one would never leave its value under rounding to nearest; the random bits are a hash of the
-element's place, the number of the optimizer's step and ``seed``, so a run can be repeated bit for bit and does not depend on the
-launch.  A
-gradient that is no number spoils its own element, and the 8-bit states of its block.
+parameters (:meth:`AdamW.flat_state`).  A tensor that is frozen has none; with its first gradient the buffers are laid
+out anew.  With ``state_bits=8`` each block of 256 elements keeps ``exp_avg`` and ``exp_avg_rms``, the square root of
+the second moment, as ``float8_e4m3fn`` times a power of two: 2.03 bytes an element instead of 8.  They are rounded at
+random (up as often as what is cut off is part of a step), because a moving average with a beta near one would never
+leave its value under rounding to nearest; the random bits are a hash of the element's place, the number of the
+optimizer's step and ``seed``, so a run can be repeated bit for bit and does not depend on the launch.  A gradient that
+is no number spoils its own element, and the 8-bit states of its block.
 """
 from __future__ import annotations
 
@@ -247,7 +247,7 @@ class AdamW(torch.optim.Optimizer):
 
     def _step(self) -> None:
         if self._frozen:
-            thawed = [p for p in self._frozen if p.grad is not None]
+            thawed = _lib.host().graded(self._frozen)
             if thawed:
                 self._take_too(thawed)
         self._place()
