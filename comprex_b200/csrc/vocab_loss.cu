@@ -12,10 +12,11 @@
 // limit, forward and backward 2.7 ms (1.23 PFLOP/s with the logits counted twice).
 //
 // P in 16 bits: a probability of a large vocabulary times the 1 / rows of a mean is below what fp16 can hold, so P is
-// stored times a power of two that brings the largest finite |g_r| to [2^13, 2^14), and both products take it out at the end.
-// One power for all rows, since dw adds rows up.  What it costs in fp16 where rows are weighted far apart: dh of a row at 2^-16 /
-// 2^-20 / 2^-24 / 2^-28 of the largest g is 2.6e-4 / 5.4e-4 / 6e-3 / 4e-2 of itself off (2.4e-4 at the largest, of which its own
-// rounding is 2.0e-4; 50257 words).  Such rows count for less in dw than its rounding, and 2^-30 is the whole range of fp16.
+// stored relative to the largest finite |g_r|, times 2^14, and both products take that out at the end, in 32 bits.  So a gradient that
+// all rows share is not rounded: times a power of two alone, its own rounding was a common error of all probabilities (bf16, 255
+// rows: 2^-8 of dh and dw).  One factor for all rows, since dw adds rows up.  What it costs in fp16 where rows are weighted far apart:
+// dh of a row at 2^-16 / 2^-20 / 2^-24 / 2^-28 of the largest g is 2.1e-4 / 3.9e-4 / 3e-3 / 3e-2 of itself off (2.0e-4 at the largest: its own
+// rounding; 50257 words).  Such rows count for less in dw than its rounding, and 2^-30 is the whole range of fp16.
 #include "cx_product.cuh"
 
 namespace {
@@ -121,8 +122,8 @@ struct Factors {
   int64_t rows, grad_stride, ignore;
   int reduction;
   float* lse2;          // [rows] lse in units of log 2
-  float* factor;        // [rows] g_r times the power of two
-  float* scale;         // its inverse
+  float* factor;        // [rows] 2^14 g_r / base
+  float* scale;         // base / 2^14
 };
 
 __device__ __forceinline__ float row_grad(const Factors& f, int64_t r) {
@@ -153,13 +154,13 @@ __global__ void __launch_bounds__(1024) factor_kernel(const __grid_constant__ Fa
   } else {
     top = __float_as_uint(*f.grad / per) & 0x7FFFFFFFu;
   }
-  // exponent e of the largest: 2^(13 - e) and back, both normal numbers for every e that is clamped to [-100, 120]
-  const int e = min(max((int)(top >> 23) - 127, -100), 120);
-  const float up = __uint_as_float((uint32_t)(13 - e + 127) << 23);
-  if (blockIdx.x == 0 && threadIdx.x == 0) *f.scale = __uint_as_float((uint32_t)(e - 13 + 127) << 23);
+  // the largest itself, or a power of two where it is so far out that a quotient or product would leave the normal numbers
+  const int e = (int)(top >> 23) - 127;
+  const float base = e < -100 ? 0x1p-100f : e > 120 ? 0x1p120f : __uint_as_float(top);
+  if (blockIdx.x == 0 && threadIdx.x == 0) *f.scale = base * 0x1p-14f;
   for (int64_t r = blockIdx.x * 1024ll + threadIdx.x; r < f.rows; r += gridDim.x * 1024ll) {
     const float g = row_grad(f, r);
-    f.factor[r] = g == 0.f ? 0.f : g / per * up;
+    f.factor[r] = g == 0.f ? 0.f : g / per / base * 0x1p14f;
     f.lse2[r] = f.lse[r] * cxprod::kLog2e;
   }
 }

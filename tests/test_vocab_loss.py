@@ -320,3 +320,21 @@ def test_many_words_in_32_bits():
     want = torch.full((vocab, 1), 3.0 / vocab, device="cuda", dtype=torch.float64)
     want[t] -= 1.0
     assert ((dw.double() - want).abs() <= 2.0 ** -18 * want.abs()).all()
+
+
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+@pytest.mark.parametrize("dtype,rows,off", [(torch.bfloat16, 4080, 2.0 ** -11), (torch.float16, 4094, 2.0 ** -14)])
+def test_gradients_have_no_common_error(device, dtype, rows, off, reduction):
+    """A gradient that all rows share, here one that lies half-way between two numbers of the type (1 / 255 and 1 / 2047 times a power of
+    two), is not rounded with every probability: what is left are roundings of their own, up to UNIT / sqrt(3) in a row and averaged over the
+    rows, five standard deviations of which are 5 * 2^-8 / 1.7 / 64 = 2^-12.4 in bf16 and 2^-15.4 in fp16."""
+    h, w, t, _ = _inputs(rows, 257, 64, dtype, device, ignored=0.0)
+    h.requires_grad_(), w.requires_grad_()
+    loss = cx.linear_cross_entropy(h, w, t, reduction=reduction)
+    up = torch.ones((), device=device) * 64.0 if reduction == "mean" else torch.full((rows,), 64.0 / rows, device=device)
+    got = torch.autograd.grad(loss, (h, w), up)
+    p = torch.softmax(h.detach().double() @ w.detach().double().T, 1)
+    p[torch.arange(rows), t] -= 1
+    p *= 64.0 / rows
+    for g, want in zip(got, (p @ w.detach().double(), p.T @ h.detach().double())):
+        assert abs((g.double() * want).sum().item() / want.square().sum().item() - 1) <= off
