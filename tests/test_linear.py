@@ -428,3 +428,17 @@ def test_saved_tensors_that_come_back_changed(device):
                     changed = True
                 # either refused, or what came back was the same after all (nothing left to change, a number in float32 already)
                 assert changed or all(p is None or torch.equal(p, q) for p, q in zip(got, want)), which
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size", [(300, 700, 1000), (1030, 67, 515), (4, 4096, 4096), (5, 3000, 130)])
+def test_larger_sizes_in_32_bits(size):
+    """Many tiles of the CUDA cores' product in all three layouts, and few rows of large weights."""
+    for act in (None, "gelu"):
+        x, w, b, r, g = _inputs(*size, torch.float32, "cuda")
+        leaves = [t.requires_grad_() for t in (x, w, b)]
+        y = cx.linear(x, w, b, activation=act, residual=r)
+        grads = torch.autograd.grad(y, leaves, g)
+        _check(*(t.detach() for t in leaves), r, g, act, y, grads)
+        again = cx.linear(x, w, b, activation=act, residual=r)
+        assert torch.equal(again, y) and all(torch.equal(a, c) for a, c in zip(torch.autograd.grad(again, leaves, g), grads))

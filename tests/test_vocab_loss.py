@@ -338,3 +338,14 @@ def test_gradients_have_no_common_error(device, dtype, rows, off, reduction):
     p *= 64.0 / rows
     for g, want in zip(got, (p @ w.detach().double(), p.T @ h.detach().double())):
         assert abs((g.double() * want).sum().item() / want.square().sum().item() - 1) <= off
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size", [(300, 1500, 130), (2700, 21000, 20)])
+def test_larger_sizes_in_32_bits(size):
+    """Many tiles, and several pieces of the vocabulary."""
+    h, w, t, g = _inputs(*size, torch.float32, "cuda")
+    h.requires_grad_(), w.requires_grad_()
+    loss = cx.linear_cross_entropy(h, w, t, reduction="none")
+    dh, dw = torch.autograd.grad(loss, (h, w), g)
+    _check(h.detach(), w.detach(), t, g, "none", loss, dh, dw)
